@@ -134,7 +134,7 @@ def frequencies(rotary, scaling):
         turns = 32768 * f / (2 * math.pi)
         keep = ((turns - 1.0) / 31.0).clamp(0.0, 1.0)
         f, factor = f * keep + f / 8.0 * (1 - keep), 0.1 * math.log(8.0) + 1.0
-    return f.float(), factor
+    return f.float(), torch.tensor(factor, dtype=torch.float32).item()
 
 
 # ----------------------------------------------------------------- inputs

@@ -127,6 +127,55 @@ typedef struct LinearParams {
   unsigned epilogue, epilogueBlock;
 } LinearParams;
 
+/* Rows rotated at positions of their own; strides in elements. */
+typedef struct RopeRowsParams {
+  unsigned tokens, heads, headDim, rotaryDim, layout; /* llmi_rope_layout */
+  unsigned inputTokenStride, inputHeadStride, outputTokenStride, outputHeadStride;
+  float factor;
+} RopeRowsParams;
+
+enum llmi_rope_layout {
+  LLMI_ROPE_HALF = 0,       /* pairs (i, i + rotaryDim / 2) */
+  LLMI_ROPE_INTERLEAVED = 1 /* pairs (2i, 2i + 1) */
+};
+
+/* How a rotation's frequencies theta^(-2i / rotaryDim) are scaled for
+ * contexts longer than originalPositions; see llmi_hip_rope_frequencies. */
+enum llmi_rope_scaling {
+  LLMI_ROPE_SCALING_NONE = 0,
+  LLMI_ROPE_SCALING_LINEAR = 1,
+  LLMI_ROPE_SCALING_NTK = 2,
+  LLMI_ROPE_SCALING_YARN = 3,
+  LLMI_ROPE_SCALING_BANDS = 4
+};
+typedef struct RopeScalingParams {
+  unsigned rotaryDim, scaling;
+  float theta, scale, originalPositions, lowTurns, highTurns;
+} RopeScalingParams;
+
+/* A pool of pages of the 4-bit cache (pages, pageSize, kvHeads, headDim) and
+ * a call's sequences: `tokens` rows, `sequences` of them, each with a row of
+ * tableStride page numbers. */
+typedef struct PagedKvParams {
+  unsigned pages, pageSize, kvHeads, headDim;
+  unsigned sequences, tableStride, tokens;
+} PagedKvParams;
+
+/* The rows of an append (strides in elements) and the rotation of its keys
+ * (rotaryDim 0: none). */
+typedef struct PagedAppendParams {
+  unsigned keyTokenStride, keyHeadStride, valueTokenStride, valueHeadStride;
+  unsigned rotaryDim, layout; /* llmi_rope_layout */
+  float factor;
+} PagedAppendParams;
+
+/* Attention over a pool: PagedKvParams, the query heads and the score's scale. */
+typedef struct PagedGqaParams {
+  PagedKvParams kv;
+  unsigned queryHeads;
+  float scale;
+} PagedGqaParams;
+
 /* LinearEpilogue, lib/Backend/Metal/Kernels/ReferenceParams.h:8-16 */
 enum llmi_linear_epilogue {
   LLMI_LINEAR_NONE = 0,
@@ -172,7 +221,11 @@ enum llmi_hip_op {
   LLMI_HIP_OP_COPY_HALF_VIEW = 21,      /* params: HalfViewParams */
   LLMI_HIP_OP_LINEAR_F16 = 22,          /* params: LinearParams */
   LLMI_HIP_OP_ADD_RMS_NORM_QUANTIZE = 23, /* params: RowParams */
-  LLMI_HIP_OP_ADD_RMS_NORM_LINEAR_W8A8 = 24 /* params: NormLinearParams */
+  LLMI_HIP_OP_ADD_RMS_NORM_LINEAR_W8A8 = 24, /* params: NormLinearParams */
+  LLMI_HIP_OP_ROPE = 25,                /* params: RopeRowsParams */
+  LLMI_HIP_OP_PAGED_APPEND = 26,        /* params: PagedKvParams */
+  LLMI_HIP_OP_PAGED_READ = 27,          /* params: PagedKvParams */
+  LLMI_HIP_OP_PAGED_GQA = 28            /* params: PagedGqaParams */
 };
 
 /* ---------------------------------------------------------------- KvAppend
@@ -379,6 +432,89 @@ LLMI_HIP_API int llmi_hip_gated_attention_activated(
     const float *q_weight, const float *k_weight, uint16_t *k_cache, uint16_t *v_cache,
     uint16_t *out, GqaParams p, unsigned rotary_dim, float epsilon, float theta,
     void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------- rotary rows, paged 4-bit cache
+ * For a program that serves several long contexts at once; the reference has
+ * no counterpart (its cache is one contiguous fp16 run of one sequence,
+ * lib/GraphIR/Graph.cpp:248-279, and its rotation is partialRope's,
+ * Graph.metal:111-129).
+ *
+ * rope: row (t, h) of `input` (headDim halves at t * inputTokenStride + h *
+ * inputHeadStride) is rotated at positions[t] and written to `output` (its
+ * strides). Pair i < rotaryDim / 2 of a row turns by positions[t] *
+ * freqs[i]: with c = fp32(factor cos), s = fp32(factor sin) (taken in
+ * double), (x, y) becomes fp16(x c - y s), fp16(y c + x s) in fp32; the rest
+ * of the row is copied. Positions may be negative. In place when output and
+ * input are the same rows with the same strides; other overlaps are
+ * undefined. rotaryDim even, at most headDim and 2048; strides at least
+ * what keeps the output's rows apart (headDim for heads, not checked where
+ * there is one). positions, freqs: device memory. */
+LLMI_HIP_API int llmi_hip_rope(const uint16_t *input, const int32_t *positions,
+                               const float *freqs, uint16_t *output, RopeRowsParams p,
+                               void *stream);
+
+/* The rotaryDim / 2 frequencies of a rotation, into host memory, and the
+ * factor its cosines and sines are multiplied by. With f = theta^(-2i /
+ * rotaryDim), s = scale and r = originalPositions f / (2 pi) (the turns of a
+ * pair over the original context):
+ *   NONE    f                          LINEAR  f / s
+ *   NTK     (theta s^(rotaryDim / (rotaryDim - 2)))^(-2i / rotaryDim)
+ *   YARN    g f + (1 - g) f / s, g = (r - lowTurns) / (highTurns - lowTurns)
+ *           clamped to [0, 1]; factor 0.1 ln(s) + 1 (1 for s <= 1)
+ *   BANDS   the frequencies of YARN with factor 1
+ * taken in double and rounded once. */
+LLMI_HIP_API int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, float *factor);
+
+/* A pool holds keys and values of headDim 64, 128 or 256 in 4 bits, a scale
+ * and a bias (fp16) for each 32 channels of each key and value: group by
+ * group s = fp16((max - min) / 15), b = fp16(min - 16 s), code = clamp(rint((
+ * x - b) / s) - 16, 0, 15), and the cache's value is fp16((16 + code) s + b).
+ * Values are kept to +-16384 (NaN as 0). It is pages x
+ * kvHeads x (pageSize / 32) blocks of 40 headDim bytes, 16-byte aligned, any
+ * bytes at first; pageSize is a multiple of 32. What lies in a block is the
+ * library's business (csrc/paged_kv.hpp); pages can be copied whole.
+ *
+ * A call's rows are those of `sequences` sequences: sequence s has rows
+ * [starts[s], starts[s + 1]) of the `tokens` rows (none is allowed), its row
+ * starts[s] + i at position past[s] + i, kept in page table[s * tableStride +
+ * position / pageSize]. starts [sequences + 1], past and table are device
+ * memory, so that a captured graph can be replayed on new lengths. Rows of no
+ * sequence are neither read nor written. A row whose position is not in its
+ * table (negative, or from tableStride * pageSize on) or whose page is not in
+ * the pool is an error that only the device can see: it sets bit 1 (2) of
+ * *invalid (when invalid is not null; never cleared here), is not appended,
+ * and is NaN where it is read or attended to. Two sequences of a call may
+ * share pages that the call does not append to.
+ *
+ * paged_append: keys and values [tokens][kvHeads][headDim] fp16 (strided;
+ * p.tokens rows) to their places; keys are rotated at their positions as
+ * llmi_hip_rope does, with the same bits, first. Sets bit 0 (1) of *invalid
+ * for a value that is not finite or past +-16384. */
+LLMI_HIP_API int llmi_hip_paged_append(const uint16_t *keys, const uint16_t *values,
+                                       const int32_t *starts, const int32_t *past,
+                                       const int32_t *table, const float *freqs, void *pool,
+                                       uint32_t *invalid, PagedKvParams p, PagedAppendParams a,
+                                       void *stream);
+
+/* The cache's values of the call's rows, into keys and values
+ * [tokens][kvHeads][headDim] fp16 (dense, 16-byte aligned). */
+LLMI_HIP_API int llmi_hip_paged_read(const void *pool, const int32_t *starts,
+                                     const int32_t *past, const int32_t *table, uint16_t *keys,
+                                     uint16_t *values, uint32_t *invalid, PagedKvParams p,
+                                     void *stream);
+
+/* CausalGqa of every row over its own sequence's cache: row (starts[s] + i,
+ * h) is the softmax over keys j <= past[s] + i of scale q . K[j, h /
+ * (queryHeads / kvHeads)], times V. q and out [tokens][queryHeads][headDim]
+ * fp16, dense, 16-byte aligned; the call's own rows are appended before.
+ * `workspace` holds llmi_hip_paged_gqa_workspace_bytes(p) bytes, 16-byte
+ * aligned: the partials of rows whose keys are divided over workgroups,
+ * written and read within the call. */
+LLMI_HIP_API int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts,
+                                    const int32_t *past, const int32_t *table, const void *pool,
+                                    uint16_t *out, uint32_t *invalid, PagedGqaParams p,
+                                    void *workspace, size_t workspace_bytes, void *stream);
+LLMI_HIP_API size_t llmi_hip_paged_gqa_workspace_bytes(PagedGqaParams p);
 
 /* ------------------------------------------------------------- DeltaUpdate
  * Replaces graphDeltaUpdate (Graph.metal:146-170 with updateDeltaColumn,

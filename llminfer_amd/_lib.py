@@ -43,11 +43,21 @@ OP_COPY_HALF_VIEW = 21
 OP_LINEAR_F16 = 22
 OP_ADD_RMS_NORM_QUANTIZE = 23
 OP_ADD_RMS_NORM_LINEAR_W8A8 = 24
+OP_ROPE = 25
+OP_PAGED_APPEND = 26
+OP_PAGED_READ = 27
+OP_PAGED_GQA = 28
 NORM_LINEAR_MAX = 4  # LLMI_HIP_NORM_LINEAR_MAX
 
 # LinearEpilogue (ReferenceParams.h:8-16)
 LINEAR_NONE, LINEAR_SILU, LINEAR_SILU_MUL, LINEAR_SIGMOID_COLUMNS = 0, 1, 2, 3
 LINEAR_SILU_F32, LINEAR_DELTA_BETA, LINEAR_DELTA_DECAY = 4, 5, 6
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1  # llmi_rope_layout
+# llmi_rope_scaling
+ROPE_SCALING_NONE, ROPE_SCALING_LINEAR, ROPE_SCALING_NTK = 0, 1, 2
+ROPE_SCALING_YARN, ROPE_SCALING_BANDS = 3, 4
+PAGED_VALUE, PAGED_PLACE = 1, 2  # bits of a paged call's invalid word
 
 NOALLOC_SCRATCH_BYTES = 8 << 20  # LLMI_HIP_NOALLOC_SCRATCH_BYTES
 
@@ -132,6 +142,34 @@ class GraphDeltaParams(C.Structure):
                 ("valueHeads", C.c_uint), ("valueDim", C.c_uint)]
 
 
+class RopeRowsParams(C.Structure):
+    _fields_ = [(n, C.c_uint) for n in ("tokens", "heads", "headDim", "rotaryDim", "layout",
+                                        "inputTokenStride", "inputHeadStride",
+                                        "outputTokenStride", "outputHeadStride")] + \
+               [("factor", C.c_float)]
+
+
+class RopeScalingParams(C.Structure):
+    _fields_ = [("rotaryDim", C.c_uint), ("scaling", C.c_uint)] + \
+               [(n, C.c_float) for n in ("theta", "scale", "originalPositions", "lowTurns",
+                                         "highTurns")]
+
+
+class PagedKvParams(C.Structure):
+    _fields_ = [(n, C.c_uint) for n in ("pages", "pageSize", "kvHeads", "headDim", "sequences",
+                                        "tableStride", "tokens")]
+
+
+class PagedAppendParams(C.Structure):
+    _fields_ = [(n, C.c_uint) for n in ("keyTokenStride", "keyHeadStride", "valueTokenStride",
+                                        "valueHeadStride", "rotaryDim", "layout")] + \
+               [("factor", C.c_float)]
+
+
+class PagedGqaParams(C.Structure):
+    _fields_ = [("kv", PagedKvParams), ("queryHeads", C.c_uint), ("scale", C.c_float)]
+
+
 class SessionConfig(C.Structure):
     _fields_ = [("capacity", C.c_uint), ("queryHeads", C.c_uint),
                 ("kvHeads", C.c_uint), ("headDim", C.c_uint),
@@ -208,6 +246,14 @@ SIGNATURES = {
                                                     NormLinearParams, _P]),
     "llmi_hip_gated_rms_norm_activated_quantize": (C.c_int, [_P, _P, _P, _P, _P, _P, _P,
                                                              RowParams, _P]),
+    "llmi_hip_rope": (C.c_int, [_P, _P, _P, _P, RopeRowsParams, _P]),
+    "llmi_hip_rope_frequencies": (C.c_int, [RopeScalingParams, C.POINTER(C.c_float),
+                                            C.POINTER(C.c_float)]),
+    "llmi_hip_paged_append": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, PagedKvParams,
+                                        PagedAppendParams, _P]),
+    "llmi_hip_paged_read": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedKvParams, _P]),
+    "llmi_hip_paged_gqa": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedGqaParams, _P, _SZ, _P]),
+    "llmi_hip_paged_gqa_workspace_bytes": (_SZ, [PagedGqaParams]),
     "llmi_hip_workspace_init": (C.c_int, [_P, _SZ, _P]),
     "llmi_hip_dispatch_count": (C.c_uint, [C.c_int, _P]),
     "llmi_hip_kernel_name": (C.c_char_p, [C.c_int, _P, C.c_uint]),

@@ -33,11 +33,13 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
 
 
 # Per-file additions. norm_rope.hip, delta_front.hip, w8a8.hip and graph_ops.hip reproduce
-# the reference's fp16 rounding points bit for bit, which needs every fp32 product rounded on its own: under
+# the reference's fp16 rounding points bit for bit (rope_rows.hip and paged_append.hip those of
+# their own formulas), which needs every fp32 product rounded on its own: under
 # the default -ffp-contract=fast the backend folds a product and the fp16
 # conversion or add after it into one fused instruction.
 FILE_FLAGS = {"norm_rope.hip": ["-ffp-contract=off"], "delta_front.hip": ["-ffp-contract=off"],
-              "w8a8.hip": ["-ffp-contract=off"], "graph_ops.hip": ["-ffp-contract=off"]}
+              "w8a8.hip": ["-ffp-contract=off"], "graph_ops.hip": ["-ffp-contract=off"],
+              "rope_rows.hip": ["-ffp-contract=off"], "paged_append.hip": ["-ffp-contract=off"]}
 
 
 def hipcc() -> str:

@@ -42,6 +42,16 @@ static bool fits32(uint64_t a, uint64_t b, uint64_t c) {
   return abc <= 0xffffffffull;
 }
 
+// Whether no two rows of tokens x heads rows of `dim` elements overlap, the
+// heads of a token inside its stride or the tokens of a head inside its.
+static bool strides_apart(uint64_t tokens, uint64_t tokenStride, uint64_t heads,
+                          uint64_t headStride, uint64_t dim) {
+  if (tokens == 1 || heads == 1)
+    return (tokens == 1 || tokenStride >= dim) && (heads == 1 || headStride >= dim);
+  return (headStride >= dim && tokenStride >= (heads - 1) * headStride + dim) ||
+         (tokenStride >= dim && headStride >= (tokens - 1) * tokenStride + dim);
+}
+
 int check_gqa(const GqaParams &p) {
   if (p.tokens == 0 || p.queryHeads == 0 || p.kvHeads == 0 || p.headDim == 0)
     return fail(LLMI_HIP_INVALID_ARGUMENT,
@@ -984,6 +994,156 @@ int llmi_hip_workspace_init(void *workspace, size_t bytes, void *stream) {
                   "workspace_init");
 }
 
+// ------------------------------------------- rotary rows, paged 4-bit cache
+
+int llmi_hip_rope(const uint16_t *input, const int32_t *positions, const float *freqs,
+                  uint16_t *output, RopeRowsParams p, void *stream) {
+  if (p.tokens == 0 || p.heads == 0 || p.headDim == 0)
+    return LLMI_HIP_OK;
+  if (!input || !output || (p.rotaryDim && (!positions || !freqs)))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: null buffer");
+  if (p.rotaryDim % 2 || p.rotaryDim > p.headDim)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: rotary width %u must be even and <= width %u",
+                p.rotaryDim, p.headDim);
+  if (p.layout > LLMI_ROPE_INTERLEAVED)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: unknown layout %u", p.layout);
+  if (!rope_rows_supported(p.rotaryDim))
+    return fail(LLMI_HIP_UNSUPPORTED, "rope: rotary width %u", p.rotaryDim);
+  if (!strides_apart(p.tokens, p.outputTokenStride, p.heads, p.outputHeadStride, p.headDim))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: the output's rows overlap");
+  if (!fits32(p.tokens, p.heads, p.headDim))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: exceeds the 32-bit index range");
+  return launched(launch_rope_rows(input, positions, freqs, output, p,
+                                   static_cast<hipStream_t>(stream)),
+                  "ropeRows");
+}
+
+int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, float *factor) {
+  if (!freqs || !factor)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "ropeFrequencies: null buffer");
+  if (p.rotaryDim % 2)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "ropeFrequencies: rotary width %u is odd", p.rotaryDim);
+  if (p.scaling > LLMI_ROPE_SCALING_BANDS)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "ropeFrequencies: unknown scaling %u", p.scaling);
+  const bool ramp = p.scaling == LLMI_ROPE_SCALING_YARN || p.scaling == LLMI_ROPE_SCALING_BANDS;
+  if (!(p.theta > 0.0f) || (p.scaling && !(p.scale > 0.0f)) ||
+      (ramp && !(p.originalPositions > 0.0f && p.highTurns > p.lowTurns)))
+    return fail(LLMI_HIP_INVALID_ARGUMENT,
+                "ropeFrequencies: theta, scale and the original positions must be positive and "
+                "the turns in order");
+  double theta = p.theta;
+  if (p.scaling == LLMI_ROPE_SCALING_NTK && p.rotaryDim > 2)
+    theta *= pow((double)p.scale, (double)p.rotaryDim / (p.rotaryDim - 2));
+  for (unsigned i = 0; i < p.rotaryDim / 2; ++i) {
+    double f = pow(theta, -2.0 * i / p.rotaryDim);
+    if (p.scaling == LLMI_ROPE_SCALING_LINEAR)
+      f /= p.scale;
+    if (ramp) {
+      const double turns = p.originalPositions * f / 6.283185307179586;
+      double keep = (turns - p.lowTurns) / ((double)p.highTurns - p.lowTurns);
+      keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+      f = keep * f + (1.0 - keep) * f / p.scale;
+    }
+    freqs[i] = (float)f;
+  }
+  *factor = p.scaling == LLMI_ROPE_SCALING_YARN && p.scale > 1.0f
+                ? (float)(0.1 * log((double)p.scale) + 1.0)
+                : 1.0f;
+  return LLMI_HIP_OK;
+}
+
+// The pool's and the sequences' shape; buffers as the caller lists them.
+static int check_paged(const char *what, const PagedKvParams &p, const int32_t *starts,
+                       const int32_t *past, const int32_t *table, const void *pool) {
+  if (p.headDim != 64 && p.headDim != 128 && p.headDim != 256)
+    return fail(LLMI_HIP_UNSUPPORTED, "%s: head_dim %u (64, 128 or 256)", what, p.headDim);
+  if (p.pageSize == 0 || p.pageSize % 32)
+    return fail(LLMI_HIP_UNSUPPORTED, "%s: page size %u is no multiple of 32", what, p.pageSize);
+  if (p.pages == 0 || p.kvHeads == 0 || p.tableStride == 0)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: pages, heads and table must not be empty", what);
+  if ((uint64_t)p.tableStride * p.pageSize > 0x7fffffffull || p.tokens > 0x7fffffffu ||
+      p.pages > 0x7fffffffu || p.sequences > 0x7fffffffu || p.kvHeads > 65535u)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: exceeds the 31-bit range of positions, rows, "
+                "pages and sequences, or 65535 heads", what);
+  if (!starts || !past || !table || !pool)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: null buffer", what);
+  if (!aligned16(pool))
+    return fail(LLMI_HIP_UNSUPPORTED, "%s: pool not 16-byte aligned", what);
+  return LLMI_HIP_OK;
+}
+
+int llmi_hip_paged_append(const uint16_t *keys, const uint16_t *values, const int32_t *starts,
+                          const int32_t *past, const int32_t *table, const float *freqs,
+                          void *pool, uint32_t *invalid, PagedKvParams p, PagedAppendParams a,
+                          void *stream) {
+  if (p.tokens == 0 || p.sequences == 0)
+    return LLMI_HIP_OK;
+  if (int rc = check_paged("pagedAppend", p, starts, past, table, pool))
+    return rc;
+  if (!keys || !values || (a.rotaryDim && !freqs))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedAppend: null buffer");
+  if (a.rotaryDim % 2 || a.rotaryDim > p.headDim || a.layout > LLMI_ROPE_INTERLEAVED)
+    return fail(LLMI_HIP_INVALID_ARGUMENT,
+                "pagedAppend: rotary width %u (even, <= %u) or layout %u", a.rotaryDim, p.headDim,
+                a.layout);
+  return launched(launch_paged_append(keys, values, starts, past, table, freqs, pool, invalid, p,
+                                      a, static_cast<hipStream_t>(stream)),
+                  "pagedAppend");
+}
+
+int llmi_hip_paged_read(const void *pool, const int32_t *starts, const int32_t *past,
+                        const int32_t *table, uint16_t *keys, uint16_t *values,
+                        uint32_t *invalid, PagedKvParams p, void *stream) {
+  if (p.tokens == 0 || p.sequences == 0)
+    return LLMI_HIP_OK;
+  if (int rc = check_paged("pagedRead", p, starts, past, table, pool))
+    return rc;
+  if (!keys || !values)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedRead: null buffer");
+  if (!aligned16(keys) || !aligned16(values))
+    return fail(LLMI_HIP_UNSUPPORTED, "pagedRead: rows not 16-byte aligned");
+  return launched(launch_paged_read(pool, starts, past, table, keys, values, invalid, p,
+                                    static_cast<hipStream_t>(stream)),
+                  "pagedRead");
+}
+
+static int check_paged_heads(const PagedGqaParams &p) {
+  if (p.queryHeads == 0 || p.kv.kvHeads == 0 || p.queryHeads % p.kv.kvHeads ||
+      p.queryHeads > 65535u)
+    return fail(LLMI_HIP_INVALID_ARGUMENT,
+                "pagedGqa: query heads %u not a multiple of KV heads %u (at most 65535)",
+                p.queryHeads, p.kv.kvHeads);
+  return LLMI_HIP_OK;
+}
+
+int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
+                       const int32_t *table, const void *pool, uint16_t *out, uint32_t *invalid,
+                       PagedGqaParams p, void *workspace, size_t workspace_bytes, void *stream) {
+  if (p.kv.tokens == 0 || p.kv.sequences == 0)
+    return LLMI_HIP_OK;
+  if (int rc = check_paged("pagedGqa", p.kv, starts, past, table, pool))
+    return rc;
+  if (int rc = check_paged_heads(p))
+    return rc;
+  if (!q || !out)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedGqa: null buffer");
+  if (!aligned16(q) || !aligned16(out))
+    return fail(LLMI_HIP_UNSUPPORTED, "pagedGqa: rows not 16-byte aligned");
+  const size_t need = paged_gqa_workspace_bytes(p.kv, p.queryHeads);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(LLMI_HIP_WORKSPACE, "pagedGqa: workspace of %zu bytes, %zu needed (16-byte "
+                "aligned)", workspace ? workspace_bytes : 0, need);
+  return launched(launch_paged_gqa(q, starts, past, table, pool, out, invalid, workspace, p.kv,
+                                   p.queryHeads, p.scale, static_cast<hipStream_t>(stream)),
+                  "pagedGqa");
+}
+
+size_t llmi_hip_paged_gqa_workspace_bytes(PagedGqaParams p) {
+  if (p.kv.tokens == 0 || p.kv.sequences == 0 || check_paged_heads(p))
+    return 0;
+  return paged_gqa_workspace_bytes(p.kv, p.queryHeads);
+}
+
 // Whether a supported CausalGqa is a prefill that divides its keys.
 static bool prefill_merges(const GqaParams &p) {
   return select_gqa(p) == GqaKernel::Prefill &&
@@ -1088,6 +1248,19 @@ unsigned llmi_hip_dispatch_count(int op, const void *params) {
   case LLMI_HIP_OP_GATED_RMS_NORM: {
     const RowParams &p = *static_cast<const RowParams *>(params);
     return p.rows && p.width ? 1 : 0;
+  }
+  case LLMI_HIP_OP_ROPE: {
+    const RopeRowsParams &p = *static_cast<const RopeRowsParams *>(params);
+    return p.tokens && p.heads && p.headDim ? 1 : 0;
+  }
+  case LLMI_HIP_OP_PAGED_APPEND:
+  case LLMI_HIP_OP_PAGED_READ: {
+    const PagedKvParams &p = *static_cast<const PagedKvParams *>(params);
+    return p.tokens && p.sequences ? 1 : 0;
+  }
+  case LLMI_HIP_OP_PAGED_GQA: {
+    const PagedGqaParams &p = *static_cast<const PagedGqaParams *>(params);
+    return p.kv.tokens && p.kv.sequences && !check_paged_heads(p) ? 1 : 0;
   }
   case LLMI_HIP_OP_GATED_ATTENTION: {
     // Launches for a rotary width the kernels take (a multiple of 16).
@@ -1198,6 +1371,14 @@ const char *llmi_hip_kernel_name(int op, const void *params, unsigned index) {
                                   nullptr, nullptr, nullptr)
                ? "sigmoidMulVec"
                : "sigmoidMulScalar";
+  case LLMI_HIP_OP_ROPE:
+    return "ropeRows";
+  case LLMI_HIP_OP_PAGED_APPEND:
+    return "pagedAppend";
+  case LLMI_HIP_OP_PAGED_READ:
+    return "pagedRead";
+  case LLMI_HIP_OP_PAGED_GQA:
+    return "pagedGqa";
   case LLMI_HIP_OP_GATED_ATTENTION:
     if (static_cast<const GqaParams *>(params)->tokens == 1)
       return index == 0 ? "gqaDecodeGated" : "gqaDecodeMergeGated";

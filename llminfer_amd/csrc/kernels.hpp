@@ -287,4 +287,22 @@ hipError_t launch_copy_half_view(const uint16_t *src, uint16_t *out, const HalfV
 hipError_t launch_linear_f16(const uint16_t *in, const uint16_t *w, void *out, const void *aux,
                              const float *bias, const LinearParams &p, hipStream_t stream);
 
+// ------------------------------------------- rotary rows, paged 4-bit cache
+// (layouts and the format: paged_kv.hpp)
+bool rope_rows_supported(unsigned rotaryDim);
+hipError_t launch_rope_rows(const uint16_t *input, const int32_t *positions, const float *freqs,
+                            uint16_t *output, const RopeRowsParams &p, hipStream_t stream);
+hipError_t launch_paged_append(const uint16_t *keys, const uint16_t *values, const int32_t *starts,
+                               const int32_t *past, const int32_t *table, const float *freqs,
+                               void *pool, uint32_t *invalid, const PagedKvParams &p,
+                               const PagedAppendParams &a, hipStream_t stream);
+hipError_t launch_paged_read(const void *pool, const int32_t *starts, const int32_t *past,
+                             const int32_t *table, uint16_t *keys, uint16_t *values,
+                             uint32_t *invalid, const PagedKvParams &p, hipStream_t stream);
+size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads);
+hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
+                            const int32_t *table, const void *pool, uint16_t *out,
+                            uint32_t *invalid, void *workspace, const PagedKvParams &p,
+                            unsigned queryHeads, float scale, hipStream_t stream);
+
 } // namespace llmi

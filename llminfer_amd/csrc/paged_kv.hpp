@@ -1,0 +1,148 @@
+// The paged 4-bit KV cache on the device: where a pool keeps a key and a
+// value, and the sequences of a call.
+//
+// A pool is [pages][kvHeads][pageSize / 32] blocks of 40 D bytes, a block the
+// 32 keys of one KV head that follow each other, as the matrix instructions
+// take them:
+//   16 D  key codes    [t 2][D/128][quad 4][row 16][32 channels]   (D 64: 16)
+//    4 D  key scales   [t 2][D/32][row 16]{scale, bias}            fp16
+//   16 D  value codes  [D/64][quad 4][D%16 16][4][8 keys]
+//    4 D  value scales [D/32]{scales, biases}[quad 4][8 keys]      fp16
+// Key 16 m + 8 t + 4 h + v of a block is row 8 m + 4 h + v of the keys' tile
+// t, and slot 4 t + v of the values' quad 2 m + h: the keys that a lane of
+// the 16x16 score tiles holds are then the eight of one value word. Slot e of
+// a word (for keys: channel 8 w + e of word w) is nibble e / 2 + 4 (e % 2),
+// so that one mask gives two neighbours, 16 bits apart.
+//
+// A group is 32 channels of one key or value: scale s = fp16((max - min) /
+// 15), bias b = fp16(min - 16 s), code = clamp(rint((x - b) / s) - 16, 0, 15),
+// and a code stands for fp16((16 + code) s + b): with the 16 in it, the value
+// is one packed fma on nibbles put behind the fp16 exponent of 16.
+#pragma once
+
+#include "hip_common.hpp"
+#include "llminfer_hip.h"
+
+namespace llmi {
+
+constexpr float kPagedLimit = 16384.0f; // values are kept to +-this: 16 s and b stay finite
+
+// invalid bits
+constexpr unsigned kPagedValue = 1u; // a value not finite or past the limit
+constexpr unsigned kPagedPlace = 2u; // a row whose place is not in its table or the pool
+
+struct PagedView {
+  const int32_t *starts, *past, *table;
+  unsigned pages, pageSize, kvHeads, dim, sequences, tableStride, tokens;
+};
+
+inline PagedView paged_view(const PagedKvParams &p, const int32_t *starts, const int32_t *past,
+                            const int32_t *table) {
+  return PagedView{starts,     past,        table,         p.pages,  p.pageSize, p.kvHeads,
+                   p.headDim, p.sequences, p.tableStride, p.tokens};
+}
+
+// Rows [row0, row0 + rows) of the call, at positions past + i. ok: they fit
+// their table.
+struct PagedSeq {
+  unsigned row0, rows, past;
+  bool ok;
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedView &g, unsigned s) {
+  const int T = (int)g.tokens;
+  const int lo = min(max(g.starts[s], 0), T), hi = min(max(g.starts[s + 1], lo), T);
+  const int past = g.past[s];
+  const long long last = (long long)past + (hi - lo);
+  PagedSeq q;
+  q.row0 = (unsigned)lo;
+  q.rows = (unsigned)(hi - lo);
+  q.past = (unsigned)past;
+  q.ok = past >= 0 && last <= (long long)g.tableStride * g.pageSize;
+  return q;
+}
+
+// Byte offset of the block of position pos (a multiple of 32 below the
+// table's end); false if its page is not in the pool.
+__device__ __forceinline__ bool paged_block(const PagedView &g, unsigned s, unsigned pos,
+                                            unsigned head, size_t &at) {
+  const unsigned slot = pos / g.pageSize;
+  const unsigned page = (unsigned)g.table[(size_t)s * g.tableStride + slot];
+  const unsigned block = (pos - slot * g.pageSize) / 32;
+  const bool ok = page < g.pages;
+  at = (((size_t)(ok ? page : 0u) * g.kvHeads + head) * (g.pageSize / 32) + block) *
+       (size_t)(40 * g.dim);
+  return ok;
+}
+
+// Places in a block. `key` is 0..31, `word` channels 8 word .. 8 word + 7.
+__host__ __device__ constexpr unsigned paged_row(unsigned key) {
+  return (key >> 4) * 8 + (key & 7);
+}
+__device__ __forceinline__ unsigned paged_key_word(unsigned D, unsigned key, unsigned word) {
+  const unsigned words = D >= 128 ? 4 : 2; // of a lane's chunk
+  const unsigned chunk = word / words;
+  return ((key >> 3) & 1) * 8 * D + (chunk / 4) * 256 * words +
+         ((chunk % 4) * 16 + paged_row(key)) * 4 * words + 4 * (word % words);
+}
+__device__ __forceinline__ unsigned paged_key_scale(unsigned D, unsigned key, unsigned group) {
+  return 16 * D + ((key >> 3) & 1) * 2 * D + (group * 16 + paged_row(key)) * 4;
+}
+__device__ __forceinline__ unsigned paged_quad(unsigned key) {
+  return (key >> 4) * 2 + ((key >> 2) & 1);
+}
+__device__ __forceinline__ unsigned paged_slot(unsigned key) {
+  return ((key >> 3) & 1) * 4 + (key & 3);
+}
+__device__ __forceinline__ unsigned paged_value_word(unsigned D, unsigned key, unsigned channel) {
+  return 20 * D + (channel / 64) * 1024 + (paged_quad(key) * 16 + channel % 16) * 16 +
+         (channel / 16 % 4) * 4;
+}
+// the scale; the bias is 64 bytes further
+__device__ __forceinline__ unsigned paged_value_scale(unsigned D, unsigned key, unsigned group) {
+  return 36 * D + group * 128 + (paged_quad(key) * 8 + paged_slot(key)) * 2;
+}
+// Bit of slot e's nibble in its word.
+__host__ __device__ constexpr unsigned paged_nibble(unsigned e) { return 4 * (e / 2) + 16 * (e % 2); }
+
+// The two values of slots 2 j and 2 j + 1 of a word, with their scales and biases.
+template <int J>
+__device__ __forceinline__ half2_t paged_pair(uint32_t word, half2_t scale, half2_t bias) {
+  // the nibble to mantissa bits 6..9 of an fp16 in [16, 32): 16 + code
+  const uint32_t moved = J == 0 ? word << 6 : J == 1 ? word << 2 : J == 2 ? word >> 2 : word >> 6;
+  const half2_t x = __builtin_bit_cast(half2_t, (moved & 0x03C003C0u) | 0x4C004C00u);
+  return __builtin_elementwise_fma(x, scale, bias);
+}
+__device__ __forceinline__ half_t paged_value(uint32_t word, unsigned e, half_t scale, half_t bias) {
+  const half_t x = (half_t)(float)(16u + ((word >> paged_nibble(e)) & 15u));
+  return __builtin_elementwise_fma(x, scale, bias);
+}
+
+// The call's unit `u` of those that count(sequence) gives each sequence, in
+// order: its sequence and its number there. Every lane of a full wave calls
+// it; false past the last unit.
+template <typename Count>
+__device__ __forceinline__ bool paged_find(const PagedView &g, unsigned u, Count count,
+                                           unsigned &seq, unsigned &local) {
+  const unsigned lane = threadIdx.x % 64;
+  unsigned before = 0;
+  for (unsigned s0 = 0; s0 < g.sequences; s0 += 64) {
+    const unsigned n = s0 + lane < g.sequences ? count(paged_seq(g, s0 + lane)) : 0u;
+    unsigned sum = n;
+    for (unsigned d = 1; d < 64; d *= 2) {
+      const unsigned up = __shfl_up(sum, d);
+      sum += lane >= d ? up : 0u;
+    }
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(u - before < sum);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      seq = s0 + (unsigned)at;
+      local = u - before - (unsigned)__shfl((int)(sum - n), at);
+      return local < (unsigned)__shfl((int)n, at); // (starts out of order: a sum that wrapped)
+    }
+    before += (unsigned)__shfl((int)sum, 63);
+  }
+  return false;
+}
+
+} // namespace llmi

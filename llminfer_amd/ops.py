@@ -958,3 +958,226 @@ def kernel_names(op: int, params) -> list[str]:
     ref = C.byref(params)
     n = lib.llmi_hip_dispatch_count(op, ref)
     return [lib.llmi_hip_kernel_name(op, ref, i).decode() for i in range(n)]
+
+
+# ------------------------------------------- rotary rows, paged 4-bit cache
+
+_LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
+_SCALINGS = {None: _lib.ROPE_SCALING_NONE, "linear": _lib.ROPE_SCALING_LINEAR,
+             "ntk": _lib.ROPE_SCALING_NTK, "yarn": _lib.ROPE_SCALING_YARN,
+             "bands": _lib.ROPE_SCALING_BANDS}
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 1e7, scaling: str | None = None,
+                     scale: float = 1.0, original_positions: float = 32768.0,
+                     low_turns: float = 1.0, high_turns: float = 32.0,
+                     device: torch.device | str = "cuda") -> tuple[torch.Tensor, float]:
+    """(frequencies fp32 [rotary_dim / 2], factor) of a rotation, for rope and
+    paged_append (llmi_hip_rope_frequencies): theta^(-2i / rotary_dim), scaled
+    for contexts longer than original_positions by `scaling`: None, "linear",
+    "ntk", "yarn" or "bands" (yarn's frequencies without its factor)."""
+    if scaling not in _SCALINGS:
+        raise ValueError(f"scaling is one of {sorted(map(str, _SCALINGS))}")
+    out = (C.c_float * max(rotary_dim // 2, 1))()
+    factor = C.c_float()
+    _lib.check(_lib.load().llmi_hip_rope_frequencies(
+        _lib.RopeScalingParams(rotary_dim, _SCALINGS[scaling], theta, scale, original_positions,
+                               low_turns, high_turns), out, C.byref(factor)))
+    freqs = torch.from_numpy(np.array(out[:rotary_dim // 2], dtype=np.float32))
+    return freqs.to(device), factor.value
+
+
+def _layout(name: str) -> int:
+    if name not in _LAYOUTS:
+        raise ValueError(f"layout is one of {sorted(_LAYOUTS)}")
+    return _LAYOUTS[name]
+
+
+def _one_device(*tensors: torch.Tensor | None) -> None:
+    """The call runs on the current stream of the current device."""
+    for t in tensors:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise ValueError("every tensor must be on the current device")
+
+
+def _require_rows(t: torch.Tensor, name: str) -> None:
+    """fp16 rows [T, H, dim]: each row's elements side by side, the rows
+    anywhere (non-negative strides)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.dtype != torch.float16:
+        raise ValueError(f"{name} must be {torch.float16}, got {t.dtype}")
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name} must be [T, H, dim] with contiguous rows")
+
+
+def bind_rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: torch.Tensor,
+              layout: str = "half", factor: float = 1.0) -> "Bound":
+    """Rows x [T, H, dim] fp16 (each row contiguous, any strides between them)
+    rotated at positions [T] (int32) by freqs [rotary_dim / 2] (fp32) into out
+    (the same shape; may be x itself): pairs (i, i + rotary_dim / 2) for layout
+    "half", (2i, 2i + 1) for "interleaved", the rest of a row copied; cosines
+    and sines times `factor` (llmi_hip_rope; rope_frequencies)."""
+    _require_rows(x, "x")
+    _require_rows(out, "out")
+    _require(positions, torch.int32, "positions")
+    _require(freqs, torch.float32, "freqs")
+    T, H, d = x.shape
+    if out.shape != x.shape or positions.shape != (T,) or freqs.dim() != 1:
+        raise ValueError("x and out are [T, H, dim], positions [T], freqs [rotary_dim / 2]")
+    _one_device(x, positions, freqs, out)
+    p = _lib.RopeRowsParams(T, H, d, 2 * freqs.numel(), _layout(layout), x.stride(0), x.stride(1),
+                            out.stride(0), out.stride(1), factor)
+    b = Bound(_lib.load().llmi_hip_rope,
+              (_ptr(x), _ptr(positions), _ptr(freqs), _ptr(out), p, _stream()), "ropeRows")
+    b._keep = (x, positions, freqs, out)
+    return b
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
+         out: torch.Tensor | None = None, layout: str = "half",
+         factor: float = 1.0) -> torch.Tensor:
+    """bind_rope, called once."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    bind_rope(x, positions, freqs, out, layout, factor)()
+    return out
+
+
+def paged_pool(pages: int, page_size: int, kv_heads: int, head_dim: int,
+               device: torch.device | str = "cuda") -> torch.Tensor:
+    """A pool of pages of the 4-bit cache: uint8 [pages, kv_heads, page_size /
+    32, 40 * head_dim] (include/llminfer_hip.h). Its shape says what it holds;
+    pages may be copied whole."""
+    if page_size <= 0 or page_size % 32 or head_dim not in (64, 128, 256):
+        raise ValueError("page_size is a multiple of 32, head_dim 64, 128 or 256")
+    return torch.zeros(pages, kv_heads, page_size // 32, 40 * head_dim, dtype=torch.uint8,
+                       device=device)
+
+
+def _paged(pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor, table: torch.Tensor,
+           tokens: int, invalid: torch.Tensor | None) -> _lib.PagedKvParams:
+    _require(pool, torch.uint8, "pool")
+    for t, n in ((starts, "starts"), (past, "past"), (table, "table")):
+        _require(t, torch.int32, n)
+    if pool.dim() != 4 or pool.shape[3] not in (40 * 64, 40 * 128, 40 * 256):
+        raise ValueError("pool is paged_pool's [pages, kv_heads, page_size / 32, 40 * head_dim]")
+    if past.dim() != 1 or starts.shape != (past.numel() + 1,) or table.dim() != 2 or \
+            table.shape[0] != past.numel():
+        raise ValueError("starts [S + 1], past [S] and table [S, pages] disagree")
+    if invalid is not None:
+        _require(invalid, torch.int32, "invalid")
+        if invalid.numel() != 1:
+            raise ValueError("invalid has one element")
+    return _lib.PagedKvParams(pool.shape[0], 32 * pool.shape[2], pool.shape[1],
+                              pool.shape[3] // 40, past.numel(), table.shape[1], tokens)
+
+
+def bind_paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor,
+                      past: torch.Tensor, table: torch.Tensor,
+                      freqs: torch.Tensor | None = None, layout: str = "half",
+                      factor: float = 1.0, invalid: torch.Tensor | None = None) -> "Bound":
+    """New keys and values k, v [T, Hkv, dim] fp16 (each row contiguous) into
+    their sequences' pages in 4 bits (llmi_hip_paged_append). Sequence s has
+    rows starts[s] .. starts[s + 1] - 1 at positions past[s] + i, position p in
+    page table[s, p // page_size]; starts [S + 1], past [S] and table [S, n]
+    are int32. freqs: keys are rotated at their positions first, as rope does.
+    invalid (int32, one element): bit 0 is set by a value that is not finite
+    or past 16384 in magnitude, bit 1 by a row with no place (such rows are
+    left out)."""
+    for t, n in ((k, "k"), (v, "v")):
+        _require_rows(t, n)
+    p = _paged(pool, starts, past, table, k.shape[0], invalid)
+    if v.shape != k.shape or tuple(k.shape[1:]) != (p.kvHeads, p.headDim):
+        raise ValueError("k and v are [T, kv_heads, head_dim] of the pool")
+    if freqs is not None:
+        _require(freqs, torch.float32, "freqs")
+        if freqs.dim() != 1:
+            raise ValueError("freqs is [rotary_dim / 2]")
+    _one_device(k, v, pool, starts, past, table, freqs, invalid)
+    a = _lib.PagedAppendParams(k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                               2 * freqs.numel() if freqs is not None else 0, _layout(layout),
+                               factor)
+    b = Bound(_lib.load().llmi_hip_paged_append,
+              (_ptr(k), _ptr(v), _ptr(starts), _ptr(past), _ptr(table), _ptr(freqs), _ptr(pool),
+               _ptr(invalid), p, a, _stream()), "pagedAppend")
+    b._keep = (k, v, pool, starts, past, table, freqs, invalid)
+    return b
+
+
+def paged_append(*args, **kwargs) -> None:
+    """bind_paged_append, called once."""
+    bind_paged_append(*args, **kwargs)()
+
+
+def bind_paged_read(pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor,
+                    table: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    invalid: torch.Tensor | None = None) -> "Bound":
+    """The cache's values of a call's rows (as bind_paged_append places them)
+    into k, v [T, Hkv, dim] fp16; a row with no place is NaN and sets bit 1 of
+    invalid. A whole sequence: past 0 and its length as rows."""
+    for t, n in ((k, "k"), (v, "v")):
+        _require(t, torch.float16, n)
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("k and v are [T, kv_heads, head_dim] of the pool")
+    p = _paged(pool, starts, past, table, k.shape[0], invalid)
+    if tuple(k.shape[1:]) != (p.kvHeads, p.headDim):
+        raise ValueError("k and v are [T, kv_heads, head_dim] of the pool")
+    _one_device(pool, starts, past, table, k, v, invalid)
+    b = Bound(_lib.load().llmi_hip_paged_read,
+              (_ptr(pool), _ptr(starts), _ptr(past), _ptr(table), _ptr(k), _ptr(v),
+               _ptr(invalid), p, _stream()), "pagedRead")
+    b._keep = (pool, starts, past, table, k, v, invalid)
+    return b
+
+
+def paged_read(pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor, table: torch.Tensor,
+               tokens: int, invalid: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """bind_paged_read of `tokens` rows, called once: (k, v). Rows of no
+    sequence are zero."""
+    shape = (tokens, pool.shape[1], pool.shape[3] // 40)
+    k, v = (torch.zeros(shape, dtype=torch.float16, device=pool.device) for _ in range(2))
+    bind_paged_read(pool, starts, past, table, k, v, invalid)()
+    return k, v
+
+
+def bind_paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor,
+                   table: torch.Tensor, out: torch.Tensor, scale: float | None = None,
+                   invalid: torch.Tensor | None = None) -> "Bound":
+    """CausalGqa of q [T, Hq, dim] fp16 over the paged 4-bit cache
+    (llmi_hip_paged_gqa): row i of sequence s attends to its keys at positions
+    up to past[s] + i, the call's own rows among them (appended before). scale
+    defaults to 1 / sqrt(dim). Rows of no sequence are left as they are; a row
+    that would read a page outside the pool, or does not fit its table, is NaN
+    and sets bit 1 of invalid."""
+    for t, n in ((q, "q"), (out, "out")):
+        _require(t, torch.float16, n)
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError("q and out are [T, Hq, head_dim]")
+    kv = _paged(pool, starts, past, table, q.shape[0], invalid)
+    if q.shape[2] != kv.headDim or q.shape[1] % max(kv.kvHeads, 1):
+        raise ValueError("q's heads do not match the pool")
+    _one_device(q, pool, starts, past, table, out, invalid)
+    lib = _lib.load()
+    p = _lib.PagedGqaParams(kv, q.shape[1],
+                            float(np.float32(1.0) / np.sqrt(np.float32(q.shape[2])))
+                            if scale is None else scale)
+    need = lib.llmi_hip_paged_gqa_workspace_bytes(p)
+    ws = workspace(need, q.device, "paged") if need else None
+    b = Bound(lib.llmi_hip_paged_gqa,
+              (_ptr(q), _ptr(starts), _ptr(past), _ptr(table), _ptr(pool), _ptr(out),
+               _ptr(invalid), p, _ptr(ws), ws.numel() if ws is not None else 0, _stream()),
+              "+".join(kernel_names(_lib.OP_PAGED_GQA, p)))
+    b._keep = (q, pool, starts, past, table, out, invalid, ws)
+    return b
+
+
+def paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor,
+              table: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
+              invalid: torch.Tensor | None = None) -> torch.Tensor:
+    """bind_paged_gqa, called once. Rows of no sequence of a new `out` are zero."""
+    if out is None:
+        out = torch.zeros_like(q)
+    bind_paged_gqa(q, pool, starts, past, table, out, scale, invalid)()
+    return out

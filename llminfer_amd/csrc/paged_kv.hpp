@@ -119,8 +119,8 @@ __device__ __forceinline__ half_t paged_value(uint32_t word, unsigned e, half_t 
 }
 
 // The call's unit `u` of those that count(sequence) gives each sequence, in
-// order: its sequence and its number there. Every lane of a full wave calls
-// it; false past the last unit.
+// order: its sequence and its number there, the same scalars in every lane.
+// Every lane of a full wave calls it; false past the last unit.
 template <typename Count>
 __device__ __forceinline__ bool paged_find(const PagedView &g, unsigned u, Count count,
                                            unsigned &seq, unsigned &local) {
@@ -137,10 +137,11 @@ __device__ __forceinline__ bool paged_find(const PagedView &g, unsigned u, Count
     if (past) {
       const int at = __builtin_ctzll(past);
       seq = s0 + (unsigned)at;
-      local = u - before - (unsigned)__shfl((int)(sum - n), at);
-      return local < (unsigned)__shfl((int)n, at); // (starts out of order: a sum that wrapped)
+      local = u - before - (unsigned)__builtin_amdgcn_readlane((int)(sum - n), at);
+      // (not so with starts out of order: a sum that wrapped)
+      return local < (unsigned)__builtin_amdgcn_readlane((int)n, at);
     }
-    before += (unsigned)__shfl((int)sum, 63);
+    before += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
   }
   return false;
 }

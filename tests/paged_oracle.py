@@ -72,6 +72,7 @@ def attention(q, k, v, past, scale):
             most = (np.abs(kk) @ np.abs(q[i, h])).max() * abs(scale)
             each = 2 * U16 + 2 * (dim + 8) * 2.0 ** -24 * most + (n + 64) * 2.0 ** -24 + 2.0 ** -21
             far[i, h] = np.abs(out[i, h]) * U16 + 2.0 ** -25 + each * (w @ np.abs(vv))
+            far[i, h] += 2.0 ** -32 * (np.abs(vv).sum(0) + n * np.abs(out[i, h]))
     return out, far
 
 

@@ -73,10 +73,12 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(
     const uint16_t *__restrict__ keys, const uint16_t *__restrict__ values, PagedView g,
     const float *__restrict__ freqs, uint8_t *pool, unsigned *invalid, AppendRows p) {
   extern __shared__ float2 sTurn[]; // [rows of this block][half]
-  unsigned seq, local;
-  if (!paged_find(g, blockIdx.x, [](const PagedSeq &q) { return touched_blocks(q); }, seq, local))
+  unsigned seq, local, before;
+  const PagedSeq own = paged_own(g);
+  if (!paged_find(g, own, blockIdx.x, [](const PagedSeq &q) { return touched_blocks(q); }, seq,
+                  local, before))
     return;
-  const PagedSeq q = paged_seq(g, seq);
+  const PagedSeq q = paged_seq_of(g, own, seq);
   const unsigned head = blockIdx.y, tid = threadIdx.x;
   // keys [first, last) of the block at position base, from the call's row `row`
   const unsigned base = q.past / 32 * 32 + 32 * local;
@@ -189,10 +191,12 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const uint8_t *__r
                                                               PagedView g, uint16_t *keys,
                                                               uint16_t *values,
                                                               unsigned *invalid) {
-  unsigned seq, local;
-  if (!paged_find(g, blockIdx.x, [](const PagedSeq &q) { return touched_blocks(q); }, seq, local))
+  unsigned seq, local, before;
+  const PagedSeq own = paged_own(g);
+  if (!paged_find(g, own, blockIdx.x, [](const PagedSeq &q) { return touched_blocks(q); }, seq,
+                  local, before))
     return;
-  const PagedSeq q = paged_seq(g, seq);
+  const PagedSeq q = paged_seq_of(g, own, seq);
   const unsigned head = blockIdx.y, tid = threadIdx.x, W = g.dim / 8;
   const unsigned base = q.past / 32 * 32 + 32 * local;
   const unsigned first = base < q.past ? q.past - base : 0u;

@@ -1,11 +1,11 @@
 // Causal GQA over the paged 4-bit cache (paged_kv.hpp): a ragged batch of
 // sequences, each with any number of new rows.
 //
-// The 16-column kernel: for one sequence and KV head, the query rows of that
-// head's group (token c / G, head c % G of column c) are 16 columns of the
-// score tiles, S^T = K Q^T with v_mfma_f32_16x16x32_f16. A workgroup takes a
-// range of the keys; each of its waves its own blocks of 32 keys, without
-// waiting for the others:
+// For one sequence and KV head, the query rows of that head's group (token c /
+// G, head c % G of column c) are columns of the score tiles, S^T = K Q^T with
+// v_mfma_f32_16x16x32_f16, CG groups of 16 a unit. A workgroup takes one unit
+// and a range of the keys; each of its waves its own blocks of 32 keys,
+// without waiting for the others:
 //  * a block is 40 D bytes in one piece, so it goes HBM -> LDS by DMA, 1 KB an
 //    instruction, several blocks ahead and without a register;
 //  * codes and scales lie in it as the matrix instructions want them: a lane
@@ -28,7 +28,7 @@
 namespace llmi {
 namespace {
 
-constexpr unsigned kColumns = 16;
+constexpr unsigned kColumns = 16; // of a group
 constexpr unsigned kWaves = 4;
 constexpr unsigned kTargetGroups = 256; // workgroups to fill: one a CU
 constexpr float kRaise = 15.0f;   // raise m when a weight would pass 2^15
@@ -41,15 +41,24 @@ __device__ __forceinline__ float4_t mfma16x16x32(half8_t a, half8_t b, float4_t 
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// The eight values of a word, as a matrix operand.
+__device__ __forceinline__ half8_t paged_eight(uint32_t u, half2_t s0, half2_t s1, half2_t s2,
+                                               half2_t s3, half2_t b0, half2_t b1, half2_t b2,
+                                               half2_t b3) {
+  const half2_t v0 = paged_pair<0>(u, s0, b0), v1 = paged_pair<1>(u, s1, b1);
+  const half2_t v2 = paged_pair<2>(u, s2, b2), v3 = paged_pair<3>(u, s3, b3);
+  return half8_t{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+
 // ---------------------------------------------------------------- the plan
 
 // Units (column blocks) of a sequence, blocks of 32 keys it holds (one where
 // it has no place, for the workgroup that says so), and how its keys are
 // divided: pieces of `chunk` blocks.
 struct Split {
-  unsigned group, chunk;
+  unsigned group, columns, chunk; // columns: of a unit
   __device__ unsigned units(const PagedSeq &q) const {
-    return (unsigned)(((uint64_t)q.rows * group + kColumns - 1) / kColumns);
+    return (unsigned)(((uint64_t)q.rows * group + columns - 1) / columns);
   }
   __device__ static unsigned blocks(const PagedSeq &q) {
     return q.ok ? (q.past + q.rows + 31) / 32 : 1u;
@@ -57,45 +66,54 @@ struct Split {
   __device__ unsigned pieces(const PagedSeq &q) const { return (blocks(q) + chunk - 1) / chunk; }
 };
 
-// The chunk for which the call's blocks make about `target` pieces: a
-// multiple of the waves, at least one block each.
-__device__ __forceinline__ Split paged_split(const PagedView &g, unsigned group, unsigned target) {
-  Split s{group, kWaves};
+// The chunk for which the call's blocks make at most `target` pieces more
+// than units: a multiple of the waves, at least one block each. (An fp32 sum is off by
+// less than the 1.0001; every workgroup and the merge add in the same order.)
+__device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
+                                             unsigned group, unsigned columns, unsigned target) {
+  Split s{group, columns, kWaves};
   const unsigned lane = threadIdx.x % 64;
-  uint64_t all = 0;
-  for (unsigned s0 = 0; s0 < g.sequences; s0 += 64)
+  float all = (float)s.units(own) * (float)Split::blocks(own);
+  for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
     if (s0 + lane < g.sequences) {
       const PagedSeq q = paged_seq(g, s0 + lane);
-      all += (uint64_t)s.units(q) * Split::blocks(q);
+      all += (float)s.units(q) * (float)Split::blocks(q);
     }
-  for (int d = 1; d < 64; d *= 2)
-    all += __shfl_xor(all, d);
-  const uint64_t chunk = (all + target - 1) / target;
-  const unsigned whole = (unsigned)((chunk + kWaves - 1) / kWaves * kWaves);
-  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(whole ? whole : kWaves));
+  all = group_sum<16>(all);
+  LanePair p = pair16(all);
+  all = p.a + p.b;
+  p = pair32(all);
+  all = p.a + p.b;
+  const unsigned chunk = (unsigned)(all * 1.0001f / (float)target) + 1;
+  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)((chunk + kWaves - 1) / kWaves * kWaves));
   return s;
 }
 
 // On the host: most units and pieces a KV head that any lengths can give.
-uint64_t most_units(const PagedKvParams &p, unsigned group) {
-  const uint64_t a = (uint64_t)p.tokens * ((group + kColumns - 1) / kColumns);
-  const uint64_t b = (uint64_t)p.tokens * group / kColumns + p.sequences;
+uint64_t most_units(const PagedKvParams &p, unsigned group, unsigned columns) {
+  const uint64_t a = (uint64_t)p.tokens * ((group + columns - 1) / columns);
+  const uint64_t b = (uint64_t)p.tokens * group / columns + p.sequences;
   return a < b ? a : b;
 }
 unsigned target_pieces(const PagedKvParams &p) {
   return (kTargetGroups + p.kvHeads - 1) / p.kvHeads;
 }
-uint64_t most_pieces(const PagedKvParams &p, unsigned group) {
-  return target_pieces(p) + most_units(p, group);
+uint64_t most_pieces(const PagedKvParams &p, unsigned group, unsigned columns) {
+  return target_pieces(p) + most_units(p, group, columns);
+}
+// Column groups of a unit, by the columns that a sequence has on average.
+unsigned column_groups(const PagedKvParams &p, unsigned group) {
+  const uint64_t columns = (uint64_t)p.tokens * group / p.sequences;
+  return columns <= 16 ? 1 : columns <= 32 || p.headDim == 256 ? 2 : 4;
 }
 
 // ------------------------------------------------------------- the kernel
 
-template <int D> struct Geo {
+template <int D, int CG> struct Geo {
   static constexpr int BLOCK = 40 * D;               // bytes of a block
   static constexpr int LOADS = (BLOCK + 1023) / 1024; // 1-KB loads of one
   static constexpr int STAGE = 1024 * LOADS;
-  static constexpr int RING = D == 256 ? 3 : D == 128 ? 5 : 6;
+  static constexpr int RING = D == 256 && CG < 4 ? 3 : D == 256 ? 2 : D == 128 ? 5 : 6;
   static constexpr int CHUNKS = D >= 128 ? D / 128 : 1; // of a lane's key
   static constexpr int WORDS = D >= 128 ? 4 : 2;        // of a chunk
   static constexpr int TILES = D / 16;                  // output tiles
@@ -104,8 +122,9 @@ template <int D> struct Geo {
 // The ring's buffers are variables of their own, so that the compiler sees
 // that a wait for one need not be a wait for all; the first also takes the
 // waves' partial outputs at the end.
-template <int D, int I> __device__ __forceinline__ char *ring_buffer() {
-  constexpr int stage = kWaves * Geo<D>::STAGE, joined = kWaves * Geo<D>::TILES * 1024;
+template <int D, int CG, int I> __device__ __forceinline__ char *ring_buffer() {
+  using Geom = Geo<D, CG>;
+  constexpr int stage = kWaves * Geom::STAGE, joined = kWaves * Geom::TILES * 1024;
   __shared__ __attribute__((aligned(1024))) char buffer[I == 0 && joined > stage ? joined : stage];
   return buffer;
 }
@@ -115,37 +134,50 @@ struct Partials {
   float *ml, *o; // [piece][KV head][column]{m, l}, [piece][KV head][column][D]
 };
 
-template <int D>
-__global__ __launch_bounds__(64 * kWaves) void paged_gqa_kernel(
-    const half_t *__restrict__ q, const uint8_t *__restrict__ pool, PagedView g, half_t *out,
-    unsigned *invalid, unsigned queryHeads, unsigned target, float c, Partials parts) {
-  using Geom = Geo<D>;
+template <int D, int CG>
+__global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
+                          amdgpu_waves_per_eu(1)))
+void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool, PagedView g,
+                      half_t *out, unsigned *invalid, unsigned queryHeads, unsigned target,
+                      float c, Partials parts) {
+  using Geom = Geo<D, CG>;
+  constexpr unsigned kUnit = CG * kColumns;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
-  const Split split = paged_split(g, G, target);
-  unsigned seq, local;
-  if (!paged_find(g, blockIdx.x,
-                  [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local))
+  const PagedSeq own = paged_own(g);
+  const Split split = paged_split(g, own, G, kUnit, target);
+  unsigned seq, local, before;
+  if (!paged_find(g, own, blockIdx.x,
+                  [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local,
+                  before))
     return;
-  const PagedSeq s = paged_seq(g, seq);
-  const unsigned pieces = split.pieces(s), unit = local / pieces, piece = local % pieces;
+  const PagedSeq s = paged_seq_of(g, own, seq);
+  // (the last units first: they see most keys)
+  const unsigned pieces = split.pieces(s), units = split.units(s);
+  const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
   const unsigned tid = threadIdx.x, lane = tid % 64, quad = lane / 16, r = lane % 16;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
 
-  // this lane's column (past the unit's last: some row's, not written)
-  const unsigned c0 = unit * kColumns, columns = min(kColumns, s.rows * G - c0), col = c0 + r;
-  const unsigned token = min(col / G, s.rows - 1), head = kvh * G + col % G;
-  const bool live = r < columns;
-  const size_t row = ((size_t)(s.row0 + token) * queryHeads + head) * D;
+  // this lane's columns, one a group (past the unit's last: some row's, not written)
+  const unsigned c0 = unit * kUnit, columns = min(kUnit, s.rows * G - c0);
+  unsigned visible[CG]; // a column's last key
+  size_t row[CG];
+#pragma unroll
+  for (int j = 0; j < CG; ++j) {
+    const unsigned col = c0 + kColumns * j + r, token = min(col / G, s.rows - 1);
+    visible[j] = s.past + token;
+    row[j] = ((size_t)(s.row0 + token) * queryHeads + kvh * G + col % G) * D;
+  }
+  auto live = [&](int j) { return kColumns * j + r < columns; };
   if (!s.ok) { // no place for this sequence
-    if (live && wave == 0)
-      for (unsigned x = quad; x < D; x += 4)
-        out[row + x] = (half_t)NAN;
+    for (int j = 0; j < CG; ++j)
+      if (live(j) && wave == 0)
+        for (unsigned x = quad; x < D; x += 4)
+          out[row[j] + x] = (half_t)NAN;
     if (invalid && tid == 0)
       atomicOr(invalid, kPagedPlace);
     return;
   }
-  const unsigned visible = s.past + token;              // the column's last key
-  const unsigned least = s.past + c0 / G;               // the first column's
+  const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
   const unsigned end = s.past + s.rows;
   const unsigned b0 = min(piece * split.chunk, most / 32 + 1);
@@ -177,19 +209,44 @@ __global__ __launch_bounds__(64 * kWaves) void paged_gqa_kernel(
                                                1024 * i + 16 * lane, 0, 0, 0);
   };
 
-  // Q^T operands: this column's channels as the key chunks have them.
-  half8_t qv[Geom::CHUNKS][Geom::WORDS];
+  // Q^T operands: the columns' channels as the key chunks have them. Where
+  // they would take the registers of the outputs they stay in LDS.
+  constexpr bool kQueriesInLds = CG * D > 512;
+  constexpr int STEPS = Geom::CHUNKS * Geom::WORDS;
+  __shared__ __attribute__((aligned(16))) half8_t sQ[kQueriesInLds ? CG * STEPS * 64 : 1];
+  half8_t qv[kQueriesInLds ? 1 : CG * STEPS];
 #pragma unroll
-  for (int i = 0; i < Geom::CHUNKS; ++i)
+  for (int j = 0; j < CG; ++j)
 #pragma unroll
-    for (int w = 0; w < Geom::WORDS; ++w)
-      qv[i][w] = load8(q + row + (4 * i + quad) * 8 * Geom::WORDS + 8 * w);
+    for (int n = 0; n < STEPS; ++n)
+      if (!kQueriesInLds || (unsigned)(j * STEPS + n) % kWaves == wave) {
+        const half8_t v = load8(q + row[j] + (4 * (n / Geom::WORDS) + quad) * 8 * Geom::WORDS +
+                                8 * (n % Geom::WORDS));
+        if constexpr (kQueriesInLds)
+          sQ[(j * STEPS + n) * 64 + lane] = v;
+        else
+          qv[j * STEPS + n] = v;
+      }
+  if constexpr (kQueriesInLds)
+    __syncthreads();
+  auto query_operand = [&](int j, int i, int w) {
+    const int n = j * STEPS + i * Geom::WORDS + w;
+    if constexpr (kQueriesInLds)
+      return sQ[n * 64 + lane];
+    else
+      return qv[n];
+  };
 
-  float m = -INFINITY, l = 0.0f;
-  float4_t o[Geom::TILES];
+  float m[CG], l[CG];
+  float4_t o[CG][Geom::TILES];
 #pragma unroll
-  for (int i = 0; i < Geom::TILES; ++i)
-    o[i] = float4_t{0, 0, 0, 0};
+  for (int j = 0; j < CG; ++j) {
+    m[j] = -INFINITY;
+    l[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Geom::TILES; ++i)
+      o[j][i] = float4_t{0, 0, 0, 0};
+  }
 
   auto consume = [&](unsigned k, char *buffer) {
     char *block = buffer + wave * Geom::STAGE;
@@ -206,70 +263,100 @@ __global__ __launch_bounds__(64 * kWaves) void paged_gqa_kernel(
           *reinterpret_cast<half_t *>(block + 36 * D + 128 * i + 2 * lane) = (half_t)0;
       }
     }
-    float x[8];
+    float4_t acc[2][CG];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float4_t acc{0, 0, 0, 0};
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < Geom::CHUNKS; ++i) {
-        uint32_t word[Geom::WORDS];
+      for (int j = 0; j < CG; ++j)
+        acc[t][j] = float4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < Geom::CHUNKS; ++i) {
+      uint32_t word[2][Geom::WORDS];
+      half2_t sc[2], bi[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         const char *at = block + t * 8 * D + i * 1024 + lane * 4 * Geom::WORDS;
         if constexpr (Geom::WORDS == 4) {
           const uint4_t v = *reinterpret_cast<const uint4_t *>(at);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            word[w] = v[w];
+            word[t][w] = v[w];
         } else {
           const uint2 v = *reinterpret_cast<const uint2 *>(at);
-          word[0] = v.x, word[1] = v.y;
+          word[t][0] = v.x, word[t][1] = v.y;
         }
         const unsigned group = D >= 128 ? 4 * i + quad : quad / 2;
         const half2_t sb = *reinterpret_cast<const half2_t *>(block + 16 * D + t * 2 * D +
                                                               (group * 16 + r) * 4);
-        const half2_t sc{sb[0], sb[0]}, bi{sb[1], sb[1]};
-#pragma unroll
-        for (int w = 0; w < Geom::WORDS; ++w) {
-          const half2_t k0 = paged_pair<0>(word[w], sc, bi), k1 = paged_pair<1>(word[w], sc, bi);
-          const half2_t k2 = paged_pair<2>(word[w], sc, bi), k3 = paged_pair<3>(word[w], sc, bi);
-          acc = mfma16x16x32(half8_t{k0[0], k0[1], k1[0], k1[1], k2[0], k2[1], k3[0], k3[1]},
-                             qv[i][w], acc);
-        }
+        sc[t] = half2_t{sb[0], sb[0]};
+        bi[t] = half2_t{sb[1], sb[1]};
       }
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        x[4 * t + v] = acc[v] * c;
+      for (int w = 0; w < Geom::WORDS; ++w) {
+        half8_t key[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          key[t] = paged_eight(word[t][w], sc[t], sc[t], sc[t], sc[t], bi[t], bi[t], bi[t], bi[t]);
+#pragma unroll
+        for (int j = 0; j < CG; ++j) {
+          const half8_t query = query_operand(j, i, w);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            acc[t][j] = mfma16x16x32(key[t], query, acc[t][j]);
+        }
+      }
     }
+    float x[CG][8];
+#pragma unroll
+    for (int j = 0; j < CG; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[j][e] = acc[e / 4][j][e % 4] * c;
     // key of slot 4 t + v of this lane
     const unsigned first = base + 16 * (quad / 2) + 4 * (quad % 2);
     if (base + 31 > least) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[e] = first + 8 * (e / 4) + e % 4 <= visible ? x[e] : -INFINITY;
+      for (int j = 0; j < CG; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          x[j][e] = first + 8 * (e / 4) + e % 4 <= visible[j] ? x[j][e] : -INFINITY;
     }
-    float top = x[0];
+    float top[CG];
+    bool raise = false;
 #pragma unroll
-    for (int e = 1; e < 8; ++e)
-      top = fmaxf(top, x[e]);
-    if (__builtin_amdgcn_ballot_w64(top > m + kRaise)) {
-      LanePair p = pair16(top);
-      top = fmaxf(p.a, p.b);
-      p = pair32(top);
-      top = fmaxf(p.a, p.b);
-      const float to = top > m + kRaise ? top - kHeadroom : m;
-      const float alpha = m == to ? 1.0f : fast_exp2(m - to);
-      m = to;
-      l *= alpha;
+    for (int j = 0; j < CG; ++j) {
+      top[j] = x[j][0];
 #pragma unroll
-      for (int i = 0; i < Geom::TILES; ++i)
-        o[i] *= alpha;
+      for (int e = 1; e < 8; ++e)
+        top[j] = fmaxf(top[j], x[j][e]);
+      raise |= top[j] > m[j] + kRaise;
     }
-    const float ref = m == -INFINITY ? 0.0f : m; // nothing seen yet: weights 0
-    half8_t w;
+    if (__builtin_amdgcn_ballot_w64(raise)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      w[e] = (half_t)fast_exp2(x[e] - ref);
+      for (int j = 0; j < CG; ++j) {
+        LanePair p = pair16(top[j]);
+        const float half = fmaxf(p.a, p.b);
+        p = pair32(half);
+        const float all = fmaxf(p.a, p.b);
+        const float to = all > m[j] + kRaise ? all - kHeadroom : m[j];
+        const float alpha = m[j] == to ? 1.0f : fast_exp2(m[j] - to);
+        m[j] = to;
+        l[j] *= alpha;
+#pragma unroll
+        for (int i = 0; i < Geom::TILES; ++i)
+          o[j][i] *= alpha;
+      }
+    }
+    half8_t w[CG];
     const half8_t ones{1, 1, 1, 1, 1, 1, 1, 1};
-    l = dot8(w, ones, l);
+#pragma unroll
+    for (int j = 0; j < CG; ++j) {
+      const float ref = m[j] == -INFINITY ? 0.0f : m[j]; // nothing seen yet: weights 0
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        w[j][e] = (half_t)fast_exp2(x[j][e] - ref);
+      l[j] = dot8(w[j], ones, l[j]);
+    }
 #pragma unroll
     for (int st = 0; st < D / 64; ++st) {
       const uint4_t word = *reinterpret_cast<const uint4_t *>(block + 20 * D + st * 1024 + lane * 16);
@@ -279,15 +366,15 @@ __global__ __launch_bounds__(64 * kWaves) void paged_gqa_kernel(
         const half8_t sc = *reinterpret_cast<const half8_t *>(at);
         const half8_t bi = *reinterpret_cast<const half8_t *>(at + 64);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t u = word[2 * half + j];
-          const half2_t v0 = paged_pair<0>(u, half2_t{sc[0], sc[1]}, half2_t{bi[0], bi[1]});
-          const half2_t v1 = paged_pair<1>(u, half2_t{sc[2], sc[3]}, half2_t{bi[2], bi[3]});
-          const half2_t v2 = paged_pair<2>(u, half2_t{sc[4], sc[5]}, half2_t{bi[4], bi[5]});
-          const half2_t v3 = paged_pair<3>(u, half2_t{sc[6], sc[7]}, half2_t{bi[6], bi[7]});
-          o[4 * st + 2 * half + j] =
-              mfma16x16x32(half8_t{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]}, w,
-                           o[4 * st + 2 * half + j]);
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t u = word[2 * half + n];
+          const half8_t value = paged_eight(
+              u, half2_t{sc[0], sc[1]}, half2_t{sc[2], sc[3]}, half2_t{sc[4], sc[5]},
+              half2_t{sc[6], sc[7]}, half2_t{bi[0], bi[1]}, half2_t{bi[2], bi[3]},
+              half2_t{bi[4], bi[5]}, half2_t{bi[6], bi[7]});
+#pragma unroll
+          for (int j = 0; j < CG; ++j)
+            o[j][4 * st + 2 * half + n] = mfma16x16x32(value, w[j], o[j][4 * st + 2 * half + n]);
         }
       }
     }
@@ -295,21 +382,21 @@ __global__ __launch_bounds__(64 * kWaves) void paged_gqa_kernel(
 
   // R blocks in flight, their buffers known at compile time.
   constexpr int R = Geom::RING;
-  static_assert(R >= 3 && R <= 6, "the buffers below");
+  static_assert(R >= 2 && R <= 6, "the buffers below");
   auto buffer = [&](int i) -> char * {
     switch (i % R) {
     case 0:
-      return ring_buffer<D, 0>();
+      return ring_buffer<D, CG, 0>();
     case 1:
-      return ring_buffer<D, 1>();
+      return ring_buffer<D, CG, 1>();
     case 2:
-      return ring_buffer<D, 2>();
+      return ring_buffer<D, CG, (R > 2 ? 2 : 0)>();
     case 3:
-      return ring_buffer<D, (R > 3 ? 3 : 0)>();
+      return ring_buffer<D, CG, (R > 3 ? 3 : 0)>();
     case 4:
-      return ring_buffer<D, (R > 4 ? 4 : 0)>();
+      return ring_buffer<D, CG, (R > 4 ? 4 : 0)>();
     default:
-      return ring_buffer<D, (R > 5 ? 5 : 0)>();
+      return ring_buffer<D, CG, (R > 5 ? 5 : 0)>();
     }
   };
 #pragma unroll
@@ -329,124 +416,147 @@ __global__ __launch_bounds__(64 * kWaves) void paged_gqa_kernel(
       consume(k + i, buffer(i));
 
   // Join the waves: (m, l) of the columns, then each wave its output tiles.
-  __shared__ float sM[kWaves][kColumns], sL[kWaves][kColumns];
-  LanePair p = pair16(l);
-  l = p.a + p.b;
-  p = pair32(l);
-  l = p.a + p.b;
-  if (__builtin_amdgcn_ballot_w64(bad)) {
-    l = NAN; // a page that is not in the pool
-    if (invalid && lane == 0)
-      atomicOr(invalid, kPagedPlace);
-  }
-  if (quad == 0) {
-    sM[wave][r] = m;
-    sL[wave][r] = l;
-  }
-  __syncthreads(); // (the ring's blocks are done with)
-  float4_t *sO = reinterpret_cast<float4_t *>(ring_buffer<D, 0>());
+  __shared__ float sM[kWaves][kUnit], sL[kWaves][kUnit];
+  const bool lost = __builtin_amdgcn_ballot_w64(bad); // a page that is not in the pool
+  if (lost && invalid && lane == 0)
+    atomicOr(invalid, kPagedPlace);
 #pragma unroll
-  for (int i = 0; i < Geom::TILES; ++i)
-    sO[(wave * Geom::TILES + i) * 64 + lane] = o[i];
-  __syncthreads();
-  float top = sM[0][r], sum = 0.0f, a[kWaves];
-#pragma unroll
-  for (unsigned w = 1; w < kWaves; ++w)
-    top = fmaxf(top, sM[w][r]);
-#pragma unroll
-  for (unsigned w = 0; w < kWaves; ++w) {
-    a[w] = sM[w][r] == -INFINITY ? 0.0f : fast_exp2(sM[w][r] - top);
-    sum += sL[w][r] * a[w]; // (a wave's NaN stays: its m is a number, or every page was bad)
+  for (int j = 0; j < CG; ++j) {
+    LanePair p = pair16(l[j]);
+    const float half = p.a + p.b;
+    p = pair32(half);
+    if (quad == 0) {
+      sM[wave][kColumns * j + r] = lost ? 0.0f : m[j];
+      sL[wave][kColumns * j + r] = lost ? NAN : p.a + p.b;
+    }
   }
-  const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * kColumns + r;
-  const float scale = pieces == 1 ? 1.0f / sum : 1.0f;
-  for (unsigned i = wave; i < (unsigned)Geom::TILES; i += kWaves) {
-    float4_t y{0, 0, 0, 0};
+  float4_t *sO = reinterpret_cast<float4_t *>(ring_buffer<D, CG, 0>());
 #pragma unroll
-    for (unsigned w = 0; w < kWaves; ++w)
-      y += sO[(w * Geom::TILES + i) * 64 + lane] * a[w];
-    if (!live)
-      continue;
-    if (pieces == 1)
-      *reinterpret_cast<half4_t *>(out + row + 16 * i + 4 * quad) =
-          half4_t{(half_t)(y[0] * scale), (half_t)(y[1] * scale), (half_t)(y[2] * scale),
-                  (half_t)(y[3] * scale)};
-    else
-      *reinterpret_cast<float4_t *>(parts.o + part * D + 16 * i + 4 * quad) = y;
+  for (int j = 0; j < CG; ++j) {
+    __syncthreads(); // (the ring's blocks, or the group before, are done with)
+#pragma unroll
+    for (int i = 0; i < Geom::TILES; ++i)
+      sO[(wave * Geom::TILES + i) * 64 + lane] = o[j][i];
+    __syncthreads();
+    const unsigned col = kColumns * j + r;
+    float top = sM[0][col], sum = 0.0f, a[kWaves];
+#pragma unroll
+    for (unsigned w = 1; w < kWaves; ++w)
+      top = fmaxf(top, sM[w][col]);
+#pragma unroll
+    for (unsigned w = 0; w < kWaves; ++w) {
+      a[w] = sM[w][col] == -INFINITY ? 0.0f : fast_exp2(sM[w][col] - top);
+      sum += sL[w][col] * a[w];
+    }
+    const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * kUnit + col;
+    const float scale = pieces == 1 ? 1.0f / sum : 1.0f;
+    for (unsigned i = wave; i < (unsigned)Geom::TILES; i += kWaves) {
+      float4_t y{0, 0, 0, 0};
+#pragma unroll
+      for (unsigned w = 0; w < kWaves; ++w)
+        y += sO[(w * Geom::TILES + i) * 64 + lane] * a[w];
+      if (!live(j))
+        continue;
+      if (pieces == 1)
+        *reinterpret_cast<half4_t *>(out + row[j] + 16 * i + 4 * quad) =
+            half4_t{(half_t)(y[0] * scale), (half_t)(y[1] * scale), (half_t)(y[2] * scale),
+                    (half_t)(y[3] * scale)};
+      else
+        *reinterpret_cast<float4_t *>(parts.o + part * D + 16 * i + 4 * quad) = y;
+    }
+    if (pieces > 1 && wave == 0 && quad == 0 && live(j))
+      *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
   }
-  if (pieces > 1 && wave == 0 && quad == 0 && live)
-    *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
 }
 
-// One workgroup a row, query head and 64 channels: four waves, each every
-// fourth piece.
+// Joins the rows whose keys were divided. An item is such a row's query head;
+// workgroups take items in turn, so that a call without any costs one round
+// of them. Each wave adds up every fourth piece, a lane D/64 channels.
 constexpr unsigned kMergeWaves = 4;
+constexpr unsigned kMergeGroups = 2048; // workgroups: eight a CU
 template <int D>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_gqa_merge_kernel(
-    PagedView g, half_t *out, unsigned queryHeads, unsigned target, Partials parts) {
+    PagedView g, half_t *out, unsigned queryHeads, unsigned unit, unsigned target,
+    Partials parts) {
+  constexpr int N = D / 64;
+  typedef float vec __attribute__((ext_vector_type(N)));
+  typedef _Float16 halves __attribute__((ext_vector_type(N)));
   const unsigned G = queryHeads / g.kvHeads;
-  const Split split = paged_split(g, G, target);
-  unsigned seq, local;
-  if (!paged_find(g, blockIdx.x, [](const PagedSeq &s) { return s.rows; }, seq, local))
-    return;
-  const PagedSeq s = paged_seq(g, seq);
-  const unsigned pieces = split.pieces(s);
-  if (!s.ok || pieces == 1)
-    return;
-  const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, h = blockIdx.y;
-  const unsigned column = local * G + h % G, kvh = h / G;
-  // the number of the first piece of this column's unit
-  unsigned first = 0;
-  for (unsigned s0 = 0; s0 < seq; s0 += 64)
-    if (s0 + lane < seq) {
-      const PagedSeq o = paged_seq(g, s0 + lane);
-      first += split.units(o) * split.pieces(o);
+  const PagedSeq own = paged_own(g);
+  const Split split = paged_split(g, own, G, unit, target);
+  const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  __shared__ float sM[kMergeWaves], sL[kMergeWaves];
+  __shared__ vec sY[kMergeWaves][64];
+  for (unsigned item = blockIdx.x;; item += gridDim.x) {
+    unsigned seq, local, before, pieceBefore = 0;
+    if (!paged_find(g, own, item,
+                    [&](const PagedSeq &s) {
+                      return s.ok && split.pieces(s) > 1 ? s.rows * queryHeads : 0u;
+                    },
+                    seq, local, before))
+      return;
+    for (unsigned s0 = 0; s0 <= seq; s0 += 64) { // pieces of the sequences before
+      const PagedSeq o = s0 ? (s0 + lane < g.sequences ? paged_seq(g, s0 + lane)
+                                                       : PagedSeq{0, 0, 0, true})
+                            : own;
+      const unsigned n = split.units(o) * split.pieces(o), sum = wave_scan(n);
+      const int at = seq - s0 < 64 ? (int)(seq - s0) : 63;
+      pieceBefore += (unsigned)__builtin_amdgcn_readlane((int)(seq - s0 < 64 ? sum - n : sum), at);
     }
-  for (int d = 1; d < 64; d *= 2)
-    first += __shfl_xor(first, d);
-  first += column / kColumns * pieces;
-  const float *ml = parts.ml + 2 * (((size_t)first * g.kvHeads + kvh) * kColumns + column % kColumns);
-  const float *po = parts.o + (((size_t)first * g.kvHeads + kvh) * kColumns + column % kColumns) * D +
-                    64 * blockIdx.z + lane;
-  const size_t step = (size_t)g.kvHeads * kColumns;
-  float m = -INFINITY, l = 0.0f, y = 0.0f;
-  for (unsigned i = wave; i < pieces; i += kMergeWaves) {
-    const float mi = ml[2 * step * i], li = ml[2 * step * i + 1], oi = po[step * i * D];
-    const float to = fmaxf(m, mi);
-    const float a = m == -INFINITY ? 0.0f : fast_exp2(m - to);
-    const float b = mi == -INFINITY ? 0.0f : fast_exp2(mi - to);
-    l = l * a + li * b;
-    y = y * a + oi * b;
-    m = to;
+    const PagedSeq s = paged_seq_of(g, own, seq);
+    const unsigned pieces = split.pieces(s), h = local % queryHeads, row = local / queryHeads;
+    const unsigned column = row * G + h % G, kvh = h / G;
+    const unsigned first = pieceBefore + (split.units(s) - 1 - column / unit) * pieces;
+    const size_t at = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
+    const size_t step = (size_t)g.kvHeads * unit;
+    const float2 *ml = reinterpret_cast<const float2 *>(parts.ml) + at;
+    const vec *po = reinterpret_cast<const vec *>(parts.o + at * D) + lane;
+    float m = -INFINITY, l = 0.0f;
+    vec y = 0.0f;
+#pragma unroll 4
+    for (unsigned i = wave; i < pieces; i += kMergeWaves) {
+      const float2 x = ml[step * i];
+      const vec o = po[step * i * 64];
+      const float to = fmaxf(m, x.x);
+      const float a = m == -INFINITY ? 0.0f : fast_exp2(m - to);
+      const float b = x.x == -INFINITY ? 0.0f : fast_exp2(x.x - to);
+      l = l * a + x.y * b;
+      y = y * a + o * b;
+      m = to;
+    }
+    sM[wave] = m;
+    sL[wave] = l;
+    sY[wave][lane] = y;
+    __syncthreads();
+    if (wave == 0) {
+      float top = sM[0];
+      for (unsigned w = 1; w < kMergeWaves; ++w)
+        top = fmaxf(top, sM[w]);
+      l = 0.0f;
+      y = 0.0f;
+      for (unsigned w = 0; w < kMergeWaves; ++w) {
+        const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - top);
+        l += sL[w] * a;
+        y += sY[w][lane] * a;
+      }
+      halves z;
+      for (int i = 0; i < N; ++i)
+        z[i] = (half_t)(y[i] / l);
+      reinterpret_cast<halves *>(out + ((size_t)(s.row0 + row) * queryHeads + h) * D)[lane] = z;
+    }
+    __syncthreads();
   }
-  __shared__ float sM[kMergeWaves], sL[kMergeWaves], sY[kMergeWaves][64];
-  sM[wave] = m;
-  sL[wave] = l;
-  sY[wave][lane] = y;
-  __syncthreads();
-  if (wave)
-    return;
-  float top = sM[0];
-  for (unsigned w = 1; w < kMergeWaves; ++w)
-    top = fmaxf(top, sM[w]);
-  l = y = 0.0f;
-  for (unsigned w = 0; w < kMergeWaves; ++w) {
-    const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - top);
-    l += sL[w] * a;
-    y += sY[w][lane] * a;
-  }
-  out[((size_t)(s.row0 + local) * queryHeads + h) * D + 64 * blockIdx.z + lane] = (half_t)(y / l);
 }
 
-size_t partials_floats(const PagedKvParams &p, unsigned group, unsigned dim) {
-  return (size_t)most_pieces(p, group) * p.kvHeads * kColumns * dim;
+size_t partial_columns(const PagedKvParams &p, unsigned group, unsigned columns) {
+  return (size_t)most_pieces(p, group, columns) * p.kvHeads * columns;
 }
 
 } // namespace
 
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads) {
   const unsigned group = queryHeads / p.kvHeads;
-  return 4 * (partials_floats(p, group, p.headDim) + partials_floats(p, group, 2));
+  return 4 * (p.headDim + 2) * partial_columns(p, group, kColumns * column_groups(p, group));
 }
 
 hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
@@ -454,24 +564,37 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
                             uint32_t *invalid, void *workspace, const PagedKvParams &p,
                             unsigned queryHeads, float scale, hipStream_t stream) {
   const unsigned group = queryHeads / p.kvHeads, target = target_pieces(p);
+  const unsigned groups = column_groups(p, group), unit = kColumns * groups;
   const PagedView g = paged_view(p, starts, past, table);
   float *ws = static_cast<float *>(workspace);
-  const Partials parts{ws + partials_floats(p, group, p.headDim), ws};
+  const Partials parts{ws + partial_columns(p, group, unit) * p.headDim, ws};
   half_t *to = reinterpret_cast<half_t *>(out);
   auto run = [&](auto kernel, auto merge) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)most_pieces(p, group), p.kvHeads), dim3(64 * kWaves),
-                       0, stream, reinterpret_cast<const half_t *>(q),
+    hipLaunchKernelGGL(kernel, dim3((unsigned)most_pieces(p, group, unit), p.kvHeads),
+                       dim3(64 * kWaves), 0, stream, reinterpret_cast<const half_t *>(q),
                        static_cast<const uint8_t *>(pool), g, to, invalid, queryHeads, target,
                        scale * kLog2e, parts);
     if (hipError_t e = hipGetLastError(); e != hipSuccess)
       return e;
-    hipLaunchKernelGGL(merge, dim3(p.tokens, queryHeads, p.headDim / 64), dim3(64 * kMergeWaves),
-                       0, stream, g, to, queryHeads, target, parts);
+    const uint64_t items = (uint64_t)p.tokens * queryHeads;
+    hipLaunchKernelGGL(merge, dim3((unsigned)(items < kMergeGroups ? items : kMergeGroups)),
+                       dim3(64 * kMergeWaves), 0, stream, g, to, queryHeads, unit, target, parts);
     return hipGetLastError();
   };
-  return p.headDim == 256   ? run(paged_gqa_kernel<256>, paged_gqa_merge_kernel<256>)
-         : p.headDim == 128 ? run(paged_gqa_kernel<128>, paged_gqa_merge_kernel<128>)
-                            : run(paged_gqa_kernel<64>, paged_gqa_merge_kernel<64>);
+  auto by_groups = [&](auto one, auto two, auto four, auto merge) {
+    return groups == 1 ? run(one, merge) : groups == 2 ? run(two, merge) : run(four, merge);
+  };
+  switch (p.headDim) {
+  case 256:
+    return by_groups(paged_gqa_kernel<256, 1>, paged_gqa_kernel<256, 2>, paged_gqa_kernel<256, 2>,
+                     paged_gqa_merge_kernel<256>);
+  case 128:
+    return by_groups(paged_gqa_kernel<128, 1>, paged_gqa_kernel<128, 2>, paged_gqa_kernel<128, 4>,
+                     paged_gqa_merge_kernel<128>);
+  default:
+    return by_groups(paged_gqa_kernel<64, 1>, paged_gqa_kernel<64, 2>, paged_gqa_kernel<64, 4>,
+                     paged_gqa_merge_kernel<64>);
+  }
 }
 
 } // namespace llmi

@@ -118,32 +118,64 @@ __device__ __forceinline__ half_t paged_value(uint32_t word, unsigned e, half_t 
   return __builtin_elementwise_fma(x, scale, bias);
 }
 
+// Sum over the wave's lanes up to this one (row shifts, then the rows' totals
+// handed on).
+template <int Ctrl, int Rows> __device__ __forceinline__ unsigned add_dpp(unsigned x) {
+  return x + (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, Ctrl, Rows, 0xF, false);
+}
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+  x = add_dpp<0x111, 0xF>(x); // row_shr 1, 2, 4, 8
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x); // row_bcast 15 into rows 1 and 3
+  return add_dpp<0x143, 0xC>(x); // row_bcast 31 into rows 2 and 3
+}
+
 // The call's unit `u` of those that count(sequence) gives each sequence, in
-// order: its sequence and its number there, the same scalars in every lane.
-// Every lane of a full wave calls it; false past the last unit.
+// order: its sequence and its number there, the same scalars in every lane,
+// and how many units come before the sequence's. Every lane of a full wave
+// calls it; false past the last unit. `own` is paged_seq of sequence `lane`
+// (nothing past the last one).
 template <typename Count>
-__device__ __forceinline__ bool paged_find(const PagedView &g, unsigned u, Count count,
-                                           unsigned &seq, unsigned &local) {
+__device__ __forceinline__ bool paged_find(const PagedView &g, const PagedSeq &own, unsigned u,
+                                           Count count, unsigned &seq, unsigned &local,
+                                           unsigned &before) {
   const unsigned lane = threadIdx.x % 64;
-  unsigned before = 0;
+  before = 0;
+  PagedSeq q = own;
   for (unsigned s0 = 0; s0 < g.sequences; s0 += 64) {
-    const unsigned n = s0 + lane < g.sequences ? count(paged_seq(g, s0 + lane)) : 0u;
-    unsigned sum = n;
-    for (unsigned d = 1; d < 64; d *= 2) {
-      const unsigned up = __shfl_up(sum, d);
-      sum += lane >= d ? up : 0u;
-    }
+    if (s0)
+      q = s0 + lane < g.sequences ? paged_seq(g, s0 + lane) : PagedSeq{0, 0, 0, true};
+    const unsigned n = count(q), sum = wave_scan(n);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(u - before < sum);
     if (past) {
       const int at = __builtin_ctzll(past);
       seq = s0 + (unsigned)at;
-      local = u - before - (unsigned)__builtin_amdgcn_readlane((int)(sum - n), at);
+      before += (unsigned)__builtin_amdgcn_readlane((int)(sum - n), at);
+      local = u - before;
       // (not so with starts out of order: a sum that wrapped)
       return local < (unsigned)__builtin_amdgcn_readlane((int)n, at);
     }
     before += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
   }
   return false;
+}
+__device__ __forceinline__ PagedSeq paged_own(const PagedView &g) {
+  const unsigned lane = threadIdx.x % 64;
+  return lane < g.sequences ? paged_seq(g, lane) : PagedSeq{0, 0, 0, true};
+}
+// One of the sequences, the same in every lane.
+__device__ __forceinline__ PagedSeq paged_seq_of(const PagedView &g, const PagedSeq &own,
+                                                 unsigned seq) {
+  if (seq >= 64)
+    return paged_seq(g, seq);
+  PagedSeq q;
+  q.row0 = (unsigned)__builtin_amdgcn_readlane((int)own.row0, (int)seq);
+  q.rows = (unsigned)__builtin_amdgcn_readlane((int)own.rows, (int)seq);
+  q.past = (unsigned)__builtin_amdgcn_readlane((int)own.past, (int)seq);
+  q.ok = __builtin_amdgcn_readlane((int)own.ok, (int)seq);
+  return q;
 }
 
 } // namespace llmi

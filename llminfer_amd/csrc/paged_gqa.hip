@@ -257,6 +257,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     const unsigned slot = lane % 8, behind = 16 * (lane / 16 % 2) + 8 * (slot / 4) +
                                              4 * (lane / 8 % 2) + slot % 4;
     if (base + 32 > end) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the block is there, before it is changed
       if (base + behind >= end) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)

@@ -16,7 +16,7 @@ namespace {
 constexpr unsigned kThreads = 256;
 
 struct AppendRows {
-  unsigned keyToken, keyHead, valueToken, valueHead, half, layout;
+  unsigned keyToken, keyHead, valueToken, valueHead, half, layout, heads; // heads: of a workgroup
   float factor;
 };
 
@@ -31,179 +31,246 @@ unsigned most_units(unsigned tokens, unsigned sequences) {
   return (unsigned)(n < tokens ? n : tokens);
 }
 
-// The value as the cache takes it; sets `bad` for one that it cannot hold.
-__device__ __forceinline__ float kept(float x, bool &bad) {
-  bad |= !(fabsf(x) <= kPagedLimit);
-  return x != x ? 0.0f : fminf(fmaxf(x, -kPagedLimit), kPagedLimit);
-}
-
-struct Group {
-  half_t scale, bias;
-  float s, b;
-};
-__device__ __forceinline__ Group group_of(float low, float high) {
-  Group g;
-  g.scale = f16_of(__fdiv_rn(__fsub_rn(high, low), 15.0f));
-  g.s = (float)g.scale;
-  g.bias = f16_of(__fsub_rn(low, mul32(16.0f, g.s)));
-  g.b = (float)g.bias;
-  return g;
-}
-// clamp(rint((x - b) / s) - 16, 0, 15). The quotient as a product with the
-// hardware's reciprocal is within 2^-17 of the exact one (at most 32, off by
-// three half steps of fp32 and the reciprocal's one); where that could change
-// the rounding, the division decides.
-struct Coder {
-  float s, b, inv;
-  __device__ explicit Coder(const Group &g)
-      : s(g.s), b(g.b), inv(g.s > 0.0f ? __builtin_amdgcn_rcpf(g.s) : 0.0f) {}
-  __device__ uint32_t operator()(float x) const {
-    const float d = __fsub_rn(x, b);
-    float q = mul32(d, inv);
-    const float r = __builtin_rintf(q);
-    // a scale below 2^-14 (fp16's subnormals) has quotients past 32: divided too
-    if (fabsf(fabsf(q - r) - 0.5f) < 0x1p-12f || s < 0x1p-14f)
-      q = s > 0.0f ? __fdiv_rn(d, s) : 0.0f;
-    return (uint32_t)fminf(fmaxf(__builtin_rintf(q) - 16.0f, 0.0f), 15.0f);
-  }
-};
-
-__device__ __forceinline__ float row_min(float x) { // over the 16 lanes of a row
-  x = fminf(x, row_ror<1>(x));
-  x = fminf(x, row_ror<2>(x));
-  x = fminf(x, row_ror<4>(x));
-  return fminf(x, row_ror<8>(x));
-}
-__device__ __forceinline__ float row_max(float x) {
-  x = fmaxf(x, row_ror<1>(x));
-  x = fmaxf(x, row_ror<2>(x));
-  x = fmaxf(x, row_ror<4>(x));
-  return fmaxf(x, row_ror<8>(x));
-}
-
 // Keys that one workgroup takes of a block: eight channels a thread.
 constexpr unsigned keys_a_group(unsigned D) { return 8 * kThreads / D; }
 constexpr unsigned key_groups(unsigned D) { return 32 / keys_a_group(D); }
 
-// VEC: eight channels of a key, and those that they are rotated with, are
-// each one 16-byte load.
-template <int D, bool VEC>
-__device__ __forceinline__ bool append_keys(const uint16_t *__restrict__ x, unsigned word,
-                                            unsigned key,
-                                            const float2 *__restrict__ turn, uint8_t *block,
-                                            const AppendRows &p) {
+// Eight neighbouring channels of a key or value, and what a group has in
+// common: a thread's eight are a quarter of one.
+struct Eight {
+  float v[8];
+};
+__device__ __forceinline__ Eight eight_of(const uint16_t (&x)[8]) {
+  Eight y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    y.v[e] = h2f(x[e]);
+  return y;
+}
+__device__ __forceinline__ void ends_of(const Eight &x, float &lo, float &hi) {
+  lo = fminf(fminf(x.v[0], x.v[1]), x.v[2]);
+  hi = fmaxf(fmaxf(x.v[0], x.v[1]), x.v[2]);
+#pragma unroll
+  for (int e = 3; e < 7; e += 2) {
+    lo = fminf(fminf(lo, x.v[e]), x.v[e + 1]);
+    hi = fmaxf(fmaxf(hi, x.v[e]), x.v[e + 1]);
+  }
+  lo = fminf(lo, x.v[7]);
+  hi = fmaxf(hi, x.v[7]);
+}
+// What the cache holds of values that are not finite or past the limit (lo
+// and hi of the others are theirs); whether there were any.
+__device__ __forceinline__ bool keep(Eight &x, float &lo, float &hi) {
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2)
+    nan |= __builtin_isunordered(x.v[e], x.v[e + 1]);
+  if (!(nan || lo < -kPagedLimit || hi > kPagedLimit))
+    return false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    x.v[e] = x.v[e] != x.v[e] ? 0.0f : __builtin_amdgcn_fmed3f(x.v[e], -kPagedLimit, kPagedLimit);
+  ends_of(x, lo, hi);
+  return true;
+}
+
+// A group's scale and bias. d / 15 as the product with 1 / 15 corrected by its
+// exact remainder is the quotient rounded once (Markstein: the reciprocal is
+// 1 / 15 rounded to nearest and nothing here underflows, d being 0 or at
+// least 2^-24).
+struct Group {
+  half_t scale, bias;
+  float s, b, inv;
+};
+__device__ __forceinline__ Group group_of(float low, float high) {
+  constexpr float k15th = 1.0f / 15.0f;
+  const float d = high - low, q = apart(d * k15th);
+  Group g;
+  g.scale = (half_t)apart(__builtin_fmaf(__builtin_fmaf(-15.0f, q, d), k15th, q));
+  g.s = (float)g.scale;
+  g.bias = (half_t)apart(__builtin_fmaf(-16.0f, g.s, low)); // (16 s is exact)
+  g.b = (float)g.bias;
+  g.inv = g.s > 0.0f ? __builtin_amdgcn_rcpf(g.s) : 0.0f;
+  return g;
+}
+// The eight codes clamp(rint((x - b) / s) - 16, 0, 15), code e in nibble e / 2
+// + 4 (e % 2). The quotients, clamped to [16, 31] first: as a product with the
+// hardware's reciprocal they are within 2^-17 of the division's (at most 32,
+// off by the reciprocal's step and two half steps of fp32), so where none of
+// the eight lies within 2^-16 of a rounding border they stand, and else the
+// divisions decide. Four codes are put together as a whole number of fp32.
+__device__ __forceinline__ uint32_t codes_of(const Eight &x, const Group &g) {
+  float q[8], r[8], border = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    q[e] = __builtin_amdgcn_fmed3f(apart(x.v[e] - g.b) * g.inv, 16.0f, 31.0f);
+    r[e] = __builtin_rintf(q[e]);
+    border = fmaxf(border, fabsf(q[e] - r[e]));
+  }
+  if (border > 0.5f - 0x1p-16f && g.s > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      r[e] = __builtin_rintf(__builtin_amdgcn_fmed3f(__fdiv_rn(x.v[e] - g.b, g.s), 16.0f, 31.0f));
+  }
+  // 16 (1 + 16 + 256 + 4096) less: the 16s of the quotients
+  uint32_t half[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    half[h] = (uint32_t)__builtin_fmaf(
+        r[6 + h], 4096.0f,
+        __builtin_fmaf(r[4 + h], 256.0f, __builtin_fmaf(r[2 + h], 16.0f, r[h] - 69904.0f)));
+  return half[0] | half[1] << 16;
+}
+
+// Eight channels of a key, and those that they are rotated with. VEC: each a
+// 16-byte load.
+struct KeyPart {
   uint16_t own[8], other[8];
+};
+template <bool VEC>
+__device__ __forceinline__ void load_eight(const uint16_t *__restrict__ x, uint16_t (&to)[8]) {
+  if constexpr (VEC)
+    *reinterpret_cast<uint4_t *>(to) = *reinterpret_cast<const uint4_t *>(x);
+  else
+#pragma unroll
+    for (unsigned e = 0; e < 8; ++e)
+      to[e] = x[e];
+}
+template <bool VEC>
+__device__ __forceinline__ KeyPart load_key(const uint16_t *__restrict__ x, unsigned word,
+                                            const AppendRows &p) {
+  KeyPart k;
   const unsigned c0 = 8 * word;
-  const bool turned = c0 < 2 * p.half; // (VEC: all eight or none)
-  const bool low = c0 < p.half;
+  load_eight<VEC>(x + c0, k.own);
   if constexpr (VEC) {
-    *reinterpret_cast<uint4_t *>(own) = *reinterpret_cast<const uint4_t *>(x + c0);
-    const unsigned far = !turned || p.layout ? c0 : low ? c0 + p.half : c0 - p.half;
-    *reinterpret_cast<uint4_t *>(other) = *reinterpret_cast<const uint4_t *>(x + far);
+    const unsigned far = c0 >= 2 * p.half || p.layout ? c0 : c0 < p.half ? c0 + p.half : c0 - p.half;
+    load_eight<VEC>(x + far, k.other);
   } else {
 #pragma unroll
     for (unsigned e = 0; e < 8; ++e) {
       const unsigned c = c0 + e;
-      own[e] = x[c];
-      other[e] = x[c >= 2 * p.half ? c : p.layout ? c ^ 1u : c < p.half ? c + p.half : c - p.half];
+      k.other[e] = x[c >= 2 * p.half ? c : p.layout ? c ^ 1u : c < p.half ? c + p.half : c - p.half];
     }
   }
-  bool bad = false;
-  float v[8];
+  return k;
+}
+
+// `word` of key `key`: rotated, quantized (four neighbours have a group),
+// stored; whether it had a value that the cache cannot hold.
+template <int D, bool VEC>
+__device__ __forceinline__ bool append_key(const KeyPart &k, unsigned word, unsigned key,
+                                           const float2 *__restrict__ turns, uint8_t *block,
+                                           const AppendRows &p) {
+  const unsigned c0 = 8 * word;
+  const uint16_t(&own)[8] = k.own, (&other)[8] = k.other;
+  const bool low = c0 < p.half;
+  uint16_t y[8];
 #pragma unroll
-  for (unsigned e = 0; e < 8; ++e) {
-    const unsigned c = c0 + e;
-    uint16_t y = own[e];
-    if (VEC ? turned : c < 2 * p.half) {
-      if (p.layout) {
-        const float2 cs = turn[c / 2];
-        const uint16_t with = VEC ? own[e ^ 1] : other[e];
-        y = e % 2 == 0 ? turn_x(h2f(y), h2f(with), cs) : turn_y(h2f(with), h2f(y), cs);
-      } else {
-        const bool first = VEC ? low : c < p.half;
-        const float2 cs = turn[first ? c : c - p.half];
-        y = first ? turn_x(h2f(y), h2f(other[e]), cs) : turn_y(h2f(other[e]), h2f(y), cs);
+  for (unsigned e = 0; e < 8; ++e)
+    y[e] = own[e];
+  if (VEC) {
+    if (c0 < 2 * p.half) { // (all eight or none)
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e) {
+        const float2 cs = turns[p.layout ? c0 / 2 + e / 2 : (low ? c0 : c0 - p.half) + e];
+        const bool first = p.layout ? e % 2 == 0 : low;
+        y[e] = turn(h2f(own[e]), h2f(p.layout ? own[e ^ 1] : other[e]), cs.x,
+                    first ? -cs.y : cs.y);
       }
     }
-    v[e] = kept(h2f(y), bad);
-  }
-  // four neighbours have a group
-  float lo = v[0], hi = v[0];
+  } else {
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    lo = fminf(lo, v[e]);
-    hi = fmaxf(hi, v[e]);
+    for (unsigned e = 0; e < 8; ++e) {
+      const unsigned c = c0 + e;
+      if (c < 2 * p.half) {
+        const bool first = p.layout ? e % 2 == 0 : c < p.half;
+        const float2 cs = turns[p.layout ? c / 2 : first ? c : c - p.half];
+        y[e] = turn(h2f(own[e]), h2f(other[e]), cs.x, first ? -cs.y : cs.y);
+      }
+    }
   }
+  Eight v = eight_of(y);
+  float lo, hi;
+  ends_of(v, lo, hi);
+  const bool bad = keep(v, lo, hi);
   lo = fminf(lo, dpp<kDppXor1>(lo));
   hi = fmaxf(hi, dpp<kDppXor1>(hi));
   lo = fminf(lo, dpp<kDppXor2>(lo));
   hi = fmaxf(hi, dpp<kDppXor2>(hi));
-  const Group grp = group_of(lo, hi);
-  const Coder code(grp);
-  uint32_t packed = 0;
-#pragma unroll
-  for (unsigned e = 0; e < 8; ++e)
-    packed |= code(v[e]) << paged_nibble(e);
-  *reinterpret_cast<uint32_t *>(block + paged_key_word(D, key, word)) = packed;
+  const Group g = group_of(lo, hi);
+  *reinterpret_cast<uint32_t *>(block + paged_key_word(D, key, word)) = codes_of(v, g);
   if (word % 4 == 0)
     *reinterpret_cast<half2_t *>(block + paged_key_scale(D, key, word / 4)) =
-        half2_t{grp.scale, grp.bias};
+        half2_t{g.scale, g.bias};
   return bad;
 }
 
-// Values of keys [first, last) of a block, 64 channels from 64 st on: a lane
-// has four of them (16 apart) for the eight keys of its quad.
+// Values: a wave has 64 channels of a quad's eight keys, lane slot + 8 c the
+// channels 8 c .. 8 c + 7 of one key (a group is the lanes whose c / 4 is the
+// same). Where the wave's eight lanes of a c have a word of channels each,
+// the cache has a word of keys for each channel: a transposition of nibbles.
+__device__ __forceinline__ unsigned value_key(unsigned quad) {
+  const unsigned slot = threadIdx.x % 8;
+  return 16 * (quad / 2) + 8 * (slot / 4) + 4 * (quad % 2) + slot % 4;
+}
+__device__ __forceinline__ uint32_t swapped(uint32_t mine, uint32_t theirs, bool upper,
+                                            uint32_t low_mask, unsigned shift) {
+  // the lower lane keeps its low parts and takes the other's to its high ones
+  return upper ? (theirs >> shift & low_mask) | (mine & ~low_mask)
+               : (mine & low_mask) | (theirs << shift & ~low_mask);
+}
+// Nibble n of lane i to nibble i of lane n, in each eight lanes.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  const unsigned i = threadIdx.x % 8;
+  uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor1, 0xF, 0xF, false);
+  x = swapped(x, other, i & 1, 0x0F0F0F0Fu, 4);
+  other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppXor2, 0xF, 0xF, false);
+  x = swapped(x, other, i & 2, 0x00FF00FFu, 8);
+  // lane i ^ 4: the half row mirrored is i ^ 7, and that quad reversed i ^ 4
+  other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kDppRowHalfMirror, 0xF, 0xF, false);
+  other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)other, 0x1B, 0xF, 0xF, false);
+  return swapped(x, other, i & 4, 0x0000FFFFu, 16);
+}
+
 template <int D>
-__device__ __forceinline__ bool append_values(const uint16_t *__restrict__ x, size_t stride,
-                                              unsigned first, unsigned last, unsigned st,
-                                              uint8_t *block) {
-  const unsigned lane = threadIdx.x % 64, quad = lane / 16, r = lane % 16;
-  auto key_of = [&](unsigned e) { return 16 * (quad / 2) + 8 * (e / 4) + 4 * (quad % 2) + e % 4; };
-  auto here = [&](unsigned e) { return key_of(e) >= first && key_of(e) < last; };
-  uint16_t raw[8][4] = {};
+__device__ __forceinline__ bool append_values(const uint16_t (&x)[8], unsigned quad, bool here,
+                                              unsigned st, uint8_t *block) {
+  const unsigned lane = threadIdx.x % 64, slot = lane % 8, c = lane / 8;
+  Eight v = eight_of(x);
+  float lo, hi;
+  ends_of(v, lo, hi);
+  const bool bad = keep(v, lo, hi) && here;
+  lo = fminf(lo, row_ror<8>(lo));
+  hi = fmaxf(hi, row_ror<8>(hi));
+  LanePair p = pair16(lo);
+  lo = fminf(p.a, p.b);
+  p = pair16(hi);
+  hi = fmaxf(p.a, p.b);
+  const Group g = group_of(lo, hi);
+  // Channel e is in nibble e / 2 + 4 (e % 2) of a word, and slot e of keys goes
+  // there too: the lanes give their words in that order, and nibble n is
+  // channel 2 (n % 4) + n / 4.
+  const unsigned turned = 2 * (slot % 4) + slot / 4;
+  uint32_t word = transposed((uint32_t)__builtin_amdgcn_ds_bpermute(
+      (int)(4 * ((lane & 56u) + turned)), (int)codes_of(v, g)));
+  const unsigned channel = 64 * st + 8 * c + turned;
+  // nibbles of keys that are here
+  const unsigned long long there = __builtin_amdgcn_ballot_w64(here) >> (lane & 56u);
+  uint32_t mask = 0;
 #pragma unroll
   for (unsigned e = 0; e < 8; ++e)
-    if (here(e)) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        raw[e][w] = x[(key_of(e) - first) * stride + 64 * st + 16 * w + r];
-    }
-  uint32_t word[4] = {0, 0, 0, 0}, mask = 0;
-  bool bad = false;
-#pragma unroll
-  for (unsigned e = 0; e < 8; ++e) {
-    if (!__builtin_amdgcn_ballot_w64(here(e)))
-      continue;
-    float v[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      v[w] = kept(h2f(raw[e][w]), bad);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const Group grp = group_of(row_min(fminf(v[2 * half], v[2 * half + 1])),
-                                 row_max(fmaxf(v[2 * half], v[2 * half + 1])));
-      const Coder code(grp);
-      word[2 * half] |= code(v[2 * half]) << paged_nibble(e);
-      word[2 * half + 1] |= code(v[2 * half + 1]) << paged_nibble(e);
-      if (here(e) && r == 0) {
-        half_t *s =
-            reinterpret_cast<half_t *>(block + paged_value_scale(D, key_of(e), 2 * st + half));
-        s[0] = grp.scale;
-        s[32] = grp.bias;
-      }
-    }
-    mask |= here(e) ? 15u << paged_nibble(e) : 0u;
-  }
-  if (mask) {
-    uint4_t *to = reinterpret_cast<uint4_t *>(block + 20 * D + st * 1024 + lane * 16);
-    uint4_t w{word[0], word[1], word[2], word[3]};
-    if (mask != 0xFFFFFFFFu) {
-      const uint4_t old = *to;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = (w[j] & mask) | (old[j] & ~mask);
-    }
-    *to = w;
+    mask |= there >> e & 1 ? 15u << paged_nibble(e) : 0u;
+  uint32_t *to = reinterpret_cast<uint32_t *>(block + 20 * D + st * 1024 +
+                                              (quad * 16 + channel % 16) * 16 +
+                                              channel / 16 % 4 * 4);
+  if (mask != 0xFFFFFFFFu)
+    word = (word & mask) | (*to & ~mask);
+  *to = word;
+  if (here && c % 4 == 0) {
+    half_t *s = reinterpret_cast<half_t *>(block + 36 * D + (2 * st + c / 4) * 128 +
+                                           (quad * 8 + slot) * 2);
+    s[0] = g.scale;
+    s[32] = g.bias;
   }
   return bad;
 }
@@ -236,36 +303,76 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(
   AppendBlock b;
   if (!find_block(g, b))
     return;
-  const unsigned head = blockIdx.y, tid = threadIdx.x;
-  const bool ofValues = blockIdx.z == key_groups(D);
-  // this workgroup's keys [first, last)
-  const unsigned first = ofValues ? b.first : max(b.first, keys_a_group(D) * blockIdx.z);
-  const unsigned last = ofValues ? b.last : min(b.last, keys_a_group(D) * (blockIdx.z + 1));
-  if (first >= last)
+  // blockIdx.z: the values of one of this workgroup's heads (first: they take
+  // longest), then groups of keys. Rows are loaded before the place they go
+  // to is known.
+  const unsigned tid = threadIdx.x, head0 = blockIdx.y * p.heads;
+  const bool ofValues = blockIdx.z < p.heads;
+  const unsigned part = blockIdx.z - p.heads;
+  const unsigned first = ofValues ? b.first : max(b.first, keys_a_group(D) * part);
+  const unsigned last = ofValues ? b.last : min(b.last, keys_a_group(D) * (part + 1));
+  const unsigned head = head0 + (ofValues ? blockIdx.z : 0u);
+  if (first >= last || head >= g.kvHeads)
     return;
-  size_t at = 0;
-  if (!b.ok || !paged_block(g, b.seq, b.base, head, at)) {
-    if (invalid && tid == 0)
-      atomicOr(invalid, kPagedPlace);
-    return;
-  }
-  uint8_t *block = pool + at;
   const size_t row = b.row + (first - b.first);
+  size_t at = 0;
   bool bad = false;
+  auto place = [&]() {
+    const bool placed = b.ok && paged_block(g, b.seq, b.base, head, at);
+    if (!placed && invalid && tid == 0)
+      atomicOr(invalid, kPagedPlace);
+    return placed;
+  };
   if (ofValues) {
-    const uint16_t *x = values + row * p.valueToken + (size_t)head * p.valueHead;
-    for (unsigned st = tid / 64; st < D / 64; st += kThreads / 64)
-      bad |= append_values<D>(x, p.valueToken, first, last, st, block);
-  } else {
-    for (unsigned i = tid; i < (last - first) * p.half; i += kThreads) {
-      const unsigned k = i / p.half;
-      sTurn[i] = rope_turn((int)(b.base + first + k), freqs[i - k * p.half], p.factor);
+    // this wave's tasks (64 channels of a quad's keys) are wave, wave + 4, ...
+    const uint16_t *x = values + row * p.valueToken + (size_t)head * p.valueHead + tid % 64 / 8 * 8;
+    constexpr unsigned kTasks = 4 * (D / 64), kEach = kTasks / (kThreads / 64);
+    uint16_t raw[kEach][8];
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) {
+      const unsigned task = tid / 64 + i * (kThreads / 64), key = value_key(task / (D / 64));
+      const unsigned from = key >= first && key < last ? key - first : 0u; // (some row of the call's)
+      load_eight<VEC>(x + (size_t)from * p.valueToken + 64 * (task % (D / 64)), raw[i]);
     }
-    __syncthreads();
+    if (!place())
+      return;
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) {
+      const unsigned task = tid / 64 + i * (kThreads / 64), key = value_key(task / (D / 64));
+      const bool here = key >= first && key < last;
+      if (__builtin_amdgcn_ballot_w64(here))
+        bad |= append_values<D>(raw[i], task / (D / 64), here, task % (D / 64), pool + at);
+    }
+  } else {
+    const unsigned heads = min(p.heads, g.kvHeads - head0);
     const unsigned k = tid / (D / 8), word = tid % (D / 8);
-    if (k < last - first) {
-      const uint16_t *x = keys + (row + k) * p.keyToken + (size_t)head * p.keyHead;
-      bad = append_keys<D, VEC>(x, word, first + k, sTurn + k * p.half, block, p);
+    const bool mine = k < last - first;
+    const uint16_t *x = keys + (row + (mine ? k : 0u)) * p.keyToken + (size_t)head * p.keyHead;
+    KeyPart next = load_key<VEC>(x, word, p);
+    if (p.half) {
+      const unsigned down = kThreads / p.half, right = kThreads % p.half;
+      unsigned n = tid / p.half, pair = tid % p.half;
+      while (n < last - first) {
+        sTurn[n * p.half + pair] = rope_turn((int)(b.base + first + n), freqs[pair], p.factor);
+        n += down;
+        pair += right;
+        if (pair >= p.half) {
+          pair -= p.half;
+          ++n;
+        }
+      }
+    }
+    if (!place())
+      return;
+    __syncthreads();
+    const size_t nextHead = (size_t)(g.pageSize / 32) * (40 * D); // (of the same page)
+    for (unsigned h = 0; h < heads; ++h) {
+      const KeyPart now = next;
+      if (h + 1 < heads)
+        next = load_key<VEC>(x + (size_t)(h + 1) * p.keyHead, word, p);
+      if (mine)
+        bad |= append_key<D, VEC>(now, word, first + k, sTurn + k * p.half,
+                                  pool + at + h * nextHead, p);
     }
   }
   if (invalid && __builtin_amdgcn_ballot_w64(bad) && tid % 64 == 0)
@@ -337,13 +444,21 @@ hipError_t launch_paged_append(const uint16_t *keys, const uint16_t *values, con
                                void *pool, uint32_t *invalid, const PagedKvParams &p,
                                const PagedAppendParams &a, hipStream_t stream) {
   const PagedView g = paged_view(p, starts, past, table);
-  const AppendRows r{a.keyTokenStride,   a.keyHeadStride,  a.valueTokenStride,
-                     a.valueHeadStride, a.rotaryDim / 2, a.layout, a.factor};
-  const dim3 grid(most_units(p.tokens, p.sequences), p.kvHeads, key_groups(p.headDim) + 1);
+  const unsigned units = most_units(p.tokens, p.sequences), groups = key_groups(p.headDim);
+  // A workgroup's turns serve as many heads as leave two workgroups a CU.
+  unsigned heads = 1;
+  while (2 * heads <= p.kvHeads &&
+         (uint64_t)units * groups * ((p.kvHeads + 2 * heads - 1) / (2 * heads)) >= 512)
+    heads *= 2;
+  const AppendRows r{a.keyTokenStride, a.keyHeadStride, a.valueTokenStride, a.valueHeadStride,
+                     a.rotaryDim / 2,  a.layout,        heads,              a.factor};
+  const dim3 grid(units, (p.kvHeads + heads - 1) / heads, groups + heads);
   const size_t lds = keys_a_group(p.headDim) * r.half * sizeof(float2);
   // (half % 8: a word's channels are all of one half, and their partners a word)
   const bool vec = (a.layout || r.half % 8 == 0) && r.half % 4 == 0 && aligned16(keys) &&
-                   (a.keyTokenStride | a.keyHeadStride) % 8 == 0;
+                   aligned16(values) &&
+                   (a.keyTokenStride | a.keyHeadStride | a.valueTokenStride | a.valueHeadStride) %
+                           8 == 0;
   auto run = [&](auto wide, auto any) {
     hipLaunchKernelGGL(vec ? wide : any, grid, dim3(kThreads), lds, stream, keys, values, g, freqs,
                        static_cast<uint8_t *>(pool), invalid, r);

@@ -50,11 +50,21 @@ __device__ __forceinline__ float2 rope_turn(int pos, float freq, float factor) {
   return make_float2((float)(co * (double)factor), (float)(si * (double)factor));
 }
 
+// The value, hidden from the optimiser like exact_fp.hpp's opaque(), but free
+// to be moved: no product is folded into the rounding after it.
+__device__ __forceinline__ float apart(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+// fp16(own c + other s): the first of a pair with -s, the second with s.
+__device__ __forceinline__ uint16_t turn(float own, float other, float c, float s) {
+  return f2h(apart(apart(own * c) + apart(other * s)));
+}
 __device__ __forceinline__ uint16_t turn_x(float x, float y, float2 cs) {
-  return f2h(opaque(mul32(x, cs.x) - mul32(y, cs.y)));
+  return turn(x, y, cs.x, -cs.y);
 }
 __device__ __forceinline__ uint16_t turn_y(float x, float y, float2 cs) {
-  return f2h(opaque(mul32(y, cs.x) + mul32(x, cs.y)));
+  return turn(y, x, cs.x, cs.y);
 }
 
 } // namespace llmi

@@ -398,17 +398,14 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const uint8_t *__r
   if (!ok && invalid && tid == 0)
     atomicOr(invalid, kPagedPlace);
   const uint8_t *block = pool + at;
+  const Nibbles nibbles;
   if (ok && blockIdx.z == 0) {
     for (unsigned i = tid; i < 4 * D; i += kThreads) { // words: key, eight channels
       const unsigned key = i / (D / 8), word = i % (D / 8);
       const uint32_t w = *reinterpret_cast<const uint32_t *>(block + paged_key_word(D, key, word));
       const half2_t m =
           *reinterpret_cast<const half2_t *>(block + paged_key_scale(D, key, word / 4));
-      const half2_t sc{m[0], m[0]}, bi{m[1], m[1]};
-      const half2_t v0 = paged_pair<0>(w, sc, bi), v1 = paged_pair<1>(w, sc, bi);
-      const half2_t v2 = paged_pair<2>(w, sc, bi), v3 = paged_pair<3>(w, sc, bi);
-      *reinterpret_cast<half8_t *>(sRow + key * PITCH + 8 * word) =
-          half8_t{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+      *reinterpret_cast<half8_t *>(sRow + key * PITCH + 8 * word) = paged_eight(w, m, nibbles);
     }
   } else if (ok) {
     const unsigned quad = lane / 16, r = lane % 16;

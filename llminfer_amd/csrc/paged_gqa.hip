@@ -22,6 +22,7 @@
 #include "hip_common.hpp"
 #include "kernels.hpp"
 #include "paged_kv.hpp"
+#include "paged_plan.hpp"
 
 #include <math.h>
 
@@ -30,63 +31,14 @@ namespace {
 
 constexpr unsigned kColumns = 16; // of a group
 constexpr unsigned kWaves = 4;
+static_assert(kPagedStep % kWaves == 0, "each wave its blocks");
 constexpr unsigned kTargetGroups = 256; // workgroups to fill: one a CU
-constexpr float kRaise = 15.0f;   // raise m when a weight would pass 2^15
-constexpr float kHeadroom = 7.0f; // after a raise the largest weight is 2^7
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 constexpr int kBufferWord3 = 0x00020000; // gfx9 raw buffer descriptor, dword 3
 
 __device__ __forceinline__ float4_t mfma16x16x32(half8_t a, half8_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// The eight values of a word, as a matrix operand.
-__device__ __forceinline__ half8_t paged_eight(uint32_t u, half2_t s0, half2_t s1, half2_t s2,
-                                               half2_t s3, half2_t b0, half2_t b1, half2_t b2,
-                                               half2_t b3) {
-  const half2_t v0 = paged_pair<0>(u, s0, b0), v1 = paged_pair<1>(u, s1, b1);
-  const half2_t v2 = paged_pair<2>(u, s2, b2), v3 = paged_pair<3>(u, s3, b3);
-  return half8_t{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
-}
-
-// ---------------------------------------------------------------- the plan
-
-// Units (column blocks) of a sequence, blocks of 32 keys it holds (one where
-// it has no place, for the workgroup that says so), and how its keys are
-// divided: pieces of `chunk` blocks.
-struct Split {
-  unsigned group, columns, chunk; // columns: of a unit
-  __device__ unsigned units(const PagedSeq &q) const {
-    return (unsigned)(((uint64_t)q.rows * group + columns - 1) / columns);
-  }
-  __device__ static unsigned blocks(const PagedSeq &q) {
-    return q.ok ? (q.past + q.rows + 31) / 32 : 1u;
-  }
-  __device__ unsigned pieces(const PagedSeq &q) const { return (blocks(q) + chunk - 1) / chunk; }
-};
-
-// The chunk for which the call's blocks make at most `target` pieces more
-// than units: a multiple of the waves, at least one block each. (An fp32 sum is off by
-// less than the 1.0001; every workgroup and the merge add in the same order.)
-__device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
-                                             unsigned group, unsigned columns, unsigned target) {
-  Split s{group, columns, kWaves};
-  const unsigned lane = threadIdx.x % 64;
-  float all = (float)s.units(own) * (float)Split::blocks(own);
-  for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
-    if (s0 + lane < g.sequences) {
-      const PagedSeq q = paged_seq(g, s0 + lane);
-      all += (float)s.units(q) * (float)Split::blocks(q);
-    }
-  all = group_sum<16>(all);
-  LanePair p = pair16(all);
-  all = p.a + p.b;
-  p = pair32(all);
-  all = p.a + p.b;
-  const unsigned chunk = (unsigned)(all * 1.0001f / (float)target) + 1;
-  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)((chunk + kWaves - 1) / kWaves * kWaves));
-  return s;
 }
 
 // On the host: most units and pieces a KV head that any lengths can give.
@@ -101,10 +53,13 @@ unsigned target_pieces(const PagedKvParams &p) {
 uint64_t most_pieces(const PagedKvParams &p, unsigned group, unsigned columns) {
   return target_pieces(p) + most_units(p, group, columns);
 }
-// Column groups of a unit, by the columns that a sequence has on average.
-unsigned column_groups(const PagedKvParams &p, unsigned group) {
+// Columns of a unit, by those that a sequence has on average: groups of 16 of
+// this file's kernel, or the units of paged_tiles.hip.
+unsigned unit_columns(const PagedKvParams &p, unsigned group) {
   const uint64_t columns = (uint64_t)p.tokens * group / p.sequences;
-  return columns <= 16 ? 1 : columns <= 32 || p.headDim == 256 ? 2 : 4;
+  if (p.headDim >= 128 && columns >= 128)
+    return paged_tiles_columns(p.headDim);
+  return columns <= 16 ? 16 : columns <= 32 || p.headDim == 256 ? 32 : 64;
 }
 
 // ------------------------------------------------------------- the kernel
@@ -129,17 +84,12 @@ template <int D, int CG, int I> __device__ __forceinline__ char *ring_buffer() {
   return buffer;
 }
 
-// Where the output or the partial of a workgroup goes.
-struct Partials {
-  float *ml, *o; // [piece][KV head][column]{m, l}, [piece][KV head][column][D]
-};
-
 template <int D, int CG>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
                           amdgpu_waves_per_eu(1)))
 void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool, PagedView g,
                       half_t *out, unsigned *invalid, unsigned queryHeads, unsigned target,
-                      float c, Partials parts) {
+                      ScoreScale c, Partials parts) {
   using Geom = Geo<D, CG>;
   constexpr unsigned kUnit = CG * kColumns;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
@@ -220,8 +170,9 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 #pragma unroll
     for (int n = 0; n < STEPS; ++n)
       if (!kQueriesInLds || (unsigned)(j * STEPS + n) % kWaves == wave) {
-        const half8_t v = load8(q + row[j] + (4 * (n / Geom::WORDS) + quad) * 8 * Geom::WORDS +
-                                8 * (n % Geom::WORDS));
+        const half8_t v = with_sign(load8(q + row[j] + (4 * (n / Geom::WORDS) + quad) * 8 *
+                                                           Geom::WORDS + 8 * (n % Geom::WORDS)),
+                                    c.sign);
         if constexpr (kQueriesInLds)
           sQ[(j * STEPS + n) * 64 + lane] = v;
         else
@@ -248,6 +199,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       o[j][i] = float4_t{0, 0, 0, 0};
   }
 
+  const Nibbles nibbles;
   auto consume = [&](unsigned k, char *buffer) {
     char *block = buffer + wave * Geom::STAGE;
     const unsigned base = 32 * (b0 + wave + kWaves * k);
@@ -273,7 +225,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 #pragma unroll
     for (int i = 0; i < Geom::CHUNKS; ++i) {
       uint32_t word[2][Geom::WORDS];
-      half2_t sc[2], bi[2];
+      half2_t both[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const char *at = block + t * 8 * D + i * 1024 + lane * 4 * Geom::WORDS;
@@ -287,17 +239,15 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
           word[t][0] = v.x, word[t][1] = v.y;
         }
         const unsigned group = D >= 128 ? 4 * i + quad : quad / 2;
-        const half2_t sb = *reinterpret_cast<const half2_t *>(block + 16 * D + t * 2 * D +
-                                                              (group * 16 + r) * 4);
-        sc[t] = half2_t{sb[0], sb[0]};
-        bi[t] = half2_t{sb[1], sb[1]};
+        both[t] = *reinterpret_cast<const half2_t *>(block + 16 * D + t * 2 * D +
+                                                     (group * 16 + r) * 4);
       }
 #pragma unroll
       for (int w = 0; w < Geom::WORDS; ++w) {
         half8_t key[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          key[t] = paged_eight(word[t][w], sc[t], sc[t], sc[t], sc[t], bi[t], bi[t], bi[t], bi[t]);
+          key[t] = paged_eight(word[t][w], both[t], nibbles);
 #pragma unroll
         for (int j = 0; j < CG; ++j) {
           const half8_t query = query_operand(j, i, w);
@@ -312,7 +262,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     for (int j = 0; j < CG; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        x[j][e] = acc[e / 4][j][e % 4] * c;
+        x[j][e] = acc[e / 4][j][e % 4];
     // key of slot 4 t + v of this lane
     const unsigned first = base + 16 * (quad / 2) + 4 * (quad % 2);
     if (base + 31 > least) {
@@ -330,7 +280,8 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 #pragma unroll
       for (int e = 1; e < 8; ++e)
         top[j] = fmaxf(top[j], x[j][e]);
-      raise |= top[j] > m[j] + kRaise;
+      top[j] *= c.c;
+      raise |= top[j] > m[j] + kPagedRaise;
     }
     if (__builtin_amdgcn_ballot_w64(raise)) {
 #pragma unroll
@@ -339,7 +290,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
         const float half = fmaxf(p.a, p.b);
         p = pair32(half);
         const float all = fmaxf(p.a, p.b);
-        const float to = all > m[j] + kRaise ? all - kHeadroom : m[j];
+        const float to = all > m[j] + kPagedRaise ? all - kPagedHeadroom : m[j];
         const float alpha = m[j] == to ? 1.0f : fast_exp2(m[j] - to);
         m[j] = to;
         l[j] *= alpha;
@@ -355,7 +306,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       const float ref = m[j] == -INFINITY ? 0.0f : m[j]; // nothing seen yet: weights 0
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        w[j][e] = (half_t)fast_exp2(x[j][e] - ref);
+        w[j][e] = (half_t)fast_exp2(fmaf(x[j][e], c.c, -ref));
       l[j] = dot8(w[j], ones, l[j]);
     }
 #pragma unroll
@@ -369,10 +320,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const uint32_t u = word[2 * half + n];
-          const half8_t value = paged_eight(
-              u, half2_t{sc[0], sc[1]}, half2_t{sc[2], sc[3]}, half2_t{sc[4], sc[5]},
-              half2_t{sc[6], sc[7]}, half2_t{bi[0], bi[1]}, half2_t{bi[2], bi[3]},
-              half2_t{bi[4], bi[5]}, half2_t{bi[6], bi[7]});
+          const half8_t value = paged_eight(u, sc, bi, nibbles);
 #pragma unroll
           for (int j = 0; j < CG; ++j)
             o[j][4 * st + 2 * half + n] = mfma16x16x32(value, w[j], o[j][4 * st + 2 * half + n]);
@@ -557,7 +505,7 @@ size_t partial_columns(const PagedKvParams &p, unsigned group, unsigned columns)
 
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads) {
   const unsigned group = queryHeads / p.kvHeads;
-  return 4 * (p.headDim + 2) * partial_columns(p, group, kColumns * column_groups(p, group));
+  return 4 * (p.headDim + 2) * partial_columns(p, group, unit_columns(p, group));
 }
 
 hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
@@ -565,37 +513,42 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
                             uint32_t *invalid, void *workspace, const PagedKvParams &p,
                             unsigned queryHeads, float scale, hipStream_t stream) {
   const unsigned group = queryHeads / p.kvHeads, target = target_pieces(p);
-  const unsigned groups = column_groups(p, group), unit = kColumns * groups;
+  const unsigned unit = unit_columns(p, group), pieces = (unsigned)most_pieces(p, group, unit);
   const PagedView g = paged_view(p, starts, past, table);
   float *ws = static_cast<float *>(workspace);
   const Partials parts{ws + partial_columns(p, group, unit) * p.headDim, ws};
   half_t *to = reinterpret_cast<half_t *>(out);
-  auto run = [&](auto kernel, auto merge) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)most_pieces(p, group, unit), p.kvHeads),
-                       dim3(64 * kWaves), 0, stream, reinterpret_cast<const half_t *>(q),
-                       static_cast<const uint8_t *>(pool), g, to, invalid, queryHeads, target,
-                       scale * kLog2e, parts);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess)
-      return e;
-    const uint64_t items = (uint64_t)p.tokens * queryHeads;
-    hipLaunchKernelGGL(merge, dim3((unsigned)(items < kMergeGroups ? items : kMergeGroups)),
+  const half_t *from = reinterpret_cast<const half_t *>(q);
+  const uint8_t *pages = static_cast<const uint8_t *>(pool);
+  auto attend = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * kWaves), 0, stream, from, pages,
+                       g, to, invalid, queryHeads, target, score_scale(scale), parts);
+    return hipGetLastError();
+  };
+  auto by_columns = [&](auto one, auto two, auto four) {
+    return unit == 16 ? attend(one) : unit == 32 ? attend(two) : attend(four);
+  };
+  hipError_t e;
+  if (unit > 64)
+    e = launch_paged_tiles(from, pages, g, to, invalid, queryHeads, target, score_scale(scale), parts,
+                           pieces, stream);
+  else if (p.headDim == 256)
+    e = unit == 16 ? attend(paged_gqa_kernel<256, 1>) : attend(paged_gqa_kernel<256, 2>);
+  else if (p.headDim == 128)
+    e = by_columns(paged_gqa_kernel<128, 1>, paged_gqa_kernel<128, 2>, paged_gqa_kernel<128, 4>);
+  else
+    e = by_columns(paged_gqa_kernel<64, 1>, paged_gqa_kernel<64, 2>, paged_gqa_kernel<64, 4>);
+  if (e != hipSuccess)
+    return e;
+  const uint64_t items = (uint64_t)p.tokens * queryHeads;
+  auto merge = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(items < kMergeGroups ? items : kMergeGroups)),
                        dim3(64 * kMergeWaves), 0, stream, g, to, queryHeads, unit, target, parts);
     return hipGetLastError();
   };
-  auto by_groups = [&](auto one, auto two, auto four, auto merge) {
-    return groups == 1 ? run(one, merge) : groups == 2 ? run(two, merge) : run(four, merge);
-  };
-  switch (p.headDim) {
-  case 256:
-    return by_groups(paged_gqa_kernel<256, 1>, paged_gqa_kernel<256, 2>, paged_gqa_kernel<256, 2>,
-                     paged_gqa_merge_kernel<256>);
-  case 128:
-    return by_groups(paged_gqa_kernel<128, 1>, paged_gqa_kernel<128, 2>, paged_gqa_kernel<128, 4>,
-                     paged_gqa_merge_kernel<128>);
-  default:
-    return by_groups(paged_gqa_kernel<64, 1>, paged_gqa_kernel<64, 2>, paged_gqa_kernel<64, 4>,
-                     paged_gqa_merge_kernel<64>);
-  }
+  return p.headDim == 256   ? merge(paged_gqa_merge_kernel<256>)
+         : p.headDim == 128 ? merge(paged_gqa_merge_kernel<128>)
+                            : merge(paged_gqa_merge_kernel<64>);
 }
 
 } // namespace llmi

@@ -105,13 +105,38 @@ __device__ __forceinline__ unsigned paged_value_scale(unsigned D, unsigned key, 
 // Bit of slot e's nibble in its word.
 __host__ __device__ constexpr unsigned paged_nibble(unsigned e) { return 4 * (e / 2) + 16 * (e % 2); }
 
+// The mask of two nibbles and the exponent that they are put behind, in
+// registers: as literals they would be two instructions and not one.
+struct Nibbles {
+  uint32_t mask = 0x03C003C0u, exponent = 0x4C004C00u;
+  __device__ __forceinline__ Nibbles() {
+    asm volatile("" : "+s"(mask));
+    asm volatile("" : "+v"(exponent));
+  }
+};
+
 // The two values of slots 2 j and 2 j + 1 of a word, with their scales and biases.
 template <int J>
-__device__ __forceinline__ half2_t paged_pair(uint32_t word, half2_t scale, half2_t bias) {
+__device__ __forceinline__ half2_t paged_pair(uint32_t word, half2_t scale, half2_t bias,
+                                              const Nibbles &n) {
   // the nibble to mantissa bits 6..9 of an fp16 in [16, 32): 16 + code
   const uint32_t moved = J == 0 ? word << 6 : J == 1 ? word << 2 : J == 2 ? word >> 2 : word >> 6;
-  const half2_t x = __builtin_bit_cast(half2_t, (moved & 0x03C003C0u) | 0x4C004C00u);
+  const half2_t x = __builtin_bit_cast(half2_t, (moved & n.mask) | n.exponent);
   return __builtin_elementwise_fma(x, scale, bias);
+}
+// The eight values of a word, in the order of its slots.
+__device__ __forceinline__ half8_t paged_eight(uint32_t u, half8_t scale, half8_t bias,
+                                               const Nibbles &n) {
+  const half2_t v0 = paged_pair<0>(u, half2_t{scale[0], scale[1]}, half2_t{bias[0], bias[1]}, n);
+  const half2_t v1 = paged_pair<1>(u, half2_t{scale[2], scale[3]}, half2_t{bias[2], bias[3]}, n);
+  const half2_t v2 = paged_pair<2>(u, half2_t{scale[4], scale[5]}, half2_t{bias[4], bias[5]}, n);
+  const half2_t v3 = paged_pair<3>(u, half2_t{scale[6], scale[7]}, half2_t{bias[6], bias[7]}, n);
+  return half8_t{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+// The same with one scale and bias, side by side in 32 bits.
+__device__ __forceinline__ half8_t paged_eight(uint32_t u, half2_t both, const Nibbles &n) {
+  const half_t s = both[0], b = both[1];
+  return paged_eight(u, half8_t{s, s, s, s, s, s, s, s}, half8_t{b, b, b, b, b, b, b, b}, n);
 }
 __device__ __forceinline__ half_t paged_value(uint32_t word, unsigned e, half_t scale, half_t bias) {
   const half_t x = (half_t)(float)(16u + ((word >> paged_nibble(e)) & 15u));

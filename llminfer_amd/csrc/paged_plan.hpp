@@ -1,0 +1,79 @@
+// What the kernels of the paged attention share: the plan that divides a
+// call's keys over workgroups, made by each of them from the lengths in device
+// memory, and where partial outputs go.
+#pragma once
+
+#include "hip_common.hpp"
+#include "paged_kv.hpp"
+
+namespace llmi {
+
+constexpr float kPagedRaise = 15.0f;   // raise m when a weight would pass 2^15
+constexpr float kPagedHeadroom = 7.0f; // after a raise the largest weight is 2^7
+constexpr unsigned kPagedStep = 4;     // a chunk is a multiple of so many blocks
+
+// The softmax scale as the kernels take it: exp2 of positive multiples of the
+// scores, so that their largest is the largest weight's, with the sign given
+// to the queries; 0 as a multiple that leaves every score 0.
+struct ScoreScale {
+  float c;
+  uint32_t sign; // of two fp16 values
+};
+inline ScoreScale score_scale(float scale) {
+  const float c = __builtin_fabsf(scale * kLog2e);
+  return {c > 1e-30f || c != c ? c : 1e-30f, scale < 0.0f ? 0x80008000u : 0u};
+}
+__device__ __forceinline__ half8_t with_sign(half8_t x, uint32_t sign) {
+  return __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_t, x) ^ sign);
+}
+
+// Units (column blocks) of a sequence, blocks of 32 keys it holds (one where
+// it has no place, for the workgroup that says so), and how its keys are
+// divided: pieces of `chunk` blocks.
+struct Split {
+  unsigned group, columns, chunk; // columns: of a unit
+  __device__ unsigned units(const PagedSeq &q) const {
+    return (unsigned)(((uint64_t)q.rows * group + columns - 1) / columns);
+  }
+  __device__ static unsigned blocks(const PagedSeq &q) {
+    return q.ok ? (q.past + q.rows + 31) / 32 : 1u;
+  }
+  __device__ unsigned pieces(const PagedSeq &q) const { return (blocks(q) + chunk - 1) / chunk; }
+};
+
+// The chunk for which the call's blocks make at most `target` pieces more
+// than units: a multiple of kPagedStep blocks. (An fp32 sum is off by
+// less than the 1.0001; every workgroup and the merge add in the same order.)
+__device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
+                                             unsigned group, unsigned columns, unsigned target) {
+  Split s{group, columns, kPagedStep};
+  const unsigned lane = threadIdx.x % 64;
+  float all = (float)s.units(own) * (float)Split::blocks(own);
+  for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
+    if (s0 + lane < g.sequences) {
+      const PagedSeq q = paged_seq(g, s0 + lane);
+      all += (float)s.units(q) * (float)Split::blocks(q);
+    }
+  all = group_sum<16>(all);
+  LanePair p = pair16(all);
+  all = p.a + p.b;
+  p = pair32(all);
+  all = p.a + p.b;
+  const unsigned chunk = (unsigned)(all * 1.0001f / (float)target) + 1;
+  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)((chunk + kPagedStep - 1) / kPagedStep * kPagedStep));
+  return s;
+}
+
+// Where the output or the partial of a workgroup goes.
+struct Partials {
+  float *ml, *o; // [piece][KV head][column]{m, l}, [piece][KV head][column][D]
+};
+
+// The kernel for sequences of many rows (paged_tiles.hip): columns of its
+// units, and its launch.
+unsigned paged_tiles_columns(unsigned headDim);
+hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedView &g, half_t *out,
+                              unsigned *invalid, unsigned queryHeads, unsigned target, ScoreScale c,
+                              Partials parts, unsigned pieces, hipStream_t stream);
+
+} // namespace llmi

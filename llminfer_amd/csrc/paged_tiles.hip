@@ -1,0 +1,360 @@
+// Causal GQA over the paged 4-bit cache for sequences of many rows: tiles of
+// keys and values decoded once for all of a workgroup's columns.
+//
+// A workgroup has 128 columns of a KV head (256 at head_dim 128), eight waves:
+// wave w the 32-column tiles of column wave w % 4, and of the keys of a step
+// the half w / 4. A step is 512 / D blocks of 32 keys:
+//  * every thread decodes 16 bytes of key codes and 16 of value codes of the
+//    next step into LDS, as fp16 operands of v_mfma_f32_32x32x16_f16 in the
+//    order in which a wave reads them (1 KB, conflict-free), while
+//  * the matrix products of this one run: S^T = K Q^T with the columns in the
+//    lanes, and O^T += V^T P^T, whose weights are the score tile's registers
+//    as they are (the slots of a value word are the keys of a lane's eight);
+//  * codes and scales are asked for two steps ahead, in registers.
+// The halves of the keys are joined at the end through the tiles' memory.
+#include "hip_common.hpp"
+#include "paged_kv.hpp"
+#include "paged_plan.hpp"
+
+#include <math.h>
+
+namespace llmi {
+namespace {
+
+constexpr unsigned kThreads = 512;
+
+template <int D> struct Tiles {
+  static constexpr int CT = 256 / D;       // 32-column tiles of a wave
+  static constexpr int UNIT = 128 * CT;    // columns of a workgroup
+  static constexpr int BLOCKS = 512 / D;   // of a step
+  static constexpr int EACH = BLOCKS / 2;  // of a half
+  static constexpr int BLOCKB = 64 * D;    // bytes of a decoded block
+  static constexpr int STEPS = D / 16;     // products over the channels
+  static constexpr int OUT = D / 32;       // output tiles
+};
+
+// Decoded keys [block][D/8][key 32][8 channels] and values [block][D/32]
+// [quad 4][channel 32][8 keys], two buffers each, variables of their own.
+template <int I> __device__ __forceinline__ char *tile_buffer() {
+  __shared__ __attribute__((aligned(1024))) char buffer[32768];
+  return buffer;
+}
+
+template <int D>
+__global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads),
+                          amdgpu_waves_per_eu(2, 2)))
+void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool,
+                        PagedView g, half_t *out, unsigned *invalid, unsigned queryHeads,
+                        unsigned target, ScoreScale c, Partials parts) {
+  using T = Tiles<D>;
+  constexpr int CT = T::CT;
+  const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
+  const PagedSeq own = paged_own(g);
+  const Split split = paged_split(g, own, G, T::UNIT, target);
+  unsigned seq, local, before;
+  if (!paged_find(g, own, blockIdx.x,
+                  [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local,
+                  before))
+    return;
+  const PagedSeq s = paged_seq_of(g, own, seq);
+  const unsigned pieces = split.pieces(s), units = split.units(s);
+  const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
+  const unsigned tid = threadIdx.x, lane = tid % 64, r = lane % 32, hi = lane / 32;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const unsigned half = wave / 4, tile0 = wave % 4 * CT;
+
+  // this lane's columns (past the unit's last: some row's, not written)
+  const unsigned c0 = unit * T::UNIT, columns = min((unsigned)T::UNIT, s.rows * G - c0);
+  unsigned visible[CT]; // a column's last key
+  size_t row[CT];
+#pragma unroll
+  for (int j = 0; j < CT; ++j) {
+    const unsigned col = c0 + 32 * (tile0 + j) + r, token = min(col / G, s.rows - 1);
+    visible[j] = s.past + token;
+    row[j] = ((size_t)(s.row0 + token) * queryHeads + kvh * G + col % G) * D;
+  }
+  auto live = [&](int j) { return 32 * (tile0 + j) + r < columns; };
+  if (!s.ok) { // no place for this sequence
+    for (int j = 0; j < CT; ++j)
+      if (live(j) && half == 0)
+        for (unsigned x = hi; x < D; x += 2)
+          out[row[j] + x] = (half_t)NAN;
+    if (invalid && tid == 0)
+      atomicOr(invalid, kPagedPlace);
+    return;
+  }
+  const unsigned least = s.past + c0 / G;                // the first column's last key
+  const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
+  const unsigned end = s.past + s.rows;
+  const unsigned b0 = min(piece * split.chunk, most / 32 + 1);
+  const unsigned b1 = min(b0 + split.chunk, most / 32 + 1);
+  const unsigned steps = (b1 - b0 + T::BLOCKS - 1) / T::BLOCKS;
+
+  // ---- decoding: this thread's 16 bytes of codes of a step's block
+  __shared__ unsigned sLost;
+  __shared__ __attribute__((aligned(16))) uint32_t sScale[kThreads];
+  if (tid == 0)
+    sLost = 0;
+  const unsigned slot = __builtin_amdgcn_readfirstlane(tid / D), unit16 = tid % D;
+  size_t place = 0;
+  bool bad = false;
+  auto block_of = [&](unsigned n) { return min(b0 + T::BLOCKS * n + slot, b1 - 1); };
+  const Nibbles nibbles;
+  uint4_t keyCodes, valueCodes;
+  uint32_t keyScale, valueScale;
+  auto fetch = [&](unsigned n) { // (n < steps; a block past the last again)
+    if (n % 64 == 0) {           // where the next 64 steps' blocks are, one a lane
+      const unsigned b = block_of(n + lane);
+      bad |= !paged_block(g, seq, 32 * b, kvh, place);
+    }
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)place, n % 64);
+    const unsigned up = __builtin_amdgcn_readlane((unsigned)(place >> 32), n % 64);
+    const uint8_t *at = pool + ((size_t)up << 32 | lo);
+    keyCodes = *reinterpret_cast<const uint4_t *>(at + 16 * unit16);
+    keyScale = *reinterpret_cast<const uint32_t *>(at + 16 * D + 4 * unit16);
+    valueCodes = *reinterpret_cast<const uint4_t *>(at + 20 * D + 16 * unit16);
+    valueScale = *reinterpret_cast<const uint32_t *>(at + 36 * D + 4 * unit16);
+  };
+  const unsigned quad = unit16 / 16 % 4, rr = unit16 % 16;
+  const unsigned keyAt = slot * T::BLOCKB + (unit16 % (D / 2) / 16) * 2048 +
+                         (16 * (rr / 8) + 8 * (unit16 / (D / 2)) + rr % 8) * 16;
+  const unsigned valueAt = slot * T::BLOCKB + (unit16 / 64) * 4096 + quad * 512 + rr * 16;
+  auto decode_keys = [&](char *to) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      *reinterpret_cast<half8_t *>(to + keyAt + 512 * w) =
+          paged_eight(keyCodes[w], __builtin_bit_cast(half2_t, keyScale), nibbles);
+  };
+  auto decode_values = [&](unsigned n, char *to) {
+    // the scales and biases of this wave's 64 channels, a word a lane
+    uint32_t *mine = sScale + 64 * wave;
+    mine[lane] = valueScale;
+    const unsigned first = 32 * block_of(n) + 16 * (quad / 2) + 4 * (quad % 2);
+    const bool tail = 32 * block_of(n) + 32 > end;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      half8_t sc = *reinterpret_cast<const half8_t *>(mine + 32 * p + 4 * quad);
+      half8_t bi = *reinterpret_cast<const half8_t *>(mine + 32 * p + 16 + 4 * quad);
+      if (tail) { // behind the sequence's last key lies anything: values of 0
+        asm volatile("" ::: "memory"); // (a branch, rarely taken, and not selects)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool in = first + 8 * (e / 4) + e % 4 < end;
+          sc[e] = in ? sc[e] : (half_t)0;
+          bi[e] = in ? bi[e] : (half_t)0;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        *reinterpret_cast<half8_t *>(to + valueAt + 2048 * p + 256 * w) =
+            paged_eight(valueCodes[2 * p + w], sc, bi, nibbles);
+    }
+  };
+
+  // ---- the products: Q^T operands, outputs
+  half8_t qv[CT][T::STEPS];
+#pragma unroll
+  for (int j = 0; j < CT; ++j)
+#pragma unroll
+    for (int n = 0; n < T::STEPS; ++n)
+      qv[j][n] = with_sign(load8(q + row[j] + 16 * n + 8 * hi), c.sign);
+  float m[CT], l[CT];
+  float16_t o[CT][T::OUT];
+#pragma unroll
+  for (int j = 0; j < CT; ++j) {
+    m[j] = -INFINITY;
+    l[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < T::OUT; ++i)
+      o[j][i] = float16_t{0};
+  }
+  auto consume = [&](unsigned b, const char *keys, const char *values) {
+    const unsigned base = 32 * b;
+    float16_t x[CT];
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+      x[j] = float16_t{0};
+#pragma unroll
+    for (int n = 0; n < T::STEPS; ++n) {
+      const half8_t key = *reinterpret_cast<const half8_t *>(keys + 1024 * n + 16 * lane);
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+        x[j] = mfma32x32x16(key, qv[j][n], x[j]);
+    }
+    if (base + 31 > least) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          x[j][v] = base + mfma_c_row(v, hi) <= visible[j] ? x[j][v] : -INFINITY;
+    }
+    float top[CT];
+    bool raise = false;
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      top[j] = x[j][0];
+#pragma unroll
+      for (int v = 1; v < 16; ++v)
+        top[j] = fmaxf(top[j], x[j][v]);
+      top[j] *= c.c;
+      raise |= top[j] > m[j] + kPagedRaise;
+    }
+    if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+      for (int j = 0; j < CT; ++j) {
+        const LanePair p = pair32(top[j]);
+        const float all = fmaxf(p.a, p.b);
+        const float to = all > m[j] + kPagedRaise ? all - kPagedHeadroom : m[j];
+        const float alpha = m[j] == to ? 1.0f : fast_exp2(m[j] - to);
+        m[j] = to;
+        l[j] *= alpha;
+#pragma unroll
+        for (int i = 0; i < T::OUT; ++i)
+          o[j][i] *= alpha;
+      }
+    }
+    half8_t w[CT][2];
+    const half8_t ones{1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      const float ref = m[j] == -INFINITY ? 0.0f : m[j]; // nothing seen yet: weights 0
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        w[j][e / 8][e % 8] = (half_t)fast_exp2(fmaf(x[j][e], c.c, -ref));
+      l[j] = dot8(w[j][0], ones, l[j]);
+      l[j] = dot8(w[j][1], ones, l[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < T::OUT; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const half8_t value =
+            *reinterpret_cast<const half8_t *>(values + 2048 * i + 1024 * n + 16 * lane);
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+          o[j][i] = mfma32x32x16(value, w[j][n], o[j][i]);
+      }
+  };
+
+  if (steps) {
+    fetch(0);
+    decode_keys(tile_buffer<0>());
+    decode_values(0, tile_buffer<2>());
+    if (steps > 1)
+      fetch(1);
+  }
+  auto step = [&](unsigned n, const char *keys, const char *values, char *nextKeys,
+                  char *nextValues) {
+    lds_sync(); // step n is decoded, and step n - 1's tiles are done with
+    auto decode = [&]() {
+      if (n + 1 < steps) {
+        decode_keys(nextKeys);
+        decode_values(n + 1, nextValues);
+        if (n + 2 < steps)
+          fetch(n + 2);
+      }
+    };
+    // The two waves of a SIMD (the halves of the keys) take turns: one decodes
+    // while the other's products run.
+    if (half == 0)
+      decode();
+#pragma unroll
+    for (int i = 0; i < T::EACH; ++i) {
+      const unsigned at = half * T::EACH + i, b = b0 + T::BLOCKS * n + at;
+      if (b < b1)
+        consume(b, keys + at * T::BLOCKB, values + at * T::BLOCKB);
+    }
+    if (half == 1)
+      decode();
+  };
+  for (unsigned n = 0; n < steps; n += 2) {
+    step(n, tile_buffer<0>(), tile_buffer<2>(), tile_buffer<1>(), tile_buffer<3>());
+    if (n + 1 < steps)
+      step(n + 1, tile_buffer<1>(), tile_buffer<3>(), tile_buffer<0>(), tile_buffer<2>());
+  }
+
+  // ---- join the halves of the keys
+  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) { // a page that is not in the pool
+    sLost = 1;
+    if (invalid)
+      atomicOr(invalid, kPagedPlace);
+  }
+  __shared__ float sM[T::UNIT], sL[T::UNIT];
+#pragma unroll
+  for (int j = 0; j < CT; ++j) {
+    const LanePair p = pair32(l[j]);
+    l[j] = p.a + p.b;
+  }
+  __syncthreads();
+  // a wave's 128 output registers, 32 KB, a buffer each
+  float4_t *mine = reinterpret_cast<float4_t *>(wave % 4 == 0   ? tile_buffer<0>()
+                                                : wave % 4 == 1 ? tile_buffer<1>()
+                                                : wave % 4 == 2 ? tile_buffer<2>()
+                                                                : tile_buffer<3>());
+  if (half == 1) {
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+      if (hi == 0) {
+        sM[32 * (tile0 + j) + r] = m[j];
+        sL[32 * (tile0 + j) + r] = l[j];
+      }
+#pragma unroll
+      for (int i = 0; i < T::OUT; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          mine[((j * T::OUT + i) * 4 + v) * 64 + lane] =
+              float4_t{o[j][i][4 * v], o[j][i][4 * v + 1], o[j][i][4 * v + 2], o[j][i][4 * v + 3]};
+    }
+  }
+  __syncthreads();
+  if (half == 1)
+    return;
+#pragma unroll
+  for (int j = 0; j < CT; ++j) {
+    const unsigned col = 32 * (tile0 + j) + r;
+    const float other = sM[col], top = sLost ? 0.0f : fmaxf(m[j], other);
+    const float a = m[j] == -INFINITY ? 0.0f : fast_exp2(m[j] - top);
+    const float b = other == -INFINITY ? 0.0f : fast_exp2(other - top);
+    const float sum = sLost ? NAN : l[j] * a + sL[col] * b;
+    const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * T::UNIT + col;
+    const float inv = 1.0f / sum;
+    if (!live(j))
+      continue;
+#pragma unroll
+    for (int i = 0; i < T::OUT; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float4_t z = mine[((j * T::OUT + i) * 4 + v) * 64 + lane];
+        float4_t y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[e] = o[j][i][4 * v + e] * a + z[e] * b;
+        const unsigned at = 32 * i + 8 * v + 4 * hi;
+        if (pieces == 1)
+          *reinterpret_cast<half4_t *>(out + row[j] + at) =
+              half4_t{(half_t)(y[0] * inv), (half_t)(y[1] * inv), (half_t)(y[2] * inv),
+                      (half_t)(y[3] * inv)};
+        else
+          *reinterpret_cast<float4_t *>(parts.o + part * D + at) = y;
+      }
+    if (pieces > 1 && hi == 0)
+      *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
+  }
+}
+
+} // namespace
+
+unsigned paged_tiles_columns(unsigned headDim) { return 128 * (256 / headDim); }
+
+hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedView &g, half_t *out,
+                              unsigned *invalid, unsigned queryHeads, unsigned target, ScoreScale c,
+                              Partials parts, unsigned pieces, hipStream_t stream) {
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(pieces, g.kvHeads), dim3(kThreads), 0, stream, q, pool, g, out,
+                       invalid, queryHeads, target, c, parts);
+    return hipGetLastError();
+  };
+  return g.dim == 256 ? run(paged_tiles_kernel<256>) : run(paged_tiles_kernel<128>);
+}
+
+} // namespace llmi

@@ -10,7 +10,9 @@
 //  * the matrix products of this one run: S^T = K Q^T with the columns in the
 //    lanes, and O^T += V^T P^T, whose weights are the score tile's registers
 //    as they are (the slots of a value word are the keys of a lane's eight);
-//  * codes and scales are asked for two steps ahead, in registers.
+//  * codes and scales go HBM -> LDS by DMA two steps ahead, each wave those
+//    that its own threads decode, so that no register holds them and only
+//    the decoded tiles need the workgroup's barrier, one a step.
 // The halves of the keys are joined at the end through the tiles' memory.
 #include "hip_common.hpp"
 #include "paged_kv.hpp"
@@ -38,6 +40,29 @@ template <int D> struct Tiles {
 template <int I> __device__ __forceinline__ char *tile_buffer() {
   __shared__ __attribute__((aligned(1024))) char buffer[32768];
   return buffer;
+}
+
+constexpr unsigned kRaw = 2560; // bytes of a wave's part of a step
+__device__ __forceinline__ char *raw_buffer() {
+  __shared__ __attribute__((aligned(1024))) char buffer[kThreads / 64 * kRaw];
+  return buffer;
+}
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+constexpr int kBufferWord3 = 0x00020000; // gfx9 raw buffer descriptor, dword 3
+
+// The order that the scheduler gives a run of products, N operands read from
+// LDS and CT products for each: some reads ahead of the first, then one after
+// each operand's products.
+template <int N, int CT> __device__ __forceinline__ void reads_ahead() {
+  constexpr int kMfma = 0x008, kRead = 0x100, kAhead = CT == 1 ? 4 : 3;
+  __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+  for (int i = 0; i < N - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, CT, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, CT * kAhead, 0);
 }
 
 template <int D>
@@ -92,7 +117,6 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 
   // ---- decoding: this thread's 16 bytes of codes of a step's block
   __shared__ unsigned sLost;
-  __shared__ __attribute__((aligned(16))) uint32_t sScale[kThreads];
   if (tid == 0)
     sLost = 0;
   const unsigned slot = __builtin_amdgcn_readfirstlane(tid / D), unit16 = tid % D;
@@ -100,8 +124,10 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   bool bad = false;
   auto block_of = [&](unsigned n) { return min(b0 + T::BLOCKS * n + slot, b1 - 1); };
   const Nibbles nibbles;
-  uint4_t keyCodes, valueCodes;
-  uint32_t keyScale, valueScale;
+  // A wave's part of a step: 1 KB of key codes and of value codes, and the
+  // scales and biases of both, a word a lane (of its 64 keys' groups, and of
+  // its 64 channels).
+  char *raw = raw_buffer() + kRaw * wave;
   auto fetch = [&](unsigned n) { // (n < steps; a block past the last again)
     if (n % 64 == 0) {           // where the next 64 steps' blocks are, one a lane
       const unsigned b = block_of(n + lane);
@@ -109,26 +135,33 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
     }
     const unsigned lo = __builtin_amdgcn_readlane((unsigned)place, n % 64);
     const unsigned up = __builtin_amdgcn_readlane((unsigned)(place >> 32), n % 64);
-    const uint8_t *at = pool + ((size_t)up << 32 | lo);
-    keyCodes = *reinterpret_cast<const uint4_t *>(at + 16 * unit16);
-    keyScale = *reinterpret_cast<const uint32_t *>(at + 16 * D + 4 * unit16);
-    valueCodes = *reinterpret_cast<const uint4_t *>(at + 20 * D + 16 * unit16);
-    valueScale = *reinterpret_cast<const uint32_t *>(at + 36 * D + 4 * unit16);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(pool + ((size_t)up << 32 | lo)), (short)0, 40 * D, kBufferWord3);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the part before has been read
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t *)raw, 16, 16 * unit16, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t *)(raw + 1024), 16,
+                                             20 * D + 16 * unit16, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t *)(raw + 2048), 4,
+                                             16 * D + 4 * unit16, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t *)(raw + 2304), 4,
+                                             36 * D + 4 * unit16, 0, 0, 0);
   };
   const unsigned quad = unit16 / 16 % 4, rr = unit16 % 16;
   const unsigned keyAt = slot * T::BLOCKB + (unit16 % (D / 2) / 16) * 2048 +
                          (16 * (rr / 8) + 8 * (unit16 / (D / 2)) + rr % 8) * 16;
   const unsigned valueAt = slot * T::BLOCKB + (unit16 / 64) * 4096 + quad * 512 + rr * 16;
   auto decode_keys = [&](char *to) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the wave's part is there
+    const uint4_t keyCodes = *reinterpret_cast<const uint4_t *>(raw + 16 * lane);
+    const half2_t keyScale = *reinterpret_cast<const half2_t *>(raw + 2048 + 4 * lane);
 #pragma unroll
     for (int w = 0; w < 4; ++w)
       *reinterpret_cast<half8_t *>(to + keyAt + 512 * w) =
-          paged_eight(keyCodes[w], __builtin_bit_cast(half2_t, keyScale), nibbles);
+          paged_eight(keyCodes[w], keyScale, nibbles);
   };
   auto decode_values = [&](unsigned n, char *to) {
-    // the scales and biases of this wave's 64 channels, a word a lane
-    uint32_t *mine = sScale + 64 * wave;
-    mine[lane] = valueScale;
+    const uint4_t valueCodes = *reinterpret_cast<const uint4_t *>(raw + 1024 + 16 * lane);
+    const uint32_t *mine = reinterpret_cast<const uint32_t *>(raw + 2304);
     const unsigned first = 32 * block_of(n) + 16 * (quad / 2) + 4 * (quad % 2);
     const bool tail = 32 * block_of(n) + 32 > end;
 #pragma unroll
@@ -181,6 +214,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
       for (int j = 0; j < CT; ++j)
         x[j] = mfma32x32x16(key, qv[j][n], x[j]);
     }
+    reads_ahead<T::STEPS, CT>();
     if (base + 31 > least) {
 #pragma unroll
       for (int j = 0; j < CT; ++j)
@@ -234,6 +268,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
         for (int j = 0; j < CT; ++j)
           o[j][i] = mfma32x32x16(value, w[j][n], o[j][i]);
       }
+    reads_ahead<2 * T::OUT, CT>();
   };
 
   if (steps) {

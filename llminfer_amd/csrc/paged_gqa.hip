@@ -32,7 +32,7 @@ namespace {
 constexpr unsigned kColumns = 16; // of a group
 constexpr unsigned kWaves = 4;
 static_assert(kPagedStep % kWaves == 0, "each wave its blocks");
-constexpr unsigned kTargetGroups = 256; // workgroups to fill: one a CU
+constexpr unsigned kCus = 256;
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 constexpr int kBufferWord3 = 0x00020000; // gfx9 raw buffer descriptor, dword 3
@@ -47,19 +47,23 @@ uint64_t most_units(const PagedKvParams &p, unsigned group, unsigned columns) {
   const uint64_t b = (uint64_t)p.tokens * group / columns + p.sequences;
   return a < b ? a : b;
 }
-unsigned target_pieces(const PagedKvParams &p) {
-  return (kTargetGroups + p.kvHeads - 1) / p.kvHeads;
-}
-uint64_t most_pieces(const PagedKvParams &p, unsigned group, unsigned columns) {
-  return target_pieces(p) + most_units(p, group, columns);
+uint64_t most_pieces(const PagedKvParams &p, unsigned group, const SplitPlan &plan) {
+  return plan.target + most_units(p, group, plan.columns);
 }
 // Columns of a unit, by those that a sequence has on average: groups of 16 of
-// this file's kernel, or the units of paged_tiles.hip.
-unsigned unit_columns(const PagedKvParams &p, unsigned group) {
+// this file's kernel, or the units of paged_tiles.hip. Pieces: as many as
+// workgroups are resident (two a CU of the 16-column kernel, four at head_dim
+// 64), and three times that for several sequences, whose lengths differ.
+SplitPlan plan_for(const PagedKvParams &p, unsigned group) {
   const uint64_t columns = (uint64_t)p.tokens * group / p.sequences;
+  auto plan = [&](unsigned unit, unsigned groups, bool nearest) {
+    return SplitPlan{unit, (groups + p.kvHeads - 1) / p.kvHeads, nearest};
+  };
   if (p.headDim >= 128 && columns >= 128)
-    return paged_tiles_columns(p.headDim);
-  return columns <= 16 ? 16 : columns <= 32 || p.headDim == 256 ? 32 : 64;
+    return plan(paged_tiles_columns(p.headDim), kCus, true);
+  if (columns <= 16)
+    return plan(16, kCus * (p.headDim == 64 ? 4 : 2) * (p.sequences > 1 ? 3 : 1), false);
+  return plan(columns <= 32 || p.headDim == 256 ? 32 : 64, kCus, false);
 }
 
 // ------------------------------------------------------------- the kernel
@@ -68,33 +72,38 @@ template <int D, int CG> struct Geo {
   static constexpr int BLOCK = 40 * D;               // bytes of a block
   static constexpr int LOADS = (BLOCK + 1023) / 1024; // 1-KB loads of one
   static constexpr int STAGE = 1024 * LOADS;
-  static constexpr int RING = D == 256 && CG < 4 ? 3 : D == 256 ? 2 : D == 128 ? 5 : 6;
+  // Blocks a wave has in LDS. One column group: as many as let two workgroups
+  // (four at head_dim 64) share a CU.
+  static constexpr int RING = CG == 1 ? (D == 256 ? 2 : D == 128 ? 4 : 3)
+                                      : (D == 256 ? 3 : D == 128 ? 5 : 6);
+  static constexpr int RESIDENT = CG > 1 ? 1 : D == 64 ? 4 : 2; // workgroups a CU
   static constexpr int CHUNKS = D >= 128 ? D / 128 : 1; // of a lane's key
   static constexpr int WORDS = D >= 128 ? 4 : 2;        // of a chunk
   static constexpr int TILES = D / 16;                  // output tiles
 };
 
 // The ring's buffers are variables of their own, so that the compiler sees
-// that a wait for one need not be a wait for all; the first also takes the
-// waves' partial outputs at the end.
+// that a wait for one need not be a wait for all. The first two also take the
+// waves' partial outputs at the end, two waves each, and the columns' (m, l).
 template <int D, int CG, int I> __device__ __forceinline__ char *ring_buffer() {
   using Geom = Geo<D, CG>;
-  constexpr int stage = kWaves * Geom::STAGE, joined = kWaves * Geom::TILES * 1024;
-  __shared__ __attribute__((aligned(1024))) char buffer[I == 0 && joined > stage ? joined : stage];
+  constexpr int size = kWaves * Geom::STAGE;
+  static_assert(2 * Geom::TILES * 1024 + kWaves * CG * kColumns * 8 <= size, "room to join");
+  __shared__ __attribute__((aligned(1024))) char buffer[size];
   return buffer;
 }
 
 template <int D, int CG>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
-                          amdgpu_waves_per_eu(1)))
+                          amdgpu_waves_per_eu(Geo<D, CG>::RESIDENT)))
 void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool, PagedView g,
-                      half_t *out, unsigned *invalid, unsigned queryHeads, unsigned target,
+                      half_t *out, unsigned *invalid, unsigned queryHeads, SplitPlan plan,
                       ScoreScale c, Partials parts) {
   using Geom = Geo<D, CG>;
   constexpr unsigned kUnit = CG * kColumns;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
   const PagedSeq own = paged_own(g);
-  const Split split = paged_split(g, own, G, kUnit, target);
+  const Split split = paged_split(g, own, G, plan);
   unsigned seq, local, before;
   if (!paged_find(g, own, blockIdx.x,
                   [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local,
@@ -130,8 +139,8 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
   const unsigned end = s.past + s.rows;
-  const unsigned b0 = min(piece * split.chunk, most / 32 + 1);
-  const unsigned b1 = min(b0 + split.chunk, most / 32 + 1);
+  const unsigned length = split.length(s), b0 = min(piece * length, most / 32 + 1);
+  const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned mine = b1 > b0 + wave ? (b1 - b0 - wave + kWaves - 1) / kWaves : 0u;
 
   // Block k of this wave is b0 + wave + 4 k; a lane knows where one in 64 is.
@@ -159,34 +168,15 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
                                                1024 * i + 16 * lane, 0, 0, 0);
   };
 
-  // Q^T operands: the columns' channels as the key chunks have them. Where
-  // they would take the registers of the outputs they stay in LDS.
-  constexpr bool kQueriesInLds = CG * D > 512;
-  constexpr int STEPS = Geom::CHUNKS * Geom::WORDS;
-  __shared__ __attribute__((aligned(16))) half8_t sQ[kQueriesInLds ? CG * STEPS * 64 : 1];
-  half8_t qv[kQueriesInLds ? 1 : CG * STEPS];
+  // Q^T operands: the columns' channels as the key chunks have them.
+  half8_t qv[CG][Geom::CHUNKS][Geom::WORDS];
 #pragma unroll
   for (int j = 0; j < CG; ++j)
 #pragma unroll
-    for (int n = 0; n < STEPS; ++n)
-      if (!kQueriesInLds || (unsigned)(j * STEPS + n) % kWaves == wave) {
-        const half8_t v = with_sign(load8(q + row[j] + (4 * (n / Geom::WORDS) + quad) * 8 *
-                                                           Geom::WORDS + 8 * (n % Geom::WORDS)),
-                                    c.sign);
-        if constexpr (kQueriesInLds)
-          sQ[(j * STEPS + n) * 64 + lane] = v;
-        else
-          qv[j * STEPS + n] = v;
-      }
-  if constexpr (kQueriesInLds)
-    __syncthreads();
-  auto query_operand = [&](int j, int i, int w) {
-    const int n = j * STEPS + i * Geom::WORDS + w;
-    if constexpr (kQueriesInLds)
-      return sQ[n * 64 + lane];
-    else
-      return qv[n];
-  };
+    for (int i = 0; i < Geom::CHUNKS; ++i)
+#pragma unroll
+      for (int w = 0; w < Geom::WORDS; ++w)
+        qv[j][i][w] = with_sign(load8(q + row[j] + (4 * i + quad) * 8 * Geom::WORDS + 8 * w), c.sign);
 
   float m[CG], l[CG];
   float4_t o[CG][Geom::TILES];
@@ -250,10 +240,9 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
           key[t] = paged_eight(word[t][w], both[t], nibbles);
 #pragma unroll
         for (int j = 0; j < CG; ++j) {
-          const half8_t query = query_operand(j, i, w);
 #pragma unroll
           for (int t = 0; t < 2; ++t)
-            acc[t][j] = mfma16x16x32(key[t], query, acc[t][j]);
+            acc[t][j] = mfma16x16x32(key[t], qv[j][i][w], acc[t][j]);
         }
       }
     }
@@ -365,7 +354,13 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       consume(k + i, buffer(i));
 
   // Join the waves: (m, l) of the columns, then each wave its output tiles.
-  __shared__ float sM[kWaves][kUnit], sL[kWaves][kUnit];
+  auto out_of = [&](unsigned w) { // wave w's tiles
+    return reinterpret_cast<float4_t *>((w < 2 ? ring_buffer<D, CG, 0>() : ring_buffer<D, CG, 1>()) +
+                                        w % 2 * Geom::TILES * 1024);
+  };
+  float *sM = reinterpret_cast<float *>(ring_buffer<D, CG, 1>() + 2 * Geom::TILES * 1024);
+  float *sL = sM + kWaves * kUnit;
+  __syncthreads(); // the ring's blocks are done with
   const bool lost = __builtin_amdgcn_ballot_w64(bad); // a page that is not in the pool
   if (lost && invalid && lane == 0)
     atomicOr(invalid, kPagedPlace);
@@ -375,27 +370,28 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     const float half = p.a + p.b;
     p = pair32(half);
     if (quad == 0) {
-      sM[wave][kColumns * j + r] = lost ? 0.0f : m[j];
-      sL[wave][kColumns * j + r] = lost ? NAN : p.a + p.b;
+      sM[wave * kUnit + kColumns * j + r] = lost ? 0.0f : m[j];
+      sL[wave * kUnit + kColumns * j + r] = lost ? NAN : p.a + p.b;
     }
   }
-  float4_t *sO = reinterpret_cast<float4_t *>(ring_buffer<D, CG, 0>());
 #pragma unroll
   for (int j = 0; j < CG; ++j) {
-    __syncthreads(); // (the ring's blocks, or the group before, are done with)
+    if (j)
+      __syncthreads(); // the group before is done with
 #pragma unroll
     for (int i = 0; i < Geom::TILES; ++i)
-      sO[(wave * Geom::TILES + i) * 64 + lane] = o[j][i];
+      out_of(wave)[i * 64 + lane] = o[j][i];
     __syncthreads();
     const unsigned col = kColumns * j + r;
-    float top = sM[0][col], sum = 0.0f, a[kWaves];
+    float top = sM[col], sum = 0.0f, a[kWaves];
 #pragma unroll
     for (unsigned w = 1; w < kWaves; ++w)
-      top = fmaxf(top, sM[w][col]);
+      top = fmaxf(top, sM[w * kUnit + col]);
 #pragma unroll
     for (unsigned w = 0; w < kWaves; ++w) {
-      a[w] = sM[w][col] == -INFINITY ? 0.0f : fast_exp2(sM[w][col] - top);
-      sum += sL[w][col] * a[w];
+      const float mw = sM[w * kUnit + col];
+      a[w] = mw == -INFINITY ? 0.0f : fast_exp2(mw - top);
+      sum += sL[w * kUnit + col] * a[w];
     }
     const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * kUnit + col;
     const float scale = pieces == 1 ? 1.0f / sum : 1.0f;
@@ -403,7 +399,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       float4_t y{0, 0, 0, 0};
 #pragma unroll
       for (unsigned w = 0; w < kWaves; ++w)
-        y += sO[(w * Geom::TILES + i) * 64 + lane] * a[w];
+        y += out_of(w)[i * 64 + lane] * a[w];
       if (!live(j))
         continue;
       if (pieces == 1)
@@ -418,25 +414,28 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   }
 }
 
-// Joins the rows whose keys were divided. An item is such a row's query head;
-// workgroups take items in turn, so that a call without any costs one round
-// of them. Each wave adds up every fourth piece, a lane D/64 channels.
-constexpr unsigned kMergeWaves = 4;
-constexpr unsigned kMergeGroups = 2048; // workgroups: eight a CU
-template <int D>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_gqa_merge_kernel(
-    PagedView g, half_t *out, unsigned queryHeads, unsigned unit, unsigned target,
-    Partials parts) {
+// Joins the rows whose keys were divided. An item is such a row's query head,
+// the work of W waves, each every W-th piece, a lane D/64 channels; items are
+// taken in turn, so that a call without any costs one round of workgroups.
+// W: 8 for calls of few rows and many pieces, 1 for the others.
+constexpr unsigned kMergeThreads = 512;
+constexpr unsigned kMergeGroups = 1024; // workgroups: four a CU
+template <int D, int W>
+__global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
+    PagedView g, half_t *out, unsigned queryHeads, SplitPlan plan, Partials parts) {
   constexpr int N = D / 64;
+  constexpr unsigned kItems = kMergeThreads / 64 / W; // of a workgroup
   typedef float vec __attribute__((ext_vector_type(N)));
   typedef _Float16 halves __attribute__((ext_vector_type(N)));
-  const unsigned G = queryHeads / g.kvHeads;
+  const unsigned G = queryHeads / g.kvHeads, unit = plan.columns;
   const PagedSeq own = paged_own(g);
-  const Split split = paged_split(g, own, G, unit, target);
-  const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  __shared__ float sM[kMergeWaves], sL[kMergeWaves];
-  __shared__ vec sY[kMergeWaves][64];
-  for (unsigned item = blockIdx.x;; item += gridDim.x) {
+  const Split split = paged_split(g, own, G, plan);
+  const unsigned lane = threadIdx.x % 64;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  __shared__ float sM[W], sL[W];
+  __shared__ vec sY[W][64];
+  // (W > 1: the same item in every wave, so all of them leave together)
+  for (unsigned item = blockIdx.x * kItems + wave / W;; item += gridDim.x * kItems) {
     unsigned seq, local, before, pieceBefore = 0;
     if (!paged_find(g, own, item,
                     [&](const PagedSeq &s) {
@@ -462,8 +461,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_gqa_merge_kernel(
     const vec *po = reinterpret_cast<const vec *>(parts.o + at * D) + lane;
     float m = -INFINITY, l = 0.0f;
     vec y = 0.0f;
-#pragma unroll 4
-    for (unsigned i = wave; i < pieces; i += kMergeWaves) {
+#pragma unroll 8
+    for (unsigned i = wave % W; i < pieces; i += W) {
       const float2 x = ml[step * i];
       const vec o = po[step * i * 64];
       const float to = fmaxf(m, x.x);
@@ -473,56 +472,60 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_gqa_merge_kernel(
       y = y * a + o * b;
       m = to;
     }
-    sM[wave] = m;
-    sL[wave] = l;
-    sY[wave][lane] = y;
-    __syncthreads();
-    if (wave == 0) {
-      float top = sM[0];
-      for (unsigned w = 1; w < kMergeWaves; ++w)
-        top = fmaxf(top, sM[w]);
+    if (W > 1) {
+      sM[wave] = m;
+      sL[wave] = l;
+      sY[wave][lane] = y;
+      __syncthreads();
+      m = sM[0];
+      for (unsigned w = 1; w < W; ++w)
+        m = fmaxf(m, sM[w]);
       l = 0.0f;
       y = 0.0f;
-      for (unsigned w = 0; w < kMergeWaves; ++w) {
-        const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - top);
+      for (unsigned w = 0; w < W; ++w) {
+        const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - m);
         l += sL[w] * a;
         y += sY[w][lane] * a;
       }
+      __syncthreads();
+    }
+    if (wave % W == 0) {
       halves z;
       for (int i = 0; i < N; ++i)
         z[i] = (half_t)(y[i] / l);
       reinterpret_cast<halves *>(out + ((size_t)(s.row0 + row) * queryHeads + h) * D)[lane] = z;
     }
-    __syncthreads();
   }
 }
 
-size_t partial_columns(const PagedKvParams &p, unsigned group, unsigned columns) {
-  return (size_t)most_pieces(p, group, columns) * p.kvHeads * columns;
+size_t partial_columns(const PagedKvParams &p, unsigned group, const SplitPlan &plan) {
+  return (size_t)most_pieces(p, group, plan) * p.kvHeads * plan.columns;
 }
 
 } // namespace
 
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads) {
   const unsigned group = queryHeads / p.kvHeads;
-  return 4 * (p.headDim + 2) * partial_columns(p, group, unit_columns(p, group));
+  return 4 * (p.headDim + 2) * partial_columns(p, group, plan_for(p, group));
 }
 
 hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
                             const int32_t *table, const void *pool, uint16_t *out,
                             uint32_t *invalid, void *workspace, const PagedKvParams &p,
                             unsigned queryHeads, float scale, hipStream_t stream) {
-  const unsigned group = queryHeads / p.kvHeads, target = target_pieces(p);
-  const unsigned unit = unit_columns(p, group), pieces = (unsigned)most_pieces(p, group, unit);
+  const unsigned group = queryHeads / p.kvHeads;
+  const SplitPlan plan = plan_for(p, group);
+  const unsigned unit = plan.columns, pieces = (unsigned)most_pieces(p, group, plan);
   const PagedView g = paged_view(p, starts, past, table);
   float *ws = static_cast<float *>(workspace);
-  const Partials parts{ws + partial_columns(p, group, unit) * p.headDim, ws};
+  const Partials parts{ws + partial_columns(p, group, plan) * p.headDim, ws};
   half_t *to = reinterpret_cast<half_t *>(out);
   const half_t *from = reinterpret_cast<const half_t *>(q);
   const uint8_t *pages = static_cast<const uint8_t *>(pool);
+  const ScoreScale c = score_scale(scale);
   auto attend = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * kWaves), 0, stream, from, pages,
-                       g, to, invalid, queryHeads, target, score_scale(scale), parts);
+                       g, to, invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };
   auto by_columns = [&](auto one, auto two, auto four) {
@@ -530,8 +533,7 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
   };
   hipError_t e;
   if (unit > 64)
-    e = launch_paged_tiles(from, pages, g, to, invalid, queryHeads, target, score_scale(scale), parts,
-                           pieces, stream);
+    e = launch_paged_tiles(from, pages, g, to, invalid, queryHeads, plan, c, parts, pieces, stream);
   else if (p.headDim == 256)
     e = unit == 16 ? attend(paged_gqa_kernel<256, 1>) : attend(paged_gqa_kernel<256, 2>);
   else if (p.headDim == 128)
@@ -540,15 +542,21 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
     e = by_columns(paged_gqa_kernel<64, 1>, paged_gqa_kernel<64, 2>, paged_gqa_kernel<64, 4>);
   if (e != hipSuccess)
     return e;
-  const uint64_t items = (uint64_t)p.tokens * queryHeads;
-  auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(items < kMergeGroups ? items : kMergeGroups)),
-                       dim3(64 * kMergeWaves), 0, stream, g, to, queryHeads, unit, target, parts);
+  auto merge = [&](auto few, auto many) {
+    const unsigned each = unit == 16 ? 1 : kMergeThreads / 64;
+    const uint64_t groups = ((uint64_t)p.tokens * queryHeads + each - 1) / each;
+    const unsigned grid = (unsigned)(groups < kMergeGroups ? groups : kMergeGroups);
+    if (unit == 16)
+      hipLaunchKernelGGL(few, dim3(grid), dim3(kMergeThreads), 0, stream, g, to, queryHeads, plan,
+                         parts);
+    else
+      hipLaunchKernelGGL(many, dim3(grid), dim3(kMergeThreads), 0, stream, g, to, queryHeads, plan,
+                         parts);
     return hipGetLastError();
   };
-  return p.headDim == 256   ? merge(paged_gqa_merge_kernel<256>)
-         : p.headDim == 128 ? merge(paged_gqa_merge_kernel<128>)
-                            : merge(paged_gqa_merge_kernel<64>);
+  return p.headDim == 256   ? merge(paged_gqa_merge_kernel<256, 8>, paged_gqa_merge_kernel<256, 1>)
+         : p.headDim == 128 ? merge(paged_gqa_merge_kernel<128, 8>, paged_gqa_merge_kernel<128, 1>)
+                            : merge(paged_gqa_merge_kernel<64, 8>, paged_gqa_merge_kernel<64, 1>);
 }
 
 } // namespace llmi

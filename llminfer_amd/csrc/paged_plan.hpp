@@ -27,26 +27,42 @@ __device__ __forceinline__ half8_t with_sign(half8_t x, uint32_t sign) {
   return __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_t, x) ^ sign);
 }
 
-// Units (column blocks) of a sequence, blocks of 32 keys it holds (one where
-// it has no place, for the workgroup that says so), and how its keys are
-// divided: pieces of `chunk` blocks.
+// How a call's work is divided: a sequence's rows into units of `columns`
+// columns, and the blocks of 32 keys that it holds (one where it has no place,
+// for the workgroup that says so) into equal pieces of about `chunk` blocks:
+// at most chunk, or (nearest) at most 1.5 of it, for a kernel whose pieces
+// cost more to join than some workgroups' longer time.
 struct Split {
-  unsigned group, columns, chunk; // columns: of a unit
+  unsigned group, columns, chunk;
+  bool nearest;
   __device__ unsigned units(const PagedSeq &q) const {
     return (unsigned)(((uint64_t)q.rows * group + columns - 1) / columns);
   }
   __device__ static unsigned blocks(const PagedSeq &q) {
     return q.ok ? (q.past + q.rows + 31) / 32 : 1u;
   }
-  __device__ unsigned pieces(const PagedSeq &q) const { return (blocks(q) + chunk - 1) / chunk; }
+  __device__ unsigned pieces(const PagedSeq &q) const {
+    const unsigned n = (blocks(q) + (nearest ? chunk / 2 : chunk - 1)) / chunk;
+    return n ? n : 1u;
+  }
+  // blocks of a piece: whole steps of the kernels
+  __device__ unsigned length(const PagedSeq &q) const {
+    const unsigned n = pieces(q), each = (blocks(q) + n - 1) / n;
+    return (each + kPagedStep - 1) / kPagedStep * kPagedStep;
+  }
 };
 
-// The chunk for which the call's blocks make at most `target` pieces more
-// than units: a multiple of kPagedStep blocks. (An fp32 sum is off by
-// less than the 1.0001; every workgroup and the merge add in the same order.)
+// How the host asks for it: `target` pieces a KV head, if the lengths give them.
+struct SplitPlan {
+  unsigned columns, target, nearest;
+};
+
+// The chunk for which the call has at most plan.target pieces more than units,
+// a multiple of kPagedStep blocks. (An fp32 sum is off by less than the
+// 1.0001; every workgroup and the merge add in the same order.)
 __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
-                                             unsigned group, unsigned columns, unsigned target) {
-  Split s{group, columns, kPagedStep};
+                                             unsigned group, const SplitPlan &plan) {
+  Split s{group, plan.columns, kPagedStep, plan.nearest != 0};
   const unsigned lane = threadIdx.x % 64;
   float all = (float)s.units(own) * (float)Split::blocks(own);
   for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
@@ -59,8 +75,9 @@ __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq 
   all = p.a + p.b;
   p = pair32(all);
   all = p.a + p.b;
-  const unsigned chunk = (unsigned)(all * 1.0001f / (float)target) + 1;
-  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)((chunk + kPagedStep - 1) / kPagedStep * kPagedStep));
+  const unsigned chunk = (unsigned)(all * 1.0001f / (float)plan.target) + 1;
+  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane(
+      (int)((chunk + kPagedStep - 1) / kPagedStep * kPagedStep));
   return s;
 }
 
@@ -73,7 +90,7 @@ struct Partials {
 // units, and its launch.
 unsigned paged_tiles_columns(unsigned headDim);
 hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedView &g, half_t *out,
-                              unsigned *invalid, unsigned queryHeads, unsigned target, ScoreScale c,
+                              unsigned *invalid, unsigned queryHeads, SplitPlan plan, ScoreScale c,
                               Partials parts, unsigned pieces, hipStream_t stream);
 
 } // namespace llmi

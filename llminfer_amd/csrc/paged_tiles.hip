@@ -70,12 +70,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads),
                           amdgpu_waves_per_eu(2, 2)))
 void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool,
                         PagedView g, half_t *out, unsigned *invalid, unsigned queryHeads,
-                        unsigned target, ScoreScale c, Partials parts) {
+                        SplitPlan plan, ScoreScale c, Partials parts) {
   using T = Tiles<D>;
   constexpr int CT = T::CT;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
   const PagedSeq own = paged_own(g);
-  const Split split = paged_split(g, own, G, T::UNIT, target);
+  const Split split = paged_split(g, own, G, plan);
   unsigned seq, local, before;
   if (!paged_find(g, own, blockIdx.x,
                   [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local,
@@ -111,8 +111,8 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
   const unsigned end = s.past + s.rows;
-  const unsigned b0 = min(piece * split.chunk, most / 32 + 1);
-  const unsigned b1 = min(b0 + split.chunk, most / 32 + 1);
+  const unsigned length = split.length(s), b0 = min(piece * length, most / 32 + 1);
+  const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned steps = (b1 - b0 + T::BLOCKS - 1) / T::BLOCKS;
 
   // ---- decoding: this thread's 16 bytes of codes of a step's block
@@ -382,11 +382,11 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 unsigned paged_tiles_columns(unsigned headDim) { return 128 * (256 / headDim); }
 
 hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedView &g, half_t *out,
-                              unsigned *invalid, unsigned queryHeads, unsigned target, ScoreScale c,
+                              unsigned *invalid, unsigned queryHeads, SplitPlan plan, ScoreScale c,
                               Partials parts, unsigned pieces, hipStream_t stream) {
   auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(pieces, g.kvHeads), dim3(kThreads), 0, stream, q, pool, g, out,
-                       invalid, queryHeads, target, c, parts);
+                       invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };
   return g.dim == 256 ? run(paged_tiles_kernel<256>) : run(paged_tiles_kernel<128>);

@@ -30,8 +30,6 @@ namespace llmi {
 namespace {
 
 constexpr unsigned kColumns = 16; // of a group
-constexpr unsigned kWaves = 4;
-static_assert(kPagedStep % kWaves == 0, "each wave its blocks");
 constexpr unsigned kCus = 256;
 
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -48,35 +46,45 @@ uint64_t most_units(const PagedKvParams &p, unsigned group, unsigned columns) {
   return a < b ? a : b;
 }
 uint64_t most_pieces(const PagedKvParams &p, unsigned group, const SplitPlan &plan) {
-  return plan.target + most_units(p, group, plan.columns);
+  return plan.target + 1 + most_units(p, group, 1u << plan.shift);
 }
 // Columns of a unit, by those that a sequence has on average: groups of 16 of
 // this file's kernel, or the units of paged_tiles.hip. Pieces: as many as
-// workgroups are resident (two a CU of the 16-column kernel, four at head_dim
-// 64), and three times that for several sequences, whose lengths differ.
-SplitPlan plan_for(const PagedKvParams &p, unsigned group) {
+// there are CUs (twice that at head_dim 64, where two workgroups share one);
+// six times as many where single tokens have units enough that their
+// different lengths count for more than the joining.
+struct GqaPlan {
+  SplitPlan split;
+  bool pooled; // eight pieces a unit or more, if the lengths give them
+};
+GqaPlan plan_for(const PagedKvParams &p, unsigned group) {
   const uint64_t columns = (uint64_t)p.tokens * group / p.sequences;
-  auto plan = [&](unsigned unit, unsigned groups, bool nearest) {
-    return SplitPlan{unit, (groups + p.kvHeads - 1) / p.kvHeads, nearest};
-  };
-  if (p.headDim >= 128 && columns >= 128)
-    return plan(paged_tiles_columns(p.headDim), kCus, true);
-  if (columns <= 16)
-    return plan(16, kCus * (p.headDim == 64 ? 4 : 2) * (p.sequences > 1 ? 3 : 1), false);
-  return plan(columns <= 32 || p.headDim == 256 ? 32 : 64, kCus, false);
+  const bool tiles = p.headDim >= 128 && columns >= 128;
+  const unsigned unit = tiles                                 ? paged_tiles_columns(p.headDim)
+                        : columns <= 16                       ? 16
+                        : columns <= 32 || p.headDim == 256 ? 32
+                                                              : 64;
+  const unsigned cus = (kCus + p.kvHeads - 1) / p.kvHeads;
+  const bool pooled = cus >= 8 * most_units(p, group, unit);
+  const unsigned rounds = unit > 16 ? 1 : !pooled ? 6 : p.headDim == 64 ? 2 : 1;
+  return {{(unsigned)__builtin_ctz(unit), pooled && unit == 16 ? 8u : 4u, rounds * cus, tiles}, pooled};
 }
 
 // ------------------------------------------------------------- the kernel
 
-template <int D, int CG> struct Geo {
+// W: waves of a workgroup. Eight where units have many pieces: the more of the
+// keys that meet in one workgroup, the fewer partials there are to join (one
+// token on 32749 keys: 23.1 us with four, two workgroups a CU, 20.4 with
+// eight); four otherwise, two workgroups a CU for single tokens, whose
+// starts and ends then overlap (48 ragged chats: 122 us, 136 with eight).
+template <int D, int CG, int W> struct Geo {
   static constexpr int BLOCK = 40 * D;               // bytes of a block
   static constexpr int LOADS = (BLOCK + 1023) / 1024; // 1-KB loads of one
   static constexpr int STAGE = 1024 * LOADS;
-  // Blocks a wave has in LDS. One column group: as many as let two workgroups
-  // (four at head_dim 64) share a CU.
+  // Blocks a wave has in LDS, and waves a SIMD.
   static constexpr int RING = CG == 1 ? (D == 256 ? 2 : D == 128 ? 4 : 3)
                                       : (D == 256 ? 3 : D == 128 ? 5 : 6);
-  static constexpr int RESIDENT = CG > 1 ? 1 : D == 64 ? 4 : 2; // workgroups a CU
+  static constexpr int RESIDENT = CG > 1 ? 1 : D == 64 ? 4 : 2;
   static constexpr int CHUNKS = D >= 128 ? D / 128 : 1; // of a lane's key
   static constexpr int WORDS = D >= 128 ? 4 : 2;        // of a chunk
   static constexpr int TILES = D / 16;                  // output tiles
@@ -84,23 +92,23 @@ template <int D, int CG> struct Geo {
 
 // The ring's buffers are variables of their own, so that the compiler sees
 // that a wait for one need not be a wait for all. The first two also take the
-// waves' partial outputs at the end, two waves each, and the columns' (m, l).
-template <int D, int CG, int I> __device__ __forceinline__ char *ring_buffer() {
-  using Geom = Geo<D, CG>;
-  constexpr int size = kWaves * Geom::STAGE;
-  static_assert(2 * Geom::TILES * 1024 + kWaves * CG * kColumns * 8 <= size, "room to join");
+// waves' partial outputs at the end, half of them each, and the columns' (m, l).
+template <int D, int CG, int W, int I> __device__ __forceinline__ char *ring_buffer() {
+  using Geom = Geo<D, CG, W>;
+  constexpr int size = W * Geom::STAGE;
+  static_assert(W / 2 * Geom::TILES * 1024 + W * CG * kColumns * 8 <= size, "room to join");
   __shared__ __attribute__((aligned(1024))) char buffer[size];
   return buffer;
 }
 
-template <int D, int CG>
-__global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
-                          amdgpu_waves_per_eu(Geo<D, CG>::RESIDENT)))
+template <int D, int CG, int W>
+__global__ __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W),
+                          amdgpu_waves_per_eu(Geo<D, CG, W>::RESIDENT)))
 void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool, PagedView g,
                       half_t *out, unsigned *invalid, unsigned queryHeads, SplitPlan plan,
                       ScoreScale c, Partials parts) {
-  using Geom = Geo<D, CG>;
-  constexpr unsigned kUnit = CG * kColumns;
+  using Geom = Geo<D, CG, W>;
+  constexpr unsigned kUnit = CG * kColumns, kWaves = W;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
   const PagedSeq own = paged_own(g);
   const Split split = paged_split(g, own, G, plan);
@@ -139,11 +147,11 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
   const unsigned end = s.past + s.rows;
-  const unsigned length = split.length(s), b0 = min(piece * length, most / 32 + 1);
+  const unsigned length = split.length(s, pieces), b0 = min(piece * length, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned mine = b1 > b0 + wave ? (b1 - b0 - wave + kWaves - 1) / kWaves : 0u;
 
-  // Block k of this wave is b0 + wave + 4 k; a lane knows where one in 64 is.
+  // Block k of this wave is b0 + wave + kWaves k; a lane knows where one in 64 is.
   size_t place = 0;
   bool bad = false;
   auto find_blocks = [&](unsigned k) {
@@ -324,17 +332,17 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   auto buffer = [&](int i) -> char * {
     switch (i % R) {
     case 0:
-      return ring_buffer<D, CG, 0>();
+      return ring_buffer<D, CG, W, 0>();
     case 1:
-      return ring_buffer<D, CG, 1>();
+      return ring_buffer<D, CG, W, 1>();
     case 2:
-      return ring_buffer<D, CG, (R > 2 ? 2 : 0)>();
+      return ring_buffer<D, CG, W, (R > 2 ? 2 : 0)>();
     case 3:
-      return ring_buffer<D, CG, (R > 3 ? 3 : 0)>();
+      return ring_buffer<D, CG, W, (R > 3 ? 3 : 0)>();
     case 4:
-      return ring_buffer<D, CG, (R > 4 ? 4 : 0)>();
+      return ring_buffer<D, CG, W, (R > 4 ? 4 : 0)>();
     default:
-      return ring_buffer<D, CG, (R > 5 ? 5 : 0)>();
+      return ring_buffer<D, CG, W, (R > 5 ? 5 : 0)>();
     }
   };
 #pragma unroll
@@ -355,10 +363,12 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 
   // Join the waves: (m, l) of the columns, then each wave its output tiles.
   auto out_of = [&](unsigned w) { // wave w's tiles
-    return reinterpret_cast<float4_t *>((w < 2 ? ring_buffer<D, CG, 0>() : ring_buffer<D, CG, 1>()) +
-                                        w % 2 * Geom::TILES * 1024);
+    return reinterpret_cast<float4_t *>(
+        (w < kWaves / 2 ? ring_buffer<D, CG, W, 0>() : ring_buffer<D, CG, W, 1>()) +
+        w % (kWaves / 2) * Geom::TILES * 1024);
   };
-  float *sM = reinterpret_cast<float *>(ring_buffer<D, CG, 1>() + 2 * Geom::TILES * 1024);
+  float *sM = reinterpret_cast<float *>(ring_buffer<D, CG, W, 1>() +
+                                       kWaves / 2 * Geom::TILES * 1024);
   float *sL = sM + kWaves * kUnit;
   __syncthreads(); // the ring's blocks are done with
   const bool lost = __builtin_amdgcn_ballot_w64(bad); // a page that is not in the pool
@@ -417,7 +427,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 // Joins the rows whose keys were divided. An item is such a row's query head,
 // the work of W waves, each every W-th piece, a lane D/64 channels; items are
 // taken in turn, so that a call without any costs one round of workgroups.
-// W: 8 for calls of few rows and many pieces, 1 for the others.
+// W: 8 where units have eight pieces or more on average, 1 otherwise.
 constexpr unsigned kMergeThreads = 512;
 constexpr unsigned kMergeGroups = 1024; // workgroups: four a CU
 template <int D, int W>
@@ -427,7 +437,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
   constexpr unsigned kItems = kMergeThreads / 64 / W; // of a workgroup
   typedef float vec __attribute__((ext_vector_type(N)));
   typedef _Float16 halves __attribute__((ext_vector_type(N)));
-  const unsigned G = queryHeads / g.kvHeads, unit = plan.columns;
+  const unsigned G = queryHeads / g.kvHeads, unit = 1u << plan.shift;
   const PagedSeq own = paged_own(g);
   const Split split = paged_split(g, own, G, plan);
   const unsigned lane = threadIdx.x % 64;
@@ -499,14 +509,14 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
 }
 
 size_t partial_columns(const PagedKvParams &p, unsigned group, const SplitPlan &plan) {
-  return (size_t)most_pieces(p, group, plan) * p.kvHeads * plan.columns;
+  return (size_t)most_pieces(p, group, plan) * p.kvHeads << plan.shift;
 }
 
 } // namespace
 
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads) {
   const unsigned group = queryHeads / p.kvHeads;
-  return 4 * (p.headDim + 2) * partial_columns(p, group, plan_for(p, group));
+  return 4 * (p.headDim + 2) * partial_columns(p, group, plan_for(p, group).split);
 }
 
 hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
@@ -514,8 +524,9 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
                             uint32_t *invalid, void *workspace, const PagedKvParams &p,
                             unsigned queryHeads, float scale, hipStream_t stream) {
   const unsigned group = queryHeads / p.kvHeads;
-  const SplitPlan plan = plan_for(p, group);
-  const unsigned unit = plan.columns, pieces = (unsigned)most_pieces(p, group, plan);
+  const GqaPlan both = plan_for(p, group);
+  const SplitPlan &plan = both.split;
+  const unsigned unit = 1u << plan.shift, pieces = (unsigned)most_pieces(p, group, plan);
   const PagedView g = paged_view(p, starts, past, table);
   float *ws = static_cast<float *>(workspace);
   const Partials parts{ws + partial_columns(p, group, plan) * p.headDim, ws};
@@ -524,29 +535,32 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
   const uint8_t *pages = static_cast<const uint8_t *>(pool);
   const ScoreScale c = score_scale(scale);
   auto attend = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * kWaves), 0, stream, from, pages,
-                       g, to, invalid, queryHeads, plan, c, parts);
+    hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * (unit == 16 ? plan.step : 4)), 0,
+                       stream, from, pages, g, to, invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };
-  auto by_columns = [&](auto one, auto two, auto four) {
-    return unit == 16 ? attend(one) : unit == 32 ? attend(two) : attend(four);
+  auto by_columns = [&](auto one, auto pooled, auto two, auto four) {
+    return unit == 16 ? attend(both.pooled ? pooled : one) : attend(unit == 32 ? two : four);
   };
   hipError_t e;
   if (unit > 64)
     e = launch_paged_tiles(from, pages, g, to, invalid, queryHeads, plan, c, parts, pieces, stream);
   else if (p.headDim == 256)
-    e = unit == 16 ? attend(paged_gqa_kernel<256, 1>) : attend(paged_gqa_kernel<256, 2>);
+    e = by_columns(paged_gqa_kernel<256, 1, 4>, paged_gqa_kernel<256, 1, 8>,
+                   paged_gqa_kernel<256, 2, 4>, paged_gqa_kernel<256, 2, 4>);
   else if (p.headDim == 128)
-    e = by_columns(paged_gqa_kernel<128, 1>, paged_gqa_kernel<128, 2>, paged_gqa_kernel<128, 4>);
+    e = by_columns(paged_gqa_kernel<128, 1, 4>, paged_gqa_kernel<128, 1, 8>,
+                   paged_gqa_kernel<128, 2, 4>, paged_gqa_kernel<128, 4, 4>);
   else
-    e = by_columns(paged_gqa_kernel<64, 1>, paged_gqa_kernel<64, 2>, paged_gqa_kernel<64, 4>);
+    e = by_columns(paged_gqa_kernel<64, 1, 4>, paged_gqa_kernel<64, 1, 8>,
+                   paged_gqa_kernel<64, 2, 4>, paged_gqa_kernel<64, 4, 4>);
   if (e != hipSuccess)
     return e;
   auto merge = [&](auto few, auto many) {
-    const unsigned each = unit == 16 ? 1 : kMergeThreads / 64;
+    const unsigned each = both.pooled ? 1 : kMergeThreads / 64;
     const uint64_t groups = ((uint64_t)p.tokens * queryHeads + each - 1) / each;
     const unsigned grid = (unsigned)(groups < kMergeGroups ? groups : kMergeGroups);
-    if (unit == 16)
+    if (both.pooled)
       hipLaunchKernelGGL(few, dim3(grid), dim3(kMergeThreads), 0, stream, g, to, queryHeads, plan,
                          parts);
     else

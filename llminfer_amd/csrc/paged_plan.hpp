@@ -10,7 +10,6 @@ namespace llmi {
 
 constexpr float kPagedRaise = 15.0f;   // raise m when a weight would pass 2^15
 constexpr float kPagedHeadroom = 7.0f; // after a raise the largest weight is 2^7
-constexpr unsigned kPagedStep = 4;     // a chunk is a multiple of so many blocks
 
 // The softmax scale as the kernels take it: exp2 of positive multiples of the
 // scores, so that their largest is the largest weight's, with the sign given
@@ -33,36 +32,44 @@ __device__ __forceinline__ half8_t with_sign(half8_t x, uint32_t sign) {
 // at most chunk, or (nearest) at most 1.5 of it, for a kernel whose pieces
 // cost more to join than some workgroups' longer time.
 struct Split {
-  unsigned group, columns, chunk;
+  unsigned group, shift, step, chunk; // units of 2^shift columns, whole steps of blocks
+  float inv;                    // 1 / chunk
   bool nearest;
   __device__ unsigned units(const PagedSeq &q) const {
-    return (unsigned)(((uint64_t)q.rows * group + columns - 1) / columns);
+    return (unsigned)(((uint64_t)q.rows * group + (1u << shift) - 1) >> shift);
   }
   __device__ static unsigned blocks(const PagedSeq &q) {
     return q.ok ? (q.past + q.rows + 31) / 32 : 1u;
   }
+  // (x + round) / chunk by the reciprocal, corrected by its remainder: at most
+  // as many pieces as the host planned for, so off by one at most
   __device__ unsigned pieces(const PagedSeq &q) const {
-    const unsigned n = (blocks(q) + (nearest ? chunk / 2 : chunk - 1)) / chunk;
+    const unsigned x = blocks(q) + (nearest ? chunk / 2 : chunk - 1);
+    unsigned n = (unsigned)((float)x * inv);
+    const int rest = (int)(x - n * chunk);
+    n = rest < 0 ? n - 1 : rest >= (int)chunk ? n + 1 : n;
     return n ? n : 1u;
   }
   // blocks of a piece: whole steps of the kernels
-  __device__ unsigned length(const PagedSeq &q) const {
-    const unsigned n = pieces(q), each = (blocks(q) + n - 1) / n;
-    return (each + kPagedStep - 1) / kPagedStep * kPagedStep;
+  __device__ unsigned length(const PagedSeq &q, unsigned pieces) const {
+    const unsigned each = (blocks(q) + pieces - 1) / pieces;
+    return (each + step - 1) & ~(step - 1);
   }
 };
 
 // How the host asks for it: `target` pieces a KV head, if the lengths give them.
+// step (a power of two): the blocks that a workgroup takes at a time.
 struct SplitPlan {
-  unsigned columns, target, nearest;
+  unsigned shift, step, target, nearest;
 };
 
 // The chunk for which the call has at most plan.target pieces more than units,
-// a multiple of kPagedStep blocks. (An fp32 sum is off by less than the
-// 1.0001; every workgroup and the merge add in the same order.)
+// whole steps. (The fp32 sum is exact below 2^24, and off
+// by less than the 1.0001 above; every workgroup and the merge add in the
+// same order.)
 __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
                                              unsigned group, const SplitPlan &plan) {
-  Split s{group, plan.columns, kPagedStep, plan.nearest != 0};
+  Split s{group, plan.shift, plan.step, plan.step, 0.0f, plan.nearest != 0};
   const unsigned lane = threadIdx.x % 64;
   float all = (float)s.units(own) * (float)Split::blocks(own);
   for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
@@ -75,9 +82,11 @@ __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq 
   all = p.a + p.b;
   p = pair32(all);
   all = p.a + p.b;
-  const unsigned chunk = (unsigned)(all * 1.0001f / (float)plan.target) + 1;
-  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane(
-      (int)((chunk + kPagedStep - 1) / kPagedStep * kPagedStep));
+  all = all < 16777216.0f ? all : all * 1.0001f;
+  const unsigned chunk = (unsigned)ceilf(all / (float)plan.target);
+  const unsigned whole = (chunk + s.step - 1) & ~(s.step - 1);
+  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(whole ? whole : s.step));
+  s.inv = __builtin_amdgcn_rcpf((float)s.chunk);
   return s;
 }
 

@@ -111,7 +111,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
   const unsigned end = s.past + s.rows;
-  const unsigned length = split.length(s), b0 = min(piece * length, most / 32 + 1);
+  const unsigned length = split.length(s, pieces), b0 = min(piece * length, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned steps = (b1 - b0 + T::BLOCKS - 1) / T::BLOCKS;
 

@@ -51,7 +51,7 @@ uint64_t most_pieces(const PagedKvParams &p, unsigned group, const SplitPlan &pl
 // Columns of a unit, by those that a sequence has on average: groups of 16 of
 // this file's kernel, or the units of paged_tiles.hip. Pieces: as many as
 // there are CUs (twice that at head_dim 64, where two workgroups share one);
-// six times as many where single tokens have units enough that their
+// up to six times as many where single tokens have units enough that their
 // different lengths count for more than the joining.
 struct GqaPlan {
   SplitPlan split;
@@ -66,8 +66,14 @@ GqaPlan plan_for(const PagedKvParams &p, unsigned group) {
                                                               : 64;
   const unsigned cus = (kCus + p.kvHeads - 1) / p.kvHeads;
   const bool pooled = cus >= 8 * most_units(p, group, unit);
-  const unsigned rounds = unit > 16 ? 1 : !pooled ? 6 : p.headDim == 64 ? 2 : 1;
-  return {{(unsigned)__builtin_ctz(unit), pooled && unit == 16 ? 8u : 4u, rounds * cus, tiles}, pooled};
+  const unsigned fill = unit == 16 && p.headDim == 64 ? 2 * cus : cus;
+  return {{(unsigned)__builtin_ctz(unit), pooled && unit == 16 ? 8u : 4u, fill,
+           unit == 16 && !pooled ? 6 * cus : fill, 64u, tiles},
+          pooled};
+}
+// Whether some lengths that fit the table divide a unit's keys.
+bool may_divide(const PagedKvParams &p, const SplitPlan &plan) {
+  return (uint64_t)p.tableStride * p.pageSize > 32 * plan.step;
 }
 
 // ------------------------------------------------------------- the kernel
@@ -427,7 +433,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 // Joins the rows whose keys were divided. An item is such a row's query head,
 // the work of W waves, each every W-th piece, a lane D/64 channels; items are
 // taken in turn, so that a call without any costs one round of workgroups.
-// W: 8 where units have eight pieces or more on average, 1 otherwise.
+// W: 8 where units have many pieces or few columns, 1 otherwise.
 constexpr unsigned kMergeThreads = 512;
 constexpr unsigned kMergeGroups = 1024; // workgroups: four a CU
 template <int D, int W>
@@ -516,6 +522,8 @@ size_t partial_columns(const PagedKvParams &p, unsigned group, const SplitPlan &
 
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads) {
   const unsigned group = queryHeads / p.kvHeads;
+  if (!may_divide(p, plan_for(p, group).split))
+    return 0;
   return 4 * (p.headDim + 2) * partial_columns(p, group, plan_for(p, group).split);
 }
 
@@ -556,11 +564,14 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
                    paged_gqa_kernel<64, 2, 4>, paged_gqa_kernel<64, 4, 4>);
   if (e != hipSuccess)
     return e;
+  if (!may_divide(p, plan))
+    return e;
+  const bool wide = both.pooled || unit <= 64;
   auto merge = [&](auto few, auto many) {
-    const unsigned each = both.pooled ? 1 : kMergeThreads / 64;
+    const unsigned each = wide ? 1 : kMergeThreads / 64;
     const uint64_t groups = ((uint64_t)p.tokens * queryHeads + each - 1) / each;
     const unsigned grid = (unsigned)(groups < kMergeGroups ? groups : kMergeGroups);
-    if (both.pooled)
+    if (wide)
       hipLaunchKernelGGL(few, dim3(grid), dim3(kMergeThreads), 0, stream, g, to, queryHeads, plan,
                          parts);
     else

@@ -57,16 +57,17 @@ struct Split {
   }
 };
 
-// How the host asks for it: `target` pieces a KV head, if the lengths give them.
-// step (a power of two): the blocks that a workgroup takes at a time.
+// How the host asks for it: `fill` pieces a KV head fill the device, and at
+// most `target`, some rounds of that, are made where pieces then still have
+// `whole` blocks. step (a power of two): the blocks that a workgroup takes at
+// a time.
 struct SplitPlan {
-  unsigned shift, step, target, nearest;
+  unsigned shift, step, fill, target, whole, nearest;
 };
 
-// The chunk for which the call has at most plan.target pieces more than units,
-// whole steps. (The fp32 sum is exact below 2^24, and off
-// by less than the 1.0001 above; every workgroup and the merge add in the
-// same order.)
+// The chunk, whole steps, for which the call has at most plan.target pieces
+// more than units. (The fp32 sum is exact below 2^24, and off by less than
+// the 1.0001 above; every workgroup and the merge add in the same order.)
 __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
                                              unsigned group, const SplitPlan &plan) {
   Split s{group, plan.shift, plan.step, plan.step, 0.0f, plan.nearest != 0};
@@ -83,9 +84,11 @@ __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq 
   p = pair32(all);
   all = p.a + p.b;
   all = all < 16777216.0f ? all : all * 1.0001f;
-  const unsigned chunk = (unsigned)ceilf(all / (float)plan.target);
-  const unsigned whole = (chunk + s.step - 1) & ~(s.step - 1);
-  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(whole ? whole : s.step));
+  const unsigned least = (unsigned)ceilf(all / (float)plan.target);
+  const unsigned one = (unsigned)ceilf(all / (float)plan.fill); // of a single round
+  const unsigned chunk = max(least, min(one, plan.whole));
+  const unsigned steps = (chunk + s.step - 1) & ~(s.step - 1);
+  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(steps ? steps : s.step));
   s.inv = __builtin_amdgcn_rcpf((float)s.chunk);
   return s;
 }

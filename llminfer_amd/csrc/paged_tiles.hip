@@ -42,6 +42,40 @@ template <int I> __device__ __forceinline__ char *tile_buffer() {
   return buffer;
 }
 
+// The call's piece `u` with the sequences of the longest pieces first (up to 64
+// sequences; in their order otherwise), so that workgroups which start late
+// have little to do (seven messages of 41 to 110 blocks, 296 workgroups:
+// RAGGED us in order, SORTED longest first).
+__device__ __forceinline__ bool find_longest(const PagedView &g, const PagedSeq &own,
+                                             const Split &split, unsigned u, unsigned &seq,
+                                             unsigned &local, unsigned &number) {
+  unsigned before;
+  if (g.sequences == 1 || g.sequences > 64) {
+    number = u;
+    return paged_find(g, own, u,
+                      [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq,
+                      local, before);
+  }
+  const unsigned lane = threadIdx.x % 64;
+  const unsigned pieces = split.pieces(own), length = split.length(own, pieces);
+  const unsigned n = split.units(own) * pieces;
+  unsigned ahead = 0;
+  for (unsigned j = 0; j < g.sequences; ++j) {
+    const unsigned lj = (unsigned)__builtin_amdgcn_readlane((int)length, (int)j);
+    const unsigned nj = (unsigned)__builtin_amdgcn_readlane((int)n, (int)j);
+    ahead += lj > length || (lj == length && j < lane) ? nj : 0u;
+  }
+  const unsigned long long here =
+      __builtin_amdgcn_ballot_w64(lane < g.sequences && u - ahead < n);
+  if (!here)
+    return false;
+  const int at = __builtin_ctzll(here);
+  seq = (unsigned)at;
+  local = u - (unsigned)__builtin_amdgcn_readlane((int)ahead, at);
+  number = (unsigned)__builtin_amdgcn_readlane((int)(wave_scan(n) - n), at) + local;
+  return true;
+}
+
 constexpr unsigned kRaw = 2560; // bytes of a wave's part of a step
 __device__ __forceinline__ char *raw_buffer() {
   __shared__ __attribute__((aligned(1024))) char buffer[kThreads / 64 * kRaw];
@@ -73,13 +107,11 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
                         SplitPlan plan, ScoreScale c, Partials parts) {
   using T = Tiles<D>;
   constexpr int CT = T::CT;
-  const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
+  const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.x % g.kvHeads;
   const PagedSeq own = paged_own(g);
   const Split split = paged_split(g, own, G, plan);
-  unsigned seq, local, before;
-  if (!paged_find(g, own, blockIdx.x,
-                  [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local,
-                  before))
+  unsigned seq, local, number; // number: of this piece, for its partials
+  if (!find_longest(g, own, split, blockIdx.x / g.kvHeads, seq, local, number))
     return;
   const PagedSeq s = paged_seq_of(g, own, seq);
   const unsigned pieces = split.pieces(s), units = split.units(s);
@@ -150,8 +182,23 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const unsigned keyAt = slot * T::BLOCKB + (unit16 % (D / 2) / 16) * 2048 +
                          (16 * (rr / 8) + 8 * (unit16 / (D / 2)) + rr % 8) * 16;
   const unsigned valueAt = slot * T::BLOCKB + (unit16 / 64) * 4096 + quad * 512 + rr * 16;
+  // The wave's part of step n has come. Behind the sequence's last key lies
+  // anything, and 0 times that may be NaN: those slots' scales and biases
+  // become 0 (a lane has two slots of one quad).
+  auto arrived = [&](unsigned n) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const unsigned base = 32 * block_of(n);
+    if (base + 32 > end) {
+      const unsigned sq = lane / 4 % 4, e = lane % 4 * 2;
+      const unsigned at = base + 16 * (sq / 2) + 4 * (sq % 2) + 8 * (e / 4) + e % 4;
+      half_t *mine = reinterpret_cast<half_t *>(raw + 2304) + 2 * lane;
+      if (at >= end)
+        mine[0] = (half_t)0;
+      if (at + 1 >= end)
+        mine[1] = (half_t)0;
+    }
+  };
   auto decode_keys = [&](char *to) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the wave's part is there
     const uint4_t keyCodes = *reinterpret_cast<const uint4_t *>(raw + 16 * lane);
     const half2_t keyScale = *reinterpret_cast<const half2_t *>(raw + 2048 + 4 * lane);
 #pragma unroll
@@ -159,24 +206,13 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
       *reinterpret_cast<half8_t *>(to + keyAt + 512 * w) =
           paged_eight(keyCodes[w], keyScale, nibbles);
   };
-  auto decode_values = [&](unsigned n, char *to) {
+  auto decode_values = [&](char *to) {
     const uint4_t valueCodes = *reinterpret_cast<const uint4_t *>(raw + 1024 + 16 * lane);
     const uint32_t *mine = reinterpret_cast<const uint32_t *>(raw + 2304);
-    const unsigned first = 32 * block_of(n) + 16 * (quad / 2) + 4 * (quad % 2);
-    const bool tail = 32 * block_of(n) + 32 > end;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      half8_t sc = *reinterpret_cast<const half8_t *>(mine + 32 * p + 4 * quad);
-      half8_t bi = *reinterpret_cast<const half8_t *>(mine + 32 * p + 16 + 4 * quad);
-      if (tail) { // behind the sequence's last key lies anything: values of 0
-        asm volatile("" ::: "memory"); // (a branch, rarely taken, and not selects)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool in = first + 8 * (e / 4) + e % 4 < end;
-          sc[e] = in ? sc[e] : (half_t)0;
-          bi[e] = in ? bi[e] : (half_t)0;
-        }
-      }
+      const half8_t sc = *reinterpret_cast<const half8_t *>(mine + 32 * p + 4 * quad);
+      const half8_t bi = *reinterpret_cast<const half8_t *>(mine + 32 * p + 16 + 4 * quad);
 #pragma unroll
       for (int w = 0; w < 2; ++w)
         *reinterpret_cast<half8_t *>(to + valueAt + 2048 * p + 256 * w) =
@@ -273,8 +309,9 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 
   if (steps) {
     fetch(0);
+    arrived(0);
     decode_keys(tile_buffer<0>());
-    decode_values(0, tile_buffer<2>());
+    decode_values(tile_buffer<2>());
     if (steps > 1)
       fetch(1);
   }
@@ -283,8 +320,9 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
     lds_sync(); // step n is decoded, and step n - 1's tiles are done with
     auto decode = [&]() {
       if (n + 1 < steps) {
+        arrived(n + 1);
         decode_keys(nextKeys);
-        decode_values(n + 1, nextValues);
+        decode_values(nextValues);
         if (n + 2 < steps)
           fetch(n + 2);
       }
@@ -351,7 +389,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
     const float a = m[j] == -INFINITY ? 0.0f : fast_exp2(m[j] - top);
     const float b = other == -INFINITY ? 0.0f : fast_exp2(other - top);
     const float sum = sLost ? NAN : l[j] * a + sL[col] * b;
-    const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * T::UNIT + col;
+    const size_t part = ((size_t)number * g.kvHeads + kvh) * T::UNIT + col;
     const float inv = 1.0f / sum;
     if (!live(j))
       continue;
@@ -385,7 +423,7 @@ hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedV
                               unsigned *invalid, unsigned queryHeads, SplitPlan plan, ScoreScale c,
                               Partials parts, unsigned pieces, hipStream_t stream) {
   auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(pieces, g.kvHeads), dim3(kThreads), 0, stream, q, pool, g, out,
+    hipLaunchKernelGGL(kernel, dim3(pieces * g.kvHeads), dim3(kThreads), 0, stream, q, pool, g, out,
                        invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };

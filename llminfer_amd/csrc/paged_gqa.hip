@@ -67,7 +67,8 @@ GqaPlan plan_for(const PagedKvParams &p, unsigned group) {
   const unsigned cus = (kCus + p.kvHeads - 1) / p.kvHeads;
   const bool pooled = cus >= 8 * most_units(p, group, unit);
   const unsigned fill = unit == 16 && p.headDim == 64 ? 2 * cus : cus;
-  return {{(unsigned)__builtin_ctz(unit), pooled && unit == 16 ? 8u : 4u, fill,
+  const unsigned step = tiles ? 512 / p.headDim : unit == 16 && pooled ? 8 : 4;
+  return {{(unsigned)__builtin_ctz(unit), step, fill,
            unit == 16 && !pooled ? 6 * cus : fill, 64u, tiles},
           pooled};
 }
@@ -543,7 +544,7 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
   const uint8_t *pages = static_cast<const uint8_t *>(pool);
   const ScoreScale c = score_scale(scale);
   auto attend = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * (unit == 16 ? plan.step : 4)), 0,
+    hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * plan.step), 0,
                        stream, from, pages, g, to, invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };

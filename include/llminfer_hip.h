@@ -483,8 +483,10 @@ LLMI_HIP_API int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, fl
  * table (negative, or from tableStride * pageSize on) or whose page is not in
  * the pool is an error that only the device can see: it sets bit 1 (2) of
  * *invalid (when invalid is not null; never cleared here), is not appended,
- * and is NaN where it is read or attended to. Two sequences of a call may
- * share pages that the call does not append to.
+ * and is NaN where it is read or attended to. Starts that go back or past
+ * `tokens` are cut to the rows there are; rows that two sequences claim may
+ * come out as either's or not at all. Two sequences of a call may share pages
+ * that the call does not append to. At most 2^22 - 1 rows or sequences.
  *
  * paged_append: keys and values [tokens][kvHeads][headDim] fp16 (strided;
  * p.tokens rows) to their places; keys are rotated at their positions as
@@ -505,11 +507,14 @@ LLMI_HIP_API int llmi_hip_paged_read(const void *pool, const int32_t *starts,
 
 /* CausalGqa of every row over its own sequence's cache: row (starts[s] + i,
  * h) is the softmax over keys j <= past[s] + i of scale q . K[j, h /
- * (queryHeads / kvHeads)], times V. q and out [tokens][queryHeads][headDim]
- * fp16, dense, 16-byte aligned; the call's own rows are appended before.
- * `workspace` holds llmi_hip_paged_gqa_workspace_bytes(p) bytes, 16-byte
- * aligned: the partials of rows whose keys are divided over workgroups,
- * written and read within the call. */
+ * (queryHeads / kvHeads)], times V: scores, softmax statistics and sums in
+ * fp32, the weights fp16. q and out [tokens][queryHeads][headDim] fp16,
+ * dense, 16-byte aligned, apart from each other; the call's own rows are
+ * appended before. `workspace` holds llmi_hip_paged_gqa_workspace_bytes(p)
+ * bytes (0: none is needed), 16-byte aligned: the partials of rows whose keys
+ * are divided over workgroups, written and read within the call. How they are
+ * divided, and so the order of the sums, goes by the lengths and the counts
+ * of rows and sequences alone. */
 LLMI_HIP_API int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts,
                                     const int32_t *past, const int32_t *table, const void *pool,
                                     uint16_t *out, uint32_t *invalid, PagedGqaParams p,

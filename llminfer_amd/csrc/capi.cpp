@@ -1011,8 +1011,8 @@ int llmi_hip_rope(const uint16_t *input, const int32_t *positions, const float *
     return fail(LLMI_HIP_UNSUPPORTED, "rope: rotary width %u", p.rotaryDim);
   if (!strides_apart(p.tokens, p.outputTokenStride, p.heads, p.outputHeadStride, p.headDim))
     return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: the output's rows overlap");
-  if (!fits32(p.tokens, p.heads, p.headDim))
-    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: exceeds the 32-bit index range");
+  if (!fits32(p.tokens, p.heads, p.headDim) || p.tokens >= 1u << 24)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "rope: exceeds the 32-bit index range or 2^24 tokens");
   return launched(launch_rope_rows(input, positions, freqs, output, p,
                                    static_cast<hipStream_t>(stream)),
                   "ropeRows");
@@ -1061,10 +1061,10 @@ static int check_paged(const char *what, const PagedKvParams &p, const int32_t *
     return fail(LLMI_HIP_UNSUPPORTED, "%s: page size %u is no multiple of 32", what, p.pageSize);
   if (p.pages == 0 || p.kvHeads == 0 || p.tableStride == 0)
     return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: pages, heads and table must not be empty", what);
-  if ((uint64_t)p.tableStride * p.pageSize > 0x7fffffffull || p.tokens > 0x7fffffffu ||
-      p.pages > 0x7fffffffu || p.sequences > 0x7fffffffu || p.kvHeads > 65535u)
-    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: exceeds the 31-bit range of positions, rows, "
-                "pages and sequences, or 65535 heads", what);
+  if ((uint64_t)p.tableStride * p.pageSize > 0x7fffffffull || p.pages > 0x7fffffffu ||
+      p.tokens >= 1u << 22 || p.sequences >= 1u << 22 || p.kvHeads > 65535u)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: exceeds the 31-bit range of positions and pages, "
+                "2^22 rows or sequences, or 65535 heads", what);
   if (!starts || !past || !table || !pool)
     return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: null buffer", what);
   if (!aligned16(pool))
@@ -1129,6 +1129,12 @@ int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *
     return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedGqa: null buffer");
   if (!aligned16(q) || !aligned16(out))
     return fail(LLMI_HIP_UNSUPPORTED, "pagedGqa: rows not 16-byte aligned");
+  if (!paged_gqa_launchable(p.kv, p.queryHeads))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedGqa: too many rows and heads for one call");
+  const uintptr_t from = reinterpret_cast<uintptr_t>(q), to = reinterpret_cast<uintptr_t>(out);
+  const size_t bytes = (size_t)p.kv.tokens * p.queryHeads * p.kv.headDim * 2;
+  if (from < to + bytes && to < from + bytes)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedGqa: out overlaps q");
   const size_t need = paged_gqa_workspace_bytes(p.kv, p.queryHeads);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(LLMI_HIP_WORKSPACE, "pagedGqa: workspace of %zu bytes, %zu needed (16-byte "
@@ -1139,7 +1145,8 @@ int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *
 }
 
 size_t llmi_hip_paged_gqa_workspace_bytes(PagedGqaParams p) {
-  if (p.kv.tokens == 0 || p.kv.sequences == 0 || check_paged_heads(p))
+  if (p.kv.tokens == 0 || p.kv.sequences == 0 || check_paged_heads(p) ||
+      !paged_gqa_launchable(p.kv, p.queryHeads))
     return 0;
   return paged_gqa_workspace_bytes(p.kv, p.queryHeads);
 }
@@ -1260,7 +1267,9 @@ unsigned llmi_hip_dispatch_count(int op, const void *params) {
   }
   case LLMI_HIP_OP_PAGED_GQA: {
     const PagedGqaParams &p = *static_cast<const PagedGqaParams *>(params);
-    return p.kv.tokens && p.kv.sequences && !check_paged_heads(p) ? 1 : 0;
+    if (!p.kv.tokens || !p.kv.sequences || check_paged_heads(p))
+      return 0;
+    return 1u + paged_gqa_joins(p.kv, p.queryHeads);
   }
   case LLMI_HIP_OP_GATED_ATTENTION: {
     // Launches for a rotary width the kernels take (a multiple of 16).
@@ -1378,7 +1387,11 @@ const char *llmi_hip_kernel_name(int op, const void *params, unsigned index) {
   case LLMI_HIP_OP_PAGED_READ:
     return "pagedRead";
   case LLMI_HIP_OP_PAGED_GQA:
-    return "pagedGqa";
+    return index ? "pagedGqaMerge"
+           : paged_gqa_tiled(static_cast<const PagedGqaParams *>(params)->kv,
+                             static_cast<const PagedGqaParams *>(params)->queryHeads)
+               ? "pagedGqaTiles"
+               : "pagedGqaSplit";
   case LLMI_HIP_OP_GATED_ATTENTION:
     if (static_cast<const GqaParams *>(params)->tokens == 1)
       return index == 0 ? "gqaDecodeGated" : "gqaDecodeMergeGated";

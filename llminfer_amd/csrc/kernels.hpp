@@ -299,6 +299,9 @@ hipError_t launch_paged_append(const uint16_t *keys, const uint16_t *values, con
 hipError_t launch_paged_read(const void *pool, const int32_t *starts, const int32_t *past,
                              const int32_t *table, uint16_t *keys, uint16_t *values,
                              uint32_t *invalid, const PagedKvParams &p, hipStream_t stream);
+bool paged_gqa_launchable(const PagedKvParams &p, unsigned queryHeads); // grids in range
+bool paged_gqa_tiled(const PagedKvParams &p, unsigned queryHeads); // the tiles' kernel runs
+bool paged_gqa_joins(const PagedKvParams &p, unsigned queryHeads); // with a launch that joins
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads);
 hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int32_t *past,
                             const int32_t *table, const void *pool, uint16_t *out,

@@ -439,7 +439,7 @@ constexpr unsigned kMergeThreads = 512;
 constexpr unsigned kMergeGroups = 1024; // workgroups: four a CU
 template <int D, int W>
 __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
-    PagedView g, half_t *out, unsigned queryHeads, SplitPlan plan, Partials parts) {
+    PagedView g, half_t *out, unsigned queryHeads, SplitPlan plan, unsigned most, Partials parts) {
   constexpr int N = D / 64;
   constexpr unsigned kItems = kMergeThreads / 64 / W; // of a workgroup
   typedef float vec __attribute__((ext_vector_type(N)));
@@ -472,6 +472,8 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
     const unsigned pieces = split.pieces(s), h = local % queryHeads, row = local / queryHeads;
     const unsigned column = row * G + h % G, kvh = h / G;
     const unsigned first = pieceBefore + (split.units(s) - 1 - column / unit) * pieces;
+    if (first + pieces > most) // starts out of order: more pieces than the rows can have
+      return;
     const size_t at = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
     const size_t step = (size_t)g.kvHeads * unit;
     const float2 *ml = reinterpret_cast<const float2 *>(parts.ml) + at;
@@ -521,9 +523,22 @@ size_t partial_columns(const PagedKvParams &p, unsigned group, const SplitPlan &
 
 } // namespace
 
+bool paged_gqa_tiled(const PagedKvParams &p, unsigned queryHeads) {
+  return (1u << plan_for(p, queryHeads / p.kvHeads).split.shift) > 64;
+}
+bool paged_gqa_joins(const PagedKvParams &p, unsigned queryHeads) {
+  return may_divide(p, plan_for(p, queryHeads / p.kvHeads).split);
+}
+bool paged_gqa_launchable(const PagedKvParams &p, unsigned queryHeads) {
+  const unsigned group = queryHeads / p.kvHeads;
+  const uint64_t rows = (uint64_t)p.tokens * queryHeads;
+  return rows <= 0x7fffffffull &&
+         (most_pieces(p, group, plan_for(p, group).split)) * p.kvHeads < (1u << 22);
+}
+
 size_t paged_gqa_workspace_bytes(const PagedKvParams &p, unsigned queryHeads) {
   const unsigned group = queryHeads / p.kvHeads;
-  if (!may_divide(p, plan_for(p, group).split))
+  if (!paged_gqa_joins(p, queryHeads))
     return 0;
   return 4 * (p.headDim + 2) * partial_columns(p, group, plan_for(p, group).split);
 }
@@ -574,10 +589,10 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
     const unsigned grid = (unsigned)(groups < kMergeGroups ? groups : kMergeGroups);
     if (wide)
       hipLaunchKernelGGL(few, dim3(grid), dim3(kMergeThreads), 0, stream, g, to, queryHeads, plan,
-                         parts);
+                         pieces, parts);
     else
       hipLaunchKernelGGL(many, dim3(grid), dim3(kMergeThreads), 0, stream, g, to, queryHeads, plan,
-                         parts);
+                         pieces, parts);
     return hipGetLastError();
   };
   return p.headDim == 256   ? merge(paged_gqa_merge_kernel<256, 8>, paged_gqa_merge_kernel<256, 1>)

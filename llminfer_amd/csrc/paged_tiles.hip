@@ -111,7 +111,8 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const PagedSeq own = paged_own(g);
   const Split split = paged_split(g, own, G, plan);
   unsigned seq, local, number; // number: of this piece, for its partials
-  if (!find_longest(g, own, split, blockIdx.x / g.kvHeads, seq, local, number))
+  if (!find_longest(g, own, split, blockIdx.x / g.kvHeads, seq, local, number) ||
+      number >= gridDim.x / g.kvHeads) // (starts out of order: more pieces than the rows can have)
     return;
   const PagedSeq s = paged_seq_of(g, own, seq);
   const unsigned pieces = split.pieces(s), units = split.units(s);

@@ -1009,6 +1009,8 @@ def _require_rows(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be {torch.float16}, got {t.dtype}")
     if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
         raise ValueError(f"{name} must be [T, H, dim] with contiguous rows")
+    if max(t.stride(0), t.stride(1)) > 0xffffffff:
+        raise ValueError(f"{name}'s strides exceed 32 bits")
 
 
 def bind_rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: torch.Tensor,
@@ -1148,9 +1150,10 @@ def bind_paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, pa
     """CausalGqa of q [T, Hq, dim] fp16 over the paged 4-bit cache
     (llmi_hip_paged_gqa): row i of sequence s attends to its keys at positions
     up to past[s] + i, the call's own rows among them (appended before). scale
-    defaults to 1 / sqrt(dim). Rows of no sequence are left as they are; a row
-    that would read a page outside the pool, or does not fit its table, is NaN
-    and sets bit 1 of invalid."""
+    defaults to 1 / sqrt(dim); out must not overlap q. Rows of no sequence are
+    left as they are; a row that would read a page outside the pool, or does
+    not fit its table, is NaN and sets bit 1 of invalid. The workspace is the
+    stream's; under capture it is the graph's own."""
     for t, n in ((q, "q"), (out, "out")):
         _require(t, torch.float16, n)
     if q.dim() != 3 or out.shape != q.shape:
@@ -1164,7 +1167,11 @@ def bind_paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, pa
                             float(np.float32(1.0) / np.sqrt(np.float32(q.shape[2])))
                             if scale is None else scale)
     need = lib.llmi_hip_paged_gqa_workspace_bytes(p)
-    ws = workspace(need, q.device, "paged") if need else None
+    if need and torch.cuda.is_current_stream_capturing():
+        # a graph's own, from its pool: replays of two graphs may overlap
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        ws = workspace(need, q.device, "paged") if need else None
     b = Bound(lib.llmi_hip_paged_gqa,
               (_ptr(q), _ptr(starts), _ptr(past), _ptr(table), _ptr(pool), _ptr(out),
                _ptr(invalid), p, _ptr(ws), ws.numel() if ws is not None else 0, _stream()),

@@ -37,6 +37,7 @@ def rope_params(**over):
     (dict(outputHeadStride=63), _lib.INVALID_ARGUMENT),          # heads overlap
     (dict(outputTokenStride=127), _lib.INVALID_ARGUMENT),        # tokens overlap
     (dict(tokens=1 << 31, heads=64), _lib.INVALID_ARGUMENT),     # 32-bit index range
+    (dict(tokens=1 << 24, heads=1, headDim=32), _lib.INVALID_ARGUMENT),
     (dict(tokens=0), _lib.OK),
 ])
 def test_rope_refusals(over, status):
@@ -53,9 +54,12 @@ def test_rope_null_buffers():
 
 
 def kv_params(**over):
-    p = dict(pages=8, pageSize=64, kvHeads=2, headDim=128, sequences=2, tableStride=4, tokens=5)
+    p = dict(pages=8, pageSize=64, kvHeads=2, headDim=128, sequences=2, tableStride=9, tokens=5)
     p.update(over)
     return _lib.PagedKvParams(**p)
+
+
+FAR = 1 << 40  # a stand-in pointer apart from A16's buffers
 
 
 def append_params(**over):
@@ -74,9 +78,9 @@ BAD_KV = [
     (dict(kvHeads=65536), _lib.INVALID_ARGUMENT),
     (dict(tableStride=0), _lib.INVALID_ARGUMENT),
     (dict(tableStride=1 << 26, pageSize=32), _lib.INVALID_ARGUMENT),  # positions past 2^31
-    (dict(tokens=1 << 31), _lib.INVALID_ARGUMENT),
+    (dict(tokens=1 << 22), _lib.INVALID_ARGUMENT),
     (dict(pages=1 << 31), _lib.INVALID_ARGUMENT),
-    (dict(sequences=1 << 31), _lib.INVALID_ARGUMENT),
+    (dict(sequences=1 << 22), _lib.INVALID_ARGUMENT),
     (dict(tokens=0), _lib.OK),
     (dict(sequences=0), _lib.OK),
 ]
@@ -88,8 +92,8 @@ def test_paged_refusals(over, status):
     p = kv_params(**over)
     assert lib.llmi_hip_paged_append(*[A16] * 8, p, append_params(), None) == status
     assert lib.llmi_hip_paged_read(*[A16] * 7, p, None) == status
-    assert lib.llmi_hip_paged_gqa(*[A16] * 7, _lib.PagedGqaParams(p, p.kvHeads, 1.0), A16, 1 << 40,
-                                  None) == status
+    assert lib.llmi_hip_paged_gqa(*[A16] * 5, FAR, A16, _lib.PagedGqaParams(p, p.kvHeads, 1.0),
+                                  A16, 1 << 40, None) == status
 
 
 def test_append_refusals():
@@ -124,10 +128,22 @@ def test_read_and_gqa_refusals():
     for heads in (0, 3, 65536):
         assert lib.llmi_hip_paged_gqa(*[A16] * 7, _lib.PagedGqaParams(kv_params(), heads, 1.0),
                                       A16, 1 << 40, None) == _lib.INVALID_ARGUMENT
-    need = lib.llmi_hip_paged_gqa_workspace_bytes(gqa)
-    if need:
-        for ws, size in ((None, 0), (A16, need - 1), (A16 + 8, need)):
-            assert lib.llmi_hip_paged_gqa(*[A16] * 7, gqa, ws, size, None) == _lib.WORKSPACE
+    call = [A16] * 5 + [FAR, A16]
+    for ws, size in ((None, 0), (A16, lib.llmi_hip_paged_gqa_workspace_bytes(gqa) - 1),
+                     (A16 + 8, 1 << 40)):
+        assert lib.llmi_hip_paged_gqa(*call, gqa, ws, size, None) == _lib.WORKSPACE
+    # a table whose keys are never divided needs none, and more rows and heads
+    # than one call takes are refused
+    small = _lib.PagedGqaParams(kv_params(tableStride=2), 4, 1.0)
+    assert lib.llmi_hip_paged_gqa_workspace_bytes(small) == 0
+    assert ops.kernel_names(_lib.OP_PAGED_GQA, small) == ["pagedGqaSplit"]
+    large = _lib.PagedGqaParams(kv_params(tokens=(1 << 22) - 1, kvHeads=512), 512 * 64, 1.0)
+    assert lib.llmi_hip_paged_gqa(*call, large, A16, 1 << 60, None) == _lib.INVALID_ARGUMENT
+    assert lib.llmi_hip_paged_gqa_workspace_bytes(large) == 0
+    # out inside q, and q inside out (5 rows of 4 heads of 128)
+    for q, out in ((A16, A16), (A16, A16 + 5104), (A16 + 5104, A16)):
+        assert lib.llmi_hip_paged_gqa(q, A16, A16, A16, A16, out, None, gqa, A16, 1 << 40,
+                                      None) == _lib.INVALID_ARGUMENT
     assert lib.llmi_hip_paged_gqa_workspace_bytes(_lib.PagedGqaParams(kv_params(), 3, 1.0)) == 0
 
 
@@ -136,7 +152,10 @@ def test_plan_names():
     assert ops.kernel_names(_lib.OP_ROPE, rope_params(tokens=0)) == []
     assert ops.kernel_names(_lib.OP_PAGED_APPEND, kv_params()) == ["pagedAppend"]
     assert ops.kernel_names(_lib.OP_PAGED_READ, kv_params()) == ["pagedRead"]
-    assert ops.kernel_names(_lib.OP_PAGED_GQA, _lib.PagedGqaParams(kv_params(), 4, 1.0))
+    assert ops.kernel_names(_lib.OP_PAGED_GQA, _lib.PagedGqaParams(kv_params(), 4, 1.0)) == \
+        ["pagedGqaSplit", "pagedGqaMerge"]
+    many = _lib.PagedGqaParams(kv_params(tokens=500, tableStride=64), 4, 1.0)
+    assert ops.kernel_names(_lib.OP_PAGED_GQA, many) == ["pagedGqaTiles", "pagedGqaMerge"]
     assert ops.kernel_names(_lib.OP_PAGED_GQA, _lib.PagedGqaParams(kv_params(), 3, 1.0)) == []
 
 

@@ -256,6 +256,7 @@ def test_rows_with_no_place(gpu):
         assert np.all(np.abs(out[lo:lo + n] - want) <= far)
     assert np.isnan(out[72:]).all()
     # starts that go back, or past the rows: nothing outside is read or written
+    # (more of it in test_starts_out_of_order)
     for bad in ([0, 50, 20, 60, 61, 62], [-5, 10, 1000, 3, 2000000000, 2], [92, 92, 92, 92, 92, 92]):
         starts = ints(*bad)
         to = torch.full((T + 8, 2 * hkv, dim), 5.0, dtype=torch.float16, device="cuda")
@@ -263,6 +264,64 @@ def test_rows_with_no_place(gpu):
         cache.append(dev(k), dev(v), starts, lens)
         ops.paged_read(cache.pool, starts, lens, cache.table, T)
         assert (to[T:] == 5).all()
+
+
+@pytest.mark.parametrize("dim, hq, rows", [(64, 4, 2), (128, 4, 2), (256, 8, 2), (128, 8, 40),
+                                           (256, 4, 40)])
+def test_starts_out_of_order(gpu, dim, hq, rows):
+    """Sequences that all claim the same rows, on long histories: more pieces of
+    keys than such rows could have; rows of none, and memory behind, stay."""
+    rng = np.random.default_rng(6)
+    S, T, n = 12, rows, 2000
+    cache = Cache(rng, S, n + rows, 1, dim, 64, fill=0)
+    q = rows16(rng, T + 4, hq, dim)
+    for starts in ([0, rows] * (S // 2) + [0], [rows] + [0] * S, [0] * S + [10 ** 9],
+                   [-10 ** 9] + [10 ** 9, 1] * (S // 2)):
+        to = torch.full((T + 4, hq, dim), 5.0, dtype=torch.float16, device="cuda")
+        k = torch.zeros(T, 1, dim, dtype=torch.float16, device="cuda")
+        ops.paged_gqa(dev(q[:T]), cache.pool, ints(*starts), ints(*[n] * S), cache.table, out=to[:T])
+        cache.append(k, k, ints(*starts), ints(*[n] * S))
+        ops.paged_read(cache.pool, ints(*starts), ints(*[n] * S), cache.table, T)
+        torch.cuda.synchronize()
+        assert (to[T:] == 5).all()
+
+
+def test_pages_that_no_row_needs(gpu):
+    """Numbers past a sequence's last page may be anything."""
+    rng = np.random.default_rng(8)
+    for rows, past in (([1, 1], [40, 700]), ([50, 3], [20, 300])):
+        cache, kv = filled(rng, rows, past, 2, 128, 32)
+        table = cache.table.cpu().numpy()
+        for s in range(2):
+            table[s, -(-(rows[s] + past[s]) // 32):] = (-1, 2 ** 31 - 1)[s]
+        cache.table = dev(table)
+        q = rows16(rng, sum(rows), 8, 128)
+        invalid = ints(0)
+        starts, lens = ints(0, *np.cumsum(rows)), ints(*past)
+        out = ops.paged_gqa(dev(q), cache.pool, starts, lens, cache.table, invalid=invalid)
+        check(out.cpu().numpy(), q, kv, rows, past, 128 ** -0.5)
+        k = rows16(rng, sum(rows), 2, 128)
+        cache.append(dev(k), dev(k), starts, lens, invalid=invalid)
+        ops.paged_read(cache.pool, starts, lens, cache.table, sum(rows), invalid)
+        assert invalid.item() == 0
+
+
+@pytest.mark.parametrize("rows, past, dim", [(1, 3000, 256), (1, 90, 64), (40, 2000, 256),
+                                             (40, 900, 128), (12, 700, 64)])
+def test_a_page_outside_the_pool_in_the_middle(gpu, rows, past, dim):
+    """Only the rows that see it are NaN, whichever workgroup meets it."""
+    rng = np.random.default_rng(9)
+    both = [rows, rows]
+    cache, kv = filled(rng, both, [past, past], 1, dim, 32)
+    at = 2 if past < 100 else 20
+    cache.table[0, at] = cache.pool.shape[0] + 5
+    q = rows16(rng, 2 * rows, 4, dim)
+    invalid = ints(0)
+    out = ops.paged_gqa(dev(q), cache.pool, ints(0, rows, 2 * rows), ints(past, past), cache.table,
+                        invalid=invalid).cpu().numpy()
+    assert invalid.item() == _lib.PAGED_PLACE
+    assert np.isnan(out[:rows]).all()
+    check(out[rows:], q[rows:], [x[1:] for x in kv], [rows], [past], dim ** -0.5)
 
 
 # ------------------------------------------------------------------ attention
@@ -287,6 +346,16 @@ GQA = [  # rows of each sequence, past of each, Hq, Hkv, dim, page
     ([70, 33], [5, 260], 6, 2, 64, 64),
     ([50], [2], 16, 1, 256, 32),
     ([150], [100], 8, 1, 128, 32),
+    ([1, 1], [9000, 4000], 2, 2, 64, 256),              # eight waves, many pieces
+    ([1] * 40, [(411 * s) % 3000 for s in range(40)], 4, 4, 128, 64),  # four waves
+    ([6, 2], [2100, 3333], 8, 2, 256, 64),              # two column groups, divided
+    ([12], [4100], 4, 1, 128, 32),                      # four
+    ([9, 20, 1], [1500, 0, 900], 12, 3, 64, 128),
+    ([40], [5000], 4, 1, 256, 64),                      # tiles, divided
+    ([70], [2500], 4, 1, 128, 96),
+    ([40, 90, 3], [700, 64, 1500], 8, 2, 256, 32),      # tiles, longest first
+    ([64], [64], 2, 1, 256, 32),                        # whole units and blocks
+    ([33, 65], [31, 63], 4, 1, 128, 32),
 ]
 
 
@@ -493,6 +562,38 @@ def test_captured_on_new_lengths(gpu):
         torch.cuda.synchronize()
         assert torch.equal(turned, a) and torch.equal(out, b) and not b.isnan().any()
         assert torch.equal(caches[0].pool, caches[1].pool)
+
+
+def test_two_graphs_at_once(gpu):
+    """Graphs captured on one stream and replayed on two at the same time: each
+    has a workspace of its own."""
+    rng = np.random.default_rng(24)
+    made, alone, graphs = [], [], []
+    side = torch.cuda.Stream()
+    for n in (5000, 3500):
+        cache, _ = filled(rng, [1], [n], 4, 128, 64)
+        call = (dev(rows16(rng, 1, 16, 128)), cache, ints(0, 1), ints(n))
+        q, c, s, p = call
+        alone.append(ops.paged_gqa(q, c.pool, s, p, c.table))
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            ops.paged_gqa(q, c.pool, s, p, c.table, out=out)
+        made.append((call, out))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for _, out in made:
+            out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(8):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), want in zip(made, alone):
+            assert torch.equal(out, want)
 
 
 def test_two_streams_at_once(gpu):

@@ -1023,6 +1023,8 @@ int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, float *factor) 
     return fail(LLMI_HIP_INVALID_ARGUMENT, "ropeFrequencies: null buffer");
   if (p.rotaryDim % 2)
     return fail(LLMI_HIP_INVALID_ARGUMENT, "ropeFrequencies: rotary width %u is odd", p.rotaryDim);
+  if (!rope_rows_supported(p.rotaryDim))
+    return fail(LLMI_HIP_UNSUPPORTED, "ropeFrequencies: rotary width %u", p.rotaryDim);
   if (p.scaling > LLMI_ROPE_SCALING_BANDS)
     return fail(LLMI_HIP_INVALID_ARGUMENT, "ropeFrequencies: unknown scaling %u", p.scaling);
   const bool ramp = p.scaling == LLMI_ROPE_SCALING_YARN || p.scaling == LLMI_ROPE_SCALING_BANDS;
@@ -1108,6 +1110,8 @@ int llmi_hip_paged_read(const void *pool, const int32_t *starts, const int32_t *
 }
 
 static int check_paged_heads(const PagedGqaParams &p) {
+  if (p.kv.headDim != 64 && p.kv.headDim != 128 && p.kv.headDim != 256)
+    return fail(LLMI_HIP_UNSUPPORTED, "pagedGqa: head_dim %u (64, 128 or 256)", p.kv.headDim);
   if (p.queryHeads == 0 || p.kv.kvHeads == 0 || p.queryHeads % p.kv.kvHeads ||
       p.queryHeads > 65535u)
     return fail(LLMI_HIP_INVALID_ARGUMENT,

@@ -472,7 +472,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
     const unsigned pieces = split.pieces(s), h = local % queryHeads, row = local / queryHeads;
     const unsigned column = row * G + h % G, kvh = h / G;
     const unsigned first = pieceBefore + (split.units(s) - 1 - column / unit) * pieces;
-    if (first + pieces > most) // starts out of order: more pieces than the rows can have
+    if (first >= most || pieces > most - first) // starts out of order: more pieces than the rows can have
       return;
     const size_t at = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
     const size_t step = (size_t)g.kvHeads * unit;

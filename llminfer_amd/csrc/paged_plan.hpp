@@ -84,8 +84,9 @@ __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq 
   p = pair32(all);
   all = p.a + p.b;
   all = all < 16777216.0f ? all : all * 1.0001f;
-  const unsigned least = (unsigned)ceilf(all / (float)plan.target);
-  const unsigned one = (unsigned)ceilf(all / (float)plan.fill); // of a single round
+  // (below 2^30: no table has more blocks)
+  const unsigned least = (unsigned)fminf(ceilf(all / (float)plan.target), 0x1p30f);
+  const unsigned one = (unsigned)fminf(ceilf(all / (float)plan.fill), 0x1p30f); // of a single round
   const unsigned chunk = max(least, min(one, plan.whole));
   const unsigned steps = (chunk + s.step - 1) & ~(s.step - 1);
   s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(steps ? steps : s.step));

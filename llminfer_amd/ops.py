@@ -978,6 +978,8 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e7, scaling: str | None = 
     "ntk", "yarn" or "bands" (yarn's frequencies without its factor)."""
     if scaling not in _SCALINGS:
         raise ValueError(f"scaling is one of {sorted(map(str, _SCALINGS))}")
+    if rotary_dim < 0:
+        raise ValueError("rotary_dim must not be negative")
     out = (C.c_float * max(rotary_dim // 2, 1))()
     factor = C.c_float()
     _lib.check(_lib.load().llmi_hip_rope_frequencies(
@@ -1153,7 +1155,7 @@ def bind_paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, pa
     defaults to 1 / sqrt(dim); out must not overlap q. Rows of no sequence are
     left as they are; a row that would read a page outside the pool, or does
     not fit its table, is NaN and sets bit 1 of invalid. The workspace is the
-    stream's; under capture it is the graph's own."""
+    call's own: calls and graphs may run at once on streams of their own."""
     for t, n in ((q, "q"), (out, "out")):
         _require(t, torch.float16, n)
     if q.dim() != 3 or out.shape != q.shape:
@@ -1167,11 +1169,9 @@ def bind_paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, pa
                             float(np.float32(1.0) / np.sqrt(np.float32(q.shape[2])))
                             if scale is None else scale)
     need = lib.llmi_hip_paged_gqa_workspace_bytes(p)
-    if need and torch.cuda.is_current_stream_capturing():
-        # a graph's own, from its pool: replays of two graphs may overlap
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    else:
-        ws = workspace(need, q.device, "paged") if need else None
+    # Not the stream's: two calls bound on one stream may be captured into
+    # graphs whose replays overlap.
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     b = Bound(lib.llmi_hip_paged_gqa,
               (_ptr(q), _ptr(starts), _ptr(past), _ptr(table), _ptr(pool), _ptr(out),
                _ptr(invalid), p, _ptr(ws), ws.numel() if ws is not None else 0, _stream()),

@@ -147,6 +147,14 @@ def test_read_and_gqa_refusals():
     assert lib.llmi_hip_paged_gqa_workspace_bytes(_lib.PagedGqaParams(kv_params(), 3, 1.0)) == 0
 
 
+@pytest.mark.parametrize("dim", [0, 32, 96, 512, 1024, 1 << 31])
+def test_plan_of_a_width_without_a_kernel(dim):
+    """The calls that plan without buffers refuse what the launch refuses."""
+    gqa = _lib.PagedGqaParams(kv_params(headDim=dim, tokens=500), 4, 1.0)
+    assert _lib.load().llmi_hip_paged_gqa_workspace_bytes(gqa) == 0
+    assert ops.kernel_names(_lib.OP_PAGED_GQA, gqa) == []
+
+
 def test_plan_names():
     assert ops.kernel_names(_lib.OP_ROPE, rope_params()) == ["ropeRows"]
     assert ops.kernel_names(_lib.OP_ROPE, rope_params(tokens=0)) == []
@@ -173,10 +181,10 @@ def test_frequencies(rotary, scaling, scale):
 
 
 def test_frequency_refusals():
-    for kwargs in (dict(scaling="twice"), ):
+    for rotary, kwargs in ((64, dict(scaling="twice")), (-2, {})):
         with pytest.raises(ValueError):
-            ops.rope_frequencies(64, device="cpu", **kwargs)
-    for args, kwargs in (((63,), {}), ((64, 0.0), {}), ((64, 1e4, "linear", 0.0), {}),
+            ops.rope_frequencies(rotary, device="cpu", **kwargs)
+    for args, kwargs in (((63,), {}), ((2050,), {}), ((64, 0.0), {}), ((64, 1e4, "linear", 0.0), {}),
                          ((64, 1e4, "yarn", 2.0, 0.0), {}),
                          ((64, 1e4, "bands", 2.0, 1024.0, 4.0, 4.0), {})):
         with pytest.raises(_lib.HipError):

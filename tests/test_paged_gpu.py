@@ -538,7 +538,7 @@ def test_captured_on_new_lengths(gpu):
 
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        step(caches[0], turned, out)  # the workspace of this stream
+        step(caches[0], turned, out)  # loads the kernels
     side.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):
@@ -582,6 +582,39 @@ def test_two_graphs_at_once(gpu):
             ops.paged_gqa(q, c.pool, s, p, c.table, out=out)
         made.append((call, out))
         graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for _, out in made:
+            out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(8):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), want in zip(made, alone):
+            assert torch.equal(out, want)
+
+
+def test_bound_calls_in_two_graphs(gpu):
+    """Calls bound one after the other on one stream, then captured each into a
+    graph: replayed at the same time they do not meet."""
+    rng = np.random.default_rng(25)
+    side = torch.cuda.Stream()
+    made, alone = [], []
+    for n in (4100, 2700):
+        cache, _ = filled(rng, [1], [n], 4, 128, 64)
+        q, starts, past = dev(rows16(rng, 1, 16, 128)), ints(0, 1), ints(n)
+        alone.append(ops.paged_gqa(q, cache.pool, starts, past, cache.table))
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            made.append((ops.bind_paged_gqa(q, cache.pool, starts, past, cache.table, out), out))
+    graphs = []
+    for bound, _ in made:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            bound()
     streams = [torch.cuda.Stream() for _ in graphs]
     for _ in range(5):
         for _, out in made:

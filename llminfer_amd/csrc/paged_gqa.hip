@@ -25,6 +25,7 @@
 #include "paged_plan.hpp"
 
 #include <math.h>
+#include <type_traits>
 
 namespace llmi {
 namespace {
@@ -480,17 +481,40 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
     const vec *po = reinterpret_cast<const vec *>(parts.o + at * D) + lane;
     float m = -INFINITY, l = 0.0f;
     vec y = 0.0f;
-#pragma unroll 8
-    for (unsigned i = wave % W; i < pieces; i += W) {
-      const float2 x = ml[step * i];
-      const vec o = po[step * i * 64];
-      const float to = fmaxf(m, x.x);
+    // `count` of this wave's pieces at a time, all of them in flight at once
+    auto take = [&](auto count, unsigned i0) {
+      constexpr unsigned kCount = decltype(count)::value;
+      float2 x[kCount];
+      vec o[kCount];
+#pragma unroll
+      for (unsigned n = 0; n < kCount; ++n) {
+        const unsigned i = min(i0 + W * n, pieces - 1);
+        x[n] = ml[step * i];
+        o[n] = po[step * i * 64];
+      }
+      float to = m;
+#pragma unroll
+      for (unsigned n = 0; n < kCount; ++n) {
+        x[n].x = i0 + W * n < pieces ? x[n].x : -INFINITY;
+        to = fmaxf(to, x[n].x);
+      }
       const float a = m == -INFINITY ? 0.0f : fast_exp2(m - to);
-      const float b = x.x == -INFINITY ? 0.0f : fast_exp2(x.x - to);
-      l = l * a + x.y * b;
-      y = y * a + o * b;
+      l *= a;
+      y *= a;
+#pragma unroll
+      for (unsigned n = 0; n < kCount; ++n)
+        if (x[n].x != -INFINITY) {
+          const float b = fast_exp2(x[n].x - to);
+          l += x[n].y * b;
+          y += o[n] * b;
+        }
       m = to;
-    }
+    };
+    unsigned i = wave % W;
+    for (; i + 4 * W < pieces; i += 8 * W)
+      take(std::integral_constant<unsigned, 8>(), i);
+    if (i < pieces)
+      take(std::integral_constant<unsigned, 4>(), i);
     if (W > 1) {
       sM[wave] = m;
       sL[wave] = l;

@@ -109,6 +109,14 @@ template <int D, int CG, int W, int I> __device__ __forceinline__ char *ring_buf
   return buffer;
 }
 
+// x, with y of the lanes Ctrl moves it from in the lanes of the banks.
+constexpr int kRowShr4 = 0x114, kRowShr8 = 0x118, kRowShr12 = 0x11C;
+template <int Ctrl, int Banks> __device__ __forceinline__ float shifted_in(float x, float y) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, x),
+                                                               __builtin_bit_cast(int, y), Ctrl,
+                                                               0xF, Banks, false));
+}
+
 template <int D, int CG, int W>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W),
                           amdgpu_waves_per_eu(Geo<D, CG, W>::RESIDENT)))
@@ -136,11 +144,14 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   const unsigned c0 = unit * kUnit, columns = min(kUnit, s.rows * G - c0);
   unsigned visible[CG]; // a column's last key
   size_t row[CG];
+  auto token_of = [&](unsigned col) { return min((c0 + col) / G, s.rows - 1); };
+  auto row_of = [&](unsigned col) {
+    return ((size_t)(s.row0 + token_of(col)) * queryHeads + kvh * G + (c0 + col) % G) * D;
+  };
 #pragma unroll
   for (int j = 0; j < CG; ++j) {
-    const unsigned col = c0 + kColumns * j + r, token = min(col / G, s.rows - 1);
-    visible[j] = s.past + token;
-    row[j] = ((size_t)(s.row0 + token) * queryHeads + kvh * G + col % G) * D;
+    visible[j] = s.past + token_of(kColumns * j + r);
+    row[j] = row_of(kColumns * j + r);
   }
   auto live = [&](int j) { return kColumns * j + r < columns; };
   if (!s.ok) { // no place for this sequence
@@ -392,15 +403,29 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       sL[wave * kUnit + kColumns * j + r] = lost ? NAN : p.a + p.b;
     }
   }
+  // Up to 16 / F columns of a group, a token's heads, are in every F-th four
+  // lanes: F tiles go side by side, lane r with column r % (16 / F) of tile
+  // F i + r / (16 / F) (a token's four heads on 4097 keys: 8.6 us, 9.7 with F 1).
+  auto join = [&](auto factor, const int j) {
+    constexpr unsigned F = decltype(factor)::value, kCols = kColumns / F;
+    constexpr unsigned kTiles = Geom::TILES / F;
 #pragma unroll
-  for (int j = 0; j < CG; ++j) {
-    if (j)
-      __syncthreads(); // the group before is done with
+    for (unsigned i = 0; i < kTiles; ++i) {
+      float4_t y = o[j][F * i];
 #pragma unroll
-    for (int i = 0; i < Geom::TILES; ++i)
-      out_of(wave)[i * 64 + lane] = o[j][i];
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (F == 2)
+          y[e] = shifted_in<kRowShr8, 0xC>(y[e], o[j][2 * i + 1][e]);
+        if constexpr (F == 4) {
+          y[e] = shifted_in<kRowShr4, 2>(y[e], o[j][4 * i + 1][e]);
+          y[e] = shifted_in<kRowShr8, 4>(y[e], o[j][4 * i + 2][e]);
+          y[e] = shifted_in<kRowShr12, 8>(y[e], o[j][4 * i + 3][e]);
+        }
+      }
+      out_of(wave)[i * 64 + lane] = y;
+    }
     __syncthreads();
-    const unsigned col = kColumns * j + r;
+    const unsigned at = r % kCols, col = kColumns * j + at;
     float top = sM[col], sum = 0.0f, a[kWaves];
 #pragma unroll
     for (unsigned w = 1; w < kWaves; ++w)
@@ -413,22 +438,36 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     }
     const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * kUnit + col;
     const float scale = pieces == 1 ? 1.0f / sum : 1.0f;
-    for (unsigned i = wave; i < (unsigned)Geom::TILES; i += kWaves) {
+    const size_t to = F == 1 ? row[j] : row_of(col);
+    for (unsigned i = wave; i < kTiles; i += kWaves) {
       float4_t y{0, 0, 0, 0};
 #pragma unroll
       for (unsigned w = 0; w < kWaves; ++w)
         y += out_of(w)[i * 64 + lane] * a[w];
-      if (!live(j))
+      if (col >= columns)
         continue;
+      const unsigned channel = 16 * (F * i + r / kCols) + 4 * quad;
       if (pieces == 1)
-        *reinterpret_cast<half4_t *>(out + row[j] + 16 * i + 4 * quad) =
+        *reinterpret_cast<half4_t *>(out + to + channel) =
             half4_t{(half_t)(y[0] * scale), (half_t)(y[1] * scale), (half_t)(y[2] * scale),
                     (half_t)(y[3] * scale)};
       else
-        *reinterpret_cast<float4_t *>(parts.o + part * D + 16 * i + 4 * quad) = y;
+        *reinterpret_cast<float4_t *>(parts.o + part * D + channel) = y;
     }
-    if (pieces > 1 && wave == 0 && quad == 0 && live(j))
+    if (pieces > 1 && wave == 0 && lane < kCols && col < columns)
       *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
+  };
+  if constexpr (CG == 1) {
+    if (columns <= 4)
+      return join(std::integral_constant<unsigned, 4>(), 0);
+    if (columns <= 8)
+      return join(std::integral_constant<unsigned, 2>(), 0);
+  }
+#pragma unroll
+  for (int j = 0; j < CG; ++j) {
+    if (j)
+      __syncthreads(); // the group before is done with
+    join(std::integral_constant<unsigned, 1>(), j);
   }
 }
 

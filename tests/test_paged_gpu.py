@@ -356,6 +356,13 @@ GQA = [  # rows of each sequence, past of each, Hq, Hkv, dim, page
     ([40, 90, 3], [700, 64, 1500], 8, 2, 256, 32),      # tiles, longest first
     ([64], [64], 2, 1, 256, 32),                        # whole units and blocks
     ([33, 65], [31, 63], 4, 1, 128, 32),
+    ([1], [2000], 3, 1, 64, 32),                        # a token's heads: 1 to 4,
+    ([2], [1500], 4, 2, 128, 32),
+    ([1], [40], 7, 1, 64, 32),                          # 5 to 8,
+    ([1, 1], [900, 33], 14, 2, 256, 32),
+    ([1], [3000], 8, 1, 128, 64),
+    ([1], [2500], 8, 1, 64, 64),
+    ([1], [70], 9, 1, 128, 32),                         # 9 to 16
 ]
 
 

@@ -49,28 +49,40 @@ uint64_t most_units(const PagedKvParams &p, unsigned group, unsigned columns) {
 uint64_t most_pieces(const PagedKvParams &p, unsigned group, const SplitPlan &plan) {
   return plan.target + 1 + most_units(p, group, 1u << plan.shift);
 }
-// Columns of a unit, by those that a sequence has on average: groups of 16 of
-// this file's kernel, or the units of paged_tiles.hip. Pieces: as many as
-// there are CUs (twice that at head_dim 64, where two workgroups share one);
-// up to six times as many where single tokens have units enough that their
-// different lengths count for more than the joining.
+// Units by the columns that a sequence has on average: 16 columns divide into
+// most pieces and join least (one sequence, 4 KV heads of 256, 8000 keys, 32
+// columns: 16.7 us, 19.8 with units of 32), more decode a key less often (64
+// columns on 16000 keys of 8 heads: 31 us, 48 with 16); the units of
+// paged_tiles.hip, decoded once, from 160 columns (192 on 31000 keys: 54 us, 84
+// with 32; 128 on 8000: 35 and 26), or 384 at head_dim 128 (768 on 16000: 101
+// and 131; 256 on 8000: 37 and 25), and from fewer in calls of many columns,
+// which they fill the device with (24 sequences of 75 columns on average on
+// 3000 keys: 48 us, 68). At head_dim 64, 16 columns up to 95 (64 on 8000 keys:
+// 13.1 us, 15.4 with 64), 64 from there (128 on 31000: 23 us, 29).
+// Pieces: as many as there are CUs (twice that at head_dim 64, where two
+// workgroups share one); where single tokens have units enough that their
+// different lengths count for more than the joining, up to six times as many,
+// of 16 blocks at least (48 chats of up to 16385 keys: 125 us, 142 in one
+// round; 12 chats of 8000: 25.7 us, 29.6 with at least 64 blocks).
 struct GqaPlan {
   SplitPlan split;
   bool pooled; // eight pieces a unit or more, if the lengths give them
 };
 GqaPlan plan_for(const PagedKvParams &p, unsigned group) {
-  const uint64_t columns = (uint64_t)p.tokens * group / p.sequences;
-  const bool tiles = p.headDim >= 128 && columns >= 128;
-  const unsigned unit = tiles                                 ? paged_tiles_columns(p.headDim)
-                        : columns <= 16                       ? 16
-                        : columns <= 32 || p.headDim == 256 ? 32
-                                                              : 64;
+  const uint64_t all = (uint64_t)p.tokens * group, columns = all / p.sequences;
+  const bool wide = p.headDim == 256, many = all * p.kvHeads >= (wide ? 2048u : 8192u);
+  const bool tiles = p.headDim >= 128 && (columns >= (wide ? 160u : 384u) ||
+                                          (many && columns >= (wide ? 48u : 96u)));
+  const unsigned unit = tiles             ? paged_tiles_columns(p.headDim)
+                        : p.headDim == 64 ? (columns < 96 ? 16 : 64)
+                                          : (columns <= 32 ? 16 : 32);
   const unsigned cus = (kCus + p.kvHeads - 1) / p.kvHeads;
   const bool pooled = cus >= 8 * most_units(p, group, unit);
   const unsigned fill = unit == 16 && p.headDim == 64 ? 2 * cus : cus;
   const unsigned step = tiles ? 512 / p.headDim : unit == 16 && pooled ? 8 : 4;
-  return {{(unsigned)__builtin_ctz(unit), step, fill,
-           unit == 16 && !pooled ? 6 * cus : fill, 64u, tiles},
+  const bool rounds = unit == 16 && !pooled;
+  return {{(unsigned)__builtin_ctz(unit), step, fill, rounds ? 6 * cus : fill,
+           columns <= 16 ? 16u : 64u, tiles, unit > 16 || pooled},
           pooled};
 }
 // Whether some lengths that fit the table divide a unit's keys.
@@ -82,9 +94,9 @@ bool may_divide(const PagedKvParams &p, const SplitPlan &plan) {
 
 // W: waves of a workgroup. Eight where units have many pieces: the more of the
 // keys that meet in one workgroup, the fewer partials there are to join (one
-// token on 32749 keys: 23.1 us with four, two workgroups a CU, 20.4 with
-// eight); four otherwise, two workgroups a CU for single tokens, whose
-// starts and ends then overlap (48 ragged chats: 122 us, 136 with eight).
+// token on 32750 keys: 18.1 us, 21.5 with four, two workgroups a CU); four
+// otherwise, two workgroups a CU for single tokens, whose starts and ends then
+// overlap (16 chats of 8000 keys: 33.7 us, 39.6 with eight).
 template <int D, int CG, int W> struct Geo {
   static constexpr int BLOCK = 40 * D;               // bytes of a block
   static constexpr int LOADS = (BLOCK + 1023) / 1024; // 1-KB loads of one
@@ -626,21 +638,21 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
                        stream, from, pages, g, to, invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };
-  auto by_columns = [&](auto one, auto pooled, auto two, auto four) {
-    return unit == 16 ? attend(both.pooled ? pooled : one) : attend(unit == 32 ? two : four);
+  auto by_columns = [&](auto one, auto pooled, auto more) {
+    return attend(unit > 16 ? more : both.pooled ? pooled : one);
   };
   hipError_t e;
   if (unit > 64)
     e = launch_paged_tiles(from, pages, g, to, invalid, queryHeads, plan, c, parts, pieces, stream);
   else if (p.headDim == 256)
     e = by_columns(paged_gqa_kernel<256, 1, 4>, paged_gqa_kernel<256, 1, 8>,
-                   paged_gqa_kernel<256, 2, 4>, paged_gqa_kernel<256, 2, 4>);
+                   paged_gqa_kernel<256, 2, 4>);
   else if (p.headDim == 128)
     e = by_columns(paged_gqa_kernel<128, 1, 4>, paged_gqa_kernel<128, 1, 8>,
-                   paged_gqa_kernel<128, 2, 4>, paged_gqa_kernel<128, 4, 4>);
+                   paged_gqa_kernel<128, 2, 4>);
   else
     e = by_columns(paged_gqa_kernel<64, 1, 4>, paged_gqa_kernel<64, 1, 8>,
-                   paged_gqa_kernel<64, 2, 4>, paged_gqa_kernel<64, 4, 4>);
+                   paged_gqa_kernel<64, 4, 4>);
   if (e != hipSuccess)
     return e;
   if (!may_divide(p, plan))

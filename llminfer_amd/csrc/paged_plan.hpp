@@ -60,9 +60,10 @@ struct Split {
 // How the host asks for it: `fill` pieces a KV head fill the device, and at
 // most `target`, some rounds of that, are made where pieces then still have
 // `whole` blocks. step (a power of two): the blocks that a workgroup takes at
-// a time.
+// a time. alone: workgroups have a CU each, so that pieces past
+// `fill` would wait for the others.
 struct SplitPlan {
-  unsigned shift, step, fill, target, whole, nearest;
+  unsigned shift, step, fill, target, whole, nearest, alone;
 };
 
 // The chunk, whole steps, for which the call has at most plan.target pieces
@@ -87,10 +88,30 @@ __device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq 
   // (below 2^30: no table has more blocks)
   const unsigned least = (unsigned)fminf(ceilf(all / (float)plan.target), 0x1p30f);
   const unsigned one = (unsigned)fminf(ceilf(all / (float)plan.fill), 0x1p30f); // of a single round
-  const unsigned chunk = max(least, min(one, plan.whole));
-  const unsigned steps = (chunk + s.step - 1) & ~(s.step - 1);
-  s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(steps ? steps : s.step));
-  s.inv = __builtin_amdgcn_rcpf((float)s.chunk);
+  auto take = [&](unsigned chunk) {
+    const unsigned steps = (chunk + s.step - 1) & ~(s.step - 1);
+    s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(steps ? steps : s.step));
+    s.inv = __builtin_amdgcn_rcpf((float)s.chunk);
+  };
+  take(max(least, min(one, plan.whole)));
+  // Every unit's last piece is rounded up, and a few pieces more than fill the
+  // device would be a second round: longer ones, where one round can be (160
+  // columns on 31000 keys at head_dim 128, units of 32: 36 us, 52 without).
+  if (plan.alone && g.sequences <= 64) {
+    auto total = [&](unsigned x) {
+      return g.sequences == 1 ? (unsigned)__builtin_amdgcn_readfirstlane((int)x)
+                              : (unsigned)__builtin_amdgcn_readlane((int)wave_scan(x), 63);
+    };
+    const unsigned units = s.units(own);
+    if (total(units) <= plan.fill)
+      for (int i = 0; i < 4; ++i) {
+        const unsigned n = total(units * s.pieces(own));
+        if (n <= plan.fill)
+          break;
+        take(max(s.chunk + 1, (unsigned)fminf((float)s.chunk * (float)n / (float)plan.fill,
+                                              0x1p30f)));
+      }
+  }
   return s;
 }
 

@@ -8,7 +8,7 @@ namespace llmi {
 namespace {
 
 constexpr unsigned kThreads = 256;
-constexpr unsigned kTurns = 1024; // cos/sin pairs that a workgroup keeps
+constexpr unsigned kTurns = 1024; // cos/sin pairs that a token may have
 
 struct RopeRows {
   unsigned heads, dim, half, layout;
@@ -25,80 +25,78 @@ template <bool VEC> struct Parts {
       : turned(VEC ? half / 8 : half), all(turned + (dim - 2 * half) / (VEC ? 8 : 1)) {}
 };
 
-// A workgroup takes `block` tokens and the heads of blockIdx.y: their cosines
-// and sines once, into LDS, then the rows of all its heads, `across` threads
-// to a row. A thread owns whole pairs, so a row may be rotated in place.
+// A workgroup takes a token and the heads of blockIdx.y: its cosines and sines
+// once, into LDS, then the rows of all its heads, `across` threads to a row. A
+// thread owns whole pairs, so a row may be rotated in place.
 // Bound by the rows' bytes: 16381 tokens of 16 heads of 256, 64 rotated, pass
-// in ROPE_16K, a copy of as many bytes in 56 us.
+// in 55 us, a copy of as many bytes in 56; 2048 tokens of 16 heads of 128 in 5.0
+// (5.9 with four tokens a workgroup).
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
     const uint16_t *in, const int *__restrict__ positions, const float *__restrict__ freqs,
-    uint16_t *out, unsigned tokens, unsigned block, unsigned headBlock, unsigned across,
-    RopeRows p) {
+    uint16_t *out, unsigned headBlock, unsigned across, RopeRows p) {
   __shared__ float2 sTurn[kTurns];
-  const unsigned t0 = blockIdx.x * block, count = min(block, tokens - t0);
+  const unsigned t = blockIdx.x;
   const unsigned h0 = blockIdx.y * headBlock, h1 = min(h0 + headBlock, p.heads);
-  for (unsigned i = threadIdx.x; i < count * p.half; i += kThreads) {
-    const unsigned t = i / p.half;
-    sTurn[i] = rope_turn(positions[t0 + t], freqs[i - t * p.half], p.factor);
-  }
+  const int position = p.half ? positions[t] : 0;
+  for (unsigned i = threadIdx.x; i < p.half; i += kThreads)
+    sTurn[i] = rope_turn(position, freqs[i], p.factor);
   __syncthreads();
   const Parts<VEC> parts(p.half, p.dim);
   const unsigned down = kThreads / across, y = threadIdx.x / across;
   if (y >= down)
     return;
   for (unsigned part = threadIdx.x % across; part < parts.all; part += across)
-    for (unsigned t = 0; t < count; ++t)
-      for (unsigned h = h0 + y; h < h1; h += down) {
-        const uint16_t *x = in + (size_t)(t0 + t) * p.inToken + (size_t)h * p.inHead;
-        uint16_t *z = out + (size_t)(t0 + t) * p.outToken + (size_t)h * p.outHead;
-        if constexpr (VEC) {
-          if (part >= parts.turned) {
-            const unsigned c = 2 * p.half + 8 * (part - parts.turned);
-            *reinterpret_cast<uint4_t *>(z + c) = *reinterpret_cast<const uint4_t *>(x + c);
-            continue;
-          }
-          const unsigned a = p.layout ? 16 * part : 8 * part, b = p.layout ? a + 8 : a + p.half;
-          const uint4_t u = *reinterpret_cast<const uint4_t *>(x + a);
-          const uint4_t v = *reinterpret_cast<const uint4_t *>(x + b);
-          uint16_t e[16], f[16];
-          *reinterpret_cast<uint4_t *>(e) = u;
-          *reinterpret_cast<uint4_t *>(e + 8) = v;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 cs = sTurn[t * p.half + 8 * part + i];
-            const float s = h2f(p.layout ? e[2 * i] : e[i]);
-            const float w = h2f(p.layout ? e[2 * i + 1] : e[8 + i]);
-            const uint16_t s1 = turn_x(s, w, cs), w1 = turn_y(s, w, cs);
-            f[i] = s1; // the turned pairs apart; put side by side below
-            f[8 + i] = w1;
-          }
-          uint4_t lo, hi;
-          if (p.layout) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              lo[i] = f[i] | (uint32_t)f[8 + i] << 16;
-              hi[i] = f[4 + i] | (uint32_t)f[12 + i] << 16;
-            }
-          } else {
-            lo = *reinterpret_cast<uint4_t *>(f);
-            hi = *reinterpret_cast<uint4_t *>(f + 8);
-          }
-          *reinterpret_cast<uint4_t *>(z + a) = lo;
-          *reinterpret_cast<uint4_t *>(z + b) = hi;
-        } else {
-          if (part >= parts.turned) {
-            const unsigned c = p.half + part;
-            z[c] = x[c];
-            continue;
-          }
-          const unsigned a = p.layout ? 2 * part : part, b = p.layout ? a + 1 : a + p.half;
-          const float2 cs = sTurn[t * p.half + part];
-          const float s = h2f(x[a]), w = h2f(x[b]);
-          z[a] = turn_x(s, w, cs);
-          z[b] = turn_y(s, w, cs);
+    for (unsigned h = h0 + y; h < h1; h += down) {
+      const uint16_t *x = in + (size_t)t * p.inToken + (size_t)h * p.inHead;
+      uint16_t *z = out + (size_t)t * p.outToken + (size_t)h * p.outHead;
+      if constexpr (VEC) {
+        if (part >= parts.turned) {
+          const unsigned c = 2 * p.half + 8 * (part - parts.turned);
+          *reinterpret_cast<uint4_t *>(z + c) = *reinterpret_cast<const uint4_t *>(x + c);
+          continue;
         }
+        const unsigned a = p.layout ? 16 * part : 8 * part, b = p.layout ? a + 8 : a + p.half;
+        const uint4_t u = *reinterpret_cast<const uint4_t *>(x + a);
+        const uint4_t v = *reinterpret_cast<const uint4_t *>(x + b);
+        uint16_t e[16], f[16];
+        *reinterpret_cast<uint4_t *>(e) = u;
+        *reinterpret_cast<uint4_t *>(e + 8) = v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 cs = sTurn[8 * part + i];
+          const float s = h2f(p.layout ? e[2 * i] : e[i]);
+          const float w = h2f(p.layout ? e[2 * i + 1] : e[8 + i]);
+          const uint16_t s1 = turn_x(s, w, cs), w1 = turn_y(s, w, cs);
+          f[i] = s1; // the turned pairs apart; put side by side below
+          f[8 + i] = w1;
+        }
+        uint4_t lo, hi;
+        if (p.layout) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            lo[i] = f[i] | (uint32_t)f[8 + i] << 16;
+            hi[i] = f[4 + i] | (uint32_t)f[12 + i] << 16;
+          }
+        } else {
+          lo = *reinterpret_cast<uint4_t *>(f);
+          hi = *reinterpret_cast<uint4_t *>(f + 8);
+        }
+        *reinterpret_cast<uint4_t *>(z + a) = lo;
+        *reinterpret_cast<uint4_t *>(z + b) = hi;
+      } else {
+        if (part >= parts.turned) {
+          const unsigned c = p.half + part;
+          z[c] = x[c];
+          continue;
+        }
+        const unsigned a = p.layout ? 2 * part : part, b = p.layout ? a + 1 : a + p.half;
+        const float2 cs = sTurn[part];
+        const float s = h2f(x[a]), w = h2f(x[b]);
+        z[a] = turn_x(s, w, cs);
+        z[b] = turn_y(s, w, cs);
       }
+    }
 }
 
 } // namespace
@@ -108,14 +106,9 @@ bool rope_rows_supported(unsigned rotaryDim) { return rotaryDim / 2 <= kTurns; }
 hipError_t launch_rope_rows(const uint16_t *input, const int32_t *positions, const float *freqs,
                             uint16_t *output, const RopeRowsParams &p, hipStream_t stream) {
   const unsigned half = p.rotaryDim / 2;
-  // four tokens a workgroup, fewer where a call has few or the turns no room
-  unsigned block = p.tokens >= 1024 ? 4 : 1;
-  if (block * half > kTurns)
-    block = kTurns / half;
   // a call of few tokens: its heads over several workgroups, four at least in each
-  const unsigned blocks = (p.tokens + block - 1) / block;
   unsigned headBlock = p.heads;
-  while (blocks * ((p.heads + headBlock - 1) / headBlock) < 256 && headBlock > 4)
+  while (p.tokens * ((p.heads + headBlock - 1) / headBlock) < 256 && headBlock > 4)
     headBlock = (headBlock + 1) / 2;
   const RopeRows r{p.heads,  p.headDim,          half,
                    p.layout, p.inputTokenStride, p.inputHeadStride,
@@ -124,10 +117,10 @@ hipError_t launch_rope_rows(const uint16_t *input, const int32_t *positions, con
                            p.outputHeadStride;
   const bool vec = half % 8 == 0 && p.headDim % 8 == 0 && strides % 8 == 0 && aligned16(input) &&
                    aligned16(output);
-  const dim3 grid(blocks, (p.heads + headBlock - 1) / headBlock);
+  const dim3 grid(p.tokens, (p.heads + headBlock - 1) / headBlock);
   auto run = [&](auto kernel, unsigned parts) {
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, input, positions, freqs, output,
-                       p.tokens, block, headBlock, parts < kThreads ? parts : kThreads, r);
+                       headBlock, parts < kThreads ? parts : kThreads, r);
     return hipGetLastError();
   };
   return vec ? run(rope_rows_kernel<true>, Parts<true>(half, p.headDim).all)

@@ -16,6 +16,15 @@
 //    words, so the weights go from the score tile into the O^T += V^T P^T
 //    product as they are;
 //  * the softmax reference moves only when a score would pass 2^15 of it.
+// The weights exp2(s - reference) are rounded to fp16, the operand of the
+// matrix product, a half step of each (2^-11 of it; below 2^-14, 2^-25 of the
+// largest possible 2^15); their sum is of the same rounded weights, so that
+// the rounding moves an output only between its values.
+//
+// Bound by memory from many or long sequences on: 48 tokens on up to 16385
+// keys of 4 heads of 256, 577 MB, in 124 us (4.65 TB/s, the rate of a copy). A
+// token on 32750 keys (42 MB) takes 18.7 us in its two launches, on 4097 keys
+// 12.6 us: latencies of the lengths, the table, the first blocks, the joins.
 // Keys are divided over workgroups by a plan that every workgroup makes for
 // itself from the lengths in device memory (a captured call may be replayed on
 // others); pagedGqaMerge joins the rows whose keys were divided.

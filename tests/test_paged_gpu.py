@@ -363,6 +363,12 @@ GQA = [  # rows of each sequence, past of each, Hq, Hkv, dim, page
     ([1], [3000], 8, 1, 128, 64),
     ([1], [2500], 8, 1, 64, 64),
     ([1], [70], 9, 1, 128, 32),                         # 9 to 16
+    ([100], [2500], 4, 1, 128, 96),                     # tiles, divided
+    ([300, 200, 3], [700, 64, 1500], 8, 2, 128, 32),    # longest first
+    ([16] * 10, [(97 * s) % 500 for s in range(10)], 16, 4, 256, 32),  # many columns
+    ([41], [3000], 4, 1, 128, 32),                      # six units on one round
+    ([25], [2000], 4, 1, 64, 64),                       # 64 columns
+    ([9], [3900], 4, 1, 256, 64),                       # 33 to 48
 ]
 
 

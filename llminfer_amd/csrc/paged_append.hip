@@ -129,19 +129,14 @@ __device__ __forceinline__ uint32_t codes_of(const Eight &x, const Group &g) {
   return half[0] | half[1] << 16;
 }
 
-// Eight channels of a key, and those that they are rotated with. VEC: each a
-// 16-byte load.
+// Eight channels of a key, and those that they are rotated with. VEC: rows at
+// 16 bytes, and a word's partners a word.
 struct KeyPart {
   uint16_t own[8], other[8];
 };
 template <bool VEC>
 __device__ __forceinline__ void load_eight(const uint16_t *__restrict__ x, uint16_t (&to)[8]) {
-  if constexpr (VEC)
-    *reinterpret_cast<uint4_t *>(to) = *reinterpret_cast<const uint4_t *>(x);
-  else
-#pragma unroll
-    for (unsigned e = 0; e < 8; ++e)
-      to[e] = x[e];
+  *reinterpret_cast<uint4_t *>(to) = load_word<VEC>(x);
 }
 template <bool VEC>
 __device__ __forceinline__ KeyPart load_key(const uint16_t *__restrict__ x, unsigned word,
@@ -149,14 +144,18 @@ __device__ __forceinline__ KeyPart load_key(const uint16_t *__restrict__ x, unsi
   KeyPart k;
   const unsigned c0 = 8 * word;
   load_eight<VEC>(x + c0, k.own);
-  if constexpr (VEC) {
-    const unsigned far = c0 >= 2 * p.half || p.layout ? c0 : c0 < p.half ? c0 + p.half : c0 - p.half;
+  const unsigned far = c0 >= 2 * p.half || p.layout ? c0 : c0 < p.half ? c0 + p.half : c0 - p.half;
+  if (VEC || far == c0 || c0 + 8 <= p.half || (c0 >= p.half && c0 + 8 <= 2 * p.half)) {
     load_eight<VEC>(x + far, k.other);
-  } else {
+    if (!VEC && p.layout)
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e)
+        k.other[e] = k.own[e ^ 1];
+  } else { // a word of both halves, or of the second and the rest
 #pragma unroll
     for (unsigned e = 0; e < 8; ++e) {
       const unsigned c = c0 + e;
-      k.other[e] = x[c >= 2 * p.half ? c : p.layout ? c ^ 1u : c < p.half ? c + p.half : c - p.half];
+      k.other[e] = x[c >= 2 * p.half ? c : c < p.half ? c + p.half : c - p.half];
     }
   }
   return k;

@@ -16,13 +16,13 @@ struct RopeRows {
   float factor;
 };
 
-// A row in parts: eight pairs a part (VEC: two 16-byte words of the row, side
-// by side where pairs are interleaved), then eight channels a part that are
-// copied; or one pair or channel a part.
-template <bool VEC> struct Parts {
+// A row in parts: eight pairs a part (two 16-byte words of the row, side by
+// side where pairs are interleaved), then eight channels a part that are
+// copied; the last of either may have fewer where the row is not VEC.
+struct Parts {
   unsigned turned, all;
   __host__ __device__ Parts(unsigned half, unsigned dim)
-      : turned(VEC ? half / 8 : half), all(turned + (dim - 2 * half) / (VEC ? 8 : 1)) {}
+      : turned((half + 7) / 8), all(turned + (dim - 2 * half + 7) / 8) {}
 };
 
 // A workgroup takes a token and the heads of blockIdx.y: its cosines and sines
@@ -30,7 +30,8 @@ template <bool VEC> struct Parts {
 // thread owns whole pairs, so a row may be rotated in place.
 // Bound by the rows' bytes: 16381 tokens of 16 heads of 256, 64 rotated, pass
 // in 55 us, a copy of as many bytes in 56; 2048 tokens of 16 heads of 128 in 5.0
-// (5.9 with four tokens a workgroup).
+// (5.9 with four tokens a workgroup). VEC: whole 16-byte words; else words at any
+// element (186 of the 256 rotated: 62 us warm, 77 channel by channel; 192, VEC: 42).
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
     const uint16_t *in, const int *__restrict__ positions, const float *__restrict__ freqs,
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
   for (unsigned i = threadIdx.x; i < p.half; i += kThreads)
     sTurn[i] = rope_turn(position, freqs[i], p.factor);
   __syncthreads();
-  const Parts<VEC> parts(p.half, p.dim);
+  const Parts parts(p.half, p.dim);
   const unsigned down = kThreads / across, y = threadIdx.x / across;
   if (y >= down)
     return;
@@ -50,52 +51,70 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
     for (unsigned h = h0 + y; h < h1; h += down) {
       const uint16_t *x = in + (size_t)t * p.inToken + (size_t)h * p.inHead;
       uint16_t *z = out + (size_t)t * p.outToken + (size_t)h * p.outHead;
-      if constexpr (VEC) {
-        if (part >= parts.turned) {
-          const unsigned c = 2 * p.half + 8 * (part - parts.turned);
-          *reinterpret_cast<uint4_t *>(z + c) = *reinterpret_cast<const uint4_t *>(x + c);
-          continue;
-        }
-        const unsigned a = p.layout ? 16 * part : 8 * part, b = p.layout ? a + 8 : a + p.half;
-        const uint4_t u = *reinterpret_cast<const uint4_t *>(x + a);
-        const uint4_t v = *reinterpret_cast<const uint4_t *>(x + b);
-        uint16_t e[16], f[16];
-        *reinterpret_cast<uint4_t *>(e) = u;
-        *reinterpret_cast<uint4_t *>(e + 8) = v;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 cs = sTurn[8 * part + i];
-          const float s = h2f(p.layout ? e[2 * i] : e[i]);
-          const float w = h2f(p.layout ? e[2 * i + 1] : e[8 + i]);
-          const uint16_t s1 = turn_x(s, w, cs), w1 = turn_y(s, w, cs);
-          f[i] = s1; // the turned pairs apart; put side by side below
-          f[8 + i] = w1;
-        }
-        uint4_t lo, hi;
-        if (p.layout) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            lo[i] = f[i] | (uint32_t)f[8 + i] << 16;
-            hi[i] = f[4 + i] | (uint32_t)f[12 + i] << 16;
+      if (part >= parts.turned) {
+        unsigned c = 2 * p.half + 8 * (part - parts.turned);
+        if (!VEC && c + 8 > p.dim) {
+          if (p.dim - 2 * p.half < 8) {
+            for (; c < p.dim; ++c)
+              z[c] = x[c];
+            continue;
           }
-        } else {
-          lo = *reinterpret_cast<uint4_t *>(f);
-          hi = *reinterpret_cast<uint4_t *>(f + 8);
+          c = p.dim - 8; // some of them by the part before as well
         }
-        *reinterpret_cast<uint4_t *>(z + a) = lo;
-        *reinterpret_cast<uint4_t *>(z + b) = hi;
-      } else {
-        if (part >= parts.turned) {
-          const unsigned c = p.half + part;
-          z[c] = x[c];
+        store_word<VEC>(z + c, load_word<VEC>(x + c));
+        continue;
+      }
+      // (the last part: eight pairs with those before it, which others write)
+      unsigned pair = 8 * part, skip = 0;
+      if (!VEC && pair + 8 > p.half) {
+        if (p.half < 8) {
+          for (; pair < p.half; ++pair) {
+            const unsigned a = p.layout ? 2 * pair : pair, b = p.layout ? a + 1 : a + p.half;
+            const float s = h2f(x[a]), w = h2f(x[b]);
+            z[a] = turn_x(s, w, sTurn[pair]);
+            z[b] = turn_y(s, w, sTurn[pair]);
+          }
           continue;
         }
-        const unsigned a = p.layout ? 2 * part : part, b = p.layout ? a + 1 : a + p.half;
-        const float2 cs = sTurn[part];
-        const float s = h2f(x[a]), w = h2f(x[b]);
-        z[a] = turn_x(s, w, cs);
-        z[b] = turn_y(s, w, cs);
+        skip = pair - (p.half - 8);
+        pair -= skip;
       }
+      const unsigned a = p.layout ? 2 * pair : pair, b = p.layout ? a + 8 : a + p.half;
+      const uint4_t u = load_word<VEC>(x + a), v = load_word<VEC>(x + b);
+      uint16_t e[16], f[16];
+      *reinterpret_cast<uint4_t *>(e) = u;
+      *reinterpret_cast<uint4_t *>(e + 8) = v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 cs = sTurn[pair + i];
+        const float s = h2f(p.layout ? e[2 * i] : e[i]);
+        const float w = h2f(p.layout ? e[2 * i + 1] : e[8 + i]);
+        const uint16_t s1 = turn_x(s, w, cs), w1 = turn_y(s, w, cs);
+        f[i] = s1; // the turned pairs apart; put side by side below
+        f[8 + i] = w1;
+      }
+      if (!VEC && skip) {
+#pragma unroll
+        for (unsigned i = 1; i < 8; ++i)
+          if (i >= skip) {
+            z[p.layout ? a + 2 * i : a + i] = f[i];
+            z[p.layout ? a + 2 * i + 1 : b + i] = f[8 + i];
+          }
+        continue;
+      }
+      uint4_t lo, hi;
+      if (p.layout) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = f[i] | (uint32_t)f[8 + i] << 16;
+          hi[i] = f[4 + i] | (uint32_t)f[12 + i] << 16;
+        }
+      } else {
+        lo = *reinterpret_cast<uint4_t *>(f);
+        hi = *reinterpret_cast<uint4_t *>(f + 8);
+      }
+      store_word<VEC>(z + a, lo);
+      store_word<VEC>(z + b, hi);
     }
 }
 
@@ -118,13 +137,13 @@ hipError_t launch_rope_rows(const uint16_t *input, const int32_t *positions, con
   const bool vec = half % 8 == 0 && p.headDim % 8 == 0 && strides % 8 == 0 && aligned16(input) &&
                    aligned16(output);
   const dim3 grid(p.tokens, (p.heads + headBlock - 1) / headBlock);
-  auto run = [&](auto kernel, unsigned parts) {
+  const unsigned parts = Parts(half, p.headDim).all;
+  auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, input, positions, freqs, output,
                        headBlock, parts < kThreads ? parts : kThreads, r);
     return hipGetLastError();
   };
-  return vec ? run(rope_rows_kernel<true>, Parts<true>(half, p.headDim).all)
-             : run(rope_rows_kernel<false>, Parts<false>(half, p.headDim).all);
+  return run(vec ? rope_rows_kernel<true> : rope_rows_kernel<false>);
 }
 
 } // namespace llmi

@@ -10,6 +10,7 @@
 #pragma once
 
 #include "exact_fp.hpp"
+#include "hip_common.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -48,6 +49,21 @@ __device__ __forceinline__ float2 rope_turn(int pos, float freq, float factor) {
   const double co = quarter == 1 || quarter == 2 ? -cc : cc;
   const double si = quarter >= 2 ? -ss : ss;
   return make_float2((float)(co * (double)factor), (float)(si * (double)factor));
+}
+
+// Sixteen bytes of a row: aligned (VEC) or at any element.
+typedef uint32_t any4_t __attribute__((ext_vector_type(4), aligned(2)));
+template <bool VEC> __device__ __forceinline__ uint4_t load_word(const uint16_t *x) {
+  if constexpr (VEC)
+    return *reinterpret_cast<const uint4_t *>(x);
+  else
+    return *reinterpret_cast<const any4_t *>(x);
+}
+template <bool VEC> __device__ __forceinline__ void store_word(uint16_t *x, uint4_t v) {
+  if constexpr (VEC)
+    *reinterpret_cast<uint4_t *>(x) = v;
+  else
+    *reinterpret_cast<any4_t *>(x) = v;
 }
 
 // The value, hidden from the optimiser like exact_fp.hpp's opaque(), but free

@@ -40,6 +40,9 @@ ROPE = [  # tokens, heads, dim, rotary, layout, first position, step, factor
     (3, 2, 64, 0, "half", 5, 1, 1.0),
     (2, 1, 2048, 2048, "half", 5, 1, 1.0),
     (65, 1, 2, 2, "interleaved", 11, 1, 1.0),
+    (5, 4, 256, 186, "half", 30_000, 1, 1.0),
+    (5, 4, 256, 186, "interleaved", 30_000, 1, 1.0),
+    (300, 2, 100, 42, "half", 17, 1, 1.0),
 ]
 
 

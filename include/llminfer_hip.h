@@ -448,7 +448,7 @@ LLMI_HIP_API int llmi_hip_gated_attention_activated(
  * input are the same rows with the same strides; other overlaps are
  * undefined. rotaryDim even, at most headDim and 2048; strides at least
  * what keeps the output's rows apart (headDim for heads, not checked where
- * there is one). positions, freqs: device memory. */
+ * there is one). At most 2^24 - 1 tokens. positions, freqs: device memory. */
 LLMI_HIP_API int llmi_hip_rope(const uint16_t *input, const int32_t *positions,
                                const float *freqs, uint16_t *output, RopeRowsParams p,
                                void *stream);
@@ -462,7 +462,7 @@ LLMI_HIP_API int llmi_hip_rope(const uint16_t *input, const int32_t *positions,
  *   YARN    g f + (1 - g) f / s, g = (r - lowTurns) / (highTurns - lowTurns)
  *           clamped to [0, 1]; factor 0.1 ln(s) + 1 (1 for s <= 1)
  *   BANDS   the frequencies of YARN with factor 1
- * taken in double and rounded once. */
+ * taken in double and rounded once. rotaryDim even and at most 2048. */
 LLMI_HIP_API int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, float *factor);
 
 /* A pool holds keys and values of headDim 64, 128 or 256 in 4 bits, a scale
@@ -486,7 +486,10 @@ LLMI_HIP_API int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, fl
  * and is NaN where it is read or attended to. Starts that go back or past
  * `tokens` are cut to the rows there are; rows that two sequences claim may
  * come out as either's or not at all. Two sequences of a call may share pages
- * that the call does not append to. At most 2^22 - 1 rows or sequences.
+ * that the call does not append to. At most 2^22 - 1 rows or sequences, and
+ * for paged_gqa 2^31 - 1 rows times query heads and about 2^22 pieces of work
+ * (a piece a KV head: 16 to 256 of its query rows, and 1536 more);
+ * INVALID_ARGUMENT beyond.
  *
  * paged_append: keys and values [tokens][kvHeads][headDim] fp16 (strided;
  * p.tokens rows) to their places; keys are rotated at their positions as

@@ -7,10 +7,10 @@
 // key's words are its own.
 //
 // 2048 rows of 4 heads of 256 take 8.4 us (11 MB: 1.3 TB/s), 6357 rows of 8
-// heads of 128 in 13 sequences 18.0 us (34 MB: 1.9 TB/s). Bound by vector
-// instructions beside the loads' latency: a value is converted, compared,
-// quantized and packed in about 20 of them, and a third of the waves' time is
-// waiting for the rows, a workgroup's only loads. Reading them back takes 5.5
+// heads of 128 in 13 sequences 17.7 us (34 MB: 1.9 TB/s). Bound by latency and
+// vector instructions, about 35 a value (converted, rotated, compared,
+// quantized, transposed; 13 of the 18 us if nothing else were): a third of the
+// waves' time is waiting for the rows, a workgroup's only loads. Reading them back takes 5.5
 // and 10.1 us (2.0 and 3.4 TB/s).
 #include "hip_common.hpp"
 #include "kernels.hpp"
@@ -66,13 +66,17 @@ __device__ __forceinline__ void ends_of(const Eight &x, float &lo, float &hi) {
   hi = fmaxf(hi, x.v[7]);
 }
 // What the cache holds of values that are not finite or past the limit (lo
-// and hi of the others are theirs); whether there were any.
-__device__ __forceinline__ bool keep(Eight &x, float &lo, float &hi) {
-  bool nan = false;
+// and hi of the others are theirs); whether there were any: without their
+// signs, the bits of fp16 values are in order, NaN behind the infinities.
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ bool keep(const uint16_t (&raw)[8], Eight &x, float &lo, float &hi) {
+  static_assert(kPagedLimit == 16384.0f, "its bits below");
+  ushort2_t most{0, 0};
 #pragma unroll
   for (int e = 0; e < 8; e += 2)
-    nan |= __builtin_isunordered(x.v[e], x.v[e + 1]);
-  if (!(nan || lo < -kPagedLimit || hi > kPagedLimit))
+    most = __builtin_elementwise_max(
+        most, ushort2_t{(uint16_t)(raw[e] & 0x7FFFu), (uint16_t)(raw[e + 1] & 0x7FFFu)});
+  if (max((unsigned)most[0], (unsigned)most[1]) <= 0x7400u)
     return false;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
@@ -198,7 +202,7 @@ __device__ __forceinline__ bool append_key(const KeyPart &k, unsigned word, unsi
   Eight v = eight_of(y);
   float lo, hi;
   ends_of(v, lo, hi);
-  const bool bad = keep(v, lo, hi);
+  const bool bad = keep(y, v, lo, hi);
   lo = fminf(lo, dpp<kDppXor1>(lo));
   hi = fmaxf(hi, dpp<kDppXor1>(hi));
   lo = fminf(lo, dpp<kDppXor2>(lo));
@@ -245,7 +249,7 @@ __device__ __forceinline__ bool append_values(const uint16_t (&x)[8], unsigned q
   Eight v = eight_of(x);
   float lo, hi;
   ends_of(v, lo, hi);
-  const bool bad = keep(v, lo, hi) && here;
+  const bool bad = keep(x, v, lo, hi) && here;
   lo = fminf(lo, row_ror<8>(lo));
   hi = fmaxf(hi, row_ror<8>(hi));
   LanePair p = pair16(lo);
@@ -260,17 +264,19 @@ __device__ __forceinline__ bool append_values(const uint16_t (&x)[8], unsigned q
   uint32_t word = transposed((uint32_t)__builtin_amdgcn_ds_bpermute(
       (int)(4 * ((lane & 56u) + turned)), (int)codes_of(v, g)));
   const unsigned channel = 64 * st + 8 * c + turned;
-  // nibbles of keys that are here
-  const unsigned long long there = __builtin_amdgcn_ballot_w64(here) >> (lane & 56u);
-  uint32_t mask = 0;
-#pragma unroll
-  for (unsigned e = 0; e < 8; ++e)
-    mask |= there >> e & 1 ? 15u << paged_nibble(e) : 0u;
   uint32_t *to = reinterpret_cast<uint32_t *>(block + 20 * D + st * 1024 +
                                               (quad * 16 + channel % 16) * 16 +
                                               channel / 16 % 4 * 4);
-  if (mask != 0xFFFFFFFFu)
-    word = (word & mask) | (*to & ~mask);
+  const unsigned long long all = __builtin_amdgcn_ballot_w64(here);
+  if (~all) { // nibbles of keys that are here
+    const unsigned long long there = all >> (lane & 56u);
+    uint32_t mask = 0;
+#pragma unroll
+    for (unsigned e = 0; e < 8; ++e)
+      mask |= there >> e & 1 ? 15u << paged_nibble(e) : 0u;
+    if (mask != 0xFFFFFFFFu)
+      word = (word & mask) | (*to & ~mask);
+  }
   *to = word;
   if (here && c % 4 == 0) {
     half_t *s = reinterpret_cast<half_t *>(block + 36 * D + (2 * st + c / 4) * 128 +

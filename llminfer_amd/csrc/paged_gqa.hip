@@ -186,18 +186,23 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   }
   const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
-  const unsigned end = s.past + s.rows;
+  // the keys that this wave has: to the sequence's end, or to a page that is not
+  // in the pool, whose columns' outputs are NaN
+  const unsigned whole = s.past + s.rows;
+  unsigned end = whole;
   const unsigned length = split.length(s, pieces), b0 = min(piece * length, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned mine = b1 > b0 + wave ? (b1 - b0 - wave + kWaves - 1) / kWaves : 0u;
 
   // Block k of this wave is b0 + wave + kWaves k; a lane knows where one in 64 is.
   size_t place = 0;
-  bool bad = false;
   auto find_blocks = [&](unsigned k) {
     const unsigned b = b0 + wave + kWaves * (k + lane);
+    bool lost = false;
     if (b < b1)
-      bad |= !paged_block(g, seq, 32 * b, kvh, place);
+      lost = !paged_block(g, seq, 32 * b, kvh, place);
+    if (const unsigned long long all = __builtin_amdgcn_ballot_w64(lost))
+      end = min(end, 32 * (b0 + wave + kWaves * (k + (unsigned)__builtin_ctzll(all))));
   };
   // A block past the last is asked for with a descriptor of no bytes: it costs
   // no traffic, and the compiler's count of the loads in flight stays exact.
@@ -241,9 +246,9 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   auto consume = [&](unsigned k, char *buffer) {
     char *block = buffer + wave * Geom::STAGE;
     const unsigned base = 32 * (b0 + wave + kWaves * k);
-    // The slots behind the sequence's last key hold anything, and 0 times that
-    // may be NaN: their values' scales and biases become 0. (A lane has one
-    // slot's scale or bias in every group.)
+    // The slots behind the last key hold anything (what is in page 0 from a
+    // missing page on), and 0 times that may be NaN: their values' scales and
+    // biases become 0. (A lane has one slot's scale or bias in every group.)
     const unsigned slot = lane % 8, behind = 16 * (lane / 16 % 2) + 8 * (slot / 4) +
                                              4 * (lane / 8 % 2) + slot % 4;
     if (base + 32 > end) {
@@ -411,8 +416,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
                                        kWaves / 2 * Geom::TILES * 1024);
   float *sL = sM + kWaves * kUnit;
   __syncthreads(); // the ring's blocks are done with
-  const bool lost = __builtin_amdgcn_ballot_w64(bad); // a page that is not in the pool
-  if (lost && invalid && lane == 0)
+  if (end < whole && invalid && lane == 0)
     atomicOr(invalid, kPagedPlace);
 #pragma unroll
   for (int j = 0; j < CG; ++j) {
@@ -420,6 +424,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     const float half = p.a + p.b;
     p = pair32(half);
     if (quad == 0) {
+      const bool lost = visible[j] >= end;
       sM[wave * kUnit + kColumns * j + r] = lost ? 0.0f : m[j];
       sL[wave * kUnit + kColumns * j + r] = lost ? NAN : p.a + p.b;
     }

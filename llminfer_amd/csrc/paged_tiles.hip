@@ -153,18 +153,20 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   }
   const unsigned least = s.past + c0 / G;                // the first column's last key
   const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
-  const unsigned end = s.past + s.rows;
+  // the keys that this wave decodes: to the sequence's end, or to a page that is
+  // not in the pool, whose columns' outputs are NaN
+  const unsigned whole = s.past + s.rows;
+  unsigned end = whole;
   const unsigned length = split.length(s, pieces), b0 = min(piece * length, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned steps = (b1 - b0 + T::BLOCKS - 1) / T::BLOCKS;
 
   // ---- decoding: this thread's 16 bytes of codes of a step's block
-  __shared__ unsigned sLost;
+  __shared__ unsigned sEnd; // the least of the waves'
   if (tid == 0)
-    sLost = 0;
+    sEnd = whole;
   const unsigned slot = __builtin_amdgcn_readfirstlane(tid / D), unit16 = tid % D;
   size_t place = 0;
-  bool bad = false;
   auto block_of = [&](unsigned n) { return min(b0 + T::BLOCKS * n + slot, b1 - 1); };
   const Nibbles nibbles;
   // A wave's part of a step: 1 KB of key codes and of value codes, and the
@@ -173,8 +175,9 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   char *raw = raw_buffer() + kRaw * wave;
   auto fetch = [&](unsigned n) { // (n < steps; a block past the last again)
     if (n % 64 == 0) {           // where the next 64 steps' blocks are, one a lane
-      const unsigned b = block_of(n + lane);
-      bad |= !paged_block(g, seq, 32 * b, kvh, place);
+      const bool lost = !paged_block(g, seq, 32 * block_of(n + lane), kvh, place);
+      if (const unsigned long long all = __builtin_amdgcn_ballot_w64(lost))
+        end = min(end, 32 * block_of(n + (unsigned)__builtin_ctzll(all)));
     }
     const unsigned lo = __builtin_amdgcn_readlane((unsigned)place, n % 64);
     const unsigned up = __builtin_amdgcn_readlane((unsigned)(place >> 32), n % 64);
@@ -193,9 +196,9 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const unsigned keyAt = slot * T::BLOCKB + (unit16 % (D / 2) / 16) * 2048 +
                          (16 * (rr / 8) + 8 * (unit16 / (D / 2)) + rr % 8) * 16;
   const unsigned valueAt = slot * T::BLOCKB + (unit16 / 64) * 4096 + quad * 512 + rr * 16;
-  // The wave's part of step n has come. Behind the sequence's last key lies
-  // anything, and 0 times that may be NaN: those slots' scales and biases
-  // become 0 (a lane has two slots of one quad).
+  // The wave's part of step n has come. Behind the last key lies anything (what
+  // is in page 0 from a missing page on), and 0 times that may be NaN: those
+  // slots' scales and biases become 0 (a lane has two slots of one quad).
   auto arrived = [&](unsigned n) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const unsigned base = 32 * block_of(n);
@@ -362,8 +365,8 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   }
 
   // ---- join the halves of the keys
-  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) { // a page that is not in the pool
-    sLost = 1;
+  if (end < whole && lane == 0) { // a page that is not in the pool
+    atomicMin(&sEnd, end);
     if (invalid)
       atomicOr(invalid, kPagedPlace);
   }
@@ -400,10 +403,11 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 #pragma unroll
   for (int j = 0; j < CT; ++j) {
     const unsigned col = 32 * (tile0 + j) + r;
-    const float other = sM[col], top = sLost ? 0.0f : fmaxf(m[j], other);
+    const bool lost = visible[j] >= sEnd;
+    const float other = sM[col], top = lost ? 0.0f : fmaxf(m[j], other);
     const float a = m[j] == -INFINITY ? 0.0f : fast_exp2(m[j] - top);
     const float b = other == -INFINITY ? 0.0f : fast_exp2(other - top);
-    const float sum = sLost ? NAN : l[j] * a + sL[col] * b;
+    const float sum = lost ? NAN : l[j] * a + sL[col] * b;
     const size_t part = ((size_t)number * g.kvHeads + kvh) * T::UNIT + col;
     const float inv = 1.0f / sum;
     if (!live(j))

@@ -304,7 +304,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     for (int j = 0; j < CG; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        x[j][e] = acc[e / 4][j][e % 4];
+        x[j][e] = scaled_score(acc[e / 4][j][e % 4], c.c);
     // key of slot 4 t + v of this lane
     const unsigned first = base + 16 * (quad / 2) + 4 * (quad % 2);
     if (base + 31 > least) {
@@ -322,8 +322,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
 #pragma unroll
       for (int e = 1; e < 8; ++e)
         top[j] = fmaxf(top[j], x[j][e]);
-      top[j] *= c.c;
-      raise |= top[j] > m[j] + kPagedRaise;
+      raise |= top[j] - m[j] > kPagedRaise;
     }
     if (__builtin_amdgcn_ballot_w64(raise)) {
 #pragma unroll
@@ -332,7 +331,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
         const float half = fmaxf(p.a, p.b);
         p = pair32(half);
         const float all = fmaxf(p.a, p.b);
-        const float to = all > m[j] + kPagedRaise ? all - kPagedHeadroom : m[j];
+        const float to = all - m[j] > kPagedRaise ? all - kPagedHeadroom : m[j];
         const float alpha = m[j] == to ? 1.0f : fast_exp2(m[j] - to);
         m[j] = to;
         l[j] *= alpha;
@@ -348,7 +347,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       const float ref = m[j] == -INFINITY ? 0.0f : m[j]; // nothing seen yet: weights 0
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        w[j][e] = (half_t)fast_exp2(fmaf(x[j][e], c.c, -ref));
+        w[j][e] = (half_t)fast_exp2(x[j][e] - ref);
       l[j] = dot8(w[j], ones, l[j]);
     }
 #pragma unroll

@@ -22,6 +22,15 @@ inline ScoreScale score_scale(float scale) {
   const float c = __builtin_fabsf(scale * kLog2e);
   return {c > 1e-30f || c != c ? c : 1e-30f, scale < 0.0f ? 0x80008000u : 0u};
 }
+// A score in those multiples, rounded, as the reference m is made of it. The fma
+// of the score, c and -m keeps what that rounding lost, 32 at 2^29, and the
+// largest weight would leave fp16 at either end: the weights take the rounded
+// product less m, exact where it counts.
+__device__ __forceinline__ float scaled_score(float x, float c) {
+  x *= c;
+  asm("" : "+v"(x)); // no fma of it
+  return x;
+}
 __device__ __forceinline__ half8_t with_sign(half8_t x, uint32_t sign) {
   return __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_t, x) ^ sign);
 }

@@ -29,6 +29,7 @@
 #include "paged_plan.hpp"
 
 #include <math.h>
+#include <type_traits>
 
 namespace llmi {
 namespace {
@@ -251,7 +252,9 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
     for (int i = 0; i < T::OUT; ++i)
       o[j][i] = float16_t{0};
   }
-  auto consume = [&](unsigned b, const char *keys, const char *values) {
+  auto consume = [&](auto wide, unsigned b, const char *keys,
+                     const char *values) __attribute__((always_inline)) {
+    constexpr bool kWide = decltype(wide)::value;
     // before the other wave's decoding, where both could go on: 2048 tokens on
     // 2048 in 149 us, 159 without, 155 with only the scores' products ahead
     __builtin_amdgcn_s_setprio(1);
@@ -268,6 +271,12 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
         x[j] = mfma32x32x16(key, qv[j][n], x[j]);
     }
     reads_ahead<T::STEPS, CT>();
+    if constexpr (kWide)
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          x[j][v] = scaled_score(x[j][v], c.c);
     if (base + 31 > least) {
 #pragma unroll
       for (int j = 0; j < CT; ++j)
@@ -283,15 +292,16 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 #pragma unroll
       for (int v = 1; v < 16; ++v)
         top[j] = fmaxf(top[j], x[j][v]);
-      top[j] *= c.c;
-      raise |= top[j] > m[j] + kPagedRaise;
+      if constexpr (!kWide)
+        top[j] *= c.c;
+      raise |= top[j] - m[j] > kPagedRaise;
     }
     if (__builtin_amdgcn_ballot_w64(raise)) {
 #pragma unroll
       for (int j = 0; j < CT; ++j) {
         const LanePair p = pair32(top[j]);
         const float all = fmaxf(p.a, p.b);
-        const float to = all > m[j] + kPagedRaise ? all - kPagedHeadroom : m[j];
+        const float to = all - m[j] > kPagedRaise ? all - kPagedHeadroom : m[j];
         const float alpha = m[j] == to ? 1.0f : fast_exp2(m[j] - to);
         m[j] = to;
         l[j] *= alpha;
@@ -307,7 +317,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
       const float ref = m[j] == -INFINITY ? 0.0f : m[j]; // nothing seen yet: weights 0
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        w[j][e / 8][e % 8] = (half_t)fast_exp2(fmaf(x[j][e], c.c, -ref));
+        w[j][e / 8][e % 8] = (half_t)fast_exp2(kWide ? x[j][e] - ref : fmaf(x[j][e], c.c, -ref));
       l[j] = dot8(w[j][0], ones, l[j]);
       l[j] = dot8(w[j][1], ones, l[j]);
     }
@@ -325,16 +335,42 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
     __builtin_amdgcn_s_setprio(0);
   };
 
+  // Whether a score may be past 2^22: |q| summed, times the largest value that an
+  // append leaves (kPagedLimit and its roundings, below 1/64 of it). Below it
+  // the fma shifts the exponents of a row by 2^-2 at most, all by the same, and
+  // its weights stay below 2^15.5. At head_dim 128 both are there, a loop each
+  // (seven ragged messages: 127 us, 135 with the rounded products alone); at 256
+  // the rounded products alone are faster (2048 tokens on 4096 keys: 135 us, 141
+  // with both).
+  constexpr bool kBoth = D == 128;
+  bool wide = !kBoth;
+  __shared__ unsigned sWide[kThreads / 64];
   if (steps) {
     fetch(0);
+#pragma unroll
+    for (int j = 0; j < (kBoth ? CT : 0); ++j) {
+      const half8_t ones{1, 1, 1, 1, 1, 1, 1, 1};
+      float all = 0.0f;
+#pragma unroll
+      for (int n = 0; n < T::STEPS; ++n)
+        all = dot8(__builtin_elementwise_abs(qv[j][n]), ones, all);
+      const LanePair p = pair32(all);
+      wide |= !((p.a + p.b) * (c.c * (kPagedLimit * 1.015625f)) < 0x1p22f);
+    }
+    if (kBoth && lane == 0)
+      sWide[wave] = __builtin_amdgcn_ballot_w64(wide) != 0;
     arrived(0);
     decode_keys(tile_buffer<0>());
     decode_values(tile_buffer<2>());
+    if (kBoth) { // the workgroup's waves take the same loop, for its barriers
+      lds_sync();
+      wide = __builtin_amdgcn_ballot_w64(sWide[lane % (kThreads / 64)] != 0);
+    }
     if (steps > 1)
       fetch(1);
   }
-  auto step = [&](unsigned n, const char *keys, const char *values, char *nextKeys,
-                  char *nextValues) {
+  auto step = [&](auto wide, unsigned n, const char *keys, const char *values, char *nextKeys,
+                  char *nextValues) __attribute__((always_inline)) {
     lds_sync(); // step n is decoded, and step n - 1's tiles are done with
     auto decode = [&]() {
       if (n + 1 < steps) {
@@ -353,16 +389,22 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
     for (int i = 0; i < T::EACH; ++i) {
       const unsigned at = half * T::EACH + i, b = b0 + T::BLOCKS * n + at;
       if (b < b1)
-        consume(b, keys + at * T::BLOCKB, values + at * T::BLOCKB);
+        consume(wide, b, keys + at * T::BLOCKB, values + at * T::BLOCKB);
     }
     if (half == 1)
       decode();
   };
-  for (unsigned n = 0; n < steps; n += 2) {
-    step(n, tile_buffer<0>(), tile_buffer<2>(), tile_buffer<1>(), tile_buffer<3>());
-    if (n + 1 < steps)
-      step(n + 1, tile_buffer<1>(), tile_buffer<3>(), tile_buffer<0>(), tile_buffer<2>());
-  }
+  auto all_steps = [&](auto wide) __attribute__((always_inline)) {
+    for (unsigned n = 0; n < steps; n += 2) {
+      step(wide, n, tile_buffer<0>(), tile_buffer<2>(), tile_buffer<1>(), tile_buffer<3>());
+      if (n + 1 < steps)
+        step(wide, n + 1, tile_buffer<1>(), tile_buffer<3>(), tile_buffer<0>(), tile_buffer<2>());
+    }
+  };
+  if (wide)
+    all_steps(std::true_type());
+  else if constexpr (kBoth)
+    all_steps(std::false_type());
 
   // ---- join the halves of the keys
   if (end < whole && lane == 0) { // a page that is not in the pool

@@ -1,12 +1,12 @@
 """GPU tests of the paged 4-bit cache where its parts meet: a missing page
-inside a unit of columns. Against paged_oracle; tolerances are counted there or
-beside the test."""
+inside a unit of columns, scores whose fp32 steps are wide. Against paged_oracle;
+tolerances are counted there or beside the test."""
 import numpy as np
 import pytest
 
 from llminfer_amd import _lib, ops
 from tests import paged_oracle as po
-from tests.test_paged_gpu import check, dev, filled, ints, rows16
+from tests.test_paged_gpu import Cache, check, dev, filled, ints, rows16
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,71 @@ def test_rows_before_a_missing_page(gpu, rows, past, hq, hkv, dim, page, slot):
     check(out[:before], q, [x[:1] for x in kv], [before], [past], dim ** -0.5)
     assert np.isnan(out[before:rows]).all()
     check(out[rows:], q[rows:], [x[1:] for x in kv], [rows], [past], dim ** -0.5)
+
+
+# ---------------------------------------------- scores with wide fp32 steps
+
+def inside(out, q, kv, past, scale):
+    """Outputs are averages of the visible values: between their least and
+    most, up to fp32 sums over n keys (twice (n + 64) half steps of the largest)
+    and a half step of fp16. Where the best score leads every other by 40 and
+    the errors of two scores in fp32 (each half a step of sum |q k| scale for
+    every product and sum), the output is its value."""
+    rows, heads, dim = out.shape
+    k, v = (x.astype(np.float64) for x in kv)
+    group = heads // k.shape[1]
+    pinned = 0
+    for i in range(rows):
+        n = past + i + 1
+        for h in range(heads):
+            kk, vv, o = k[:n, h // group], v[:n, h // group], out[i, h].astype(np.float64)
+            qq = q[i, h].astype(np.float64)
+            far = 2 * (n + 64) * 2.0 ** -24 * np.abs(vv).max(0) + np.abs(o) * po.U16 + 2.0 ** -25
+            assert np.isfinite(o).all(), (i, h)
+            assert np.all(o >= vv.min(0) - far) and np.all(o <= vv.max(0) + far), (i, h)
+            x = kk @ qq * scale
+            wrong = 2 * (dim + 8) * 2.0 ** -24 * (np.abs(kk) @ np.abs(qq)).max() * scale
+            best = int(x.argmax())
+            if n == 1 or x[best] - np.delete(x, best).max() > 40 + wrong:
+                pinned += 1
+                rest = n * np.exp(-40.0) * np.abs(vv).max(0)
+                assert np.all(np.abs(o - vv[best]) <= far + rest), (i, h)
+    return pinned
+
+
+@pytest.mark.parametrize("rows, past, dim", [(1, 0, 256), (1, 5, 128), (1, 700, 64), (1, 1500, 256),
+                                             (9, 3, 128), (20, 40, 64), (50, 0, 256), (45, 900, 256),
+                                             (110, 500, 128)])
+@pytest.mark.parametrize("size", [50.0, 300.0, 2000.0, 30000.0])
+@pytest.mark.parametrize("kind", ["apart", "near", "random", "mixed"])
+def test_scores_of_any_size(gpu, rows, past, dim, size, kind):
+    """Keys near the format's limit and large queries: scores of up to 2^34, whose
+    fp32 steps are wider than the softmax. `apart`: keys of one value each, so
+    that one leads by far; `near`: their scores differ by less than a step;
+    `mixed`: one head's queries are as large, the others' ordinary."""
+    rng = np.random.default_rng(int(size) + rows + past + dim)
+    n, hq = rows + past, 4
+    q = np.full((rows, hq, dim), size, np.float16)
+    if kind in ("random", "mixed"):
+        k = rng.uniform(-16384, 16384, (n, 1, dim)).astype(np.float16)
+        q = rows16(rng, rows, hq, dim, size=min(size, 8000.0))
+        if kind == "mixed":
+            q[:, :3] = rows16(rng, rows, 3, dim, size=2.0 ** -12)
+    elif kind == "apart":
+        k = np.repeat((16384 - 16.0 * rng.permutation(n)).astype(np.float16)[:, None, None], dim, 2)
+        q[:, ::2] *= -1
+    else:
+        k = np.full((n, 1, dim), 16000.0, np.float16)
+        k[:, 0, 0] -= 8 * rng.integers(0, 60, n).astype(np.float16)
+        q[..., 0] = 1.0
+    v = rows16(rng, n, 1, dim)
+    cache = Cache(rng, 1, n, 1, dim, 64, fill=0xFF)
+    invalid = ints(0)
+    cache.append(dev(k), dev(v), ints(0, n), ints(0), invalid=invalid)
+    assert invalid.item() == 0
+    kv = [x[0] for x in cache.read([n])]
+    scale = float(np.float32(dim) ** np.float32(-0.5))
+    out = ops.paged_gqa(dev(q), cache.pool, ints(0, rows), ints(past), cache.table)
+    pinned = inside(out.cpu().numpy(), q, kv, past, scale)
+    if kind == "apart":
+        assert pinned == rows * hq  # 16 apart in every channel: a lead of 100 steps and more

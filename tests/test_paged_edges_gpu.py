@@ -1,8 +1,10 @@
 """GPU tests of the paged 4-bit cache where its parts meet: a missing page
-inside a unit of columns, scores whose fp32 steps are wide. Against paged_oracle;
-tolerances are counted there or beside the test."""
+inside a unit of columns, scores whose fp32 steps are wide, appends whose
+workgroups have several heads. Against paged_oracle; tolerances are counted
+there or beside the test."""
 import numpy as np
 import pytest
+import torch
 
 from llminfer_amd import _lib, ops
 from tests import paged_oracle as po
@@ -129,3 +131,51 @@ def test_scores_of_any_size(gpu, rows, past, dim, size, kind):
     pinned = inside(out.cpu().numpy(), q, kv, past, scale)
     if kind == "apart":
         assert pinned == rows * hq  # 16 apart in every channel: a lead of 100 steps and more
+
+
+# --------------------------------------- appends with several heads a workgroup
+
+MANY = [  # rows of each sequence, past of each, Hkv, dim, page, rotary, layout, an odd element first
+    ([500] * 13, [37 * s for s in range(13)], 8, 128, 32, 128, "interleaved", 0),  # 4 heads
+    ([700, 1, 0, 2100, 33, 1500], [5, 31, 9, 0, 64, 1001], 3, 128, 64, 64, "half", 0),  # 2, then 1
+    ([2100], [17], 3, 256, 128, 64, "half", 0),
+    ([2100], [17], 3, 256, 128, 62, "half", 1),
+    ([3000, 2600], [3, 70], 5, 64, 32, 64, "half", 0),                # 2, 2 and 1
+    ([8300], [11], 5, 64, 64, 64, "interleaved", 1),                  # 4 and 1
+    ([1100, 1200], [0, 31], 8, 256, 64, 0, "half", 0),                # 4, not rotated
+]
+
+
+@pytest.mark.parametrize("rows, past, hkv, dim, page, rot, layout, lead", MANY)
+def test_append_of_many_rows(gpu, rows, past, hkv, dim, page, rot, layout, lead):
+    """Calls in which a workgroup has several heads, a last one with fewer:
+    every head's keys and values are the format's, bit for bit."""
+    units = min(sum(rows), sum(rows) // 32 + 2 * len(rows))
+    assert units * (dim // 64) * -(-hkv // 2) >= 512  # two heads or more
+    rng = np.random.default_rng(sum(rows) + dim)
+    S, T = len(rows), sum(rows)
+    cache = Cache(rng, S, max(r + p for r, p in zip(rows, past)), hkv, dim, page, fill=0xA5)
+    wide = dev(rows16(rng, T, 2 * hkv * dim + 8, size=2.0))
+    both = wide[:, lead:lead + 2 * hkv * dim].unflatten(1, (2 * hkv, dim))
+    k, v = both[:, :hkv], both[:, hkv:]
+    freqs, _ = ops.rope_frequencies(rot, 1e4)
+    invalid = ints(0)
+    starts, lens = ints(0, *np.cumsum(rows)), ints(*past)
+    before = cache.pool.clone()
+    cache.append(k, v, starts, lens, freqs=freqs if rot else None, layout=layout, invalid=invalid)
+    gk, gv = ops.paged_read(cache.pool, starts, lens, cache.table, T, invalid)
+    assert invalid.item() == 0
+    turned = k
+    if rot:
+        pos = np.concatenate([np.arange(p, p + r) for r, p in zip(rows, past)]).astype(np.int32)
+        turned = ops.rope(k, dev(pos), freqs, layout=layout)
+    for got, want in ((gk, turned), (gv, v)):
+        got, want = got.cpu().numpy(), po.kept(want.contiguous().cpu().numpy())
+        assert np.array_equal(got, want), np.argwhere((got != want).any(-1))[:8]
+    # pages that hold none of the rows stay
+    held = torch.zeros(before.shape[0], dtype=torch.bool)
+    for s in range(S):
+        if rows[s]:
+            first, last = past[s] // page, (past[s] + rows[s] - 1) // page
+            held[cache.table[s, first:last + 1].long().cpu()] = True
+    assert torch.equal(before[~held], cache.pool[~held])

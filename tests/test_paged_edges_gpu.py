@@ -1,7 +1,7 @@
 """GPU tests of the paged 4-bit cache where its parts meet: a missing page
 inside a unit of columns, scores whose fp32 steps are wide, appends whose
-workgroups have several heads. Against paged_oracle; tolerances are counted
-there or beside the test."""
+workgroups have several heads, calls of more than 64 sequences. Against
+paged_oracle; tolerances are counted there or beside the test."""
 import numpy as np
 import pytest
 import torch
@@ -179,3 +179,42 @@ def test_append_of_many_rows(gpu, rows, past, hkv, dim, page, rot, layout, lead)
             first, last = past[s] // page, (past[s] + rows[s] - 1) // page
             held[cache.table[s, first:last + 1].long().cpu()] = True
     assert torch.equal(before[~held], cache.pool[~held])
+
+
+# ------------------------------------------------- more than 64 sequences
+
+def late(count, most, small):
+    """Pasts of `count` sequences: short, but for some behind the 64th."""
+    past = [(37 * s) % small for s in range(count)]
+    for s, n in most.items():
+        past[s] = n
+    return past
+
+
+CROWDS = [  # rows of each sequence, past of each, Hq, Hkv, dim, page
+    ([1] * 70, late(70, {3: 2000, 64: 4100, 69: 3000}, 90), 4, 1, 128, 64),
+    ([1] * 130, late(130, {63: 900, 64: 2500, 65: 40, 128: 5000, 129: 1700}, 60), 8, 2, 64, 32),
+    ([1] * 66, late(66, {65: 6000}, 50), 16, 4, 256, 64),
+    ([5] * 80, late(80, {10: 1500, 66: 3000, 79: 2222}, 70), 8, 1, 256, 32),      # 32 columns
+    ([26] * 67, late(67, {64: 2600, 66: 1900}, 40), 4, 1, 64, 64),                # 64
+    ([12] * 70, late(70, {0: 1000, 64: 3000, 69: 2500}, 80), 4, 1, 256, 32),      # tiles
+    ([24] * 70, late(70, {33: 900, 65: 2400, 69: 2000}, 60), 8, 2, 128, 64),
+    ([8, 0, 30] * 44, late(132, {2: 1200, 128: 3100, 131: 2700}, 50), 4, 1, 256, 64),
+]
+
+
+@pytest.mark.parametrize("rows, past, hq, hkv, dim, page", CROWDS)
+def test_more_than_64_sequences(gpu, rows, past, hq, hkv, dim, page):
+    """Sequences behind the 64th whose keys are divided and joined."""
+    rng = np.random.default_rng(len(rows) + dim)
+    cache, kv = filled(rng, rows, past, hkv, dim, page)
+    T = sum(rows)
+    q = rows16(rng, T + 2, hq, dim, size=1.5)
+    out = torch.full((T + 2, hq, dim), 9.0, dtype=torch.float16, device="cuda")
+    invalid = ints(0)
+    ops.paged_gqa(dev(q), cache.pool, ints(0, *np.cumsum(rows)), ints(*past), cache.table, out=out,
+                  invalid=invalid)
+    assert invalid.item() == 0
+    out = out.cpu().numpy()
+    assert (out[T:] == 9).all()
+    check(out, q, kv, rows, past, dim ** -0.5)

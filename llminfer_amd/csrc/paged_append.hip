@@ -264,9 +264,7 @@ __device__ __forceinline__ bool append_values(const uint16_t (&x)[8], unsigned q
   uint32_t word = transposed((uint32_t)__builtin_amdgcn_ds_bpermute(
       (int)(4 * ((lane & 56u) + turned)), (int)codes_of(v, g)));
   const unsigned channel = 64 * st + 8 * c + turned;
-  uint32_t *to = reinterpret_cast<uint32_t *>(block + 20 * D + st * 1024 +
-                                              (quad * 16 + channel % 16) * 16 +
-                                              channel / 16 % 4 * 4);
+  uint32_t *to = reinterpret_cast<uint32_t *>(block + paged_value_word(D, quad, channel));
   const unsigned long long all = __builtin_amdgcn_ballot_w64(here);
   if (~all) { // nibbles of keys that are here
     const unsigned long long there = all >> (lane & 56u);
@@ -279,8 +277,8 @@ __device__ __forceinline__ bool append_values(const uint16_t (&x)[8], unsigned q
   }
   *to = word;
   if (here && c % 4 == 0) {
-    half_t *s = reinterpret_cast<half_t *>(block + 36 * D + (2 * st + c / 4) * 128 +
-                                           (quad * 8 + slot) * 2);
+    half_t *s =
+        reinterpret_cast<half_t *>(block + paged_value_scale(D, quad, slot, 2 * st + c / 4));
     s[0] = g.scale;
     s[32] = g.bias;
   }
@@ -422,10 +420,11 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const uint8_t *__r
   } else if (ok) {
     const unsigned quad = lane / 16, r = lane % 16;
     for (unsigned st = tid / 64; st < D / 64; st += kThreads / 64) {
-      const uint4_t w = *reinterpret_cast<const uint4_t *>(block + 20 * D + st * 1024 + lane * 16);
+      const uint4_t w =
+          *reinterpret_cast<const uint4_t *>(block + paged_value_word(D, quad, 64 * st + r));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint8_t *m = block + 36 * D + (2 * st + j / 2) * 128 + quad * 16;
+        const uint8_t *m = block + paged_value_scale(D, quad, 0, 2 * st + j / 2);
         const half8_t sc = *reinterpret_cast<const half8_t *>(m);
         const half8_t bi = *reinterpret_cast<const half8_t *>(m + 64);
 #pragma unroll

@@ -88,19 +88,14 @@ __device__ __forceinline__ unsigned paged_key_word(unsigned D, unsigned key, uns
 __device__ __forceinline__ unsigned paged_key_scale(unsigned D, unsigned key, unsigned group) {
   return 16 * D + ((key >> 3) & 1) * 2 * D + (group * 16 + paged_row(key)) * 4;
 }
-__device__ __forceinline__ unsigned paged_quad(unsigned key) {
-  return (key >> 4) * 2 + ((key >> 2) & 1);
+// A value's, of the quad and slot that hold its key; the bias is 64 bytes
+// behind the scale.
+__device__ __forceinline__ unsigned paged_value_word(unsigned D, unsigned quad, unsigned channel) {
+  return 20 * D + (channel / 64) * 1024 + (quad * 16 + channel % 16) * 16 + (channel / 16 % 4) * 4;
 }
-__device__ __forceinline__ unsigned paged_slot(unsigned key) {
-  return ((key >> 3) & 1) * 4 + (key & 3);
-}
-__device__ __forceinline__ unsigned paged_value_word(unsigned D, unsigned key, unsigned channel) {
-  return 20 * D + (channel / 64) * 1024 + (paged_quad(key) * 16 + channel % 16) * 16 +
-         (channel / 16 % 4) * 4;
-}
-// the scale; the bias is 64 bytes further
-__device__ __forceinline__ unsigned paged_value_scale(unsigned D, unsigned key, unsigned group) {
-  return 36 * D + group * 128 + (paged_quad(key) * 8 + paged_slot(key)) * 2;
+__device__ __forceinline__ unsigned paged_value_scale(unsigned D, unsigned quad, unsigned slot,
+                                                      unsigned group) {
+  return 36 * D + group * 128 + (quad * 8 + slot) * 2;
 }
 // Bit of slot e's nibble in its word.
 __host__ __device__ constexpr unsigned paged_nibble(unsigned e) { return 4 * (e / 2) + 16 * (e % 2); }

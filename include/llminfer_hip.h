@@ -460,7 +460,10 @@ LLMI_HIP_API int llmi_hip_rope(const uint16_t *input, const int32_t *positions,
  *   NONE    f                          LINEAR  f / s
  *   NTK     (theta s^(rotaryDim / (rotaryDim - 2)))^(-2i / rotaryDim)
  *   YARN    g f + (1 - g) f / s, g = (r - lowTurns) / (highTurns - lowTurns)
- *           clamped to [0, 1]; factor 0.1 ln(s) + 1 (1 for s <= 1)
+ *           clamped to [0, 1]; factor 0.1 ln(s) + 1 (1 for s <= 1). Linear in
+ *           the turns r; a model trained with a ramp over the pair's index i
+ *           differs inside it and brings frequencies of its own (rope and
+ *           paged_append take any)
  *   BANDS   the frequencies of YARN with factor 1
  * taken in double and rounded once. rotaryDim even and at most 2048. */
 LLMI_HIP_API int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, float *factor);
@@ -479,11 +482,14 @@ LLMI_HIP_API int llmi_hip_rope_frequencies(RopeScalingParams p, float *freqs, fl
  * starts[s] + i at position past[s] + i, kept in page table[s * tableStride +
  * position / pageSize]. starts [sequences + 1], past and table are device
  * memory, so that a captured graph can be replayed on new lengths. Rows of no
- * sequence are neither read nor written. A row whose position is not in its
- * table (negative, or from tableStride * pageSize on) or whose page is not in
- * the pool is an error that only the device can see: it sets bit 1 (2) of
- * *invalid (when invalid is not null; never cleared here), is not appended,
- * and is NaN where it is read or attended to. Starts that go back or past
+ * sequence are neither read nor written. Two errors only the device can see;
+ * both set bit 1 (2) of *invalid (when invalid is not null; never cleared
+ * here). A sequence that does not fit its table (past negative, or past + rows
+ * above tableStride * pageSize) has no place as a whole: none of its rows is
+ * appended, all are NaN where they are read or attended to. A page that is not
+ * in the pool: the rows in it are not appended and are NaN where they are
+ * read, and the rows that would attend to keys in it are NaN; the sequence's
+ * other rows are as they would be. Starts that go back or past
  * `tokens` are cut to the rows there are; rows that two sequences claim may
  * come out as either's or not at all. Two sequences of a call may share pages
  * that the call does not append to. At most 2^22 - 1 rows or sequences, and
@@ -515,7 +521,9 @@ LLMI_HIP_API int llmi_hip_paged_read(const void *pool, const int32_t *starts,
  * dense, 16-byte aligned, apart from each other; the call's own rows are
  * appended before. `workspace` holds llmi_hip_paged_gqa_workspace_bytes(p)
  * bytes (0: none is needed), 16-byte aligned: the partials of rows whose keys
- * are divided over workgroups, written and read within the call. How they are
+ * are divided over workgroups, written and read within the call. It is for
+ * the most that any lengths could divide, so it grows with the rows (16 / 4
+ * heads of 256: 69 MB for 2048, 576 MB for 32768). How they are
  * divided, and so the order of the sums, goes by the lengths and the counts
  * of rows and sequences alone. */
 LLMI_HIP_API int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts,

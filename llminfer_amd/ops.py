@@ -975,7 +975,9 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e7, scaling: str | None = 
     """(frequencies fp32 [rotary_dim / 2], factor) of a rotation, for rope and
     paged_append (llmi_hip_rope_frequencies): theta^(-2i / rotary_dim), scaled
     for contexts longer than original_positions by `scaling`: None, "linear",
-    "ntk", "yarn" or "bands" (yarn's frequencies without its factor)."""
+    "ntk", "yarn" or "bands" (yarn's frequencies without its factor). yarn's ramp
+    is linear in a pair's turns; for a model trained with a ramp over the pairs'
+    index, pass frequencies of its own to rope and paged_append."""
     if scaling not in _SCALINGS:
         raise ValueError(f"scaling is one of {sorted(map(str, _SCALINGS))}")
     if rotary_dim < 0:
@@ -1087,8 +1089,9 @@ def bind_paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, star
     page table[s, p // page_size]; starts [S + 1], past [S] and table [S, n]
     are int32. freqs: keys are rotated at their positions first, as rope does.
     invalid (int32, one element): bit 0 is set by a value that is not finite
-    or past 16384 in magnitude, bit 1 by a row with no place (such rows are
-    left out)."""
+    or past 16384 in magnitude, bit 1 by rows with no place, which are left out:
+    those whose page is outside the pool, and all of a sequence that does not
+    fit its table."""
     for t, n in ((k, "k"), (v, "v")):
         _require_rows(t, n)
     p = _paged(pool, starts, past, table, k.shape[0], invalid)
@@ -1118,8 +1121,8 @@ def bind_paged_read(pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor
                     table: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                     invalid: torch.Tensor | None = None) -> "Bound":
     """The cache's values of a call's rows (as bind_paged_append places them)
-    into k, v [T, Hkv, dim] fp16; a row with no place is NaN and sets bit 1 of
-    invalid. A whole sequence: past 0 and its length as rows."""
+    into k, v [T, Hkv, dim] fp16; rows with no place, as there, are NaN and set
+    bit 1 of invalid. A whole sequence: past 0 and its length as rows."""
     for t, n in ((k, "k"), (v, "v")):
         _require(t, torch.float16, n)
     if k.dim() != 3 or v.shape != k.shape:
@@ -1153,9 +1156,11 @@ def bind_paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, pa
     (llmi_hip_paged_gqa): row i of sequence s attends to its keys at positions
     up to past[s] + i, the call's own rows among them (appended before). scale
     defaults to 1 / sqrt(dim); out must not overlap q. Rows of no sequence are
-    left as they are; a row that would read a page outside the pool, or does
-    not fit its table, is NaN and sets bit 1 of invalid. The workspace is the
-    call's own: calls and graphs may run at once on streams of their own."""
+    left as they are; a row that would read a page outside the pool, and every
+    row of a sequence that does not fit its table, is NaN and sets bit 1 of
+    invalid. The workspace is the bound call's own (tens of MB for thousands of
+    rows): calls and graphs may run at once on streams of their own. Keep a bound
+    call as long as a graph that it was captured into."""
     for t, n in ((q, "q"), (out, "out")):
         _require(t, torch.float16, n)
     if q.dim() != 3 or out.shape != q.shape:

@@ -6,12 +6,13 @@
 // in and written back by the one workgroup that has them, without atomics; a
 // key's words are its own.
 //
-// 2048 rows of 4 heads of 256 take 8.4 us (11 MB: 1.3 TB/s), 6357 rows of 8
-// heads of 128 in 13 sequences 17.7 us (34 MB: 1.9 TB/s). Bound by latency and
-// vector instructions, about 35 a value (converted, rotated, compared,
-// quantized, transposed; 13 of the 18 us if nothing else were): a third of the
-// waves' time is waiting for the rows, a workgroup's only loads. Reading them back takes 5.5
-// and 10.1 us (2.0 and 3.4 TB/s).
+// Traced, 2048 rows of 4 heads of 256 take 8.4 us (11 MB: 1.3 TB/s), 6357 rows of
+// 8 heads of 128 in 13 sequences 17.6 us (34 MB: 1.9 TB/s). Bound by vector
+// instructions, about 35 a value (converted, rotated, compared, quantized,
+// transposed; 12 of the 17.6 us and 4 of the 8.4 if nothing else were), and by
+// latency: lengths, table and rows, one load after the other. Reading them back
+// takes 5.6 and 10.2 us (2.0 and 3.4 TB/s), the values' codes through two-byte
+// writes to LDS.
 #include "hip_common.hpp"
 #include "kernels.hpp"
 #include "paged_kv.hpp"

@@ -15,13 +15,20 @@
 //    the decoded tiles need the workgroup's barrier, one a step.
 // The halves of the keys are joined at the end through the tiles' memory.
 //
-// 2048 tokens of 16 heads of 256 on 4096 keys take 131 us, 103 GFLOP; the last
-// units see 4096 keys and the first 2080, and the kernel takes the time of the
-// last ones: 128 blocks at 0.97 us, 1.1 PFLOP/s while all of them run. Bound by
-// the products and the vector instructions of a SIMD's two waves, which overlap
-// little: 99 and 75 thousand cycles of the 200 thousand that an average
-// workgroup runs (half of the vector instructions decode, without them the
-// kernel takes 64 % of its time; LDS is busy for 85 thousand).
+// 2048 tokens of 16 heads of 256 on 4096 keys take 131 us (traced, after some
+// hundred passes; the first take 138 and more; 134 to 138 in their call with
+// the join's launch, by the card), 103 GFLOP; the last units see 4096 keys and
+// the first 2080, and the kernel takes the time of the last ones: 128 blocks at
+// 0.97 us, 1.1 PFLOP/s while all of them run. Bound by the products and the
+// vector instructions of a SIMD's two waves, which overlap little: 99 and 78
+// thousand cycles of the 208 thousand that a SIMD's workgroups run (half of the
+// vector instructions decode, without them the kernel takes 64 % of its time;
+// LDS is busy for 86 thousand).
+// At head_dim 128 the kernel has more than its 256 registers hold: addresses are
+// reloaded from scratch between a step's DMA loads, each reload a wait for all
+// loads before it. SQ_WAIT_ANY is 56 million in seven ragged messages (125 us
+// traced, 127 to 131 in their call) and 28 million in the call above, whose
+// products are more.
 // Of a short call (61 tokens on 16472 keys: 30 us inside the kernel) 6 us are
 // the plan, the table and the first blocks, 5 the joining and the partials.
 #include "hip_common.hpp"
@@ -56,7 +63,7 @@ template <int I> __device__ __forceinline__ char *tile_buffer() {
 // The call's piece `u` with the sequences of the longest pieces first (up to 64
 // sequences; in their order otherwise), so that workgroups which start late
 // have little to do (seven messages of 41 to 110 blocks, 296 workgroups:
-// 195 us in order, 148 longest first).
+// 174 us in order, 130 longest first).
 __device__ __forceinline__ bool find_longest(const PagedView &g, const PagedSeq &own,
                                              const Split &split, unsigned u, unsigned &seq,
                                              unsigned &local, unsigned &number) {
@@ -256,7 +263,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
                      const char *values) __attribute__((always_inline)) {
     constexpr bool kWide = decltype(wide)::value;
     // before the other wave's decoding, where both could go on: 2048 tokens on
-    // 2048 in 149 us, 159 without, 155 with only the scores' products ahead
+    // 4096 keys in 138 us, 144 without, 143 with only the scores' products ahead
     __builtin_amdgcn_s_setprio(1);
     const unsigned base = 32 * b;
     float16_t x[CT];
@@ -341,7 +348,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   // its weights stay below 2^15.5. At head_dim 128 both are there, a loop each
   // (seven ragged messages: 127 us, 135 with the rounded products alone); at 256
   // the rounded products alone are faster (2048 tokens on 4096 keys: 135 us, 141
-  // with both).
+  // with both on the same card).
   constexpr bool kBoth = D == 128;
   bool wide = !kBoth;
   __shared__ unsigned sWide[kThreads / 64];

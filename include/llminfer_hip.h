@@ -176,6 +176,23 @@ typedef struct PagedGqaParams {
   float scale;
 } PagedGqaParams;
 
+/* Attention whose sequences are in groups with a prefix in common. */
+typedef struct PagedSharedParams {
+  PagedGqaParams gqa;
+  unsigned groups;
+} PagedSharedParams;
+
+/* `children` rows of tableStride page numbers made from `sequences` ones. */
+typedef struct PagedForkParams {
+  unsigned pages, pageSize, kvHeads, headDim;
+  unsigned sequences, tableStride, children;
+} PagedForkParams;
+
+/* The tables of `sequences` sequences over a pool's pages. */
+typedef struct PagedFreeParams {
+  unsigned pages, pageSize, sequences, tableStride;
+} PagedFreeParams;
+
 /* LinearEpilogue, lib/Backend/Metal/Kernels/ReferenceParams.h:8-16 */
 enum llmi_linear_epilogue {
   LLMI_LINEAR_NONE = 0,
@@ -225,7 +242,11 @@ enum llmi_hip_op {
   LLMI_HIP_OP_ROPE = 25,                /* params: RopeRowsParams */
   LLMI_HIP_OP_PAGED_APPEND = 26,        /* params: PagedKvParams */
   LLMI_HIP_OP_PAGED_READ = 27,          /* params: PagedKvParams */
-  LLMI_HIP_OP_PAGED_GQA = 28            /* params: PagedGqaParams */
+  LLMI_HIP_OP_PAGED_GQA = 28,           /* params: PagedGqaParams */
+  LLMI_HIP_OP_PAGED_GQA_SHARED = 29,    /* params: PagedSharedParams */
+  LLMI_HIP_OP_PAGED_FORK = 30,          /* params: PagedForkParams */
+  LLMI_HIP_OP_PAGED_FREE = 31,          /* params: PagedFreeParams */
+  LLMI_HIP_OP_PAGED_MOVE = 32           /* params: PagedKvParams */
 };
 
 /* ---------------------------------------------------------------- KvAppend
@@ -531,6 +552,82 @@ LLMI_HIP_API int llmi_hip_paged_gqa(const uint16_t *q, const int32_t *starts,
                                     uint16_t *out, uint32_t *invalid, PagedGqaParams p,
                                     void *workspace, size_t workspace_bytes, void *stream);
 LLMI_HIP_API size_t llmi_hip_paged_gqa_workspace_bytes(PagedGqaParams p);
+
+/* paged_gqa of sequences that have pages in common: group g is sequences
+ * [groups[g], groups[g + 1]) of the call, whose first prefix[g] keys are the
+ * same (device memory: groups [p.groups + 1], in order, and prefix [p.groups]).
+ * Those keys, in whole blocks of 32, are read once for all rows of the group,
+ * through the table of its first sequence, also where that has no rows; the
+ * result is paged_gqa's but for the order of the sums. The group's sequences
+ * have the shared pages in their own tables as well: what of the prefix is no
+ * whole block is read there. A prefix below 32 shares nothing (a negative one
+ * is 0); a sequence whose past is shorter than its group's prefix has no place,
+ * as one that does not fit its table; a sequence of no group shares nothing.
+ * Groups whose rows are not in order (as starts) or that claim the same
+ * sequences leave those rows as either's, or as they were. p.groups 0 is
+ * paged_gqa. Sizes, limits, errors and the workspace
+ * (llmi_hip_paged_gqa_shared_workspace_bytes) are as there; groups at most
+ * 2^22 - 1. */
+LLMI_HIP_API int llmi_hip_paged_gqa_shared(const uint16_t *q, const int32_t *starts,
+                                           const int32_t *past, const int32_t *table,
+                                           const int32_t *groups, const int32_t *prefix,
+                                           const void *pool, uint16_t *out, uint32_t *invalid,
+                                           PagedSharedParams p, void *workspace,
+                                           size_t workspace_bytes, void *stream);
+LLMI_HIP_API size_t llmi_hip_paged_gqa_shared_workspace_bytes(PagedSharedParams p);
+
+/* Children of sequences. Child i continues sequence parent[i] (any number of
+ * children may have one parent), of length L = past[parent[i]]: its row of
+ * tableOut has the parent's first L / pageSize pages, then spare[i], a page of
+ * its own, into which the blocks of the parent's next page that hold its last L
+ * % pageSize keys are copied, then -1 to the row's end; pastOut[i] = L. With
+ * spare[i] negative it takes over the parent's row as it is, which at most one
+ * child of a parent can do. (A full row has no place for a spare page, which
+ * stays unused.)
+ * Spare pages are apart and none of a sequence's. The tables are [sequences]
+ * and [children] rows of tableStride page numbers, apart from each other;
+ * tableOut and pastOut overlap no input. An engine with a pool for each layer
+ * calls this for each, with the same tables. A parent that is not one of the
+ * sequences, or whose length is negative or does not fit its row: the child's
+ * row is all -1 and its length -1 (no place anywhere). A spare page, or the page
+ * copied, that is not in the pool: -1 in its place. Both set bit 1 (2) of
+ * *invalid. At most 2^22 - 1 children, and 2^24 - 1 of them times kvHeads times
+ * blocks of a page. */
+LLMI_HIP_API int llmi_hip_paged_fork(const int32_t *table, const int32_t *past,
+                                     const int32_t *parent, const int32_t *spare,
+                                     int32_t *tableOut, int32_t *pastOut, void *pool,
+                                     uint32_t *invalid, PagedForkParams p, void *stream);
+
+/* The pages that no sequence holds: sequence s holds the first ceil(lengths[s]
+ * / pageSize) pages of its row of the table. free [pages] gets them, ascending,
+ * and -1 behind them, *count how many they are; both apart from the inputs. A
+ * sequence whose length is negative or does not fit its row holds all of the
+ * row, and entries that are not in the pool hold nothing; both set bit 1 (2)
+ * of *invalid. No sequences hold no page. `workspace` holds
+ * llmi_hip_paged_free_workspace_bytes(p) bytes (0: none is needed), 16-byte
+ * aligned. At most 2^31 - 1 pages, positions of a row and entries of the table. */
+LLMI_HIP_API int llmi_hip_paged_free(const int32_t *table, const int32_t *lengths, int32_t *free,
+                                     int32_t *count, uint32_t *invalid, PagedFreeParams p,
+                                     void *workspace, size_t workspace_bytes, void *stream);
+LLMI_HIP_API size_t llmi_hip_paged_free_workspace_bytes(PagedFreeParams p);
+
+/* Keys and values moved as they are, in 4 bits: row starts[s] + i of the call
+ * is the key and value at position source[starts[s] + i] (in any order, any
+ * number of times) of row s of sourceTable, and goes to position past[s] + i of
+ * row s of table. All are read before any is written, so the tables may be the
+ * same and rows may move within a sequence (a context without the keys it can
+ * do without; drafts of which some are kept). Keys stay rotated as they were.
+ * sourceTable has the shape of table (tokens of source: device memory). A row
+ * whose source has no place is not moved, what is at its target stays; the
+ * other errors, and the sequences, are as in paged_append. Two rows of a call
+ * must not go to one place. `workspace` holds
+ * llmi_hip_paged_move_workspace_bytes(p) bytes, 16-byte aligned. */
+LLMI_HIP_API int llmi_hip_paged_move(const int32_t *source, const int32_t *sourceTable,
+                                     const int32_t *starts, const int32_t *past,
+                                     const int32_t *table, void *pool, uint32_t *invalid,
+                                     PagedKvParams p, void *workspace, size_t workspace_bytes,
+                                     void *stream);
+LLMI_HIP_API size_t llmi_hip_paged_move_workspace_bytes(PagedKvParams p);
 
 /* ------------------------------------------------------------- DeltaUpdate
  * Replaces graphDeltaUpdate (Graph.metal:146-170 with updateDeltaColumn,

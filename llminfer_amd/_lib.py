@@ -47,6 +47,10 @@ OP_ROPE = 25
 OP_PAGED_APPEND = 26
 OP_PAGED_READ = 27
 OP_PAGED_GQA = 28
+OP_PAGED_GQA_SHARED = 29
+OP_PAGED_FORK = 30
+OP_PAGED_FREE = 31
+OP_PAGED_MOVE = 32
 NORM_LINEAR_MAX = 4  # LLMI_HIP_NORM_LINEAR_MAX
 
 # LinearEpilogue (ReferenceParams.h:8-16)
@@ -170,6 +174,19 @@ class PagedGqaParams(C.Structure):
     _fields_ = [("kv", PagedKvParams), ("queryHeads", C.c_uint), ("scale", C.c_float)]
 
 
+class PagedSharedParams(C.Structure):
+    _fields_ = [("gqa", PagedGqaParams), ("groups", C.c_uint)]
+
+
+class PagedForkParams(C.Structure):
+    _fields_ = [(n, C.c_uint) for n in ("pages", "pageSize", "kvHeads", "headDim", "sequences",
+                                        "tableStride", "children")]
+
+
+class PagedFreeParams(C.Structure):
+    _fields_ = [(n, C.c_uint) for n in ("pages", "pageSize", "sequences", "tableStride")]
+
+
 class SessionConfig(C.Structure):
     _fields_ = [("capacity", C.c_uint), ("queryHeads", C.c_uint),
                 ("kvHeads", C.c_uint), ("headDim", C.c_uint),
@@ -254,6 +271,14 @@ SIGNATURES = {
     "llmi_hip_paged_read": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedKvParams, _P]),
     "llmi_hip_paged_gqa": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedGqaParams, _P, _SZ, _P]),
     "llmi_hip_paged_gqa_workspace_bytes": (_SZ, [PagedGqaParams]),
+    "llmi_hip_paged_gqa_shared": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, PagedSharedParams,
+                                            _P, _SZ, _P]),
+    "llmi_hip_paged_gqa_shared_workspace_bytes": (_SZ, [PagedSharedParams]),
+    "llmi_hip_paged_fork": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, PagedForkParams, _P]),
+    "llmi_hip_paged_free": (C.c_int, [_P, _P, _P, _P, _P, PagedFreeParams, _P, _SZ, _P]),
+    "llmi_hip_paged_free_workspace_bytes": (_SZ, [PagedFreeParams]),
+    "llmi_hip_paged_move": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedKvParams, _P, _SZ, _P]),
+    "llmi_hip_paged_move_workspace_bytes": (_SZ, [PagedKvParams]),
     "llmi_hip_workspace_init": (C.c_int, [_P, _SZ, _P]),
     "llmi_hip_dispatch_count": (C.c_uint, [C.c_int, _P]),
     "llmi_hip_kernel_name": (C.c_char_p, [C.c_int, _P, C.c_uint]),

@@ -1155,6 +1155,154 @@ size_t llmi_hip_paged_gqa_workspace_bytes(PagedGqaParams p) {
   return paged_gqa_workspace_bytes(p.kv, p.queryHeads);
 }
 
+static int check_workspace(const char *what, const void *workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need || !aligned16(workspace)))
+    return fail(LLMI_HIP_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what,
+                workspace ? bytes : 0, need);
+  return LLMI_HIP_OK;
+}
+// Whether two ranges of memory have bytes in common.
+static bool overlap(const void *a, size_t aBytes, const void *b, size_t bBytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + bBytes && y < x + aBytes;
+}
+
+int llmi_hip_paged_gqa_shared(const uint16_t *q, const int32_t *starts, const int32_t *past,
+                              const int32_t *table, const int32_t *groups, const int32_t *prefix,
+                              const void *pool, uint16_t *out, uint32_t *invalid,
+                              PagedSharedParams p, void *workspace, size_t workspace_bytes,
+                              void *stream) {
+  const PagedKvParams &kv = p.gqa.kv;
+  if (p.groups == 0)
+    return llmi_hip_paged_gqa(q, starts, past, table, pool, out, invalid, p.gqa, workspace,
+                              workspace_bytes, stream);
+  if (kv.tokens == 0 || kv.sequences == 0)
+    return LLMI_HIP_OK;
+  const char *what = "pagedGqaShared";
+  if (int rc = check_paged(what, kv, starts, past, table, pool))
+    return rc;
+  if (int rc = check_paged_heads(p.gqa))
+    return rc;
+  if (!q || !out || !groups || !prefix)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: null buffer", what);
+  if (!aligned16(q) || !aligned16(out))
+    return fail(LLMI_HIP_UNSUPPORTED, "%s: rows not 16-byte aligned", what);
+  if (p.groups >= 1u << 22 || !paged_shared_launchable(kv, p.gqa.queryHeads, p.groups))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: too many rows, heads or groups for one call", what);
+  const size_t bytes = (size_t)kv.tokens * p.gqa.queryHeads * kv.headDim * 2;
+  if (overlap(q, bytes, out, bytes))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: out overlaps q", what);
+  if (int rc = check_workspace(what, workspace, workspace_bytes,
+                               paged_shared_workspace_bytes(kv, p.gqa.queryHeads, p.groups)))
+    return rc;
+  return launched(launch_paged_gqa_shared(q, starts, past, table, groups, prefix, pool, out, invalid,
+                                          workspace, kv, p.gqa.queryHeads, p.gqa.scale, p.groups,
+                                          static_cast<hipStream_t>(stream)),
+                  what);
+}
+
+size_t llmi_hip_paged_gqa_shared_workspace_bytes(PagedSharedParams p) {
+  if (p.groups == 0)
+    return llmi_hip_paged_gqa_workspace_bytes(p.gqa);
+  if (p.gqa.kv.tokens == 0 || p.gqa.kv.sequences == 0 || check_paged_heads(p.gqa) ||
+      p.groups >= 1u << 22 || !paged_shared_launchable(p.gqa.kv, p.gqa.queryHeads, p.groups))
+    return 0;
+  return paged_shared_workspace_bytes(p.gqa.kv, p.gqa.queryHeads, p.groups);
+}
+
+int llmi_hip_paged_fork(const int32_t *table, const int32_t *past, const int32_t *parent,
+                        const int32_t *spare, int32_t *tableOut, int32_t *pastOut, void *pool,
+                        uint32_t *invalid, PagedForkParams p, void *stream) {
+  if (p.children == 0)
+    return LLMI_HIP_OK;
+  const char *what = "pagedFork";
+  if (p.sequences == 0)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: no sequences to continue", what);
+  const PagedKvParams kv{p.pages,     p.pageSize,    p.kvHeads, p.headDim,
+                         p.sequences, p.tableStride, 1};
+  if (int rc = check_paged(what, kv, past, past, table, pool))
+    return rc;
+  if (!parent || !spare || !tableOut || !pastOut)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: null buffer", what);
+  if (p.children >= 1u << 22 || !fits32(256 * (uint64_t)p.children, p.kvHeads, p.pageSize / 32))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: too many children, heads or blocks for one call",
+                what);
+  const size_t row = (size_t)p.tableStride * 4, tableBytes = p.sequences * row;
+  const size_t outBytes = p.children * row, n = (size_t)p.children * 4;
+  const size_t pastBytes = (size_t)p.sequences * 4;
+  const struct {
+    const void *at;
+    size_t bytes;
+  } in[] = {{table, tableBytes}, {past, pastBytes}, {parent, n}, {spare, n}};
+  for (const auto &x : in)
+    if (overlap(x.at, x.bytes, tableOut, outBytes) || overlap(x.at, x.bytes, pastOut, n))
+      return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: an output overlaps an input", what);
+  if (overlap(tableOut, outBytes, pastOut, n))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "%s: the outputs overlap", what);
+  return launched(launch_paged_fork(table, past, parent, spare, tableOut, pastOut, pool, invalid, p,
+                                    static_cast<hipStream_t>(stream)),
+                  what);
+}
+
+static int check_free(const PagedFreeParams &p) {
+  if (p.pageSize == 0 || p.pageSize % 32)
+    return fail(LLMI_HIP_UNSUPPORTED, "pagedFree: page size %u is no multiple of 32", p.pageSize);
+  if (p.pages == 0 || p.tableStride == 0)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedFree: pages and table must not be empty");
+  if (p.pages > 0x7fffffffu || (uint64_t)p.tableStride * p.pageSize > 0x7fffffffull ||
+      (uint64_t)p.sequences * p.tableStride > 0x7fffffffull)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedFree: exceeds the 31-bit range of pages, "
+                "positions or entries");
+  return LLMI_HIP_OK;
+}
+
+int llmi_hip_paged_free(const int32_t *table, const int32_t *lengths, int32_t *free, int32_t *count,
+                        uint32_t *invalid, PagedFreeParams p, void *workspace,
+                        size_t workspace_bytes, void *stream) {
+  if (int rc = check_free(p))
+    return rc;
+  if ((p.sequences && (!table || !lengths)) || !free || !count)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedFree: null buffer");
+  const size_t entries = (size_t)p.sequences * p.tableStride * 4, out = (size_t)p.pages * 4;
+  if (overlap(table, entries, free, out) || overlap(lengths, (size_t)p.sequences * 4, free, out) ||
+      overlap(table, entries, count, 4) || overlap(lengths, (size_t)p.sequences * 4, count, 4) ||
+      overlap(free, out, count, 4))
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedFree: an output overlaps another buffer");
+  if (int rc = check_workspace("pagedFree", workspace, workspace_bytes,
+                               paged_free_workspace_bytes(p)))
+    return rc;
+  return launched(launch_paged_free(table, lengths, free, count, invalid, workspace, p,
+                                    static_cast<hipStream_t>(stream)),
+                  "pagedFree");
+}
+
+size_t llmi_hip_paged_free_workspace_bytes(PagedFreeParams p) {
+  return check_free(p) ? 0 : paged_free_workspace_bytes(p);
+}
+
+int llmi_hip_paged_move(const int32_t *source, const int32_t *sourceTable, const int32_t *starts,
+                        const int32_t *past, const int32_t *table, void *pool, uint32_t *invalid,
+                        PagedKvParams p, void *workspace, size_t workspace_bytes, void *stream) {
+  if (p.tokens == 0 || p.sequences == 0)
+    return LLMI_HIP_OK;
+  if (int rc = check_paged("pagedMove", p, starts, past, table, pool))
+    return rc;
+  if (!source || !sourceTable)
+    return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedMove: null buffer");
+  if (int rc = check_workspace("pagedMove", workspace, workspace_bytes,
+                               paged_move_workspace_bytes(p)))
+    return rc;
+  return launched(launch_paged_move(source, sourceTable, starts, past, table, pool, invalid,
+                                    workspace, p, static_cast<hipStream_t>(stream)),
+                  "pagedMove");
+}
+
+size_t llmi_hip_paged_move_workspace_bytes(PagedKvParams p) {
+  if (p.tokens == 0 || p.sequences == 0 || (p.headDim != 64 && p.headDim != 128 && p.headDim != 256))
+    return 0;
+  return paged_move_workspace_bytes(p);
+}
+
 // Whether a supported CausalGqa is a prefill that divides its keys.
 static bool prefill_merges(const GqaParams &p) {
   return select_gqa(p) == GqaKernel::Prefill &&
@@ -1274,6 +1422,24 @@ unsigned llmi_hip_dispatch_count(int op, const void *params) {
     if (!p.kv.tokens || !p.kv.sequences || check_paged_heads(p))
       return 0;
     return 1u + paged_gqa_joins(p.kv, p.queryHeads);
+  }
+  case LLMI_HIP_OP_PAGED_GQA_SHARED: {
+    const PagedSharedParams &p = *static_cast<const PagedSharedParams *>(params);
+    if (!p.groups)
+      return llmi_hip_dispatch_count(LLMI_HIP_OP_PAGED_GQA, &p.gqa);
+    if (!p.gqa.kv.tokens || !p.gqa.kv.sequences || check_paged_heads(p.gqa))
+      return 0;
+    return paged_shared_launches(p.gqa.kv, p.gqa.queryHeads, p.groups);
+  }
+  case LLMI_HIP_OP_PAGED_FORK:
+    return static_cast<const PagedForkParams *>(params)->children ? 1 : 0;
+  case LLMI_HIP_OP_PAGED_FREE: {
+    const PagedFreeParams &p = *static_cast<const PagedFreeParams *>(params);
+    return check_free(p) ? 0 : paged_free_launches(p);
+  }
+  case LLMI_HIP_OP_PAGED_MOVE: {
+    const PagedKvParams &p = *static_cast<const PagedKvParams *>(params);
+    return p.tokens && p.sequences ? 2 : 0;
   }
   case LLMI_HIP_OP_GATED_ATTENTION: {
     // Launches for a rotary width the kernels take (a multiple of 16).
@@ -1396,6 +1562,23 @@ const char *llmi_hip_kernel_name(int op, const void *params, unsigned index) {
                              static_cast<const PagedGqaParams *>(params)->queryHeads)
                ? "pagedGqaTiles"
                : "pagedGqaSplit";
+  case LLMI_HIP_OP_PAGED_GQA_SHARED: {
+    const PagedSharedParams &p = *static_cast<const PagedSharedParams *>(params);
+    if (!p.groups)
+      return llmi_hip_kernel_name(LLMI_HIP_OP_PAGED_GQA, &p.gqa, index);
+    if (index + 1 == llmi_hip_dispatch_count(op, params))
+      return "pagedSharedMerge";
+    return paged_shared_tiled(p.gqa.kv, p.gqa.queryHeads, p.groups, index) ? "pagedGqaTiles"
+                                                                          : "pagedGqaSplit";
+  }
+  case LLMI_HIP_OP_PAGED_FORK:
+    return "pagedFork";
+  case LLMI_HIP_OP_PAGED_FREE:
+    return llmi_hip_dispatch_count(op, params) == 1 ? "pagedFree"
+           : index                                  ? "pagedFreeList"
+                                                    : "pagedFreeMark";
+  case LLMI_HIP_OP_PAGED_MOVE:
+    return index ? "pagedPlace" : "pagedGather";
   case LLMI_HIP_OP_GATED_ATTENTION:
     if (static_cast<const GqaParams *>(params)->tokens == 1)
       return index == 0 ? "gqaDecodeGated" : "gqaDecodeMergeGated";

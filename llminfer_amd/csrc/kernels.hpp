@@ -308,4 +308,32 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
                             uint32_t *invalid, void *workspace, const PagedKvParams &p,
                             unsigned queryHeads, float scale, hipStream_t stream);
 
+// Sequences in groups with shared keys; `groups` of them, at least one.
+bool paged_shared_launchable(const PagedKvParams &p, unsigned queryHeads, unsigned groups);
+size_t paged_shared_workspace_bytes(const PagedKvParams &p, unsigned queryHeads, unsigned groups);
+unsigned paged_shared_launches(const PagedKvParams &p, unsigned queryHeads, unsigned groups);
+// Whether the tiles' kernel runs for the shared keys, or for the others.
+bool paged_shared_tiled(const PagedKvParams &p, unsigned queryHeads, unsigned groups, bool rest);
+hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, const int32_t *past,
+                                   const int32_t *table, const int32_t *groups,
+                                   const int32_t *prefix, const void *pool, uint16_t *out,
+                                   uint32_t *invalid, void *workspace, const PagedKvParams &p,
+                                   unsigned queryHeads, float scale, unsigned count,
+                                   hipStream_t stream);
+
+// The pages of the cache (paged_pages.hip).
+hipError_t launch_paged_fork(const int32_t *table, const int32_t *past, const int32_t *parent,
+                             const int32_t *spare, int32_t *tableOut, int32_t *pastOut, void *pool,
+                             uint32_t *invalid, const PagedForkParams &p, hipStream_t stream);
+unsigned paged_free_launches(const PagedFreeParams &p);
+size_t paged_free_workspace_bytes(const PagedFreeParams &p);
+hipError_t launch_paged_free(const int32_t *table, const int32_t *lengths, int32_t *free,
+                             int32_t *count, uint32_t *invalid, void *workspace,
+                             const PagedFreeParams &p, hipStream_t stream);
+size_t paged_move_workspace_bytes(const PagedKvParams &p);
+hipError_t launch_paged_move(const int32_t *source, const int32_t *sourceTable,
+                             const int32_t *starts, const int32_t *past, const int32_t *table,
+                             void *pool, uint32_t *invalid, void *workspace, const PagedKvParams &p,
+                             hipStream_t stream);
+
 } // namespace llmi

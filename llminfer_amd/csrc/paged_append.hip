@@ -28,17 +28,6 @@ struct AppendRows {
   float factor;
 };
 
-// Blocks that a sequence's rows touch.
-__device__ __forceinline__ unsigned touched_blocks(const PagedSeq &q) {
-  return q.rows ? (q.past % 32 + q.rows + 31) / 32 : 0u;
-}
-// At most as many units as that over any sequences: n rows touch at most
-// (n + 62) / 32 blocks, and at most n.
-unsigned most_units(unsigned tokens, unsigned sequences) {
-  const uint64_t n = (uint64_t)tokens / 32 + 2 * (uint64_t)sequences;
-  return (unsigned)(n < tokens ? n : tokens);
-}
-
 // Keys that one workgroup takes of a block: eight channels a thread.
 constexpr unsigned keys_a_group(unsigned D) { return 8 * kThreads / D; }
 constexpr unsigned key_groups(unsigned D) { return 32 / keys_a_group(D); }
@@ -286,33 +275,13 @@ __device__ __forceinline__ bool append_values(const uint16_t (&x)[8], unsigned q
   return bad;
 }
 
-// Where a workgroup's block lies in its sequence and in the call.
-struct AppendBlock {
-  unsigned seq, base, first, last, row; // keys [first, last) at position base, from row `row`
-  bool ok;
-};
-__device__ __forceinline__ bool find_block(const PagedView &g, AppendBlock &b) {
-  unsigned local, before;
-  const PagedSeq own = paged_own(g);
-  if (!paged_find(g, own, blockIdx.x, [](const PagedSeq &q) { return touched_blocks(q); }, b.seq,
-                  local, before))
-    return false;
-  const PagedSeq q = paged_seq_of(g, own, b.seq);
-  b.base = q.past / 32 * 32 + 32 * local;
-  b.first = b.base < q.past ? q.past - b.base : 0u;
-  b.last = min(32u, q.past + q.rows - b.base);
-  b.row = q.row0 + (b.base + b.first - q.past);
-  b.ok = q.ok;
-  return true;
-}
-
 template <int D, bool VEC>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(
     const uint16_t *__restrict__ keys, const uint16_t *__restrict__ values, PagedView g,
     const float *__restrict__ freqs, uint8_t *pool, unsigned *invalid, AppendRows p) {
   extern __shared__ float2 sTurn[]; // [key of this workgroup][half]
-  AppendBlock b;
-  if (!find_block(g, b))
+  PagedRun b;
+  if (!paged_run(g, b))
     return;
   // blockIdx.z: the values of one of this workgroup's heads (first: they take
   // longest), then groups of keys. Rows are loaded before the place they go
@@ -400,8 +369,8 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(const uint8_t *__r
                                                               unsigned *invalid) {
   constexpr unsigned PITCH = D + 8;
   __shared__ __attribute__((aligned(16))) half_t sRow[32 * PITCH];
-  AppendBlock b;
-  if (!find_block(g, b))
+  PagedRun b;
+  if (!paged_run(g, b))
     return;
   const unsigned head = blockIdx.y, tid = threadIdx.x, lane = tid % 64;
   size_t at = 0;
@@ -453,7 +422,7 @@ hipError_t launch_paged_append(const uint16_t *keys, const uint16_t *values, con
                                void *pool, uint32_t *invalid, const PagedKvParams &p,
                                const PagedAppendParams &a, hipStream_t stream) {
   const PagedView g = paged_view(p, starts, past, table);
-  const unsigned units = most_units(p.tokens, p.sequences), groups = key_groups(p.headDim);
+  const unsigned units = paged_most_runs(p.tokens, p.sequences), groups = key_groups(p.headDim);
   // A workgroup's turns serve as many heads as leave two workgroups a CU (6357
   // rows of 8 heads of 128, all of them rotated: 28.6 us with their reading
   // back, 34.3 with a head a workgroup).
@@ -490,7 +459,7 @@ hipError_t launch_paged_read(const void *pool, const int32_t *starts, const int3
                              uint32_t *invalid, const PagedKvParams &p, hipStream_t stream) {
   const PagedView g = paged_view(p, starts, past, table);
   auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(most_units(p.tokens, p.sequences), p.kvHeads, 2),
+    hipLaunchKernelGGL(kernel, dim3(paged_most_runs(p.tokens, p.sequences), p.kvHeads, 2),
                        dim3(kThreads), 0, stream, static_cast<const uint8_t *>(pool), g, keys,
                        values, invalid);
     return hipGetLastError();

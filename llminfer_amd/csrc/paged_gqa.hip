@@ -32,6 +32,7 @@
 #include "kernels.hpp"
 #include "paged_kv.hpp"
 #include "paged_plan.hpp"
+#include "paged_shared.hpp"
 
 #include <math.h>
 #include <type_traits>
@@ -138,23 +139,23 @@ template <int Ctrl, int Banks> __device__ __forceinline__ float shifted_in(float
                                                                0xF, Banks, false));
 }
 
-template <int D, int CG, int W>
+template <int D, int CG, int W, typename View>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * W, 64 * W),
                           amdgpu_waves_per_eu(Geo<D, CG, W>::RESIDENT)))
-void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool, PagedView g,
+void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool, View g,
                       half_t *out, unsigned *invalid, unsigned queryHeads, SplitPlan plan,
                       ScoreScale c, Partials parts) {
   using Geom = Geo<D, CG, W>;
   constexpr unsigned kUnit = CG * kColumns, kWaves = W;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.y;
-  const PagedSeq own = paged_own(g);
+  const auto own = paged_own(g);
   const Split split = paged_split(g, own, G, plan);
   unsigned seq, local, before;
   if (!paged_find(g, own, blockIdx.x,
-                  [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq, local,
+                  [&](const auto &s) { return split.units(s) * split.pieces(s); }, seq, local,
                   before))
     return;
-  const PagedSeq s = paged_seq_of(g, own, seq);
+  const auto s = paged_seq_of(g, own, seq);
   // (the last units first: they see most keys)
   const unsigned pieces = split.pieces(s), units = split.units(s);
   const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
@@ -171,7 +172,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   };
 #pragma unroll
   for (int j = 0; j < CG; ++j) {
-    visible[j] = s.past + token_of(kColumns * j + r);
+    visible[j] = s.last(token_of(kColumns * j + r));
     row[j] = row_of(kColumns * j + r);
   }
   auto live = [&](int j) { return kColumns * j + r < columns; };
@@ -184,13 +185,14 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       atomicOr(invalid, kPagedPlace);
     return;
   }
-  const unsigned least = s.past + c0 / G;                // the first column's last key
-  const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
+  const unsigned least = s.last(c0 / G);                // the first column's last key
+  const unsigned most = s.last((c0 + columns - 1) / G); // the last column's
   // the keys that this wave has: to the sequence's end, or to a page that is not
   // in the pool, whose columns' outputs are NaN
-  const unsigned whole = s.past + s.rows;
+  const unsigned whole = s.keys();
   unsigned end = whole;
-  const unsigned length = split.length(s, pieces), b0 = min(piece * length, most / 32 + 1);
+  const unsigned length = split.length(s, pieces);
+  const unsigned b0 = min(s.first() + piece * length, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned mine = b1 > b0 + wave ? (b1 - b0 - wave + kWaves - 1) / kWaves : 0u;
 
@@ -200,7 +202,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
     const unsigned b = b0 + wave + kWaves * (k + lane);
     bool lost = false;
     if (b < b1)
-      lost = !paged_block(g, seq, 32 * b, kvh, place);
+      lost = !paged_block(g, s.table(seq), 32 * b, kvh, place);
     if (const unsigned long long all = __builtin_amdgcn_ballot_w64(lost))
       end = min(end, 32 * (b0 + wave + kWaves * (k + (unsigned)__builtin_ctzll(all))));
   };
@@ -462,7 +464,7 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       sum += sL[w * kUnit + col] * a[w];
     }
     const size_t part = ((size_t)blockIdx.x * g.kvHeads + kvh) * kUnit + col;
-    const float scale = pieces == 1 ? 1.0f / sum : 1.0f;
+    const float scale = pieces == 1 && !s.joined() ? 1.0f / sum : 1.0f;
     const size_t to = F == 1 ? row[j] : row_of(col);
     for (unsigned i = wave; i < kTiles; i += kWaves) {
       float4_t y{0, 0, 0, 0};
@@ -472,14 +474,14 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
       if (col >= columns)
         continue;
       const unsigned channel = 16 * (F * i + r / kCols) + 4 * quad;
-      if (pieces == 1)
+      if (pieces == 1 && !s.joined())
         *reinterpret_cast<half4_t *>(out + to + channel) =
             half4_t{(half_t)(y[0] * scale), (half_t)(y[1] * scale), (half_t)(y[2] * scale),
                     (half_t)(y[3] * scale)};
       else
         *reinterpret_cast<float4_t *>(parts.o + part * D + channel) = y;
     }
-    if (pieces > 1 && wave == 0 && lane < kCols && col < columns)
+    if ((pieces > 1 || s.joined()) && wave == 0 && lane < kCols && col < columns)
       *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
   };
   if constexpr (CG == 1) {
@@ -605,6 +607,170 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
   }
 }
 
+// ------------------------------------------------ sequences in groups
+
+// A launch over a SharedView: its plan, its partials and how many pieces it has.
+struct SharedPart {
+  SharedView g;
+  SplitPlan plan;
+  Partials parts;
+  unsigned most;
+};
+
+// Pieces of the sequences before `seq`.
+template <typename View>
+__device__ __forceinline__ unsigned pieces_before(const View &g, const typename View::Seq &own,
+                                                  const Split &split, unsigned seq) {
+  const unsigned lane = threadIdx.x % 64;
+  unsigned before = 0;
+  for (unsigned s0 = 0; s0 <= seq; s0 += 64) {
+    const typename View::Seq o =
+        s0 ? (s0 + lane < g.sequences ? paged_seq(g, s0 + lane) : typename View::Seq{0, 0, 0, true})
+           : own;
+    const unsigned n = split.units(o) * split.pieces(o), sum = wave_scan(n);
+    const int at = seq - s0 < 64 ? (int)(seq - s0) : 63;
+    before += (unsigned)__builtin_amdgcn_readlane((int)(seq - s0 < 64 ? sum - n : sum), at);
+  }
+  return before;
+}
+
+// Joins a row's partials: those of its sequence's own keys and those of its
+// group's shared ones, from one launch (`apart` false: both parts are the same)
+// or from two. An item is a query head of a row, as in paged_gqa_merge_kernel,
+// the work of a workgroup's eight waves.
+template <int D>
+__global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
+    SharedPart shared, SharedPart rest, bool apart, half_t *out, unsigned queryHeads) {
+  constexpr int N = D / 64;
+  constexpr unsigned W = kMergeThreads / 64;
+  typedef float vec __attribute__((ext_vector_type(N)));
+  typedef _Float16 halves __attribute__((ext_vector_type(N)));
+  const SharedView &g = rest.g;
+  const unsigned G = queryHeads / g.kvHeads;
+  const SharedSeq own = paged_own(g);
+  const Split split = paged_split(g, own, G, rest.plan);
+  const SharedSeq ownShared = apart ? paged_own(shared.g) : own;
+  const Split splitShared = apart ? paged_split(shared.g, ownShared, G, shared.plan) : split;
+  const unsigned lane = threadIdx.x % 64;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  __shared__ float sM[W], sL[W];
+  __shared__ vec sY[W][64];
+  // (the same item in every wave, so all of them leave together)
+  for (unsigned item = blockIdx.x;; item += gridDim.x) {
+    unsigned seq, local, before;
+    if (!paged_find(g, own, item,
+                    [&](const SharedSeq &s) {
+                      return s.step && s.ok && (s.joined() || split.pieces(s) > 1)
+                                 ? s.rows * queryHeads
+                                 : 0u;
+                    },
+                    seq, local, before))
+      return;
+    const SharedSeq s = paged_seq_of(g, own, seq);
+    const unsigned h = local % queryHeads, row = local / queryHeads, kvh = h / G;
+    float m = -INFINITY, l = 0.0f;
+    vec y = 0.0f;
+    // column `column` of the pieces of a sequence; false where starts out of
+    // order make more of them than the rows can have
+    auto join = [&](const SharedPart &part, const SharedSeq &of, const Split &by, unsigned at,
+                    const SharedSeq &lanes, unsigned column, unsigned turn) {
+      const unsigned unit = 1u << part.plan.shift, pieces = by.pieces(of), units = by.units(of);
+      const unsigned first =
+          pieces_before(part.g, lanes, by, at) + (units - 1 - column / unit) * pieces;
+      if (column / unit >= units || first >= part.most || pieces > part.most - first)
+        return false;
+      const size_t place = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
+      const size_t step = (size_t)g.kvHeads * unit;
+      const float2 *ml = reinterpret_cast<const float2 *>(part.parts.ml) + place;
+      const vec *po = reinterpret_cast<const vec *>(part.parts.o + place * D) + lane;
+      for (unsigned i0 = (wave + turn) % W; i0 < pieces; i0 += 4 * W) {
+        float2 x[4];
+        vec o[4];
+#pragma unroll
+        for (unsigned n = 0; n < 4; ++n) {
+          const unsigned i = min(i0 + W * n, pieces - 1);
+          x[n] = ml[step * i];
+          o[n] = po[step * i * 64];
+        }
+        float to = m;
+#pragma unroll
+        for (unsigned n = 0; n < 4; ++n) {
+          x[n].x = i0 + W * n < pieces ? x[n].x : -INFINITY;
+          to = fmaxf(to, x[n].x);
+        }
+        const float a = m == -INFINITY ? 0.0f : fast_exp2(m - to);
+        l *= a;
+        y *= a;
+#pragma unroll
+        for (unsigned n = 0; n < 4; ++n)
+          if (x[n].x != -INFINITY) {
+            const float b = fast_exp2(x[n].x - to);
+            l += x[n].y * b;
+            y += o[n] * b;
+          }
+        m = to;
+      }
+      return true;
+    };
+    bool whole = join(rest, s, split, seq, own, row * G + h % G, 0);
+    if (s.begin) {
+      unsigned group = 0;
+      shared_group(g, s.from, group);
+      const SharedSeq p = paged_seq_of(shared.g, ownShared, group);
+      whole = join(shared, p, splitShared, group, ownShared,
+                   (s.row0 + row - p.row0) * G + h % G, split.pieces(s)) && whole;
+    }
+    sM[wave] = m;
+    sL[wave] = l;
+    sY[wave][lane] = y;
+    __syncthreads();
+    m = sM[0];
+    for (unsigned w = 1; w < W; ++w)
+      m = fmaxf(m, sM[w]);
+    l = 0.0f;
+    y = 0.0f;
+    for (unsigned w = 0; w < W; ++w) {
+      const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - m);
+      l += sL[w] * a;
+      y += sY[w][lane] * a;
+    }
+    __syncthreads();
+    if (wave == 0 && whole) {
+      halves z;
+      for (int i = 0; i < N; ++i)
+        z[i] = (half_t)(y[i] / l);
+      reinterpret_cast<halves *>(out + ((size_t)(s.row0 + row) * queryHeads + h) * D)[lane] = z;
+    }
+  }
+}
+
+// The kernel of a plan, over the sequences of a view.
+template <typename View>
+hipError_t launch_attend(const half_t *q, const uint8_t *pool, const View &g, half_t *out,
+                         unsigned *invalid, unsigned queryHeads, const GqaPlan &by, ScoreScale c,
+                         Partials parts, unsigned pieces, hipStream_t stream) {
+  const SplitPlan &plan = by.split;
+  const unsigned unit = 1u << plan.shift;
+  auto attend = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(pieces, g.kvHeads), dim3(64 * plan.step), 0, stream, q, pool, g,
+                       out, invalid, queryHeads, plan, c, parts);
+    return hipGetLastError();
+  };
+  auto by_columns = [&](auto one, auto pooled, auto more) {
+    return attend(unit > 16 ? more : by.pooled ? pooled : one);
+  };
+  if (unit > 64)
+    return launch_paged_tiles(q, pool, g, out, invalid, queryHeads, plan, c, parts, pieces, stream);
+  if (g.dim == 256)
+    return by_columns(paged_gqa_kernel<256, 1, 4, View>, paged_gqa_kernel<256, 1, 8, View>,
+                      paged_gqa_kernel<256, 2, 4, View>);
+  if (g.dim == 128)
+    return by_columns(paged_gqa_kernel<128, 1, 4, View>, paged_gqa_kernel<128, 1, 8, View>,
+                      paged_gqa_kernel<128, 2, 4, View>);
+  return by_columns(paged_gqa_kernel<64, 1, 4, View>, paged_gqa_kernel<64, 1, 8, View>,
+                    paged_gqa_kernel<64, 4, 4, View>);
+}
+
 size_t partial_columns(const PagedKvParams &p, unsigned group, const SplitPlan &plan) {
   return (size_t)most_pieces(p, group, plan) * p.kvHeads << plan.shift;
 }
@@ -646,26 +812,8 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
   const half_t *from = reinterpret_cast<const half_t *>(q);
   const uint8_t *pages = static_cast<const uint8_t *>(pool);
   const ScoreScale c = score_scale(scale);
-  auto attend = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(pieces, p.kvHeads), dim3(64 * plan.step), 0,
-                       stream, from, pages, g, to, invalid, queryHeads, plan, c, parts);
-    return hipGetLastError();
-  };
-  auto by_columns = [&](auto one, auto pooled, auto more) {
-    return attend(unit > 16 ? more : both.pooled ? pooled : one);
-  };
-  hipError_t e;
-  if (unit > 64)
-    e = launch_paged_tiles(from, pages, g, to, invalid, queryHeads, plan, c, parts, pieces, stream);
-  else if (p.headDim == 256)
-    e = by_columns(paged_gqa_kernel<256, 1, 4>, paged_gqa_kernel<256, 1, 8>,
-                   paged_gqa_kernel<256, 2, 4>);
-  else if (p.headDim == 128)
-    e = by_columns(paged_gqa_kernel<128, 1, 4>, paged_gqa_kernel<128, 1, 8>,
-                   paged_gqa_kernel<128, 2, 4>);
-  else
-    e = by_columns(paged_gqa_kernel<64, 1, 4>, paged_gqa_kernel<64, 1, 8>,
-                   paged_gqa_kernel<64, 4, 4>);
+  const hipError_t e =
+      launch_attend(from, pages, g, to, invalid, queryHeads, both, c, parts, pieces, stream);
   if (e != hipSuccess)
     return e;
   if (!may_divide(p, plan))
@@ -686,6 +834,106 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
   return p.headDim == 256   ? merge(paged_gqa_merge_kernel<256, 8>, paged_gqa_merge_kernel<256, 1>)
          : p.headDim == 128 ? merge(paged_gqa_merge_kernel<128, 8>, paged_gqa_merge_kernel<128, 1>)
                             : merge(paged_gqa_merge_kernel<64, 8>, paged_gqa_merge_kernel<64, 1>);
+}
+
+// ------------------------------------------------ sequences in groups
+
+namespace {
+
+// The groups' shared keys and the sequences' own: in one launch, or apart where
+// the shared keys have columns for a kernel that would waste most of itself on
+// a sequence's few.
+struct SharedPlan {
+  bool apart;
+  GqaPlan shared, rest;
+  uint64_t sharedPieces, restPieces; // a KV head, at most
+};
+SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) {
+  PagedKvParams of = p;
+  of.sequences = groups;
+  SharedPlan s;
+  s.shared = plan_for(of, group);
+  s.rest = plan_for(p, group);
+  s.apart = s.shared.split.shift > 5;
+  s.sharedPieces = most_pieces(of, group, s.shared.split);
+  if (!s.apart) {
+    s.rest = s.shared;
+    s.sharedPieces += most_units(p, group, 1u << s.shared.split.shift);
+    s.restPieces = s.sharedPieces;
+  } else
+    s.restPieces = most_pieces(p, group, s.rest.split);
+  return s;
+}
+size_t shared_columns(const PagedKvParams &p, const SharedPlan &s) {
+  return (size_t)s.sharedPieces * p.kvHeads << s.shared.split.shift;
+}
+size_t rest_columns(const PagedKvParams &p, const SharedPlan &s) {
+  return s.apart ? (size_t)s.restPieces * p.kvHeads << s.rest.split.shift : 0;
+}
+
+} // namespace
+
+bool paged_shared_launchable(const PagedKvParams &p, unsigned queryHeads, unsigned groups) {
+  const SharedPlan s = shared_plan(p, queryHeads / p.kvHeads, groups);
+  return (uint64_t)p.tokens * queryHeads <= 0x7fffffffull &&
+         s.sharedPieces * p.kvHeads < (1u << 22) && s.restPieces * p.kvHeads < (1u << 22);
+}
+size_t paged_shared_workspace_bytes(const PagedKvParams &p, unsigned queryHeads, unsigned groups) {
+  const SharedPlan s = shared_plan(p, queryHeads / p.kvHeads, groups);
+  return 4 * (p.headDim + 2) * (shared_columns(p, s) + rest_columns(p, s));
+}
+unsigned paged_shared_launches(const PagedKvParams &p, unsigned queryHeads, unsigned groups) {
+  return shared_plan(p, queryHeads / p.kvHeads, groups).apart ? 3 : 2;
+}
+bool paged_shared_tiled(const PagedKvParams &p, unsigned queryHeads, unsigned groups, bool rest) {
+  const SharedPlan s = shared_plan(p, queryHeads / p.kvHeads, groups);
+  return (rest ? s.rest : s.shared).split.shift > 6;
+}
+
+hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, const int32_t *past,
+                                   const int32_t *table, const int32_t *groups,
+                                   const int32_t *prefix, const void *pool, uint16_t *out,
+                                   uint32_t *invalid, void *workspace, const PagedKvParams &p,
+                                   unsigned queryHeads, float scale, unsigned count,
+                                   hipStream_t stream) {
+  const SharedPlan s = shared_plan(p, queryHeads / p.kvHeads, count);
+  const ScoreScale c = score_scale(scale);
+  const half_t *from = reinterpret_cast<const half_t *>(q);
+  const uint8_t *pages = static_cast<const uint8_t *>(pool);
+  half_t *to = reinterpret_cast<half_t *>(out);
+  float *ws = static_cast<float *>(workspace);
+  const size_t sharedColumns = shared_columns(p, s), restColumns = rest_columns(p, s);
+  auto part = [&](const GqaPlan &by, uint64_t pieces, float *at, size_t columns, unsigned base,
+                  unsigned sequences) {
+    SharedPart x{SharedView{paged_view(p, starts, past, table), groups, prefix, count, p.sequences,
+                            base},
+                 by.split, Partials{at + columns * p.headDim, at}, (unsigned)pieces};
+    x.g.sequences = sequences;
+    return x;
+  };
+  const SharedPart shared = part(s.shared, s.sharedPieces, ws, sharedColumns, 0,
+                                 s.apart ? count : count + p.sequences);
+  const SharedPart rest =
+      s.apart ? part(s.rest, s.restPieces, ws + sharedColumns * (p.headDim + 2), restColumns, count,
+                     p.sequences)
+              : shared;
+  auto attend = [&](const SharedPart &x, const GqaPlan &by) {
+    return launch_attend(from, pages, x.g, to, invalid, queryHeads, by, c, x.parts, x.most, stream);
+  };
+  hipError_t e = attend(shared, s.shared);
+  if (e == hipSuccess && s.apart)
+    e = attend(rest, s.rest);
+  if (e != hipSuccess)
+    return e;
+  auto merge = [&](auto kernel) {
+    const uint64_t items = (uint64_t)p.tokens * queryHeads;
+    hipLaunchKernelGGL(kernel, dim3(items < kMergeGroups ? (unsigned)items : kMergeGroups),
+                       dim3(kMergeThreads), 0, stream, shared, rest, s.apart, to, queryHeads);
+    return hipGetLastError();
+  };
+  return p.headDim == 256   ? merge(paged_shared_merge_kernel<256>)
+         : p.headDim == 128 ? merge(paged_shared_merge_kernel<128>)
+                            : merge(paged_shared_merge_kernel<64>);
 }
 
 } // namespace llmi

@@ -31,7 +31,23 @@ constexpr float kPagedLimit = 16384.0f; // values are kept to +-this: 16 s and b
 constexpr unsigned kPagedValue = 1u; // a value not finite or past the limit
 constexpr unsigned kPagedPlace = 2u; // a row whose place is not in its table or the pool
 
+// Rows [row0, row0 + rows) of the call, at positions past + i. ok: they fit
+// their table.
+struct PagedSeq {
+  unsigned row0, rows, past;
+  bool ok;
+  // What the attention asks of a sequence (SharedSeq has other answers): its
+  // keys, the block of 32 that they begin with, the last key that a row sees,
+  // its row of the table, whether other keys are joined to these.
+  __device__ unsigned keys() const { return past + rows; }
+  __device__ unsigned first() const { return 0; }
+  __device__ unsigned last(unsigned row) const { return past + row; }
+  __device__ unsigned table(unsigned seq) const { return seq; }
+  __device__ bool joined() const { return false; }
+};
+
 struct PagedView {
+  typedef PagedSeq Seq;
   const int32_t *starts, *past, *table;
   unsigned pages, pageSize, kvHeads, dim, sequences, tableStride, tokens;
 };
@@ -41,13 +57,6 @@ inline PagedView paged_view(const PagedKvParams &p, const int32_t *starts, const
   return PagedView{starts,     past,        table,         p.pages,  p.pageSize, p.kvHeads,
                    p.headDim, p.sequences, p.tableStride, p.tokens};
 }
-
-// Rows [row0, row0 + rows) of the call, at positions past + i. ok: they fit
-// their table.
-struct PagedSeq {
-  unsigned row0, rows, past;
-  bool ok;
-};
 
 __device__ __forceinline__ PagedSeq paged_seq(const PagedView &g, unsigned s) {
   const int T = (int)g.tokens;
@@ -157,16 +166,17 @@ __device__ __forceinline__ unsigned wave_scan(unsigned x) {
 // and how many units come before the sequence's. Every lane of a full wave
 // calls it; false past the last unit. `own` is paged_seq of sequence `lane`
 // (nothing past the last one).
-template <typename Count>
-__device__ __forceinline__ bool paged_find(const PagedView &g, const PagedSeq &own, unsigned u,
-                                           Count count, unsigned &seq, unsigned &local,
+template <typename View, typename Count>
+__device__ __forceinline__ bool paged_find(const View &g, const typename View::Seq &own,
+                                           unsigned u, Count count, unsigned &seq, unsigned &local,
                                            unsigned &before) {
   const unsigned lane = threadIdx.x % 64;
+  typedef typename View::Seq Seq;
   before = 0;
-  PagedSeq q = own;
+  Seq q = own;
   for (unsigned s0 = 0; s0 < g.sequences; s0 += 64) {
     if (s0)
-      q = s0 + lane < g.sequences ? paged_seq(g, s0 + lane) : PagedSeq{0, 0, 0, true};
+      q = s0 + lane < g.sequences ? paged_seq(g, s0 + lane) : Seq{0, 0, 0, true};
     const unsigned n = count(q), sum = wave_scan(n);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(u - before < sum);
     if (past) {
@@ -181,21 +191,56 @@ __device__ __forceinline__ bool paged_find(const PagedView &g, const PagedSeq &o
   }
   return false;
 }
-__device__ __forceinline__ PagedSeq paged_own(const PagedView &g) {
+template <typename View> __device__ __forceinline__ typename View::Seq paged_own(const View &g) {
   const unsigned lane = threadIdx.x % 64;
-  return lane < g.sequences ? paged_seq(g, lane) : PagedSeq{0, 0, 0, true};
+  return lane < g.sequences ? paged_seq(g, lane) : typename View::Seq{0, 0, 0, true};
 }
 // One of the sequences, the same in every lane.
-__device__ __forceinline__ PagedSeq paged_seq_of(const PagedView &g, const PagedSeq &own,
-                                                 unsigned seq) {
-  if (seq >= 64)
-    return paged_seq(g, seq);
+__device__ __forceinline__ PagedSeq paged_from_lane(const PagedSeq &own, unsigned lane) {
   PagedSeq q;
-  q.row0 = (unsigned)__builtin_amdgcn_readlane((int)own.row0, (int)seq);
-  q.rows = (unsigned)__builtin_amdgcn_readlane((int)own.rows, (int)seq);
-  q.past = (unsigned)__builtin_amdgcn_readlane((int)own.past, (int)seq);
-  q.ok = __builtin_amdgcn_readlane((int)own.ok, (int)seq);
+  q.row0 = (unsigned)__builtin_amdgcn_readlane((int)own.row0, (int)lane);
+  q.rows = (unsigned)__builtin_amdgcn_readlane((int)own.rows, (int)lane);
+  q.past = (unsigned)__builtin_amdgcn_readlane((int)own.past, (int)lane);
+  q.ok = __builtin_amdgcn_readlane((int)own.ok, (int)lane);
   return q;
+}
+template <typename View>
+__device__ __forceinline__ typename View::Seq paged_seq_of(const View &g,
+                                                           const typename View::Seq &own,
+                                                           unsigned seq) {
+  return seq >= 64 ? paged_seq(g, seq) : paged_from_lane(own, seq);
+}
+
+// Blocks that a sequence's rows touch.
+__device__ __forceinline__ unsigned touched_blocks(const PagedSeq &q) {
+  return q.rows ? (q.past % 32 + q.rows + 31) / 32 : 0u;
+}
+// At most as many as that over any sequences: n rows touch at most (n + 62) /
+// 32 blocks, and at most n.
+inline unsigned paged_most_runs(unsigned tokens, unsigned sequences) {
+  const uint64_t n = (uint64_t)tokens / 32 + 2 * (uint64_t)sequences;
+  return (unsigned)(n < tokens ? n : tokens);
+}
+
+// Where the rows of a workgroup (blockIdx.x) lie, those of one block, in their
+// sequence and in the call.
+struct PagedRun {
+  unsigned seq, base, first, last, row; // keys [first, last) at position base, from row `row`
+  bool ok;
+};
+__device__ __forceinline__ bool paged_run(const PagedView &g, PagedRun &b) {
+  unsigned local, before;
+  const PagedSeq own = paged_own(g);
+  if (!paged_find(g, own, blockIdx.x, [](const PagedSeq &q) { return touched_blocks(q); }, b.seq,
+                  local, before))
+    return false;
+  const PagedSeq q = paged_seq_of(g, own, b.seq);
+  b.base = q.past / 32 * 32 + 32 * local;
+  b.first = b.base < q.past ? q.past - b.base : 0u;
+  b.last = min(32u, q.past + q.rows - b.base);
+  b.row = q.row0 + (b.base + b.first - q.past);
+  b.ok = q.ok;
+  return true;
 }
 
 } // namespace llmi

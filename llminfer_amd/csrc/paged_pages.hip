@@ -1,0 +1,488 @@
+// The pages of the paged 4-bit cache (paged_kv.hpp) as sequences come and go:
+// children that share their parents' pages (fork), the pages that no sequence
+// holds (free), chosen keys and values put side by side (move). No arithmetic,
+// so bytes and latency are what there is to gain.
+#include "hip_common.hpp"
+#include "kernels.hpp"
+#include "paged_kv.hpp"
+
+namespace llmi {
+namespace {
+
+// -------------------------------------------------------------------- fork
+
+constexpr unsigned kForkThreads = 256;
+
+struct ForkView {
+  const int32_t *table, *past, *parent, *spare;
+  int32_t *tableOut, *pastOut;
+  unsigned pages, pageSize, kvHeads, sequences, tableStride;
+};
+
+// A workgroup copies one block of one head of a child's last page; the first
+// of a child writes its row of the table too.
+template <int D>
+__global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(ForkView g, uint4_t *pool,
+                                                                  unsigned *invalid) {
+  constexpr unsigned kWords = 40 * D / 16, kEach = (kWords + kForkThreads - 1) / kForkThreads;
+  const unsigned blocks = g.pageSize / 32, parts = g.kvHeads * blocks;
+  const unsigned child = blockIdx.x / parts, part = blockIdx.x % parts, tid = threadIdx.x;
+  const unsigned parent = (unsigned)g.parent[child];
+  const int spare = g.spare[child];
+  const int held = parent < g.sequences ? g.past[parent] : -1;
+  const bool ok = held >= 0 && (long long)held <= (long long)g.tableStride * g.pageSize;
+  const unsigned length = ok ? (unsigned)held : 0u, whole = length / g.pageSize;
+  const unsigned rest = length - whole * g.pageSize;
+  const int32_t *row = g.table + (size_t)(ok ? parent : 0u) * g.tableStride;
+  const bool taken = spare < 0; // the parent's pages as they are
+  const unsigned from = ok && rest ? (unsigned)row[whole] : 0u;
+  const bool fits = taken || ((unsigned)spare < g.pages && from < g.pages) ||
+                    whole == g.tableStride; // (a full table needs no page)
+  if (part == 0) {
+    int32_t *to = g.tableOut + (size_t)child * g.tableStride;
+    for (unsigned j = tid; j < g.tableStride; j += kForkThreads)
+      to[j] = !ok                 ? -1
+              : taken || j < whole ? row[j]
+              : j == whole && fits ? spare
+                                   : -1;
+    if (tid == 0) {
+      g.pastOut[child] = ok ? held : -1;
+      if (invalid && !(ok && fits))
+        atomicOr(invalid, kPagedPlace);
+    }
+  }
+  const unsigned block = part % blocks, head = part / blocks;
+  if (!ok || taken || !fits || 32 * block >= rest)
+    return;
+  const size_t at = ((size_t)head * blocks + block) * kWords;
+  const size_t page = (size_t)g.kvHeads * blocks * kWords;
+  const uint4_t *src = pool + from * page + at;
+  uint4_t *dst = pool + (unsigned)spare * page + at, x[kEach];
+#pragma unroll
+  for (unsigned i = 0; i < kEach; ++i)
+    if (tid + i * kForkThreads < kWords)
+      x[i] = src[tid + i * kForkThreads];
+#pragma unroll
+  for (unsigned i = 0; i < kEach; ++i)
+    if (tid + i * kForkThreads < kWords)
+      dst[tid + i * kForkThreads] = x[i];
+}
+
+// -------------------------------------------------------------------- free
+
+constexpr unsigned kFreeThreads = 1024;
+constexpr unsigned kFreeWaves = kFreeThreads / 64;
+constexpr unsigned kWindow = 1u << 19; // pages whose marks one workgroup has in LDS
+constexpr unsigned kListed = 8192;     // pages whose entries one workgroup writes
+constexpr unsigned kMarkers = 8;       // workgroups that mark, at most
+
+struct FreeView {
+  const int32_t *table, *lengths;
+  unsigned pages, pageSize, sequences, tableStride;
+};
+
+// The pages of window `window` that rows `part`, part + parts, ... of the
+// 1024-entry pieces of the tables name, as bits.
+__device__ __forceinline__ void mark_held(const FreeView &g, unsigned part, unsigned parts,
+                                          unsigned window, uint32_t *marks, unsigned *invalid) {
+  constexpr unsigned kAhead = 8;
+  const unsigned tid = threadIdx.x, first = window * kWindow;
+  const unsigned mine = min(kWindow, g.pages - first);
+  for (unsigned w = tid; w < (mine + 31) / 32; w += kFreeThreads)
+    marks[w] = 0;
+  __syncthreads();
+  const unsigned pieces = (g.tableStride + kFreeThreads - 1) / kFreeThreads; // of a row
+  const uint64_t all = (uint64_t)g.sequences * pieces;
+  bool lost = false;
+  for (uint64_t i0 = part; i0 < all; i0 += (uint64_t)kAhead * parts) {
+    int entry[kAhead];
+    bool held[kAhead];
+#pragma unroll
+    for (unsigned n = 0; n < kAhead; ++n) {
+      const uint64_t i = i0 + (uint64_t)n * parts;
+      const unsigned s = i < all ? (unsigned)(i / pieces) : 0u;
+      const unsigned slot = (unsigned)(i % pieces) * kFreeThreads + tid;
+      const int length = g.lengths[s];
+      const bool bad = length < 0 || (long long)length > (long long)g.tableStride * g.pageSize;
+      lost |= bad && i < all;
+      // (a sequence that does not fit its row holds all of it)
+      held[n] = i < all && slot < g.tableStride && (bad || (uint64_t)slot * g.pageSize < (unsigned)length);
+      entry[n] = held[n] ? g.table[(size_t)s * g.tableStride + slot] : 0;
+    }
+#pragma unroll
+    for (unsigned n = 0; n < kAhead; ++n) {
+      if (!held[n])
+        continue;
+      const unsigned page = (unsigned)entry[n];
+      lost |= page >= g.pages;
+      if (page < g.pages && page - first < mine)
+        atomicOr(&marks[(page - first) / 32], 1u << (page - first) % 32);
+    }
+  }
+  if (lost && invalid)
+    atomicOr(invalid, kPagedPlace);
+  __syncthreads();
+}
+
+// Entries of the pages [first, first + count), `before` of the pages before
+// them free: a free page at its rank, and for each other one a -1 from the end.
+// word(i) has the marks of pages 32 i .. 32 i + 31.
+template <typename Word>
+__device__ __forceinline__ void list_free(unsigned first, unsigned count, unsigned before,
+                                          unsigned pages, int32_t *free, int32_t *number,
+                                          Word word) {
+  __shared__ unsigned sBefore[kListed / 64 + 1];
+  const unsigned tid = threadIdx.x, lane = tid % 64;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const unsigned groups = (count + 63) / 64; // of 64 pages
+  auto held = [&](unsigned i) { // of group i; those behind the last page held
+    const unsigned at = first / 32 + 2 * i, left = count - 64 * i;
+    uint64_t x = word(at);
+    if (left > 32)
+      x |= (uint64_t)word(at + 1) << 32;
+    return left < 64 ? x | ~0ull << left : x;
+  };
+  // (kListed / 64 = 128 groups: two a lane of the first wave)
+  static_assert(kListed == 128 * 64, "two groups a lane below");
+  if (wave == 0) {
+    const unsigned a = 2 * lane < groups ? 64 - __builtin_popcountll(held(2 * lane)) : 0u;
+    const unsigned b = 2 * lane + 1 < groups ? 64 - __builtin_popcountll(held(2 * lane + 1)) : 0u;
+    const unsigned sum = before + wave_scan(a + b);
+    sBefore[2 * lane] = sum - a - b;
+    sBefore[2 * lane + 1] = sum - b;
+    if (lane == 63)
+      sBefore[kListed / 64] = sum;
+  }
+  __syncthreads();
+  for (unsigned i = wave; i < groups; i += kFreeWaves) {
+    const uint64_t x = held(i);
+    const unsigned page = first + 64 * i + lane;
+    const unsigned rank = sBefore[i] + (unsigned)__builtin_popcountll(~x & ((1ull << lane) - 1));
+    if (64 * i + lane < count) {
+      const bool isFree = !(x >> lane & 1);
+      free[isFree ? rank : pages - 1 - (page - rank)] = isFree ? (int)page : -1;
+    }
+  }
+  if (first + count == pages && tid == 0)
+    *number = (int)sBefore[kListed / 64];
+  __syncthreads();
+}
+
+// All of a small pool in one workgroup.
+__global__ __launch_bounds__(kFreeThreads) void paged_free_small_kernel(FreeView g, int32_t *free,
+                                                                        int32_t *count,
+                                                                        unsigned *invalid) {
+  __shared__ uint32_t marks[kListed / 32];
+  mark_held(g, 0, 1, 0, marks, invalid);
+  list_free(0, g.pages, 0, g.pages, free, count, [&](unsigned i) { return marks[i]; });
+}
+
+// Marks: [part][(pages + 31) / 32].
+__global__ __launch_bounds__(kFreeThreads) void paged_free_mark_kernel(FreeView g, uint32_t *out,
+                                                                       unsigned *invalid) {
+  __shared__ uint32_t marks[kWindow / 32];
+  const unsigned window = blockIdx.y, words = (g.pages + 31) / 32;
+  mark_held(g, blockIdx.x, gridDim.x, window, marks, invalid);
+  uint32_t *to = out + (size_t)blockIdx.x * words + window * (kWindow / 32);
+  const unsigned mine = min(kWindow / 32, words - window * (kWindow / 32));
+  for (unsigned w = threadIdx.x; w < mine; w += kFreeThreads)
+    to[w] = marks[w];
+}
+
+// kListed pages a workgroup, behind the free ones of all before.
+__global__ __launch_bounds__(kFreeThreads) void paged_free_list_kernel(const uint32_t *marks,
+                                                                       unsigned parts,
+                                                                       unsigned pages, int32_t *free,
+                                                                       int32_t *count) {
+  const unsigned words = (pages + 31) / 32, first = blockIdx.x * kListed, tid = threadIdx.x;
+  __shared__ unsigned sFree[kFreeWaves];
+  __shared__ uint32_t sWord[kListed / 32];
+  auto word = [&](unsigned i) {
+    uint32_t x = 0;
+    for (unsigned p = 0; p < parts; ++p)
+      x |= marks[(size_t)p * words + i];
+    return x;
+  };
+  unsigned n = 0;
+  for (unsigned i = tid; i < first / 32; i += kFreeThreads)
+    n += 32 - __builtin_popcount(word(i));
+  n = wave_scan(n);
+  if (tid % 64 == 63)
+    sFree[tid / 64] = n;
+  const unsigned mine = min(kListed, pages - first);
+  for (unsigned i = tid; i < (mine + 31) / 32; i += kFreeThreads)
+    sWord[i] = word(first / 32 + i);
+  __syncthreads();
+  n = 0;
+  for (unsigned w = 0; w < kFreeWaves; ++w)
+    n += sFree[w];
+  list_free(first, mine, n, pages, free, count,
+            [&](unsigned i) { return sWord[i - first / 32]; });
+}
+
+unsigned free_markers(const PagedFreeParams &p) {
+  const uint64_t slots = (uint64_t)p.sequences * p.tableStride, parts = slots / 16384;
+  return parts < 1 ? 1u : parts < kMarkers ? (unsigned)parts : kMarkers;
+}
+bool free_small(const PagedFreeParams &p) { return p.pages <= kListed && free_markers(p) == 1; }
+
+// -------------------------------------------------------------------- move
+//
+// Two launches, so that all rows are read before any is written, whichever
+// pages they come from and go to: the first makes the blocks as they will be
+// (kept keys of a block in a word), the second puts them into their places.
+// Codes and scales are laid out for the matrix instructions (paged_kv.hpp), so
+// what moves is 16 bytes (8 at D 64) for 32 (16) channels of a key, but a
+// nibble of a word for a channel of a value: a thread has four channels of eight
+// keys, eight loads for a store.
+
+constexpr unsigned kMoveThreads = 256;
+
+// A block's 16-byte words: key codes, key scales, value codes, value scales.
+template <int D> struct Words {
+  static constexpr unsigned KEYS = D, SCALES = D / 4, ALL = 40 * D / 16;
+  static_assert(ALL == 2 * (KEYS + SCALES), "the block's parts");
+};
+
+// The key of row `row` of the keys' tile t, and of slot e of the values' quad.
+__device__ __forceinline__ unsigned key_of_row(unsigned t, unsigned row) {
+  return row / 8 * 16 + 8 * t + row % 8;
+}
+__device__ __forceinline__ unsigned key_of_slot(unsigned quad, unsigned e) {
+  return 16 * (quad / 2) + 4 * (quad % 2) + 8 * (e / 4) + e % 4;
+}
+__device__ __forceinline__ unsigned quad_of(unsigned key) { return key / 16 * 2 + key / 4 % 2; }
+__device__ __forceinline__ unsigned slot_of(unsigned key) { return key / 8 % 2 * 4 + key % 4; }
+
+// The bits of 32-bit word j of the block's 16-byte word c that belong to the
+// keys of `live`.
+template <int D> __device__ __forceinline__ uint32_t bits_of(unsigned c, unsigned j, uint32_t live) {
+  using W = Words<D>;
+  auto all = [&](unsigned key) { return live >> key & 1 ? ~0u : 0u; };
+  if (c < W::KEYS) { // (a tile's are D / 2; at D 64 two rows a word)
+    const unsigned t = c / (D / 2), row = D >= 128 ? c % 16 : c % 8 * 2 + j / 2;
+    return all(key_of_row(t, row));
+  }
+  c -= W::KEYS;
+  if (c < W::SCALES)
+    return all(key_of_row(c / (D / 8), c % 4 * 4 + j));
+  c -= W::SCALES;
+  uint32_t bits = 0;
+  if (c < W::KEYS) {
+    for (unsigned e = 0; e < 8; ++e)
+      bits |= live >> key_of_slot(c / 16 % 4, e) & 1 ? 15u << paged_nibble(e) : 0u;
+    return bits;
+  }
+  c -= W::KEYS;
+  for (unsigned e = 0; e < 2; ++e)
+    bits |= live >> key_of_slot(c % 4, 2 * j + e) & 1 ? 0xFFFFu << 16 * e : 0u;
+  return bits;
+}
+
+template <int D>
+__global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
+    const uint8_t *__restrict__ pool, PagedView g, const int32_t *__restrict__ source,
+    const int32_t *__restrict__ sourceTable, uint32_t *live, uint4_t *blocks, unsigned *invalid) {
+  using W = Words<D>;
+  PagedRun b;
+  if (!paged_run(g, b))
+    return;
+  const unsigned tid = threadIdx.x, head = blockIdx.y;
+  const size_t unit = (size_t)blockIdx.x * g.kvHeads + head;
+  __shared__ const uint8_t *sBlock[32]; // of the keys of this block
+  __shared__ unsigned sKey[32], sLive;
+  if (tid < 64) {
+    const bool mine = b.ok && tid >= b.first && tid < b.last;
+    const int from = mine ? source[b.row + (tid - b.first)] : -1;
+    PagedView of = g;
+    of.table = sourceTable;
+    size_t at = 0;
+    const bool found = from >= 0 && (long long)from < (long long)g.tableStride * g.pageSize &&
+                       paged_block(of, b.seq, (unsigned)from, head, at);
+    if (tid < 32) {
+      sBlock[tid] = pool + (found ? at : 0u); // (some block's, not put anywhere)
+      sKey[tid] = found ? (unsigned)from % 32 : 0u;
+    }
+    const uint32_t keys = (uint32_t)__builtin_amdgcn_ballot_w64(found);
+    if (tid == 0) {
+      sLive = live[unit] = keys;
+      if (invalid && (!b.ok || __builtin_popcount(keys) != (int)(b.last - b.first)))
+        atomicOr(invalid, kPagedPlace);
+    }
+  }
+  __syncthreads();
+  if (!sLive)
+    return;
+  uint4_t *to = blocks + unit * W::ALL;
+  for (unsigned word = tid; word < W::ALL; word += kMoveThreads) {
+    unsigned c = word;
+    uint4_t x = 0;
+    if (c < W::KEYS) {
+      const unsigned t = c / (D / 2), chunk = c % (D / 2) / (D >= 128 ? 16 : 8);
+      if constexpr (D >= 128) {
+        const unsigned key = key_of_row(t, c % 16), from = sKey[key];
+        x = *reinterpret_cast<const uint4_t *>(sBlock[key] + from / 8 % 2 * 8 * D +
+                                               (chunk * 16 + paged_row(from)) * 16);
+      } else {
+        for (unsigned n = 0; n < 2; ++n) {
+          const unsigned key = key_of_row(t, c % 8 * 2 + n), from = sKey[key];
+          const uint2 y = *reinterpret_cast<const uint2 *>(sBlock[key] + from / 8 % 2 * 8 * D +
+                                                           (chunk * 16 + paged_row(from)) * 8);
+          x[2 * n] = y.x;
+          x[2 * n + 1] = y.y;
+        }
+      }
+    } else if ((c -= W::KEYS) < W::SCALES) {
+      const unsigned t = c / (D / 8), group = c % (D / 8) / 4;
+      for (unsigned j = 0; j < 4; ++j) {
+        const unsigned key = key_of_row(t, c % 4 * 4 + j);
+        x[j] = *reinterpret_cast<const uint32_t *>(sBlock[key] + paged_key_scale(D, sKey[key], group));
+      }
+    } else if ((c -= W::SCALES) < W::KEYS) {
+      const unsigned st = c / 64, quad = c / 16 % 4, r = c % 16;
+      uint4_t y[8];
+      unsigned from[8];
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e) {
+        const unsigned key = key_of_slot(quad, e);
+        from[e] = sKey[key];
+        y[e] = *reinterpret_cast<const uint4_t *>(sBlock[key] +
+                                                  paged_value_word(D, quad_of(from[e]), 64 * st + r));
+      }
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e)
+        x |= (y[e] >> paged_nibble(slot_of(from[e])) & 15u) << paged_nibble(e);
+    } else {
+      c -= W::KEYS;
+      const unsigned group = c / 8, bias = c / 4 % 2, quad = c % 4;
+#pragma unroll
+      for (unsigned e = 0; e < 8; ++e) {
+        const unsigned key = key_of_slot(quad, e), from = sKey[key];
+        const uint32_t y = *reinterpret_cast<const uint16_t *>(
+            sBlock[key] + paged_value_scale(D, quad_of(from), slot_of(from), group) + 64 * bias);
+        x[e / 2] |= y << 16 * (e % 2);
+      }
+    }
+    to[word] = x;
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kMoveThreads) void paged_place_kernel(uint8_t *pool, PagedView g,
+                                                                   const uint32_t *__restrict__ live,
+                                                                   const uint4_t *__restrict__ blocks,
+                                                                   unsigned *invalid) {
+  using W = Words<D>;
+  constexpr unsigned kEach = (W::ALL + kMoveThreads - 1) / kMoveThreads;
+  PagedRun b;
+  if (!paged_run(g, b) || !b.ok)
+    return;
+  const unsigned tid = threadIdx.x, head = blockIdx.y;
+  const size_t unit = (size_t)blockIdx.x * g.kvHeads + head;
+  const uint32_t keys = live[unit];
+  size_t at;
+  if (!paged_block(g, b.seq, b.base, head, at)) {
+    if (invalid && tid == 0)
+      atomicOr(invalid, kPagedPlace);
+    return;
+  }
+  if (!keys)
+    return;
+  const uint4_t *from = blocks + unit * W::ALL;
+  uint4_t *to = reinterpret_cast<uint4_t *>(pool + at), x[kEach];
+#pragma unroll
+  for (unsigned i = 0; i < kEach; ++i)
+    if (tid + i * kMoveThreads < W::ALL)
+      x[i] = from[tid + i * kMoveThreads];
+  if (keys != ~0u) {
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) {
+      const unsigned c = tid + i * kMoveThreads;
+      if (c >= W::ALL)
+        continue;
+      const uint4_t old = to[c];
+#pragma unroll
+      for (unsigned j = 0; j < 4; ++j) {
+        const uint32_t bits = bits_of<D>(c, j, keys);
+        x[i][j] = (old[j] & ~bits) | (x[i][j] & bits);
+      }
+    }
+  }
+#pragma unroll
+  for (unsigned i = 0; i < kEach; ++i)
+    if (tid + i * kMoveThreads < W::ALL)
+      to[tid + i * kMoveThreads] = x[i];
+}
+
+size_t move_units(const PagedKvParams &p) {
+  return (size_t)paged_most_runs(p.tokens, p.sequences) * p.kvHeads;
+}
+
+} // namespace
+
+hipError_t launch_paged_fork(const int32_t *table, const int32_t *past, const int32_t *parent,
+                             const int32_t *spare, int32_t *tableOut, int32_t *pastOut, void *pool,
+                             uint32_t *invalid, const PagedForkParams &p, hipStream_t stream) {
+  const ForkView g{table,   past,       parent,    spare,       tableOut,     pastOut,
+                   p.pages, p.pageSize, p.kvHeads, p.sequences, p.tableStride};
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(p.children * p.kvHeads * (p.pageSize / 32)), dim3(kForkThreads),
+                       0, stream, g, static_cast<uint4_t *>(pool), invalid);
+    return hipGetLastError();
+  };
+  return p.headDim == 256   ? run(paged_fork_kernel<256>)
+         : p.headDim == 128 ? run(paged_fork_kernel<128>)
+                            : run(paged_fork_kernel<64>);
+}
+
+unsigned paged_free_launches(const PagedFreeParams &p) { return free_small(p) ? 1 : 2; }
+size_t paged_free_workspace_bytes(const PagedFreeParams &p) {
+  return free_small(p) ? 0 : (size_t)free_markers(p) * (((size_t)p.pages + 31) / 32) * 4;
+}
+hipError_t launch_paged_free(const int32_t *table, const int32_t *lengths, int32_t *free,
+                             int32_t *count, uint32_t *invalid, void *workspace,
+                             const PagedFreeParams &p, hipStream_t stream) {
+  const FreeView g{table, lengths, p.pages, p.pageSize, p.sequences, p.tableStride};
+  if (free_small(p)) {
+    hipLaunchKernelGGL(paged_free_small_kernel, dim3(1), dim3(kFreeThreads), 0, stream, g, free,
+                       count, invalid);
+    return hipGetLastError();
+  }
+  uint32_t *marks = static_cast<uint32_t *>(workspace);
+  const unsigned parts = free_markers(p), windows = (p.pages + kWindow - 1) / kWindow;
+  hipLaunchKernelGGL(paged_free_mark_kernel, dim3(parts, windows), dim3(kFreeThreads), 0, stream, g,
+                     marks, invalid);
+  if (hipError_t e = hipGetLastError())
+    return e;
+  hipLaunchKernelGGL(paged_free_list_kernel, dim3((p.pages + kListed - 1) / kListed),
+                     dim3(kFreeThreads), 0, stream, marks, parts, p.pages, free, count);
+  return hipGetLastError();
+}
+
+size_t paged_move_workspace_bytes(const PagedKvParams &p) {
+  const size_t units = move_units(p);
+  return units * 40 * p.headDim + (units * 4 + 15) / 16 * 16;
+}
+hipError_t launch_paged_move(const int32_t *source, const int32_t *sourceTable,
+                             const int32_t *starts, const int32_t *past, const int32_t *table,
+                             void *pool, uint32_t *invalid, void *workspace, const PagedKvParams &p,
+                             hipStream_t stream) {
+  const PagedView g = paged_view(p, starts, past, table);
+  uint4_t *blocks = static_cast<uint4_t *>(workspace);
+  uint32_t *live = reinterpret_cast<uint32_t *>(blocks + move_units(p) * (40 * p.headDim / 16));
+  const dim3 grid(paged_most_runs(p.tokens, p.sequences), p.kvHeads);
+  uint8_t *pages = static_cast<uint8_t *>(pool);
+  auto run = [&](auto gather, auto place) {
+    hipLaunchKernelGGL(gather, grid, dim3(kMoveThreads), 0, stream, pages, g, source, sourceTable,
+                       live, blocks, invalid);
+    if (hipError_t e = hipGetLastError())
+      return e;
+    hipLaunchKernelGGL(place, grid, dim3(kMoveThreads), 0, stream, pages, g, live, blocks, invalid);
+    return hipGetLastError();
+  };
+  return p.headDim == 256   ? run(paged_gather_kernel<256>, paged_place_kernel<256>)
+         : p.headDim == 128 ? run(paged_gather_kernel<128>, paged_place_kernel<128>)
+                            : run(paged_gather_kernel<64>, paged_place_kernel<64>);
+}
+
+} // namespace llmi

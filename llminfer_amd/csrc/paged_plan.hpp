@@ -44,15 +44,15 @@ struct Split {
   unsigned group, shift, step, chunk; // units of 2^shift columns, whole steps of blocks
   float inv;                    // 1 / chunk
   bool nearest;
-  __device__ unsigned units(const PagedSeq &q) const {
+  template <typename Seq> __device__ unsigned units(const Seq &q) const {
     return (unsigned)(((uint64_t)q.rows * group + (1u << shift) - 1) >> shift);
   }
-  __device__ static unsigned blocks(const PagedSeq &q) {
-    return q.ok ? (q.past + q.rows + 31) / 32 : 1u;
+  template <typename Seq> __device__ static unsigned blocks(const Seq &q) {
+    return q.ok ? (q.keys() + 31) / 32 - q.first() : 1u;
   }
   // (x + round) / chunk by the reciprocal, corrected by its remainder: at most
   // as many pieces as the host planned for, so off by one at most
-  __device__ unsigned pieces(const PagedSeq &q) const {
+  template <typename Seq> __device__ unsigned pieces(const Seq &q) const {
     const unsigned x = blocks(q) + (nearest ? chunk / 2 : chunk - 1);
     unsigned n = (unsigned)((float)x * inv);
     const int rest = (int)(x - n * chunk);
@@ -60,7 +60,7 @@ struct Split {
     return n ? n : 1u;
   }
   // blocks of a piece: whole steps of the kernels
-  __device__ unsigned length(const PagedSeq &q, unsigned pieces) const {
+  template <typename Seq> __device__ unsigned length(const Seq &q, unsigned pieces) const {
     const unsigned each = (blocks(q) + pieces - 1) / pieces;
     return (each + step - 1) & ~(step - 1);
   }
@@ -78,14 +78,15 @@ struct SplitPlan {
 // The chunk, whole steps, for which the call has at most plan.target pieces
 // more than units. (The fp32 sum is exact below 2^24, and off by less than
 // the 1.0001 above; every workgroup and the merge add in the same order.)
-__device__ __forceinline__ Split paged_split(const PagedView &g, const PagedSeq &own,
+template <typename View>
+__device__ __forceinline__ Split paged_split(const View &g, const typename View::Seq &own,
                                              unsigned group, const SplitPlan &plan) {
   Split s{group, plan.shift, plan.step, plan.step, 0.0f, plan.nearest != 0};
   const unsigned lane = threadIdx.x % 64;
   float all = (float)s.units(own) * (float)Split::blocks(own);
   for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
     if (s0 + lane < g.sequences) {
-      const PagedSeq q = paged_seq(g, s0 + lane);
+      const typename View::Seq q = paged_seq(g, s0 + lane);
       all += (float)s.units(q) * (float)Split::blocks(q);
     }
   all = group_sum<16>(all);
@@ -132,7 +133,8 @@ struct Partials {
 // The kernel for sequences of many rows (paged_tiles.hip): columns of its
 // units, and its launch.
 unsigned paged_tiles_columns(unsigned headDim);
-hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedView &g, half_t *out,
+template <typename View>
+hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const View &g, half_t *out,
                               unsigned *invalid, unsigned queryHeads, SplitPlan plan, ScoreScale c,
                               Partials parts, unsigned pieces, hipStream_t stream);
 

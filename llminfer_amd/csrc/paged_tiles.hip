@@ -34,6 +34,7 @@
 #include "hip_common.hpp"
 #include "paged_kv.hpp"
 #include "paged_plan.hpp"
+#include "paged_shared.hpp"
 
 #include <math.h>
 #include <type_traits>
@@ -64,14 +65,15 @@ template <int I> __device__ __forceinline__ char *tile_buffer() {
 // sequences; in their order otherwise), so that workgroups which start late
 // have little to do (seven messages of 41 to 110 blocks, 296 workgroups:
 // 174 us in order, 130 longest first).
-__device__ __forceinline__ bool find_longest(const PagedView &g, const PagedSeq &own,
+template <typename View>
+__device__ __forceinline__ bool find_longest(const View &g, const typename View::Seq &own,
                                              const Split &split, unsigned u, unsigned &seq,
                                              unsigned &local, unsigned &number) {
   unsigned before;
   if (g.sequences == 1 || g.sequences > 64) {
     number = u;
     return paged_find(g, own, u,
-                      [&](const PagedSeq &s) { return split.units(s) * split.pieces(s); }, seq,
+                      [&](const auto &s) { return split.units(s) * split.pieces(s); }, seq,
                       local, before);
   }
   const unsigned lane = threadIdx.x % 64;
@@ -117,22 +119,22 @@ template <int N, int CT> __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(kMfma, CT * kAhead, 0);
 }
 
-template <int D>
+template <int D, typename View>
 __global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads),
                           amdgpu_waves_per_eu(2, 2)))
 void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool,
-                        PagedView g, half_t *out, unsigned *invalid, unsigned queryHeads,
+                        View g, half_t *out, unsigned *invalid, unsigned queryHeads,
                         SplitPlan plan, ScoreScale c, Partials parts) {
   using T = Tiles<D>;
   constexpr int CT = T::CT;
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.x % g.kvHeads;
-  const PagedSeq own = paged_own(g);
+  const auto own = paged_own(g);
   const Split split = paged_split(g, own, G, plan);
   unsigned seq, local, number; // number: of this piece, for its partials
   if (!find_longest(g, own, split, blockIdx.x / g.kvHeads, seq, local, number) ||
       number >= gridDim.x / g.kvHeads) // (starts out of order: more pieces than the rows can have)
     return;
-  const PagedSeq s = paged_seq_of(g, own, seq);
+  const auto s = paged_seq_of(g, own, seq);
   const unsigned pieces = split.pieces(s), units = split.units(s);
   const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
   const unsigned tid = threadIdx.x, lane = tid % 64, r = lane % 32, hi = lane / 32;
@@ -146,7 +148,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 #pragma unroll
   for (int j = 0; j < CT; ++j) {
     const unsigned col = c0 + 32 * (tile0 + j) + r, token = min(col / G, s.rows - 1);
-    visible[j] = s.past + token;
+    visible[j] = s.last(token);
     row[j] = ((size_t)(s.row0 + token) * queryHeads + kvh * G + col % G) * D;
   }
   auto live = [&](int j) { return 32 * (tile0 + j) + r < columns; };
@@ -159,13 +161,14 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
       atomicOr(invalid, kPagedPlace);
     return;
   }
-  const unsigned least = s.past + c0 / G;                // the first column's last key
-  const unsigned most = s.past + (c0 + columns - 1) / G; // the last column's
+  const unsigned least = s.last(c0 / G);                // the first column's last key
+  const unsigned most = s.last((c0 + columns - 1) / G); // the last column's
   // the keys that this wave decodes: to the sequence's end, or to a page that is
   // not in the pool, whose columns' outputs are NaN
-  const unsigned whole = s.past + s.rows;
+  const unsigned whole = s.keys();
   unsigned end = whole;
-  const unsigned length = split.length(s, pieces), b0 = min(piece * length, most / 32 + 1);
+  const unsigned length = split.length(s, pieces);
+  const unsigned b0 = min(s.first() + piece * length, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned steps = (b1 - b0 + T::BLOCKS - 1) / T::BLOCKS;
 
@@ -183,7 +186,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   char *raw = raw_buffer() + kRaw * wave;
   auto fetch = [&](unsigned n) { // (n < steps; a block past the last again)
     if (n % 64 == 0) {           // where the next 64 steps' blocks are, one a lane
-      const bool lost = !paged_block(g, seq, 32 * block_of(n + lane), kvh, place);
+      const bool lost = !paged_block(g, s.table(seq), 32 * block_of(n + lane), kvh, place);
       if (const unsigned long long all = __builtin_amdgcn_ballot_w64(lost))
         end = min(end, 32 * block_of(n + (unsigned)__builtin_ctzll(all)));
     }
@@ -471,14 +474,14 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
         for (int e = 0; e < 4; ++e)
           y[e] = o[j][i][4 * v + e] * a + z[e] * b;
         const unsigned at = 32 * i + 8 * v + 4 * hi;
-        if (pieces == 1)
+        if (pieces == 1 && !s.joined())
           *reinterpret_cast<half4_t *>(out + row[j] + at) =
               half4_t{(half_t)(y[0] * inv), (half_t)(y[1] * inv), (half_t)(y[2] * inv),
                       (half_t)(y[3] * inv)};
         else
           *reinterpret_cast<float4_t *>(parts.o + part * D + at) = y;
       }
-    if (pieces > 1 && hi == 0)
+    if ((pieces > 1 || s.joined()) && hi == 0)
       *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
   }
 }
@@ -487,7 +490,8 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
 
 unsigned paged_tiles_columns(unsigned headDim) { return 128 * (256 / headDim); }
 
-hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedView &g, half_t *out,
+template <typename View>
+hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const View &g, half_t *out,
                               unsigned *invalid, unsigned queryHeads, SplitPlan plan, ScoreScale c,
                               Partials parts, unsigned pieces, hipStream_t stream) {
   auto run = [&](auto kernel) {
@@ -495,7 +499,15 @@ hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const PagedV
                        invalid, queryHeads, plan, c, parts);
     return hipGetLastError();
   };
-  return g.dim == 256 ? run(paged_tiles_kernel<256>) : run(paged_tiles_kernel<128>);
+  return g.dim == 256 ? run(paged_tiles_kernel<256, View>) : run(paged_tiles_kernel<128, View>);
 }
+template hipError_t launch_paged_tiles<PagedView>(const half_t *, const uint8_t *,
+                                                  const PagedView &, half_t *, unsigned *, unsigned,
+                                                  SplitPlan, ScoreScale, Partials, unsigned,
+                                                  hipStream_t);
+template hipError_t launch_paged_tiles<SharedView>(const half_t *, const uint8_t *,
+                                                   const SharedView &, half_t *, unsigned *,
+                                                   unsigned, SplitPlan, ScoreScale, Partials,
+                                                   unsigned, hipStream_t);
 
 } // namespace llmi

@@ -1193,3 +1193,194 @@ def paged_gqa(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor, past: t
         out = torch.zeros_like(q)
     bind_paged_gqa(q, pool, starts, past, table, out, scale, invalid)()
     return out
+
+
+# ------------------------------------- sequences that share pages of the cache
+
+def _private(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """A bound call's own workspace: two calls bound on one stream may be
+    captured into graphs whose replays overlap."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _size(ws: torch.Tensor | None) -> int:
+    return ws.numel() if ws is not None else 0
+
+
+def _require_pool(pool: torch.Tensor) -> None:
+    _require(pool, torch.uint8, "pool")
+    if pool.dim() != 4 or pool.shape[3] not in (40 * 64, 40 * 128, 40 * 256):
+        raise ValueError("pool is paged_pool's [pages, kv_heads, page_size / 32, 40 * head_dim]")
+
+
+def _require_invalid(invalid: torch.Tensor | None) -> None:
+    if invalid is not None:
+        _require(invalid, torch.int32, "invalid")
+        if invalid.numel() != 1:
+            raise ValueError("invalid has one element")
+
+
+def bind_paged_gqa_shared(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor,
+                          past: torch.Tensor, table: torch.Tensor, groups: torch.Tensor,
+                          prefix: torch.Tensor, out: torch.Tensor, scale: float | None = None,
+                          invalid: torch.Tensor | None = None) -> "Bound":
+    """bind_paged_gqa of sequences that have pages in common, as bind_paged_fork
+    leaves them (llmi_hip_paged_gqa_shared): the first prefix[g] keys (int32
+    [G]) of sequences groups[g] .. groups[g + 1] - 1 (int32 [G + 1], in order)
+    are the same and are read once for all of the group's rows, through the
+    table of its first sequence. A sequence whose past is shorter than its
+    group's prefix has no place: NaN, and bit 1 of invalid. Pays from two
+    sequences on a prefix of some thousand keys. The workspace is the bound
+    call's own; keep a bound call as long as a graph that it was captured
+    into."""
+    for t, n in ((q, "q"), (out, "out")):
+        _require(t, torch.float16, n)
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError("q and out are [T, Hq, head_dim]")
+    kv = _paged(pool, starts, past, table, q.shape[0], invalid)
+    if q.shape[2] != kv.headDim or q.shape[1] % max(kv.kvHeads, 1):
+        raise ValueError("q's heads do not match the pool")
+    for t, n in ((groups, "groups"), (prefix, "prefix")):
+        _require(t, torch.int32, n)
+    if prefix.dim() != 1 or groups.shape != (prefix.numel() + 1,):
+        raise ValueError("groups [G + 1] and prefix [G] disagree")
+    _one_device(q, pool, starts, past, table, groups, prefix, out, invalid)
+    lib = _lib.load()
+    p = _lib.PagedSharedParams(
+        _lib.PagedGqaParams(kv, q.shape[1], float(np.float32(1.0) / np.sqrt(np.float32(q.shape[2])))
+                            if scale is None else scale), prefix.numel())
+    ws = _private(lib.llmi_hip_paged_gqa_shared_workspace_bytes(p), q.device)
+    b = Bound(lib.llmi_hip_paged_gqa_shared,
+              (_ptr(q), _ptr(starts), _ptr(past), _ptr(table), _ptr(groups), _ptr(prefix),
+               _ptr(pool), _ptr(out), _ptr(invalid), p, _ptr(ws), _size(ws), _stream()),
+              "+".join(kernel_names(_lib.OP_PAGED_GQA_SHARED, p)))
+    b._keep = (q, pool, starts, past, table, groups, prefix, out, invalid, ws)
+    return b
+
+
+def paged_gqa_shared(q: torch.Tensor, pool: torch.Tensor, starts: torch.Tensor,
+                     past: torch.Tensor, table: torch.Tensor, groups: torch.Tensor,
+                     prefix: torch.Tensor, out: torch.Tensor | None = None,
+                     scale: float | None = None,
+                     invalid: torch.Tensor | None = None) -> torch.Tensor:
+    """bind_paged_gqa_shared, called once. Rows of no sequence of a new `out`
+    are zero."""
+    if out is None:
+        out = torch.zeros_like(q)
+    bind_paged_gqa_shared(q, pool, starts, past, table, groups, prefix, out, scale, invalid)()
+    return out
+
+
+def bind_paged_fork(pool: torch.Tensor, table: torch.Tensor, past: torch.Tensor,
+                    parent: torch.Tensor, spare: torch.Tensor, table_out: torch.Tensor,
+                    past_out: torch.Tensor, invalid: torch.Tensor | None = None) -> "Bound":
+    """Children of sequences (llmi_hip_paged_fork): child i continues sequence
+    parent[i] of table [S, n] and past [S] as row i of table_out [N, n] and
+    past_out [N] (all int32). It shares the parent's whole pages and gets a copy
+    of the page that is not full in page spare[i], or with spare[i] negative
+    takes over the parent's row as it is. Spare pages are apart and none of a
+    sequence's (paged_free has them). A parent that is not one of the
+    sequences, or does not fit its row: a row of -1 of length -1; a page that is
+    not in the pool: -1 in its place; both set bit 1 of invalid."""
+    _require_pool(pool)
+    for t, n in ((table, "table"), (past, "past"), (parent, "parent"), (spare, "spare"),
+                 (table_out, "table_out"), (past_out, "past_out")):
+        _require(t, torch.int32, n)
+    _require_invalid(invalid)
+    if table.dim() != 2 or past.shape != table.shape[:1]:
+        raise ValueError("table [S, pages] and past [S] disagree")
+    if parent.dim() != 1 or spare.shape != parent.shape or past_out.shape != parent.shape or \
+            table_out.shape != (parent.numel(), table.shape[1]):
+        raise ValueError("parent, spare, past_out [N] and table_out [N, pages] disagree")
+    _one_device(pool, table, past, parent, spare, table_out, past_out, invalid)
+    p = _lib.PagedForkParams(pool.shape[0], 32 * pool.shape[2], pool.shape[1], pool.shape[3] // 40,
+                             table.shape[0], table.shape[1], parent.numel())
+    b = Bound(_lib.load().llmi_hip_paged_fork,
+              (_ptr(table), _ptr(past), _ptr(parent), _ptr(spare), _ptr(table_out), _ptr(past_out),
+               _ptr(pool), _ptr(invalid), p, _stream()), "pagedFork")
+    b._keep = (pool, table, past, parent, spare, table_out, past_out, invalid)
+    return b
+
+
+def paged_fork(pool: torch.Tensor, table: torch.Tensor, past: torch.Tensor, parent: torch.Tensor,
+               spare: torch.Tensor, invalid: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """bind_paged_fork, called once: (table_out, past_out)."""
+    table_out = torch.empty(parent.numel(), table.shape[-1], dtype=torch.int32, device=parent.device)
+    past_out = torch.empty_like(parent)
+    bind_paged_fork(pool, table, past, parent, spare, table_out, past_out, invalid)()
+    return table_out, past_out
+
+
+def bind_paged_free(table: torch.Tensor, lengths: torch.Tensor, page_size: int, free: torch.Tensor,
+                    count: torch.Tensor, invalid: torch.Tensor | None = None) -> "Bound":
+    """The pages that no sequence holds (llmi_hip_paged_free), into free [pages]
+    (int32: their numbers, ascending, and -1 behind them) and count (one
+    element). Sequence s holds the pages of its first lengths[s] keys, by its
+    row of table [S, n]; one whose length does not fit the row holds all of it,
+    entries that are not in the pool hold nothing, and both set bit 1 of
+    invalid. The workspace is the bound call's own; keep a bound call as long
+    as a graph that it was captured into."""
+    for t, n in ((table, "table"), (lengths, "lengths"), (free, "free"), (count, "count")):
+        _require(t, torch.int32, n)
+    _require_invalid(invalid)
+    if table.dim() != 2 or lengths.shape != table.shape[:1]:
+        raise ValueError("table [S, pages] and lengths [S] disagree")
+    if free.dim() != 1 or count.numel() != 1:
+        raise ValueError("free is [pages], count has one element")
+    if page_size <= 0 or page_size % 32:
+        raise ValueError("page_size is a multiple of 32")
+    _one_device(table, lengths, free, count, invalid)
+    lib = _lib.load()
+    p = _lib.PagedFreeParams(free.numel(), page_size, *table.shape)
+    ws = _private(lib.llmi_hip_paged_free_workspace_bytes(p), free.device)
+    b = Bound(lib.llmi_hip_paged_free,
+              (_ptr(table), _ptr(lengths), _ptr(free), _ptr(count), _ptr(invalid), p, _ptr(ws),
+               _size(ws), _stream()), "+".join(kernel_names(_lib.OP_PAGED_FREE, p)))
+    b._keep = (table, lengths, free, count, invalid, ws)
+    return b
+
+
+def paged_free(table: torch.Tensor, lengths: torch.Tensor, page_size: int, pages: int,
+               invalid: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """bind_paged_free of a pool of `pages` pages, called once: (free, count)."""
+    free = torch.empty(pages, dtype=torch.int32, device=table.device)
+    count = torch.empty(1, dtype=torch.int32, device=table.device)
+    bind_paged_free(table, lengths, page_size, free, count, invalid)()
+    return free, count
+
+
+def bind_paged_move(pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor,
+                    table: torch.Tensor, source: torch.Tensor,
+                    source_table: torch.Tensor | None = None,
+                    invalid: torch.Tensor | None = None) -> "Bound":
+    """Keys and values moved as they are (llmi_hip_paged_move): those at
+    positions source [T] (int32, in any order) of their sequences' rows of
+    source_table (default: table) to positions past[s] + i of table, row i of
+    sequence s being source[starts[s] + i]. All are read before any is written,
+    so a sequence may be made shorter in its own pages. Keys stay rotated as
+    they were. A row whose source or target has no place is not moved and sets
+    bit 1 of invalid. The workspace is the bound call's own; keep a bound call
+    as long as a graph that it was captured into."""
+    _require(source, torch.int32, "source")
+    if source.dim() != 1:
+        raise ValueError("source is [T]")
+    p = _paged(pool, starts, past, table, source.numel(), invalid)
+    if source_table is None:
+        source_table = table
+    _require(source_table, torch.int32, "source_table")
+    if source_table.shape != table.shape:
+        raise ValueError("source_table has the shape of table")
+    _one_device(pool, starts, past, table, source, source_table, invalid)
+    lib = _lib.load()
+    ws = _private(lib.llmi_hip_paged_move_workspace_bytes(p), pool.device)
+    b = Bound(lib.llmi_hip_paged_move,
+              (_ptr(source), _ptr(source_table), _ptr(starts), _ptr(past), _ptr(table), _ptr(pool),
+               _ptr(invalid), p, _ptr(ws), _size(ws), _stream()), "pagedGather+pagedPlace")
+    b._keep = (pool, starts, past, table, source, source_table, invalid, ws)
+    return b
+
+
+def paged_move(*args, **kwargs) -> None:
+    """bind_paged_move, called once."""
+    bind_paged_move(*args, **kwargs)()

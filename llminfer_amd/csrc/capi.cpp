@@ -1575,8 +1575,9 @@ const char *llmi_hip_kernel_name(int op, const void *params, unsigned index) {
     return "pagedFork";
   case LLMI_HIP_OP_PAGED_FREE:
     return llmi_hip_dispatch_count(op, params) == 1 ? "pagedFree"
-           : index                                  ? "pagedFreeList"
-                                                    : "pagedFreeMark";
+           : index == 0                             ? "pagedFreeMark"
+           : index == 1                             ? "pagedFreeJoin"
+                                                    : "pagedFreeList";
   case LLMI_HIP_OP_PAGED_MOVE:
     return index ? "pagedPlace" : "pagedGather";
   case LLMI_HIP_OP_GATED_ATTENTION:

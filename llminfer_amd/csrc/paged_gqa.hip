@@ -32,7 +32,6 @@
 #include "kernels.hpp"
 #include "paged_kv.hpp"
 #include "paged_plan.hpp"
-#include "paged_shared.hpp"
 
 #include <math.h>
 #include <type_traits>
@@ -159,6 +158,8 @@ void paged_gqa_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ 
   // (the last units first: they see most keys)
   const unsigned pieces = split.pieces(s), units = split.units(s);
   const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
+  if (local == 0 && kvh == 0 && threadIdx.x == 0)
+    leave_note(g, s, seq, before, pieces, units);
   const unsigned tid = threadIdx.x, lane = tid % 64, quad = lane / 16, r = lane % 16;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
 
@@ -617,67 +618,61 @@ struct SharedPart {
   unsigned most;
 };
 
-// Pieces of the sequences before `seq`.
-template <typename View>
-__device__ __forceinline__ unsigned pieces_before(const View &g, const typename View::Seq &own,
-                                                  const Split &split, unsigned seq) {
-  const unsigned lane = threadIdx.x % 64;
-  unsigned before = 0;
-  for (unsigned s0 = 0; s0 <= seq; s0 += 64) {
-    const typename View::Seq o =
-        s0 ? (s0 + lane < g.sequences ? paged_seq(g, s0 + lane) : typename View::Seq{0, 0, 0, true})
-           : own;
-    const unsigned n = split.units(o) * split.pieces(o), sum = wave_scan(n);
-    const int at = seq - s0 < 64 ? (int)(seq - s0) : 63;
-    before += (unsigned)__builtin_amdgcn_readlane((int)(seq - s0 < 64 ? sum - n : sum), at);
-  }
-  return before;
-}
-
 // Joins a row's partials: those of its sequence's own keys and those of its
-// group's shared ones, from one launch (`apart` false: both parts are the same)
-// or from two. An item is a query head of a row, as in paged_gqa_merge_kernel,
-// the work of a workgroup's eight waves.
-template <int D>
+// group's shared ones, from one launch (the two parts are the same) or from
+// two. A workgroup has a row and 8 / W of its query heads, W waves each, every
+// W-th piece a wave; where the pieces are is in the notes that the launches left,
+// so that nothing of the plan is made again. W: 8 where the shared keys have
+// many pieces, 1 otherwise.
+template <int D, int W>
 __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
-    SharedPart shared, SharedPart rest, bool apart, half_t *out, unsigned queryHeads) {
+    SharedPart shared, SharedPart rest, half_t *out, unsigned queryHeads) {
   constexpr int N = D / 64;
-  constexpr unsigned W = kMergeThreads / 64;
+  constexpr unsigned kItems = kMergeThreads / 64 / W; // heads of a workgroup
   typedef float vec __attribute__((ext_vector_type(N)));
   typedef _Float16 halves __attribute__((ext_vector_type(N)));
   const SharedView &g = rest.g;
-  const unsigned G = queryHeads / g.kvHeads;
-  const SharedSeq own = paged_own(g);
-  const Split split = paged_split(g, own, G, rest.plan);
-  const SharedSeq ownShared = apart ? paged_own(shared.g) : own;
-  const Split splitShared = apart ? paged_split(shared.g, ownShared, G, shared.plan) : split;
+  const unsigned G = queryHeads / g.kvHeads, row = blockIdx.x;
   const unsigned lane = threadIdx.x % 64;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  __shared__ unsigned sCount[kMergeThreads / 64];
   __shared__ float sM[W], sL[W];
   __shared__ vec sY[W][64];
-  // (the same item in every wave, so all of them leave together)
-  for (unsigned item = blockIdx.x;; item += gridDim.x) {
-    unsigned seq, local, before;
-    if (!paged_find(g, own, item,
-                    [&](const SharedSeq &s) {
-                      return s.step && s.ok && (s.joined() || split.pieces(s) > 1)
-                                 ? s.rows * queryHeads
-                                 : 0u;
-                    },
-                    seq, local, before))
+  // the row's sequence: the last one that begins at or before it
+  unsigned n = 0;
+  for (unsigned i = threadIdx.x; i < g.all; i += kMergeThreads)
+    n += g.starts[i] <= (int)row;
+  n = wave_scan(n);
+  if (lane == 63)
+    sCount[wave] = n;
+  __syncthreads();
+  n = 0;
+  for (unsigned w = 0; w < kMergeThreads / 64; ++w)
+    n += sCount[w];
+  if (n == 0)
+    return;
+  const unsigned seq = n - 1;
+  const int lo = max(g.starts[seq], 0), hi = g.starts[seq + 1];
+  const SharedNote mine = g.notes[g.count + seq];
+  if ((int)row < lo || (int)row >= hi || mine.pieces == 0 || mine.other > g.count)
+    return; // of no sequence, or its output is there
+  const bool both = mine.other != 0;
+  SharedNote of{0, 0, 0, 0};
+  if (both)
+    of = shared.g.notes[mine.other - 1];
+  for (unsigned h0 = blockIdx.y * kItems; h0 < queryHeads; h0 += gridDim.y * kItems) {
+    const unsigned h = h0 + wave / W, kvh = h / G;
+    if (W == 1 && h >= queryHeads)
       return;
-    const SharedSeq s = paged_seq_of(g, own, seq);
-    const unsigned h = local % queryHeads, row = local / queryHeads, kvh = h / G;
     float m = -INFINITY, l = 0.0f;
     vec y = 0.0f;
-    // column `column` of the pieces of a sequence; false where starts out of
-    // order make more of them than the rows can have
-    auto join = [&](const SharedPart &part, const SharedSeq &of, const Split &by, unsigned at,
-                    const SharedSeq &lanes, unsigned column, unsigned turn) {
-      const unsigned unit = 1u << part.plan.shift, pieces = by.pieces(of), units = by.units(of);
-      const unsigned first =
-          pieces_before(part.g, lanes, by, at) + (units - 1 - column / unit) * pieces;
-      if (column / unit >= units || first >= part.most || pieces > part.most - first)
+    // column `column` of a note's pieces; false where starts out of order make
+    // more of them than the rows can have
+    auto join = [&](const SharedPart &part, const SharedNote &note, unsigned column, unsigned turn) {
+      const unsigned unit = 1u << part.plan.shift, pieces = note.pieces;
+      const unsigned long long first =
+          note.first + (unsigned long long)(note.units - 1 - column / unit) * pieces;
+      if (column / unit >= note.units || first + pieces > part.most)
         return false;
       const size_t place = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
       const size_t step = (size_t)g.kvHeads * unit;
@@ -712,34 +707,33 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
       }
       return true;
     };
-    bool whole = join(rest, s, split, seq, own, row * G + h % G, 0);
-    if (s.begin) {
-      unsigned group = 0;
-      shared_group(g, s.from, group);
-      const SharedSeq p = paged_seq_of(shared.g, ownShared, group);
-      whole = join(shared, p, splitShared, group, ownShared,
-                   (s.row0 + row - p.row0) * G + h % G, split.pieces(s)) && whole;
+    bool whole = join(rest, mine, (row - lo) * G + h % G, 0);
+    if (both) // (`other` of a group: its first row)
+      whole = join(shared, of, (row - of.other) * G + h % G, mine.pieces) && whole;
+    if (W > 1) {
+      sM[wave] = m;
+      sL[wave] = l;
+      sY[wave][lane] = y;
+      __syncthreads();
+      if (wave == 0) {
+        m = sM[0];
+        for (unsigned w = 1; w < W; ++w)
+          m = fmaxf(m, sM[w]);
+        l = 0.0f;
+        y = 0.0f;
+        for (unsigned w = 0; w < W; ++w) {
+          const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - m);
+          l += sL[w] * a;
+          y += sY[w][lane] * a;
+        }
+      }
+      __syncthreads();
     }
-    sM[wave] = m;
-    sL[wave] = l;
-    sY[wave][lane] = y;
-    __syncthreads();
-    m = sM[0];
-    for (unsigned w = 1; w < W; ++w)
-      m = fmaxf(m, sM[w]);
-    l = 0.0f;
-    y = 0.0f;
-    for (unsigned w = 0; w < W; ++w) {
-      const float a = sM[w] == -INFINITY ? 0.0f : fast_exp2(sM[w] - m);
-      l += sL[w] * a;
-      y += sY[w][lane] * a;
-    }
-    __syncthreads();
-    if (wave == 0 && whole) {
+    if (wave % W == 0 && whole) {
       halves z;
       for (int i = 0; i < N; ++i)
         z[i] = (half_t)(y[i] / l);
-      reinterpret_cast<halves *>(out + ((size_t)(s.row0 + row) * queryHeads + h) * D)[lane] = z;
+      reinterpret_cast<halves *>(out + ((size_t)row * queryHeads + h) * D)[lane] = z;
     }
   }
 }
@@ -870,6 +864,9 @@ size_t shared_columns(const PagedKvParams &p, const SharedPlan &s) {
 size_t rest_columns(const PagedKvParams &p, const SharedPlan &s) {
   return s.apart ? (size_t)s.restPieces * p.kvHeads << s.rest.split.shift : 0;
 }
+size_t notes_bytes(const PagedKvParams &p, unsigned groups) {
+  return ((size_t)groups + p.sequences) * sizeof(SharedNote);
+}
 
 } // namespace
 
@@ -880,7 +877,7 @@ bool paged_shared_launchable(const PagedKvParams &p, unsigned queryHeads, unsign
 }
 size_t paged_shared_workspace_bytes(const PagedKvParams &p, unsigned queryHeads, unsigned groups) {
   const SharedPlan s = shared_plan(p, queryHeads / p.kvHeads, groups);
-  return 4 * (p.headDim + 2) * (shared_columns(p, s) + rest_columns(p, s));
+  return notes_bytes(p, groups) + 4 * (p.headDim + 2) * (shared_columns(p, s) + rest_columns(p, s));
 }
 unsigned paged_shared_launches(const PagedKvParams &p, unsigned queryHeads, unsigned groups) {
   return shared_plan(p, queryHeads / p.kvHeads, groups).apart ? 3 : 2;
@@ -901,12 +898,13 @@ hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, con
   const half_t *from = reinterpret_cast<const half_t *>(q);
   const uint8_t *pages = static_cast<const uint8_t *>(pool);
   half_t *to = reinterpret_cast<half_t *>(out);
-  float *ws = static_cast<float *>(workspace);
+  SharedNote *notes = static_cast<SharedNote *>(workspace);
+  float *ws = reinterpret_cast<float *>(notes + count + p.sequences);
   const size_t sharedColumns = shared_columns(p, s), restColumns = rest_columns(p, s);
   auto part = [&](const GqaPlan &by, uint64_t pieces, float *at, size_t columns, unsigned base,
                   unsigned sequences) {
-    SharedPart x{SharedView{paged_view(p, starts, past, table), groups, prefix, count, p.sequences,
-                            base},
+    SharedPart x{SharedView{paged_view(p, starts, past, table), groups, prefix, notes, count,
+                            p.sequences, base},
                  by.split, Partials{at + columns * p.headDim, at}, (unsigned)pieces};
     x.g.sequences = sequences;
     return x;
@@ -925,15 +923,20 @@ hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, con
     e = attend(rest, s.rest);
   if (e != hipSuccess)
     return e;
-  auto merge = [&](auto kernel) {
-    const uint64_t items = (uint64_t)p.tokens * queryHeads;
-    hipLaunchKernelGGL(kernel, dim3(items < kMergeGroups ? (unsigned)items : kMergeGroups),
-                       dim3(kMergeThreads), 0, stream, shared, rest, s.apart, to, queryHeads);
+  // pieces of a unit of shared keys, about, where all of them are as long
+  const unsigned unit = 1u << s.shared.split.shift;
+  const uint64_t units = ((uint64_t)p.tokens * (queryHeads / p.kvHeads) + unit - 1) / unit;
+  const bool many = s.shared.split.target >= 8 * units;
+  auto merge = [&](auto wide, auto narrow) {
+    const unsigned each = many ? 1 : kMergeThreads / 64, parts = (queryHeads + each - 1) / each;
+    hipLaunchKernelGGL(many ? wide : narrow, dim3(p.tokens, parts < 65535 ? parts : 65535),
+                       dim3(kMergeThreads), 0, stream, shared, rest, to, queryHeads);
     return hipGetLastError();
   };
-  return p.headDim == 256   ? merge(paged_shared_merge_kernel<256>)
-         : p.headDim == 128 ? merge(paged_shared_merge_kernel<128>)
-                            : merge(paged_shared_merge_kernel<64>);
+  return p.headDim == 256 ? merge(paged_shared_merge_kernel<256, 8>, paged_shared_merge_kernel<256, 1>)
+         : p.headDim == 128
+             ? merge(paged_shared_merge_kernel<128, 8>, paged_shared_merge_kernel<128, 1>)
+             : merge(paged_shared_merge_kernel<64, 8>, paged_shared_merge_kernel<64, 1>);
 }
 
 } // namespace llmi

@@ -195,6 +195,7 @@ template <typename View> __device__ __forceinline__ typename View::Seq paged_own
   const unsigned lane = threadIdx.x % 64;
   return lane < g.sequences ? paged_seq(g, lane) : typename View::Seq{0, 0, 0, true};
 }
+__device__ __forceinline__ const PagedSeq &paged_first(const PagedSeq &own) { return own; }
 // One of the sequences, the same in every lane.
 __device__ __forceinline__ PagedSeq paged_from_lane(const PagedSeq &own, unsigned lane) {
   PagedSeq q;

@@ -73,51 +73,64 @@ __global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(ForkView g, ui
 constexpr unsigned kFreeThreads = 1024;
 constexpr unsigned kFreeWaves = kFreeThreads / 64;
 constexpr unsigned kWindow = 1u << 19; // pages whose marks one workgroup has in LDS
-constexpr unsigned kListed = 8192;     // pages whose entries one workgroup writes
-constexpr unsigned kMarkers = 8;       // workgroups that mark, at most
+constexpr unsigned kListed = 4096;     // pages whose entries one workgroup writes
+constexpr unsigned kSmall = 8192;      // pages of a pool that one workgroup has alone
+constexpr unsigned kMarkers = 32;      // workgroups that mark, at most
 
 struct FreeView {
   const int32_t *table, *lengths;
   unsigned pages, pageSize, sequences, tableStride;
 };
 
-// The pages of window `window` that rows `part`, part + parts, ... of the
-// 1024-entry pieces of the tables name, as bits.
+// The pages of window `window` that the tables name, as bits; this is workgroup
+// `part` of `parts`. A wave takes 512 slots of a row at a time, four of these
+// pieces of rows in flight.
 __device__ __forceinline__ void mark_held(const FreeView &g, unsigned part, unsigned parts,
                                           unsigned window, uint32_t *marks, unsigned *invalid) {
-  constexpr unsigned kAhead = 8;
-  const unsigned tid = threadIdx.x, first = window * kWindow;
+  constexpr unsigned kRows = 4, kSlots = 8;
+  const unsigned tid = threadIdx.x, lane = tid % 64, first = window * kWindow;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const unsigned mine = min(kWindow, g.pages - first);
+  const unsigned pieces = (g.tableStride + 64 * kSlots - 1) / (64 * kSlots); // of a row
+  const unsigned all = g.sequences * pieces, step = parts * kFreeWaves;      // (< 2^31)
+  bool lost = false;
   for (unsigned w = tid; w < (mine + 31) / 32; w += kFreeThreads)
     marks[w] = 0;
   __syncthreads();
-  const unsigned pieces = (g.tableStride + kFreeThreads - 1) / kFreeThreads; // of a row
-  const uint64_t all = (uint64_t)g.sequences * pieces;
-  bool lost = false;
-  for (uint64_t i0 = part; i0 < all; i0 += (uint64_t)kAhead * parts) {
-    int entry[kAhead];
-    bool held[kAhead];
+  for (unsigned i0 = part * kFreeWaves + wave; i0 < all; i0 += kRows * step) {
+    unsigned from[kRows], count[kRows]; // slots of the rows that hold pages
+    size_t row[kRows];
+    int page[kRows][kSlots];
 #pragma unroll
-    for (unsigned n = 0; n < kAhead; ++n) {
-      const uint64_t i = i0 + (uint64_t)n * parts;
-      const unsigned s = i < all ? (unsigned)(i / pieces) : 0u;
-      const unsigned slot = (unsigned)(i % pieces) * kFreeThreads + tid;
+    for (unsigned n = 0; n < kRows; ++n) {
+      const unsigned i = min(i0 + n * step, all - 1), s = i / pieces;
       const int length = g.lengths[s];
       const bool bad = length < 0 || (long long)length > (long long)g.tableStride * g.pageSize;
-      lost |= bad && i < all;
+      lost |= bad;
       // (a sequence that does not fit its row holds all of it)
-      held[n] = i < all && slot < g.tableStride && (bad || (uint64_t)slot * g.pageSize < (unsigned)length);
-      entry[n] = held[n] ? g.table[(size_t)s * g.tableStride + slot] : 0;
+      count[n] = i0 + n * step >= all ? 0u
+                 : bad                ? g.tableStride
+                                      : ((unsigned)length + g.pageSize - 1) / g.pageSize;
+      from[n] = i % pieces * 64 * kSlots + lane;
+      row[n] = (size_t)s * g.tableStride;
     }
 #pragma unroll
-    for (unsigned n = 0; n < kAhead; ++n) {
-      if (!held[n])
-        continue;
-      const unsigned page = (unsigned)entry[n];
-      lost |= page >= g.pages;
-      if (page < g.pages && page - first < mine)
-        atomicOr(&marks[(page - first) / 32], 1u << (page - first) % 32);
-    }
+    for (unsigned n = 0; n < kRows; ++n)
+#pragma unroll
+      for (unsigned k = 0; k < kSlots; ++k)
+        if (from[n] + 64 * k < count[n])
+          page[n][k] = g.table[row[n] + from[n] + 64 * k];
+#pragma unroll
+    for (unsigned n = 0; n < kRows; ++n)
+#pragma unroll
+      for (unsigned k = 0; k < kSlots; ++k) {
+        if (from[n] + 64 * k >= count[n])
+          continue;
+        const unsigned x = (unsigned)page[n][k];
+        lost |= x >= g.pages;
+        if (x < g.pages && x - first < mine)
+          atomicOr(&marks[(x - first) / 32], 1u << (x - first) % 32);
+      }
   }
   if (lost && invalid)
     atomicOr(invalid, kPagedPlace);
@@ -127,14 +140,16 @@ __device__ __forceinline__ void mark_held(const FreeView &g, unsigned part, unsi
 // Entries of the pages [first, first + count), `before` of the pages before
 // them free: a free page at its rank, and for each other one a -1 from the end.
 // word(i) has the marks of pages 32 i .. 32 i + 31.
-template <typename Word>
+template <unsigned Most, typename Word>
 __device__ __forceinline__ void list_free(unsigned first, unsigned count, unsigned before,
                                           unsigned pages, int32_t *free, int32_t *number,
                                           Word word) {
-  __shared__ unsigned sBefore[kListed / 64 + 1];
+  constexpr unsigned kGroups = Most / 64, kEach = kGroups / 64; // of 64 pages; of a lane
+  static_assert(kEach * 4096 == Most, "whole groups a lane");
+  __shared__ unsigned sBefore[kGroups + 1];
   const unsigned tid = threadIdx.x, lane = tid % 64;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  const unsigned groups = (count + 63) / 64; // of 64 pages
+  const unsigned groups = (count + 63) / 64;
   auto held = [&](unsigned i) { // of group i; those behind the last page held
     const unsigned at = first / 32 + 2 * i, left = count - 64 * i;
     uint64_t x = word(at);
@@ -142,16 +157,20 @@ __device__ __forceinline__ void list_free(unsigned first, unsigned count, unsign
       x |= (uint64_t)word(at + 1) << 32;
     return left < 64 ? x | ~0ull << left : x;
   };
-  // (kListed / 64 = 128 groups: two a lane of the first wave)
-  static_assert(kListed == 128 * 64, "two groups a lane below");
   if (wave == 0) {
-    const unsigned a = 2 * lane < groups ? 64 - __builtin_popcountll(held(2 * lane)) : 0u;
-    const unsigned b = 2 * lane + 1 < groups ? 64 - __builtin_popcountll(held(2 * lane + 1)) : 0u;
-    const unsigned sum = before + wave_scan(a + b);
-    sBefore[2 * lane] = sum - a - b;
-    sBefore[2 * lane + 1] = sum - b;
+    unsigned n[kEach], sum = 0;
+    for (unsigned j = 0; j < kEach; ++j) {
+      const unsigned i = kEach * lane + j;
+      n[j] = i < groups ? 64 - __builtin_popcountll(held(i)) : 0u;
+      sum += n[j];
+    }
+    unsigned at = before + wave_scan(sum) - sum;
+    for (unsigned j = 0; j < kEach; ++j) {
+      sBefore[kEach * lane + j] = at;
+      at += n[j];
+    }
     if (lane == 63)
-      sBefore[kListed / 64] = sum;
+      sBefore[kGroups] = at;
   }
   __syncthreads();
   for (unsigned i = wave; i < groups; i += kFreeWaves) {
@@ -164,67 +183,102 @@ __device__ __forceinline__ void list_free(unsigned first, unsigned count, unsign
     }
   }
   if (first + count == pages && tid == 0)
-    *number = (int)sBefore[kListed / 64];
-  __syncthreads();
+    *number = (int)sBefore[kGroups];
 }
 
 // All of a small pool in one workgroup.
 __global__ __launch_bounds__(kFreeThreads) void paged_free_small_kernel(FreeView g, int32_t *free,
                                                                         int32_t *count,
                                                                         unsigned *invalid) {
-  __shared__ uint32_t marks[kListed / 32];
+  __shared__ uint32_t marks[kSmall / 32];
   mark_held(g, 0, 1, 0, marks, invalid);
-  list_free(0, g.pages, 0, g.pages, free, count, [&](unsigned i) { return marks[i]; });
+  list_free<kSmall>(0, g.pages, 0, g.pages, free, count, [&](unsigned i) { return marks[i]; });
 }
 
-// Marks: [part][(pages + 31) / 32].
+// What the launches leave each other: [part][words] marks, the words of a part
+// whole 16 bytes, [words] of all of them and how many pages of each kListed are
+// free.
+struct FreeMarks {
+  uint32_t *parts, *all, *count;
+};
+__host__ __device__ constexpr unsigned free_words(unsigned pages) {
+  return (pages / 32 + 4) / 4 * 4;
+}
+
 __global__ __launch_bounds__(kFreeThreads) void paged_free_mark_kernel(FreeView g, uint32_t *out,
                                                                        unsigned *invalid) {
   __shared__ uint32_t marks[kWindow / 32];
-  const unsigned window = blockIdx.y, words = (g.pages + 31) / 32;
+  const unsigned window = blockIdx.y, words = free_words(g.pages);
   mark_held(g, blockIdx.x, gridDim.x, window, marks, invalid);
   uint32_t *to = out + (size_t)blockIdx.x * words + window * (kWindow / 32);
-  const unsigned mine = min(kWindow / 32, words - window * (kWindow / 32));
-  for (unsigned w = threadIdx.x; w < mine; w += kFreeThreads)
+  const unsigned mine = min(kWindow, g.pages - window * kWindow);
+  for (unsigned w = threadIdx.x; w < (mine + 31) / 32; w += kFreeThreads)
     to[w] = marks[w];
 }
 
+// The marks of all parts, kListed pages a workgroup: 16 bytes of every eighth
+// part a thread.
+constexpr unsigned kJoinThreads = kListed / 128 * 8;
+__global__ __launch_bounds__(kJoinThreads) void paged_free_join_kernel(FreeMarks m, unsigned parts,
+                                                                       unsigned pages) {
+  constexpr unsigned kFours = kListed / 128;
+  const unsigned words = free_words(pages), i = threadIdx.x % kFours, p0 = threadIdx.x / kFours;
+  const unsigned at = 4 * (blockIdx.x * kFours + i), first = blockIdx.x * kListed + 128 * i;
+  __shared__ uint4_t sMarks[8][kFours];
+  uint4_t x = 0;
+  if (at < words) {
+#pragma unroll
+    for (unsigned n = 0; n < kMarkers / 8; ++n) // (the last part again)
+      x |= *reinterpret_cast<const uint4_t *>(m.parts + (size_t)min(p0 + 8 * n, parts - 1) * words + at);
+  }
+  sMarks[p0][i] = x;
+  __syncthreads();
+  if (threadIdx.x >= 64)
+    return;
+  unsigned n = 0;
+  if (p0 == 0 && at < words) {
+    for (unsigned p = 1; p < 8; ++p)
+      x |= sMarks[p][i];
+    *reinterpret_cast<uint4_t *>(m.all + at) = x;
+    for (unsigned j = 0; j < 4; ++j) {
+      const unsigned page = first + 32 * j, left = page < pages ? min(pages - page, 32u) : 0u;
+      n += left - __builtin_popcount(left < 32 ? x[j] & ((1u << left) - 1) : x[j]);
+    }
+  }
+  n = wave_scan(n);
+  if (threadIdx.x == 63)
+    m.count[blockIdx.x] = n;
+}
+
 // kListed pages a workgroup, behind the free ones of all before.
-__global__ __launch_bounds__(kFreeThreads) void paged_free_list_kernel(const uint32_t *marks,
-                                                                       unsigned parts,
-                                                                       unsigned pages, int32_t *free,
+__global__ __launch_bounds__(kFreeThreads) void paged_free_list_kernel(FreeMarks m, unsigned pages,
+                                                                       int32_t *free,
                                                                        int32_t *count) {
-  const unsigned words = (pages + 31) / 32, first = blockIdx.x * kListed, tid = threadIdx.x;
+  const unsigned first = blockIdx.x * kListed, tid = threadIdx.x;
   __shared__ unsigned sFree[kFreeWaves];
   __shared__ uint32_t sWord[kListed / 32];
-  auto word = [&](unsigned i) {
-    uint32_t x = 0;
-    for (unsigned p = 0; p < parts; ++p)
-      x |= marks[(size_t)p * words + i];
-    return x;
-  };
+  const unsigned mine = min(kListed, pages - first);
   unsigned n = 0;
-  for (unsigned i = tid; i < first / 32; i += kFreeThreads)
-    n += 32 - __builtin_popcount(word(i));
+  for (unsigned i = tid; i < blockIdx.x; i += kFreeThreads)
+    n += m.count[i];
+  if (tid < (mine + 31) / 32)
+    sWord[tid] = m.all[first / 32 + tid];
   n = wave_scan(n);
   if (tid % 64 == 63)
     sFree[tid / 64] = n;
-  const unsigned mine = min(kListed, pages - first);
-  for (unsigned i = tid; i < (mine + 31) / 32; i += kFreeThreads)
-    sWord[i] = word(first / 32 + i);
   __syncthreads();
   n = 0;
   for (unsigned w = 0; w < kFreeWaves; ++w)
     n += sFree[w];
-  list_free(first, mine, n, pages, free, count,
-            [&](unsigned i) { return sWord[i - first / 32]; });
+  list_free<kListed>(first, mine, n, pages, free, count,
+                     [&](unsigned i) { return sWord[i - first / 32]; });
 }
 
 unsigned free_markers(const PagedFreeParams &p) {
   const uint64_t slots = (uint64_t)p.sequences * p.tableStride, parts = slots / 16384;
   return parts < 1 ? 1u : parts < kMarkers ? (unsigned)parts : kMarkers;
 }
-bool free_small(const PagedFreeParams &p) { return p.pages <= kListed && free_markers(p) == 1; }
+bool free_small(const PagedFreeParams &p) { return p.pages <= kSmall && free_markers(p) == 1; }
 
 // -------------------------------------------------------------------- move
 //
@@ -435,9 +489,10 @@ hipError_t launch_paged_fork(const int32_t *table, const int32_t *past, const in
                             : run(paged_fork_kernel<64>);
 }
 
-unsigned paged_free_launches(const PagedFreeParams &p) { return free_small(p) ? 1 : 2; }
+unsigned paged_free_launches(const PagedFreeParams &p) { return free_small(p) ? 1 : 3; }
 size_t paged_free_workspace_bytes(const PagedFreeParams &p) {
-  return free_small(p) ? 0 : (size_t)free_markers(p) * (((size_t)p.pages + 31) / 32) * 4;
+  const size_t lists = (p.pages + kListed - 1) / kListed;
+  return free_small(p) ? 0 : 4 * ((free_markers(p) + 1) * (size_t)free_words(p.pages) + lists);
 }
 hipError_t launch_paged_free(const int32_t *table, const int32_t *lengths, int32_t *free,
                              int32_t *count, uint32_t *invalid, void *workspace,
@@ -448,14 +503,21 @@ hipError_t launch_paged_free(const int32_t *table, const int32_t *lengths, int32
                        count, invalid);
     return hipGetLastError();
   }
-  uint32_t *marks = static_cast<uint32_t *>(workspace);
   const unsigned parts = free_markers(p), windows = (p.pages + kWindow - 1) / kWindow;
+  const unsigned lists = (p.pages + kListed - 1) / kListed;
+  const size_t words = free_words(p.pages);
+  uint32_t *marks = static_cast<uint32_t *>(workspace);
+  const FreeMarks m{marks, marks + parts * words, marks + (parts + 1) * words};
   hipLaunchKernelGGL(paged_free_mark_kernel, dim3(parts, windows), dim3(kFreeThreads), 0, stream, g,
-                     marks, invalid);
+                     m.parts, invalid);
   if (hipError_t e = hipGetLastError())
     return e;
-  hipLaunchKernelGGL(paged_free_list_kernel, dim3((p.pages + kListed - 1) / kListed),
-                     dim3(kFreeThreads), 0, stream, marks, parts, p.pages, free, count);
+  hipLaunchKernelGGL(paged_free_join_kernel, dim3(lists), dim3(kJoinThreads), 0, stream, m, parts,
+                     p.pages);
+  if (hipError_t e = hipGetLastError())
+    return e;
+  hipLaunchKernelGGL(paged_free_list_kernel, dim3(lists), dim3(kFreeThreads), 0, stream, m, p.pages,
+                     free, count);
   return hipGetLastError();
 }
 

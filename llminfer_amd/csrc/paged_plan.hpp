@@ -5,6 +5,7 @@
 
 #include "hip_common.hpp"
 #include "paged_kv.hpp"
+#include "paged_shared.hpp"
 
 namespace llmi {
 
@@ -78,18 +79,34 @@ struct SplitPlan {
 // The chunk, whole steps, for which the call has at most plan.target pieces
 // more than units. (The fp32 sum is exact below 2^24, and off by less than
 // the 1.0001 above; every workgroup and the merge add in the same order.)
-template <typename View>
-__device__ __forceinline__ Split paged_split(const View &g, const typename View::Seq &own,
-                                             unsigned group, const SplitPlan &plan) {
-  Split s{group, plan.shift, plan.step, plan.step, 0.0f, plan.nearest != 0};
+template <typename Seq>
+__device__ __forceinline__ float lane_blocks(const Split &s, const Seq &q) {
+  return (float)s.units(q) * (float)Split::blocks(q);
+}
+__device__ __forceinline__ float all_blocks(const Split &s, const PagedView &g,
+                                            const PagedSeq &own) {
   const unsigned lane = threadIdx.x % 64;
-  float all = (float)s.units(own) * (float)Split::blocks(own);
+  float all = lane_blocks(s, own);
   for (unsigned s0 = 64; s0 < g.sequences; s0 += 64)
-    if (s0 + lane < g.sequences) {
-      const typename View::Seq q = paged_seq(g, s0 + lane);
-      all += (float)s.units(q) * (float)Split::blocks(q);
-    }
-  all = group_sum<16>(all);
+    if (s0 + lane < g.sequences)
+      all += lane_blocks(s, paged_seq(g, s0 + lane));
+  return all;
+}
+__device__ __forceinline__ float all_blocks(const Split &s, const SharedView &g,
+                                            const SharedLanes &own) {
+  float all = 0.0f;
+  shared_chunks(g, own, [&](unsigned, const SharedSeq &q) {
+    all += lane_blocks(s, q);
+    return false;
+  });
+  return all;
+}
+template <typename View, typename Own>
+__device__ __forceinline__ Split paged_split(const View &g, const Own &lanes, unsigned group,
+                                             const SplitPlan &plan) {
+  Split s{group, plan.shift, plan.step, plan.step, 0.0f, plan.nearest != 0};
+  const auto &own = paged_first(lanes);
+  float all = group_sum<16>(all_blocks(s, g, lanes));
   LanePair p = pair16(all);
   all = p.a + p.b;
   p = pair32(all);

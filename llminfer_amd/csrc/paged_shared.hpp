@@ -12,15 +12,23 @@ namespace llmi {
 
 // Rows [row0, row0 + rows) over the keys from block `begin` to `end`: row i
 // sees those up to past + i (step 1) or past (step 0, a group's shared keys).
+// from: the row of the table. group: a sequence's, if it has shared keys.
 struct SharedSeq {
   unsigned row0, rows, past;
   bool ok;
-  unsigned begin, end, step, from; // from: the row of the table
+  unsigned begin, end, step, from, group;
   __device__ unsigned keys() const { return end; }
   __device__ unsigned first() const { return begin; }
   __device__ unsigned last(unsigned row) const { return past + step * row; }
   __device__ unsigned table(unsigned) const { return from; }
   __device__ bool joined() const { return begin != 0 || step == 0; }
+};
+
+// What the workgroups of a sequence leave for the join: its first piece, how
+// many a unit has, its units, and the group whose partials are joined to them
+// (+ 1; 0: none), for a group its first row.
+struct SharedNote {
+  unsigned first, pieces, units, other;
 };
 
 // Sequences base .. base + sequences - 1 of `count` groups and then `all`
@@ -29,58 +37,104 @@ struct SharedSeq {
 struct SharedView : PagedView {
   typedef SharedSeq Seq;
   const int32_t *groups, *prefix;
+  SharedNote *notes; // [count + all]
   unsigned count, all, base;
 };
 
-// A group's shared keys that are read as one: whole blocks.
-__device__ __forceinline__ unsigned shared_keys(const SharedView &g, unsigned group) {
-  return (unsigned)max(g.prefix[group], 0) & ~31u;
+// The groups' arrays, those of group `lane` in registers.
+struct SharedGroups {
+  int first, behind, prefix;
+};
+__device__ __forceinline__ SharedGroups shared_groups(const SharedView &g) {
+  const unsigned i = min(threadIdx.x % 64, g.count - 1);
+  return {g.groups[i], g.groups[i + 1], g.prefix[i]};
 }
 
-// The group of a sequence, by bisection (groups are in order); false if it is
-// in none.
-__device__ __forceinline__ bool shared_group(const SharedView &g, unsigned seq, unsigned &group) {
-  unsigned lo = 0, hi = g.count; // groups[lo] <= seq < groups[hi], if any
-  while (hi - lo > 1) {
-    const unsigned mid = (lo + hi) / 2;
-    if (g.groups[mid] <= (int)seq)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  group = lo;
-  return g.groups[lo] <= (int)seq && (int)seq < g.groups[lo + 1];
-}
-
-// A sequence's own keys. One that is shorter than its group's prefix has no
-// place.
-__device__ __forceinline__ SharedSeq shared_own_keys(const SharedView &g, unsigned seq) {
-  const PagedSeq p = paged_seq(static_cast<const PagedView &>(g), seq);
-  SharedSeq q{p.row0, p.rows, p.past, p.ok, 0, p.past + p.rows, 1, seq};
-  unsigned group;
-  if (shared_group(g, seq, group)) {
-    const int prefix = g.prefix[group];
-    q.ok = q.ok && prefix <= (int)p.past;
-    q.begin = q.ok ? shared_keys(g, group) / 32 : 0u;
+// Sequence s of the view (nothing past the last one), a different one in every
+// lane; all lanes call it. Groups and sequences take the same steps, so that the
+// loads of both are in flight together.
+__device__ __forceinline__ SharedSeq shared_seq(const SharedView &g, const SharedGroups &lanes,
+                                                unsigned s) {
+  const bool none = s >= g.sequences, few = g.count <= 64;
+  const unsigned v = (none ? g.sequences - 1 : s) + g.base;
+  const bool ofGroup = v < g.count;
+  const unsigned seq = ofGroup ? 0u : v - g.count;
+  auto group_of = [&](int mine, const int32_t *array, unsigned i) {
+    return few ? __shfl(mine, (int)i) : array[i];
+  };
+  // the last group that begins at or before the sequence, by bisection
+  unsigned group = 0;
+  for (unsigned n = g.count; n > 1; n -= n / 2)
+    if (group_of(lanes.first, g.groups, group + n / 2) <= (int)seq)
+      group += n / 2;
+  group = ofGroup ? v : group;
+  const int from = group_of(lanes.first, g.groups, group);
+  const int to = group_of(lanes.behind, g.groups + 1, group);
+  const int prefix = group_of(lanes.prefix, g.prefix, group);
+  const int S = (int)g.all, T = (int)g.tokens;
+  const int s0 = ofGroup ? min(max(from, 0), S) : (int)seq;
+  const int s1 = ofGroup ? min(max(to, s0), S) : (int)seq + 1;
+  const int lo = min(max(g.starts[s0], 0), T), hi = min(max(g.starts[s1], lo), T);
+  const int past = g.past[seq];
+  const unsigned keys = (unsigned)max(prefix, 0) & ~31u; // those that are read as one
+  const long long most = (long long)g.tableStride * g.pageSize;
+  SharedSeq q;
+  q.row0 = (unsigned)lo;
+  q.rows = none ? 0u : (unsigned)(hi - lo);
+  q.step = ofGroup ? 0u : 1u;
+  q.from = (unsigned)s0;
+  q.group = group;
+  if (ofGroup) {
+    // (more keys than a row of the table has: no sequence has a place)
+    const bool any = s1 > s0 && keys && keys <= most;
+    q.rows = any ? q.rows : 0u;
+    q.past = keys - 1;
+    q.ok = true;
+    q.begin = 0;
+    q.end = any ? keys : 0u;
+  } else {
+    // one that is shorter than its group's prefix has no place
+    const bool in = from <= (int)seq && (int)seq < to;
+    q.past = (unsigned)past;
+    q.ok = none || (past >= 0 && (long long)past + (hi - lo) <= most && !(in && prefix > past));
+    q.begin = in && q.ok ? keys / 32 : 0u;
+    q.end = q.past + (unsigned)(hi - lo);
   }
   return q;
 }
 
-// A group's shared keys, for all of its rows.
-__device__ __forceinline__ SharedSeq shared_prefix_keys(const SharedView &g, unsigned group) {
-  const int S = (int)g.all, T = (int)g.tokens;
-  const int s0 = min(max(g.groups[group], 0), S), s1 = min(max(g.groups[group + 1], s0), S);
-  const int lo = min(max(g.starts[s0], 0), T), hi = min(max(g.starts[s1], lo), T);
-  const unsigned keys = shared_keys(g, group);
-  // (more keys than a row of the table has: no sequence has a place)
-  const bool any = s1 > s0 && keys && keys <= (unsigned)(g.tableStride * g.pageSize);
-  return SharedSeq{(unsigned)lo, any ? (unsigned)(hi - lo) : 0u, keys - 1,       true, 0,
-                   any ? keys : 0u, 0, (unsigned)s0};
+// The first 256 sequences, one a lane and member (no array, which would be in
+// memory): most calls read the lengths once, all of them in flight.
+struct SharedLanes {
+  SharedGroups groups;
+  SharedSeq a, b, c, d;
+};
+__device__ __forceinline__ SharedLanes paged_own(const SharedView &g) {
+  const unsigned lane = threadIdx.x % 64;
+  SharedLanes own;
+  own.groups = shared_groups(g);
+  own.a = shared_seq(g, own.groups, lane);
+  own.b = own.c = own.d = SharedSeq{0, 0, 0, true};
+  if (g.sequences > 64) {
+    own.b = shared_seq(g, own.groups, 64 + lane);
+    own.c = shared_seq(g, own.groups, 128 + lane);
+    own.d = shared_seq(g, own.groups, 192 + lane);
+  }
+  return own;
 }
+__device__ __forceinline__ const SharedSeq &paged_first(const SharedLanes &own) { return own.a; }
 
-__device__ __forceinline__ SharedSeq paged_seq(const SharedView &g, unsigned s) {
-  s += g.base;
-  return s < g.count ? shared_prefix_keys(g, s) : shared_own_keys(g, s - g.count);
+// `each(number of the 64, its sequences)` for all of them, in order, until it
+// says true.
+template <typename Each>
+__device__ __forceinline__ void shared_chunks(const SharedView &g, const SharedLanes &own, Each each) {
+  if (each(0u, own.a) || g.sequences <= 64)
+    return;
+  if (each(1u, own.b) || each(2u, own.c) || each(3u, own.d))
+    return;
+  for (unsigned c = 4; 64 * c < g.sequences; ++c)
+    if (each(c, shared_seq(g, own.groups, 64 * c + threadIdx.x % 64)))
+      return;
 }
 
 __device__ __forceinline__ SharedSeq paged_from_lane(const SharedSeq &own, unsigned lane) {
@@ -94,7 +148,54 @@ __device__ __forceinline__ SharedSeq paged_from_lane(const SharedSeq &own, unsig
   q.end = at(own.end);
   q.step = at(own.step);
   q.from = at(own.from);
+  q.group = at(own.group);
   return q;
+}
+__device__ __forceinline__ SharedSeq paged_seq_of(const SharedView &g, const SharedLanes &own,
+                                                  unsigned seq) {
+  SharedSeq q;
+  shared_chunks(g, own, [&](unsigned c, const SharedSeq &s) {
+    if (c != seq / 64)
+      return false;
+    q = paged_from_lane(s, seq % 64);
+    return true;
+  });
+  return q;
+}
+
+template <typename Count>
+__device__ __forceinline__ bool paged_find(const SharedView &g, const SharedLanes &own, unsigned u,
+                                           Count count, unsigned &seq, unsigned &local,
+                                           unsigned &before) {
+  bool found = false;
+  before = 0;
+  shared_chunks(g, own, [&](unsigned c, const SharedSeq &q) {
+    const unsigned n = count(q), sum = wave_scan(n);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(u - before < sum);
+    if (!past) {
+      before += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+      return false;
+    }
+    const int at = __builtin_ctzll(past);
+    seq = 64 * c + (unsigned)at;
+    before += (unsigned)__builtin_amdgcn_readlane((int)(sum - n), at);
+    local = u - before;
+    // (not so with starts out of order: a sum that wrapped)
+    found = local < (unsigned)__builtin_amdgcn_readlane((int)n, at);
+    return true;
+  });
+  return found;
+}
+
+// What the join needs of a sequence, left by its first workgroup of the first
+// KV head. One without a place has its output already, and nothing to join.
+__device__ __forceinline__ void leave_note(const PagedView &, const PagedSeq &, unsigned, unsigned,
+                                           unsigned, unsigned) {}
+__device__ __forceinline__ void leave_note(const SharedView &g, const SharedSeq &s, unsigned seq,
+                                           unsigned first, unsigned pieces, unsigned units) {
+  const bool join = s.ok && (s.joined() || pieces > 1);
+  g.notes[g.base + seq] =
+      SharedNote{first, join ? pieces : 0u, units, s.step == 0 ? s.row0 : s.begin ? s.group + 1 : 0u};
 }
 
 } // namespace llmi

@@ -34,7 +34,6 @@
 #include "hip_common.hpp"
 #include "paged_kv.hpp"
 #include "paged_plan.hpp"
-#include "paged_shared.hpp"
 
 #include <math.h>
 #include <type_traits>
@@ -65,14 +64,15 @@ template <int I> __device__ __forceinline__ char *tile_buffer() {
 // sequences; in their order otherwise), so that workgroups which start late
 // have little to do (seven messages of 41 to 110 blocks, 296 workgroups:
 // 174 us in order, 130 longest first).
-template <typename View>
-__device__ __forceinline__ bool find_longest(const View &g, const typename View::Seq &own,
-                                             const Split &split, unsigned u, unsigned &seq,
-                                             unsigned &local, unsigned &number) {
+template <typename View, typename Own>
+__device__ __forceinline__ bool find_longest(const View &g, const Own &lanes, const Split &split,
+                                             unsigned u, unsigned &seq, unsigned &local,
+                                             unsigned &number) {
+  const auto &own = paged_first(lanes);
   unsigned before;
   if (g.sequences == 1 || g.sequences > 64) {
     number = u;
-    return paged_find(g, own, u,
+    return paged_find(g, lanes, u,
                       [&](const auto &s) { return split.units(s) * split.pieces(s); }, seq,
                       local, before);
   }
@@ -137,6 +137,8 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const auto s = paged_seq_of(g, own, seq);
   const unsigned pieces = split.pieces(s), units = split.units(s);
   const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
+  if (local == 0 && kvh == 0 && threadIdx.x == 0)
+    leave_note(g, s, seq, number, pieces, units);
   const unsigned tid = threadIdx.x, lane = tid % 64, r = lane % 32, hi = lane / 32;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const unsigned half = wave / 4, tile0 = wave % 4 * CT;

@@ -153,8 +153,8 @@ def test_launches():
     assert ops.kernel_names(_lib.OP_PAGED_FORK, fork_params()) == ["pagedFork"]
     assert ops.kernel_names(_lib.OP_PAGED_FORK, fork_params(children=0)) == []
     assert ops.kernel_names(_lib.OP_PAGED_FREE, free_params()) == ["pagedFree"]
-    assert ops.kernel_names(_lib.OP_PAGED_FREE, free_params(pages=10**5)) == ["pagedFreeMark",
-                                                                             "pagedFreeList"]
+    assert ops.kernel_names(_lib.OP_PAGED_FREE, free_params(pages=10**5)) == [
+        "pagedFreeMark", "pagedFreeJoin", "pagedFreeList"]
     assert ops.kernel_names(_lib.OP_PAGED_MOVE, kv_params()) == ["pagedGather", "pagedPlace"]
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED, shared_params(heads=4))
     assert names[-1] == "pagedSharedMerge" and names[0] == "pagedGqaSplit"

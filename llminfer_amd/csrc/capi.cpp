@@ -1566,10 +1566,7 @@ const char *llmi_hip_kernel_name(int op, const void *params, unsigned index) {
     const PagedSharedParams &p = *static_cast<const PagedSharedParams *>(params);
     if (!p.groups)
       return llmi_hip_kernel_name(LLMI_HIP_OP_PAGED_GQA, &p.gqa, index);
-    if (index + 1 == llmi_hip_dispatch_count(op, params))
-      return "pagedSharedMerge";
-    return paged_shared_tiled(p.gqa.kv, p.gqa.queryHeads, p.groups, index) ? "pagedGqaTiles"
-                                                                          : "pagedGqaSplit";
+    return paged_shared_kernel(p.gqa.kv, p.gqa.queryHeads, p.groups, index);
   }
   case LLMI_HIP_OP_PAGED_FORK:
     return "pagedFork";

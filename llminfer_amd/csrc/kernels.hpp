@@ -312,8 +312,8 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
 bool paged_shared_launchable(const PagedKvParams &p, unsigned queryHeads, unsigned groups);
 size_t paged_shared_workspace_bytes(const PagedKvParams &p, unsigned queryHeads, unsigned groups);
 unsigned paged_shared_launches(const PagedKvParams &p, unsigned queryHeads, unsigned groups);
-// Whether the tiles' kernel runs for the shared keys, or for the others.
-bool paged_shared_tiled(const PagedKvParams &p, unsigned queryHeads, unsigned groups, bool rest);
+const char *paged_shared_kernel(const PagedKvParams &p, unsigned queryHeads, unsigned groups,
+                                unsigned index); // of those launches
 hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, const int32_t *past,
                                    const int32_t *table, const int32_t *groups,
                                    const int32_t *prefix, const void *pool, uint16_t *out,

@@ -610,10 +610,11 @@ __global__ __launch_bounds__(kMergeThreads) void paged_gqa_merge_kernel(
 
 // ------------------------------------------------ sequences in groups
 
-// A launch over a SharedView: its plan, its partials and how many pieces it has.
+// A launch over a SharedView: units of 2^shift columns, its partials and how many
+// pieces it has at most.
 struct SharedPart {
   SharedView g;
-  SplitPlan plan;
+  unsigned shift;
   Partials parts;
   unsigned most;
 };
@@ -669,7 +670,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
     // column `column` of a note's pieces; false where starts out of order make
     // more of them than the rows can have
     auto join = [&](const SharedPart &part, const SharedNote &note, unsigned column, unsigned turn) {
-      const unsigned unit = 1u << part.plan.shift, pieces = note.pieces;
+      const unsigned unit = 1u << part.shift, pieces = note.pieces;
       const unsigned long long first =
           note.first + (unsigned long long)(note.units - 1 - column / unit) * pieces;
       if (column / unit >= note.units || first + pieces > part.most)
@@ -834,35 +835,57 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
 
 namespace {
 
-// The groups' shared keys and the sequences' own: in one launch, or apart where
-// the shared keys have columns for a kernel that would waste most of itself on
-// a sequence's few.
+// How the groups' shared keys and the sequences' own are taken: both in units of
+// the same columns by one launch (Same); shared keys in tiles beside own keys in
+// units of 16, by one launch (Mixed); each by a launch of its own (Apart), where
+// the sequences have many rows themselves, or more units of shared keys than
+// workgroups.
 struct SharedPlan {
-  bool apart;
+  enum { Same, Mixed, Apart } how;
   GqaPlan shared, rest;
+  MixedPlan mixed;
+  unsigned sharedShift, restShift; // columns of a unit
   uint64_t sharedPieces, restPieces; // a KV head, at most
 };
 SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) {
   PagedKvParams of = p;
   of.sequences = groups;
-  SharedPlan s;
+  const uint64_t columns = (uint64_t)p.tokens * group / groups;
+  SharedPlan s{};
   s.shared = plan_for(of, group);
   s.rest = plan_for(p, group);
-  s.apart = s.shared.split.shift > 5;
-  s.sharedPieces = most_pieces(of, group, s.shared.split);
-  if (!s.apart) {
-    s.rest = s.shared;
-    s.sharedPieces += most_units(p, group, 1u << s.shared.split.shift);
-    s.restPieces = s.sharedPieces;
-  } else
+  s.restShift = s.rest.split.shift;
+  s.mixed.shift = p.headDim == 256 || columns < 256 ? 7 : 8;
+  s.mixed.step = 512 / p.headDim;
+  s.mixed.cus = kCus / p.kvHeads ? kCus / p.kvHeads : 1;
+  s.mixed.sharedCost = p.headDim == 256 ? 1.0f : 0.5f;
+  s.mixed.ownCost = 0.17f * p.headDim / 256;
+  s.mixed.ownFixed = 6.0f;
+  const uint64_t units = most_units(of, group, 1u << s.mixed.shift);
+  if (columns >= 64 && s.restShift == 4 && units < s.mixed.cus) {
+    s.how = SharedPlan::Mixed;
+    s.sharedShift = s.mixed.shift;
+    s.sharedPieces = s.mixed.cus;
+    s.restPieces = 4 * s.mixed.cus + 2 + most_units(p, group, kColumns);
+  } else if (s.shared.split.shift > 5) {
+    s.how = SharedPlan::Apart;
+    s.sharedShift = s.shared.split.shift;
+    s.sharedPieces = most_pieces(of, group, s.shared.split);
     s.restPieces = most_pieces(p, group, s.rest.split);
+  } else {
+    s.how = SharedPlan::Same;
+    s.rest = s.shared;
+    s.sharedShift = s.restShift = s.shared.split.shift;
+    s.sharedPieces = s.restPieces =
+        most_pieces(of, group, s.shared.split) + most_units(p, group, 1u << s.restShift);
+  }
   return s;
 }
 size_t shared_columns(const PagedKvParams &p, const SharedPlan &s) {
-  return (size_t)s.sharedPieces * p.kvHeads << s.shared.split.shift;
+  return (size_t)s.sharedPieces * p.kvHeads << s.sharedShift;
 }
 size_t rest_columns(const PagedKvParams &p, const SharedPlan &s) {
-  return s.apart ? (size_t)s.restPieces * p.kvHeads << s.rest.split.shift : 0;
+  return s.how == SharedPlan::Same ? 0 : (size_t)s.restPieces * p.kvHeads << s.restShift;
 }
 size_t notes_bytes(const PagedKvParams &p, unsigned groups) {
   return ((size_t)groups + p.sequences) * sizeof(SharedNote);
@@ -880,11 +903,16 @@ size_t paged_shared_workspace_bytes(const PagedKvParams &p, unsigned queryHeads,
   return notes_bytes(p, groups) + 4 * (p.headDim + 2) * (shared_columns(p, s) + rest_columns(p, s));
 }
 unsigned paged_shared_launches(const PagedKvParams &p, unsigned queryHeads, unsigned groups) {
-  return shared_plan(p, queryHeads / p.kvHeads, groups).apart ? 3 : 2;
+  return shared_plan(p, queryHeads / p.kvHeads, groups).how == SharedPlan::Apart ? 3 : 2;
 }
-bool paged_shared_tiled(const PagedKvParams &p, unsigned queryHeads, unsigned groups, bool rest) {
+const char *paged_shared_kernel(const PagedKvParams &p, unsigned queryHeads, unsigned groups,
+                                unsigned index) {
   const SharedPlan s = shared_plan(p, queryHeads / p.kvHeads, groups);
-  return (rest ? s.rest : s.shared).split.shift > 6;
+  if (index == (s.how == SharedPlan::Apart ? 2u : 1u))
+    return "pagedSharedMerge";
+  if (s.how == SharedPlan::Mixed)
+    return "pagedGqaMixed";
+  return (index ? s.restShift : s.sharedShift) > 6 ? "pagedGqaTiles" : "pagedGqaSplit";
 }
 
 hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, const int32_t *past,
@@ -901,32 +929,38 @@ hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, con
   SharedNote *notes = static_cast<SharedNote *>(workspace);
   float *ws = reinterpret_cast<float *>(notes + count + p.sequences);
   const size_t sharedColumns = shared_columns(p, s), restColumns = rest_columns(p, s);
-  auto part = [&](const GqaPlan &by, uint64_t pieces, float *at, size_t columns, unsigned base,
+  const bool same = s.how == SharedPlan::Same, apart = s.how == SharedPlan::Apart;
+  auto part = [&](unsigned shift, uint64_t pieces, float *at, size_t columns, unsigned base,
                   unsigned sequences) {
     SharedPart x{SharedView{paged_view(p, starts, past, table), groups, prefix, notes, count,
                             p.sequences, base},
-                 by.split, Partials{at + columns * p.headDim, at}, (unsigned)pieces};
+                 shift, Partials{at + columns * p.headDim, at}, (unsigned)pieces};
     x.g.sequences = sequences;
     return x;
   };
-  const SharedPart shared = part(s.shared, s.sharedPieces, ws, sharedColumns, 0,
-                                 s.apart ? count : count + p.sequences);
+  const SharedPart shared = part(s.sharedShift, s.sharedPieces, ws, sharedColumns, 0,
+                                 apart ? count : count + p.sequences);
   const SharedPart rest =
-      s.apart ? part(s.rest, s.restPieces, ws + sharedColumns * (p.headDim + 2), restColumns, count,
-                     p.sequences)
-              : shared;
+      same ? shared
+           : part(s.restShift, s.restPieces, ws + sharedColumns * (p.headDim + 2), restColumns,
+                  count, p.sequences);
   auto attend = [&](const SharedPart &x, const GqaPlan &by) {
     return launch_attend(from, pages, x.g, to, invalid, queryHeads, by, c, x.parts, x.most, stream);
   };
-  hipError_t e = attend(shared, s.shared);
-  if (e == hipSuccess && s.apart)
+  hipError_t e;
+  if (s.how == SharedPlan::Mixed)
+    e = launch_paged_mixed(from, pages, shared.g, to, invalid, queryHeads, s.mixed, c, shared.parts,
+                           rest.parts, shared.most, rest.most, stream);
+  else
+    e = attend(shared, s.shared);
+  if (e == hipSuccess && apart)
     e = attend(rest, s.rest);
   if (e != hipSuccess)
     return e;
   // pieces of a unit of shared keys, about, where all of them are as long
-  const unsigned unit = 1u << s.shared.split.shift;
+  const unsigned unit = 1u << s.sharedShift;
   const uint64_t units = ((uint64_t)p.tokens * (queryHeads / p.kvHeads) + unit - 1) / unit;
-  const bool many = s.shared.split.target >= 8 * units;
+  const bool many = (s.how == SharedPlan::Mixed ? s.mixed.cus : s.shared.split.target) >= 8 * units;
   auto merge = [&](auto wide, auto narrow) {
     const unsigned each = many ? 1 : kMergeThreads / 64, parts = (queryHeads + each - 1) / each;
     hipLaunchKernelGGL(many ? wide : narrow, dim3(p.tokens, parts < 65535 ? parts : 65535),

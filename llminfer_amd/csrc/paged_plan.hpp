@@ -155,4 +155,17 @@ hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const View &
                               unsigned *invalid, unsigned queryHeads, SplitPlan plan, ScoreScale c,
                               Partials parts, unsigned pieces, hipStream_t stream);
 
+// The kernel for groups with many rows in all and sequences with few
+// (paged_mixed.hip): units of 2^shift columns of the shared keys, whole steps of
+// blocks, on `cus` workgroups a KV head, and what a block of shared and of own
+// keys and a piece of own keys take.
+struct MixedPlan {
+  unsigned shift, step, cus;
+  float sharedCost, ownCost, ownFixed;
+};
+hipError_t launch_paged_mixed(const half_t *q, const uint8_t *pool, const SharedView &g, half_t *out,
+                              unsigned *invalid, unsigned queryHeads, const MixedPlan &plan,
+                              ScoreScale c, Partials shared, Partials rest, unsigned mostShared,
+                              unsigned mostOwn, hipStream_t stream);
+
 } // namespace llmi

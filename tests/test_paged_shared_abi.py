@@ -160,7 +160,10 @@ def test_launches():
     assert names[-1] == "pagedSharedMerge" and names[0] == "pagedGqaSplit"
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED,
                              shared_params(heads=16, kvHeads=4, headDim=256, tokens=48, sequences=48))
-    assert names == ["pagedGqaTiles", "pagedGqaSplit", "pagedSharedMerge"]
+    assert names == ["pagedGqaMixed", "pagedSharedMerge"]
+    names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED,
+                             shared_params(heads=16, kvHeads=4, headDim=256, tokens=400, sequences=4))
+    assert names == ["pagedGqaTiles", "pagedGqaTiles", "pagedSharedMerge"]
     plain = shared_params(groups=0, heads=4)
     assert ops.kernel_names(_lib.OP_PAGED_GQA_SHARED, plain) == \
         ops.kernel_names(_lib.OP_PAGED_GQA, plain.gqa)

@@ -617,6 +617,7 @@ struct SharedPart {
   unsigned shift;
   Partials parts;
   unsigned most;
+  bool runs; // own keys as paged_mixed_kernel divides them
 };
 
 // Joins a row's partials: those of its sequence's own keys and those of its
@@ -655,6 +656,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
   const unsigned seq = n - 1;
   const int lo = max(g.starts[seq], 0), hi = g.starts[seq + 1];
   const SharedNote mine = g.notes[g.count + seq];
+  const unsigned run = rest.runs ? g.notes[g.count + g.all].first : 0u;
   if ((int)row < lo || (int)row >= hi || mine.pieces == 0 || mine.other > g.count)
     return; // of no sequence, or its output is there
   const bool both = mine.other != 0;
@@ -667,13 +669,12 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
       return;
     float m = -INFINITY, l = 0.0f;
     vec y = 0.0f;
-    // column `column` of a note's pieces; false where starts out of order make
-    // more of them than the rows can have
-    auto join = [&](const SharedPart &part, const SharedNote &note, unsigned column, unsigned turn) {
-      const unsigned unit = 1u << part.shift, pieces = note.pieces;
-      const unsigned long long first =
-          note.first + (unsigned long long)(note.units - 1 - column / unit) * pieces;
-      if (column / unit >= note.units || first + pieces > part.most)
+    // column `column` of pieces [first, first + pieces); false where starts out of
+    // order make more of them than the rows can have
+    auto join = [&](const SharedPart &part, unsigned long long first, unsigned pieces,
+                    unsigned column, unsigned turn) {
+      const unsigned unit = 1u << part.shift;
+      if (first + pieces > part.most)
         return false;
       const size_t place = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
       const size_t step = (size_t)g.kvHeads * unit;
@@ -708,9 +709,30 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
       }
       return true;
     };
-    bool whole = join(rest, mine, (row - lo) * G + h % G, 0);
+    // units of `units` that have `pieces` each, the last unit's first
+    auto join_units = [&](const SharedPart &part, const SharedNote &note, unsigned column,
+                          unsigned turn) {
+      const unsigned unit = column >> part.shift;
+      return unit < note.units &&
+             join(part, note.first + (unsigned long long)(note.units - 1 - unit) * note.pieces,
+                  note.pieces, column, turn);
+    };
+    const unsigned column = (row - lo) * G + h % G;
+    bool whole;
+    unsigned turn = mine.pieces;
+    if (rest.runs) { // (the note: first block, blocks of a unit, first unit)
+      const unsigned unit = column >> rest.shift;
+      const unsigned long long a = mine.first + (unsigned long long)unit * mine.pieces;
+      const unsigned long long from = a / run, to = (a + mine.pieces - 1) / run;
+      turn = (unsigned)(to - from + 1);
+      if (turn == 1 && !both)
+        whole = false; // its output is there
+      else
+        whole = join(rest, from + mine.units + unit, turn, column, 0);
+    } else
+      whole = join_units(rest, mine, column, 0);
     if (both) // (`other` of a group: its first row)
-      whole = join(shared, of, (row - of.other) * G + h % G, mine.pieces) && whole;
+      whole = join_units(shared, of, (row - of.other) * G + h % G, turn) && whole;
     if (W > 1) {
       sM[wave] = m;
       sL[wave] = l;
@@ -835,11 +857,19 @@ hipError_t launch_paged_gqa(const uint16_t *q, const int32_t *starts, const int3
 
 namespace {
 
-// How the groups' shared keys and the sequences' own are taken: both in units of
-// the same columns by one launch (Same); shared keys in tiles beside own keys in
-// units of 16, by one launch (Mixed); each by a launch of its own (Apart), where
-// the sequences have many rows themselves, or more units of shared keys than
-// workgroups.
+// How the groups' shared keys and the sequences' own are taken:
+//  Same   both in units of 16 columns, by one launch of the few-column kernel;
+//  Mixed  shared keys in tiles of 128 columns, beside them own keys in units of
+//         16, by one launch (paged_mixed.hip);
+//  Apart  each by a launch of its own, as its columns ask for.
+// Mixed from 96 columns a group and 640 in all KV heads on (128 columns of 8
+// heads of 128 on 8192 keys: 29 us, 35 Same; 768 of 4 heads of 256 on 16384: 44
+// and 61; below, its beginning and end cost more: 64 of 4 heads on 4096 keys 25
+// us, 18 Same; 128 of one head 18 and 12), as long as each unit has a workgroup.
+// Apart where it has not, or where the sequences have many rows themselves.
+// Same has the pieces of its kernel's eight waves where the units are few (8
+// sequences on 4299 keys: 15.3 us, 17.2 with four), two rounds of four waves
+// otherwise (4 groups of 8 on 8192 keys: 25 us, 30 with six rounds or one).
 struct SharedPlan {
   enum { Same, Mixed, Apart } how;
   GqaPlan shared, rest;
@@ -850,34 +880,37 @@ struct SharedPlan {
 SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) {
   PagedKvParams of = p;
   of.sequences = groups;
-  const uint64_t columns = (uint64_t)p.tokens * group / groups;
+  const uint64_t all = (uint64_t)p.tokens * group;
   SharedPlan s{};
   s.shared = plan_for(of, group);
   s.rest = plan_for(p, group);
+  s.sharedShift = s.shared.split.shift;
   s.restShift = s.rest.split.shift;
-  s.mixed.shift = p.headDim == 256 || columns < 256 ? 7 : 8;
-  s.mixed.step = 512 / p.headDim;
-  s.mixed.cus = kCus / p.kvHeads ? kCus / p.kvHeads : 1;
-  s.mixed.sharedCost = p.headDim == 256 ? 1.0f : 0.5f;
-  s.mixed.ownCost = 0.17f * p.headDim / 256;
-  s.mixed.ownFixed = 6.0f;
-  const uint64_t units = most_units(of, group, 1u << s.mixed.shift);
-  if (columns >= 64 && s.restShift == 4 && units < s.mixed.cus) {
+  // (costs in us, of a workgroup: a block of 128 columns takes 1 at head_dim 256
+  // and 0.5 at 128 and 64, a wave's own block of 10 KB 2.2)
+  s.mixed = {7, 512 / p.headDim, kCus / p.kvHeads ? kCus / p.kvHeads : 1,
+             p.headDim == 256 ? 1.0f : 0.5f, 0.2f * p.headDim / 256, 0.5f};
+  const uint64_t units = most_units(of, group, 128), ownUnits = most_units(p, group, kColumns);
+  // own blocks of all units, which are counted in 32 bits
+  const uint64_t blocks = ownUnits * ((uint64_t)p.tableStride * p.pageSize / 32 + 1);
+  if (s.restShift != 4 || units >= s.mixed.cus || blocks >= 1u << 31) {
+    s.how = SharedPlan::Apart;
+    s.sharedPieces = most_pieces(of, group, s.shared.split);
+    s.restPieces = most_pieces(p, group, s.rest.split);
+  } else if (all / groups >= 96 && all * p.kvHeads >= 640) {
     s.how = SharedPlan::Mixed;
     s.sharedShift = s.mixed.shift;
     s.sharedPieces = s.mixed.cus;
-    s.restPieces = 4 * s.mixed.cus + 2 + most_units(p, group, kColumns);
-  } else if (s.shared.split.shift > 5) {
-    s.how = SharedPlan::Apart;
-    s.sharedShift = s.shared.split.shift;
-    s.sharedPieces = most_pieces(of, group, s.shared.split);
-    s.restPieces = most_pieces(p, group, s.rest.split);
+    s.restPieces = kMixedWaves * s.mixed.cus + ownUnits;
   } else {
     s.how = SharedPlan::Same;
+    const unsigned cus = (kCus + p.kvHeads - 1) / p.kvHeads;
+    const unsigned fill = p.headDim == 64 ? 2 * cus : cus;
+    const bool pooled = cus >= 8 * most_units(of, group, kColumns);
+    s.shared = {{4, pooled ? 8u : 4u, fill, pooled ? fill : 2 * cus, 16, 0, pooled}, pooled};
     s.rest = s.shared;
-    s.sharedShift = s.restShift = s.shared.split.shift;
-    s.sharedPieces = s.restPieces =
-        most_pieces(of, group, s.shared.split) + most_units(p, group, 1u << s.restShift);
+    s.sharedShift = 4;
+    s.sharedPieces = s.restPieces = most_pieces(of, group, s.shared.split) + ownUnits;
   }
   return s;
 }
@@ -888,7 +921,7 @@ size_t rest_columns(const PagedKvParams &p, const SharedPlan &s) {
   return s.how == SharedPlan::Same ? 0 : (size_t)s.restPieces * p.kvHeads << s.restShift;
 }
 size_t notes_bytes(const PagedKvParams &p, unsigned groups) {
-  return ((size_t)groups + p.sequences) * sizeof(SharedNote);
+  return ((size_t)groups + p.sequences + 1) * sizeof(SharedNote);
 }
 
 } // namespace
@@ -927,14 +960,15 @@ hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, con
   const uint8_t *pages = static_cast<const uint8_t *>(pool);
   half_t *to = reinterpret_cast<half_t *>(out);
   SharedNote *notes = static_cast<SharedNote *>(workspace);
-  float *ws = reinterpret_cast<float *>(notes + count + p.sequences);
+  float *ws = reinterpret_cast<float *>(notes + count + p.sequences + 1);
   const size_t sharedColumns = shared_columns(p, s), restColumns = rest_columns(p, s);
   const bool same = s.how == SharedPlan::Same, apart = s.how == SharedPlan::Apart;
   auto part = [&](unsigned shift, uint64_t pieces, float *at, size_t columns, unsigned base,
                   unsigned sequences) {
     SharedPart x{SharedView{paged_view(p, starts, past, table), groups, prefix, notes, count,
                             p.sequences, base},
-                 shift, Partials{at + columns * p.headDim, at}, (unsigned)pieces};
+                 shift, Partials{at + columns * p.headDim, at}, (unsigned)pieces,
+                 s.how == SharedPlan::Mixed};
     x.g.sequences = sequences;
     return x;
   };
@@ -960,7 +994,7 @@ hipError_t launch_paged_gqa_shared(const uint16_t *q, const int32_t *starts, con
   // pieces of a unit of shared keys, about, where all of them are as long
   const unsigned unit = 1u << s.sharedShift;
   const uint64_t units = ((uint64_t)p.tokens * (queryHeads / p.kvHeads) + unit - 1) / unit;
-  const bool many = (s.how == SharedPlan::Mixed ? s.mixed.cus : s.shared.split.target) >= 8 * units;
+  const bool many = (s.how == SharedPlan::Mixed ? s.mixed.cus : s.shared.split.target) >= 16 * units;
   auto merge = [&](auto wide, auto narrow) {
     const unsigned each = many ? 1 : kMergeThreads / 64, parts = (queryHeads + each - 1) / each;
     hipLaunchKernelGGL(many ? wide : narrow, dim3(p.tokens, parts < 65535 ? parts : 65535),

@@ -1,15 +1,18 @@
 // Causal GQA of groups of sequences behind shared keys, in one launch: some
 // workgroups have tiles of a group's shared keys, with all its rows as columns
-// (paged_tiles.hpp: bound by the matrix cores), the others the sequences' own
-// keys, sixteen columns a unit (bound by memory), so that both run at once. The
-// partials of the two are joined by paged_shared_merge_kernel.
+// (paged_tiles.hpp: bound by the matrix cores), the waves of the others the
+// sequences' own keys, sixteen columns a unit (bound by memory and decoding), so
+// that both run at once. The partials of the two are joined by
+// paged_shared_merge_kernel.
 #include "paged_tiles.hpp"
 
 namespace llmi {
 namespace {
 
 constexpr unsigned kColumns = 16; // of a unit of own keys
-constexpr unsigned kWaves = kThreads / 64;
+constexpr unsigned kWaves = kMixedWaves;
+static_assert(kWaves == kThreads / 64, "the tiles' waves");
+constexpr unsigned kLeastRun = 2; // blocks
 
 __device__ __forceinline__ float4_t mfma16x16x32(half8_t a, half8_t b, float4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -31,16 +34,15 @@ template <int D> struct OwnBlock {
   uint32_t key[2][CHUNKS][WORDS], scale[2][CHUNKS];
 };
 
-// Unit `unit` of a sequence's own keys over its piece `piece` of `pieces`: a wave
-// has every eighth block of 32 keys. As paged_gqa_kernel, which has the
-// arithmetic.
+// Blocks [b0, b1) of a sequence's own keys with the columns of unit `unit`, by one
+// wave, which waits for no other. As paged_gqa_kernel, which has the arithmetic.
 template <int D>
 __device__ __forceinline__ void own_piece(const half_t *__restrict__ q,
                                           const uint8_t *__restrict__ pool, const SharedView &g,
                                           half_t *out, unsigned *invalid, unsigned queryHeads,
-                                          const Split &split, ScoreScale c, const Partials &parts,
-                                          const SharedSeq &s, unsigned kvh, unsigned unit,
-                                          unsigned piece, unsigned pieces, unsigned number) {
+                                          ScoreScale c, const Partials &parts, const SharedSeq &s,
+                                          unsigned kvh, unsigned unit, unsigned b0, unsigned b1,
+                                          bool direct, unsigned number) {
   using Block = OwnBlock<D>;
   constexpr int TILES = D / 16;
   const unsigned G = queryHeads / g.kvHeads;
@@ -54,32 +56,31 @@ __device__ __forceinline__ void own_piece(const half_t *__restrict__ q,
   const unsigned visible = s.last(token_of(r)); // this lane's column's last key
   const size_t row = row_of(r);
   if (!s.ok) { // no place for this sequence
-    if (r < columns && wave == 0)
+    if (r < columns)
 #pragma unroll 1
       for (unsigned x = quad; x < D; x += 4)
         out[row + x] = (half_t)NAN;
-    if (invalid && tid == 0)
+    if (invalid && lane == 0)
       atomicOr(invalid, kPagedPlace);
     return;
   }
   const unsigned least = s.last(c0 / G), most = s.last((c0 + columns - 1) / G);
   // the keys that this wave has: to the sequence's end, or to a page that is not
   // in the pool, whose columns' outputs are NaN
-  const unsigned whole = s.keys(), length = split.length(s, pieces);
+  const unsigned whole = s.keys();
   unsigned end = whole;
-  const unsigned b0 = min(s.first() + piece * length, most / 32 + 1);
-  const unsigned b1 = min(b0 + length, most / 32 + 1);
-  const unsigned mine = b1 > b0 + wave ? (b1 - b0 - wave + kWaves - 1) / kWaves : 0u;
+  b1 = min(b1, most / 32 + 1);
+  const unsigned mine = b1 > b0 ? b1 - b0 : 0u;
 
-  // Block k of this wave is b0 + wave + kWaves k; a lane knows where one in 64 is.
+  // A lane knows where one block in 64 is.
   size_t place = 0;
   auto find_blocks = [&](unsigned k) {
-    const unsigned b = b0 + wave + kWaves * (k + lane);
+    const unsigned b = b0 + k + lane;
     bool lost = false;
     if (b < b1)
       lost = !paged_block(g, s.from, 32 * b, kvh, place);
     if (const unsigned long long all = __builtin_amdgcn_ballot_w64(lost))
-      end = min(end, 32 * (b0 + wave + kWaves * (k + (unsigned)__builtin_ctzll(all))));
+      end = min(end, 32 * (b0 + k + (unsigned)__builtin_ctzll(all)));
   };
   // (a block past the last is asked for with a descriptor of no bytes)
   auto issue = [&](unsigned k, Block &block, char *values, char *scales) {
@@ -136,7 +137,7 @@ __device__ __forceinline__ void own_piece(const half_t *__restrict__ q,
                      char *scales) __attribute__((always_inline)) {
     values += 16 * D * wave;
     scales += 1024 * wave;
-    const unsigned base = 32 * (b0 + wave + kWaves * k);
+    const unsigned base = 32 * (b0 + k);
     float4_t acc[2] = {float4_t{0, 0, 0, 0}, float4_t{0, 0, 0, 0}};
 #pragma unroll
     for (int i = 0; i < Block::CHUNKS; ++i)
@@ -215,75 +216,48 @@ __device__ __forceinline__ void own_piece(const half_t *__restrict__ q,
   };
   Block a, b;
   issue(0, a, tile_buffer<0>(), tile_buffer<2>());
-  for (unsigned k = 0; k < mine; k += 2) {
+  unsigned k = 0;
+  for (; k + 2 <= mine; k += 2) {
     issue(k + 1, b, tile_buffer<1>(), tile_buffer<3>());
     consume(k, a, tile_buffer<0>(), tile_buffer<2>());
     issue(k + 2, a, tile_buffer<0>(), tile_buffer<2>());
-    if (k + 1 < mine)
-      consume(k + 1, b, tile_buffer<1>(), tile_buffer<3>());
+    consume(k + 1, b, tile_buffer<1>(), tile_buffer<3>());
   }
+  if (k < mine)
+    consume(k, a, tile_buffer<0>(), tile_buffer<2>());
 
-  // Join the waves: (m, l) of the columns, then each wave its output tiles.
-  auto out_of = [&](unsigned w) { // wave w's tiles
-    return reinterpret_cast<float4_t *>((w / 2 == 0   ? tile_buffer<0>()
-                                         : w / 2 == 1 ? tile_buffer<1>()
-                                         : w / 2 == 2 ? tile_buffer<2>()
-                                                      : tile_buffer<3>()) +
-                                        w % 2 * TILES * 1024);
-  };
-  __shared__ float sM[kWaves * kColumns], sL[kWaves * kColumns];
-  __syncthreads(); // the blocks are done with
   if (end < whole && invalid && lane == 0)
     atomicOr(invalid, kPagedPlace);
   LanePair p = pair16(l);
   const float half = p.a + p.b;
   p = pair32(half);
-  if (quad == 0) {
-    const bool lost = visible >= end;
-    sM[wave * kColumns + r] = lost ? 0.0f : m;
-    sL[wave * kColumns + r] = lost ? NAN : p.a + p.b;
-  }
-#pragma unroll
-  for (int i = 0; i < TILES; ++i)
-    out_of(wave)[i * 64 + lane] = o[i];
-  __syncthreads();
-  float top = sM[r], sum = 0.0f, by[kWaves];
-#pragma unroll
-  for (unsigned w = 1; w < kWaves; ++w)
-    top = fmaxf(top, sM[w * kColumns + r]);
-#pragma unroll
-  for (unsigned w = 0; w < kWaves; ++w) {
-    const float mw = sM[w * kColumns + r];
-    by[w] = mw == -INFINITY ? 0.0f : fast_exp2(mw - top);
-    sum += sL[w * kColumns + r] * by[w];
-  }
-  const size_t part = ((size_t)number * g.kvHeads + kvh) * kColumns + r;
-  const bool direct = pieces == 1 && !s.joined();
-  const float scale = direct ? 1.0f / sum : 1.0f;
+  const bool lost = visible >= end;
+  const float sum = lost ? NAN : p.a + p.b;
   if (r >= columns)
     return;
-  for (unsigned i = wave; i < TILES; i += kWaves) {
-    float4_t y{0, 0, 0, 0};
+  const size_t part = ((size_t)number * g.kvHeads + kvh) * kColumns + r;
+  const float scale = 1.0f / sum;
 #pragma unroll
-    for (unsigned w = 0; w < kWaves; ++w)
-      y += out_of(w)[i * 64 + lane] * by[w];
+  for (int i = 0; i < TILES; ++i) {
     const unsigned channel = 16 * i + 4 * quad;
     if (direct)
       *reinterpret_cast<half4_t *>(out + row + channel) =
-          half4_t{(half_t)(y[0] * scale), (half_t)(y[1] * scale), (half_t)(y[2] * scale),
-                  (half_t)(y[3] * scale)};
+          half4_t{(half_t)(o[i][0] * scale), (half_t)(o[i][1] * scale), (half_t)(o[i][2] * scale),
+                  (half_t)(o[i][3] * scale)};
     else
-      *reinterpret_cast<float4_t *>(parts.o + part * D + channel) = y;
+      *reinterpret_cast<float4_t *>(parts.o + part * D + channel) = o[i];
   }
-  if (!direct && wave == 0 && quad == 0)
-    *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
+  if (!direct && quad == 0)
+    *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(lost ? 0.0f : m, sum);
 }
 
-// The two divisions: of the groups' shared keys over `workers` workgroups a KV
-// head, of the sequences' own keys over the others.
+// The two divisions. Groups' shared keys: pieces as Split has them, on `workers`
+// workgroups a KV head, one each. The sequences' own keys: the blocks of all
+// their units, one after the other, cut into runs of `run` blocks, one for each
+// wave of the other workgroups; a unit's pieces are where its blocks lie in them.
 struct Mixed {
-  Split shared, own;
-  unsigned workers;
+  Split shared;
+  unsigned workers, run;
 };
 __device__ __forceinline__ float wave_sum(float x) {
   x = group_sum<16>(x);
@@ -292,44 +266,45 @@ __device__ __forceinline__ float wave_sum(float x) {
   p = pair32(x);
   return p.a + p.b;
 }
+__device__ __forceinline__ unsigned own_units(const SharedSeq &q, unsigned group) {
+  return q.step ? (q.rows * group + kColumns - 1) / kColumns : 0u;
+}
 __device__ __forceinline__ Mixed mixed_split(const SharedView &g, const SharedLanes &lanes,
                                              unsigned group, const MixedPlan &plan) {
-  Mixed x{Split{group, plan.shift, plan.step, plan.step, 0.0f, true},
-          Split{group, 4, kWaves, kWaves, 0.0f, false}, 0};
-  float shared = 0.0f, own = 0.0f, units = 0.0f;
+  Mixed x{Split{group, plan.shift, plan.step, plan.step, 0.0f, true}, 0, 1};
+  float shared = 0.0f, units = 0.0f;
+  unsigned own = 0; // (the host sees to it that they are no more than 2^31)
   shared_chunks(g, lanes, [&](unsigned, const SharedSeq &q) {
-    if (q.step == 0)
-      shared += lane_blocks(x.shared, q);
-    else {
-      own += lane_blocks(x.own, q);
-      units += (float)x.own.units(q);
-    }
+    shared += q.step == 0 ? lane_blocks(x.shared, q) : 0.0f;
+    const unsigned n = own_units(q, group);
+    own += n * Split::blocks(q);
+    units += (float)n;
     return false;
   });
   shared = wave_sum(shared);
-  own = wave_sum(own);
   units = wave_sum(units);
+  own = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(own), 63);
   auto whole = [](float v) { // (below 2^30: no table has more blocks)
-    return (unsigned)__builtin_amdgcn_readfirstlane((int)fminf(ceilf(v), 0x1p30f));
+    return uniform((unsigned)fminf(ceilf(v), 0x1p30f));
   };
-  const float a = shared * plan.sharedCost, b = own * plan.ownCost + units * plan.ownFixed;
+  const float a = shared * plan.sharedCost, b = (float)own * plan.ownCost + units * plan.ownFixed;
   const float cus = (float)plan.cus;
   unsigned workers = shared == 0.0f ? 0u : max(1u, whole(cus * a / (a + b) - 0.5f));
-  workers = b == 0.0f ? plan.cus : min(workers, plan.cus - 1);
+  workers = own == 0 ? plan.cus : min(workers, plan.cus - 1);
   auto take = [](Split &s, unsigned chunk) {
     const unsigned steps = (chunk + s.step - 1) & ~(s.step - 1);
-    s.chunk = (unsigned)__builtin_amdgcn_readfirstlane((int)(steps ? steps : s.step));
+    s.chunk = uniform(steps ? steps : s.step);
     s.inv = __builtin_amdgcn_rcpf((float)s.chunk);
   };
   take(x.shared, whole(shared * 1.0001f / (float)max(workers, 1u)));
   // Every unit's last piece is rounded up: longer ones until each has a
   // workgroup, undivided units at last (the host sees to it that they fit).
-  auto pieces = [&](bool undivided) {
+  auto pieces = [&](bool undivided) { // (the groups come first)
     unsigned n = 0;
-    shared_chunks(g, lanes, [&](unsigned, const SharedSeq &q) {
+    shared_chunks(g, lanes, [&](unsigned c, const SharedSeq &q) {
       if (q.step == 0)
         n += x.shared.units(q) * (undivided ? 1u : x.shared.pieces(q));
-      return false;
+      return 64 * (c + 1) >= g.count;
     });
     return (unsigned)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
   };
@@ -343,15 +318,39 @@ __device__ __forceinline__ Mixed mixed_split(const SharedView &g, const SharedLa
     take(x.shared, 1u << 30);
     n = pieces(true);
   }
-  x.workers = workers = min(n, plan.cus);
-  // own keys: as many pieces as the other workgroups, but of 16 blocks at least,
-  // and in up to four rounds where they would be longer than 64
-  const float rest = (float)max(plan.cus - workers, 1u), even = own * 1.0001f / rest;
-  take(x.own, max(16u, whole(fminf(even, fmaxf(64.0f, even * 0.25f)))));
+  x.workers = min(n, plan.cus);
+  const unsigned waves = max(kWaves * (plan.cus - x.workers), 1u);
+  x.run = max(uniform((own + waves - 1) / waves), kLeastRun);
   return x;
 }
 
-template <int D, int CT>
+// The sequence that has block `at` of all own units: its first block and its
+// first unit among them; false behind the last.
+__device__ __forceinline__ bool find_own(const SharedView &g, const SharedLanes &lanes,
+                                         unsigned group, unsigned at, unsigned &seq,
+                                         unsigned &firstBlock, unsigned &firstUnit) {
+  bool found = false;
+  firstBlock = firstUnit = 0;
+  shared_chunks(g, lanes, [&](unsigned c, const SharedSeq &q) {
+    const unsigned units = own_units(q, group), n = units * Split::blocks(q);
+    const unsigned blocks = wave_scan(n), sum = wave_scan(units);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(at - firstBlock < blocks);
+    if (!past) {
+      firstBlock += (unsigned)__builtin_amdgcn_readlane((int)blocks, 63);
+      firstUnit += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+      return false;
+    }
+    const int lane = __builtin_ctzll(past);
+    seq = 64 * c + (unsigned)lane;
+    firstBlock += (unsigned)__builtin_amdgcn_readlane((int)(blocks - n), lane);
+    firstUnit += (unsigned)__builtin_amdgcn_readlane((int)(sum - units), lane);
+    found = at - firstBlock < (unsigned)__builtin_amdgcn_readlane((int)n, lane);
+    return true;
+  });
+  return found;
+}
+
+template <int D>
 __global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads),
                           amdgpu_waves_per_eu(2, 2)))
 void paged_mixed_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool,
@@ -360,45 +359,53 @@ void paged_mixed_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
                         unsigned mostShared, unsigned mostOwn) {
   const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.x % g.kvHeads;
   const unsigned me = blockIdx.x / g.kvHeads;
-  SharedLanes lanes = paged_own(g);
-  Mixed x = mixed_split(g, lanes, G, plan);
-  // piece u of shared or of own keys: whether there is one, and where
-  SharedSeq s;
-  unsigned seq, unit, piece, pieces;
-  auto find = [&](const Split &split, unsigned step, unsigned u, unsigned most) {
-    unsigned local, before;
-    if (u >= most || // (starts out of order make more pieces than the rows can have)
-        !paged_find(g, lanes, u,
+  const SharedLanes lanes = paged_own(g);
+  const Mixed x = mixed_split(g, lanes, G, plan);
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    g.notes[g.count + g.all].first = x.run;
+  if (me < x.workers) {
+    unsigned seq, local, before;
+    if (me >= mostShared || // (starts out of order make more pieces than the rows can have)
+        !paged_find(g, lanes, me,
                     [&](const SharedSeq &q) {
-                      return q.step == step ? split.units(q) * split.pieces(q) : 0u;
+                      return q.step == 0 ? x.shared.units(q) * x.shared.pieces(q) : 0u;
                     },
                     seq, local, before))
-      return false;
-    seq = uniform(seq);
-    local = uniform(local);
-    s = paged_from_lane(paged_seq_of(g, lanes, seq), 0);
-    pieces = uniform(split.pieces(s));
-    const unsigned units = split.units(s);
-    unit = units - 1 - local / pieces;
-    piece = local % pieces;
+      return;
+    const SharedSeq s = paged_seq_of(g, lanes, seq);
+    const unsigned pieces = x.shared.pieces(s), units = x.shared.units(s);
+    const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
     if (local == 0 && kvh == 0 && threadIdx.x == 0)
       leave_note(g, s, seq, before, pieces, units);
-    return true;
-  };
-  if (me < x.workers) {
-    if (find(x.shared, 0, me, mostShared))
-      tiles_piece<D, CT>(q, pool, g, out, invalid, queryHeads, x.shared, c, shared, s, seq, kvh,
-                         unit, piece, pieces, me);
+    tiles_piece<D, 1>(q, pool, g, out, invalid, queryHeads, x.shared, c, shared, s, seq, kvh, unit,
+                      piece, pieces, me);
     return;
   }
-  for (unsigned u = me - x.workers; find(x.own, 1, u, mostOwn); u += plan.cus - x.workers) {
-    own_piece<D>(q, pool, g, out, invalid, queryHeads, x.own, c, rest, s, kvh, unit, piece, pieces,
-                 u);
-    __syncthreads(); // done with its LDS
-    // (made again for the next: kept, the lengths would need registers that the
-    // pieces have none of)
-    lanes = paged_own(g);
-    x = mixed_split(g, lanes, G, plan);
+  // this wave's run of own blocks
+  const unsigned worker = uniform((me - x.workers) * kWaves + threadIdx.x / 64);
+  unsigned at = worker * x.run, seq, firstBlock, firstUnit;
+  const unsigned stop = at + x.run;
+  if (!find_own(g, lanes, G, at, seq, firstBlock, firstUnit))
+    return;
+  SharedSeq s = paged_from_lane(paged_seq_of(g, lanes, seq), 0);
+  while (true) {
+    const unsigned units = uniform(own_units(s, G)), blocks = uniform(Split::blocks(s));
+    for (; at < stop && at - firstBlock < units * blocks;) {
+      const unsigned unit = (at - firstBlock) / blocks, b0 = (at - firstBlock) % blocks;
+      const unsigned length = min(blocks - b0, stop - at), number = worker + firstUnit + unit;
+      if (at == firstBlock && kvh == 0 && threadIdx.x % 64 == 0)
+        g.notes[seq] = SharedNote{firstBlock, s.ok ? blocks : 0u, firstUnit, s.begin ? s.group + 1 : 0u};
+      if (number >= mostOwn)
+        return;
+      own_piece<D>(q, pool, g, out, invalid, queryHeads, c, rest, s, kvh, unit, s.begin + b0,
+                   s.begin + b0 + length, length == blocks && !s.joined(), number);
+      at += length;
+    }
+    if (at >= stop || ++seq >= g.sequences)
+      return;
+    firstBlock += units * blocks;
+    firstUnit += units;
+    s = paged_from_lane(shared_seq(g, lanes.groups, seq), 0);
   }
 }
 
@@ -413,11 +420,9 @@ hipError_t launch_paged_mixed(const half_t *q, const uint8_t *pool, const Shared
                        out, invalid, queryHeads, plan, c, shared, rest, mostShared, mostOwn);
     return hipGetLastError();
   };
-  if (g.dim == 256)
-    return run(paged_mixed_kernel<256, 1>);
-  if (g.dim == 128)
-    return plan.shift == 8 ? run(paged_mixed_kernel<128, 2>) : run(paged_mixed_kernel<128, 1>);
-  return plan.shift == 8 ? run(paged_mixed_kernel<64, 2>) : run(paged_mixed_kernel<64, 1>);
+  return g.dim == 256   ? run(paged_mixed_kernel<256>)
+         : g.dim == 128 ? run(paged_mixed_kernel<128>)
+                        : run(paged_mixed_kernel<64>);
 }
 
 } // namespace llmi

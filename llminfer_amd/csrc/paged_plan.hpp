@@ -157,8 +157,9 @@ hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const View &
 
 // The kernel for groups with many rows in all and sequences with few
 // (paged_mixed.hip): units of 2^shift columns of the shared keys, whole steps of
-// blocks, on `cus` workgroups a KV head, and what a block of shared and of own
-// keys and a piece of own keys take.
+// blocks, on `cus` workgroups a KV head, and the time that a block of a unit of
+// shared keys, a block of a unit of own keys and a unit of own keys take of one.
+constexpr unsigned kMixedWaves = 8; // of a workgroup
 struct MixedPlan {
   unsigned shift, step, cus;
   float sharedCost, ownCost, ownFixed;

@@ -26,7 +26,9 @@ struct SharedSeq {
 
 // What the workgroups of a sequence leave for the join: its first piece, how
 // many a unit has, its units, and the group whose partials are joined to them
-// (+ 1; 0: none), for a group its first row.
+// (+ 1; 0: none), for a group its first row. Own keys in runs of blocks
+// (paged_mixed.hip): the first of its blocks among all, the blocks of a unit, its
+// first unit among all, and the group.
 struct SharedNote {
   unsigned first, pieces, units, other;
 };
@@ -37,7 +39,7 @@ struct SharedNote {
 struct SharedView : PagedView {
   typedef SharedSeq Seq;
   const int32_t *groups, *prefix;
-  SharedNote *notes; // [count + all]
+  SharedNote *notes; // [count + all], and one with the blocks of a run
   unsigned count, all, base;
 };
 
@@ -53,14 +55,15 @@ __device__ __forceinline__ SharedGroups shared_groups(const SharedView &g) {
 // Sequence s of the view (nothing past the last one), a different one in every
 // lane; all lanes call it. Groups and sequences take the same steps, so that the
 // loads of both are in flight together.
-__device__ __forceinline__ SharedSeq shared_seq(const SharedView &g, const SharedGroups &lanes,
-                                                unsigned s) {
-  const bool none = s >= g.sequences, few = g.count <= 64;
+template <bool Few> // at most 64 groups, all of them in `lanes`
+__device__ __forceinline__ SharedSeq shared_seq_of(const SharedView &g, const SharedGroups &lanes,
+                                                   unsigned s) {
+  const bool none = s >= g.sequences;
   const unsigned v = (none ? g.sequences - 1 : s) + g.base;
   const bool ofGroup = v < g.count;
   const unsigned seq = ofGroup ? 0u : v - g.count;
   auto group_of = [&](int mine, const int32_t *array, unsigned i) {
-    return few ? __shfl(mine, (int)i) : array[i];
+    return Few ? __shfl(mine, (int)i) : array[i];
   };
   // the last group that begins at or before the sequence, by bisection
   unsigned group = 0;
@@ -103,6 +106,11 @@ __device__ __forceinline__ SharedSeq shared_seq(const SharedView &g, const Share
   return q;
 }
 
+__device__ __forceinline__ SharedSeq shared_seq(const SharedView &g, const SharedGroups &lanes,
+                                                unsigned s) {
+  return g.count <= 64 ? shared_seq_of<true>(g, lanes, s) : shared_seq_of<false>(g, lanes, s);
+}
+
 // The first 256 sequences, one a lane and member (no array, which would be in
 // memory): most calls read the lengths once, all of them in flight.
 struct SharedLanes {
@@ -113,12 +121,19 @@ __device__ __forceinline__ SharedLanes paged_own(const SharedView &g) {
   const unsigned lane = threadIdx.x % 64;
   SharedLanes own;
   own.groups = shared_groups(g);
-  own.a = shared_seq(g, own.groups, lane);
-  own.b = own.c = own.d = SharedSeq{0, 0, 0, true};
-  if (g.sequences > 64) {
-    own.b = shared_seq(g, own.groups, 64 + lane);
-    own.c = shared_seq(g, own.groups, 128 + lane);
-    own.d = shared_seq(g, own.groups, 192 + lane);
+  if (g.sequences <= 64) {
+    own.a = shared_seq(g, own.groups, lane);
+    own.b = own.c = own.d = SharedSeq{0, 0, 0, true};
+  } else if (g.count <= 64) {
+    own.a = shared_seq_of<true>(g, own.groups, lane);
+    own.b = shared_seq_of<true>(g, own.groups, 64 + lane);
+    own.c = shared_seq_of<true>(g, own.groups, 128 + lane);
+    own.d = shared_seq_of<true>(g, own.groups, 192 + lane);
+  } else {
+    own.a = shared_seq_of<false>(g, own.groups, lane);
+    own.b = shared_seq_of<false>(g, own.groups, 64 + lane);
+    own.c = shared_seq_of<false>(g, own.groups, 128 + lane);
+    own.d = shared_seq_of<false>(g, own.groups, 192 + lane);
   }
   return own;
 }

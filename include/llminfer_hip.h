@@ -188,6 +188,13 @@ typedef struct PagedForkParams {
   unsigned sequences, tableStride, children;
 } PagedForkParams;
 
+/* Rows moved in a pool: within the sequences' own pages, or (apart) from other
+ * pages into them. */
+typedef struct PagedMoveParams {
+  PagedKvParams kv;
+  unsigned apart;
+} PagedMoveParams;
+
 /* The tables of `sequences` sequences over a pool's pages. */
 typedef struct PagedFreeParams {
   unsigned pages, pageSize, sequences, tableStride;
@@ -246,7 +253,7 @@ enum llmi_hip_op {
   LLMI_HIP_OP_PAGED_GQA_SHARED = 29,    /* params: PagedSharedParams */
   LLMI_HIP_OP_PAGED_FORK = 30,          /* params: PagedForkParams */
   LLMI_HIP_OP_PAGED_FREE = 31,          /* params: PagedFreeParams */
-  LLMI_HIP_OP_PAGED_MOVE = 32           /* params: PagedKvParams */
+  LLMI_HIP_OP_PAGED_MOVE = 32           /* params: PagedMoveParams */
 };
 
 /* ---------------------------------------------------------------- KvAppend
@@ -611,23 +618,25 @@ LLMI_HIP_API int llmi_hip_paged_free(const int32_t *table, const int32_t *length
                                      void *workspace, size_t workspace_bytes, void *stream);
 LLMI_HIP_API size_t llmi_hip_paged_free_workspace_bytes(PagedFreeParams p);
 
-/* Keys and values moved as they are, in 4 bits: row starts[s] + i of the call
- * is the key and value at position source[starts[s] + i] (in any order, any
- * number of times) of row s of sourceTable, and goes to position past[s] + i of
- * row s of table. All are read before any is written, so the tables may be the
- * same and rows may move within a sequence (a context without the keys it can
- * do without; drafts of which some are kept). Keys stay rotated as they were.
- * sourceTable has the shape of table (tokens of source: device memory). A row
- * whose source has no place is not moved, what is at its target stays; the
+/* Keys and values moved as they are, in 4 bits: row starts[s] + i of the call is
+ * the key and value at position source[starts[s] + i] (device memory; in any
+ * order, any number of times) of sequence s, and goes to position past[s] + i of
+ * row s of table. p.apart 0: the source is row s of table too, and all rows are
+ * read before any is written, so that rows move within a sequence (a context
+ * without the keys that it can do without; drafts of which some are kept). p.apart
+ * 1: the source is row s of sourceTable, of the table's shape; the pages that rows
+ * are read from are none that rows go to. Keys stay rotated as they were. A
+ * row whose source has no place is not moved, what is at its target stays; the
  * other errors, and the sequences, are as in paged_append. Two rows of a call
- * must not go to one place. `workspace` holds
- * llmi_hip_paged_move_workspace_bytes(p) bytes, 16-byte aligned. */
+ * must not go to one place, and no sequence's rows to a page that another's are
+ * read from. `workspace` holds llmi_hip_paged_move_workspace_bytes(p) bytes (0:
+ * none is needed), 16-byte aligned. */
 LLMI_HIP_API int llmi_hip_paged_move(const int32_t *source, const int32_t *sourceTable,
                                      const int32_t *starts, const int32_t *past,
                                      const int32_t *table, void *pool, uint32_t *invalid,
-                                     PagedKvParams p, void *workspace, size_t workspace_bytes,
+                                     PagedMoveParams p, void *workspace, size_t workspace_bytes,
                                      void *stream);
-LLMI_HIP_API size_t llmi_hip_paged_move_workspace_bytes(PagedKvParams p);
+LLMI_HIP_API size_t llmi_hip_paged_move_workspace_bytes(PagedMoveParams p);
 
 /* ------------------------------------------------------------- DeltaUpdate
  * Replaces graphDeltaUpdate (Graph.metal:146-170 with updateDeltaColumn,

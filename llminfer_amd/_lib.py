@@ -183,6 +183,10 @@ class PagedForkParams(C.Structure):
                                         "tableStride", "children")]
 
 
+class PagedMoveParams(C.Structure):
+    _fields_ = [("kv", PagedKvParams), ("apart", C.c_uint)]
+
+
 class PagedFreeParams(C.Structure):
     _fields_ = [(n, C.c_uint) for n in ("pages", "pageSize", "sequences", "tableStride")]
 
@@ -277,8 +281,8 @@ SIGNATURES = {
     "llmi_hip_paged_fork": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, PagedForkParams, _P]),
     "llmi_hip_paged_free": (C.c_int, [_P, _P, _P, _P, _P, PagedFreeParams, _P, _SZ, _P]),
     "llmi_hip_paged_free_workspace_bytes": (_SZ, [PagedFreeParams]),
-    "llmi_hip_paged_move": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedKvParams, _P, _SZ, _P]),
-    "llmi_hip_paged_move_workspace_bytes": (_SZ, [PagedKvParams]),
+    "llmi_hip_paged_move": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, PagedMoveParams, _P, _SZ, _P]),
+    "llmi_hip_paged_move_workspace_bytes": (_SZ, [PagedMoveParams]),
     "llmi_hip_workspace_init": (C.c_int, [_P, _SZ, _P]),
     "llmi_hip_dispatch_count": (C.c_uint, [C.c_int, _P]),
     "llmi_hip_kernel_name": (C.c_char_p, [C.c_int, _P, C.c_uint]),

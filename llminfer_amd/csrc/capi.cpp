@@ -1282,25 +1282,27 @@ size_t llmi_hip_paged_free_workspace_bytes(PagedFreeParams p) {
 
 int llmi_hip_paged_move(const int32_t *source, const int32_t *sourceTable, const int32_t *starts,
                         const int32_t *past, const int32_t *table, void *pool, uint32_t *invalid,
-                        PagedKvParams p, void *workspace, size_t workspace_bytes, void *stream) {
-  if (p.tokens == 0 || p.sequences == 0)
+                        PagedMoveParams p, void *workspace, size_t workspace_bytes, void *stream) {
+  if (p.kv.tokens == 0 || p.kv.sequences == 0)
     return LLMI_HIP_OK;
-  if (int rc = check_paged("pagedMove", p, starts, past, table, pool))
+  if (int rc = check_paged("pagedMove", p.kv, starts, past, table, pool))
     return rc;
-  if (!source || !sourceTable)
+  if (!source || (p.apart && !sourceTable))
     return fail(LLMI_HIP_INVALID_ARGUMENT, "pagedMove: null buffer");
   if (int rc = check_workspace("pagedMove", workspace, workspace_bytes,
-                               paged_move_workspace_bytes(p)))
+                               llmi_hip_paged_move_workspace_bytes(p)))
     return rc;
-  return launched(launch_paged_move(source, sourceTable, starts, past, table, pool, invalid,
-                                    workspace, p, static_cast<hipStream_t>(stream)),
+  return launched(launch_paged_move(source, p.apart ? sourceTable : nullptr, starts, past, table,
+                                    pool, invalid, workspace, p.kv,
+                                    static_cast<hipStream_t>(stream)),
                   "pagedMove");
 }
 
-size_t llmi_hip_paged_move_workspace_bytes(PagedKvParams p) {
-  if (p.tokens == 0 || p.sequences == 0 || (p.headDim != 64 && p.headDim != 128 && p.headDim != 256))
+size_t llmi_hip_paged_move_workspace_bytes(PagedMoveParams p) {
+  const unsigned dim = p.kv.headDim;
+  if (p.apart || p.kv.tokens == 0 || p.kv.sequences == 0 || (dim != 64 && dim != 128 && dim != 256))
     return 0;
-  return paged_move_workspace_bytes(p);
+  return paged_move_workspace_bytes(p.kv);
 }
 
 // Whether a supported CausalGqa is a prefill that divides its keys.
@@ -1438,8 +1440,8 @@ unsigned llmi_hip_dispatch_count(int op, const void *params) {
     return check_free(p) ? 0 : paged_free_launches(p);
   }
   case LLMI_HIP_OP_PAGED_MOVE: {
-    const PagedKvParams &p = *static_cast<const PagedKvParams *>(params);
-    return p.tokens && p.sequences ? 2 : 0;
+    const PagedMoveParams &p = *static_cast<const PagedMoveParams *>(params);
+    return !p.kv.tokens || !p.kv.sequences ? 0 : p.apart ? 1 : 2;
   }
   case LLMI_HIP_OP_GATED_ATTENTION: {
     // Launches for a rotary width the kernels take (a multiple of 16).
@@ -1576,7 +1578,9 @@ const char *llmi_hip_kernel_name(int op, const void *params, unsigned index) {
            : index == 1                             ? "pagedFreeJoin"
                                                     : "pagedFreeList";
   case LLMI_HIP_OP_PAGED_MOVE:
-    return index ? "pagedPlace" : "pagedGather";
+    return index                                                 ? "pagedPlace"
+           : static_cast<const PagedMoveParams *>(params)->apart ? "pagedMove"
+                                                                 : "pagedGather";
   case LLMI_HIP_OP_GATED_ATTENTION:
     if (static_cast<const GqaParams *>(params)->tokens == 1)
       return index == 0 ? "gqaDecodeGated" : "gqaDecodeMergeGated";

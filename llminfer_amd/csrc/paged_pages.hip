@@ -282,10 +282,10 @@ bool free_small(const PagedFreeParams &p) { return p.pages <= kSmall && free_mar
 
 // -------------------------------------------------------------------- move
 //
-// Two launches, so that all rows are read before any is written, whichever
-// pages they come from and go to: the first makes the blocks as they will be
-// (kept keys of a block in a word), the second puts them into their places.
-// Codes and scales are laid out for the matrix instructions (paged_kv.hpp), so
+// Within the same pages two launches, so that all rows are read before any is
+// written: the first makes the blocks as they will be (which keys, in a word), the
+// second puts them into their places. Between pages that are apart one launch
+// does both. Codes and scales are laid out for the matrix instructions (paged_kv.hpp), so
 // what moves is 16 bytes (8 at D 64) for 32 (16) channels of a key, but a
 // nibble of a word for a channel of a value: a thread has four channels of eight
 // keys, eight loads for a store.
@@ -333,9 +333,20 @@ template <int D> __device__ __forceinline__ uint32_t bits_of(unsigned c, unsigne
   return bits;
 }
 
+// Word c of a block, x in the bits of the keys of `live`.
 template <int D>
+__device__ __forceinline__ uint4_t with_keys(uint4_t old, uint4_t x, unsigned c, uint32_t live) {
+#pragma unroll
+  for (unsigned j = 0; j < 4; ++j) {
+    const uint32_t bits = bits_of<D>(c, j, live);
+    x[j] = (old[j] & ~bits) | (x[j] & bits);
+  }
+  return x;
+}
+
+template <int D, bool APART>
 __global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
-    const uint8_t *__restrict__ pool, PagedView g, const int32_t *__restrict__ source,
+    uint8_t *pool, PagedView g, const int32_t *__restrict__ source,
     const int32_t *__restrict__ sourceTable, uint32_t *live, uint4_t *blocks, unsigned *invalid) {
   using W = Words<D>;
   PagedRun b;
@@ -343,6 +354,15 @@ __global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
     return;
   const unsigned tid = threadIdx.x, head = blockIdx.y;
   const size_t unit = (size_t)blockIdx.x * g.kvHeads + head;
+  size_t target = 0;
+  if (APART) {
+    const bool placed = b.ok && paged_block(g, b.seq, b.base, head, target);
+    if (!placed) {
+      if (invalid && tid == 0)
+        atomicOr(invalid, kPagedPlace);
+      return;
+    }
+  }
   __shared__ const uint8_t *sBlock[32]; // of the keys of this block
   __shared__ unsigned sKey[32], sLive;
   if (tid < 64) {
@@ -359,15 +379,18 @@ __global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
     }
     const uint32_t keys = (uint32_t)__builtin_amdgcn_ballot_w64(found);
     if (tid == 0) {
-      sLive = live[unit] = keys;
+      sLive = keys;
+      if (!APART)
+        live[unit] = keys;
       if (invalid && (!b.ok || __builtin_popcount(keys) != (int)(b.last - b.first)))
         atomicOr(invalid, kPagedPlace);
     }
   }
   __syncthreads();
-  if (!sLive)
+  const uint32_t keys = sLive;
+  if (!keys)
     return;
-  uint4_t *to = blocks + unit * W::ALL;
+  uint4_t *to = APART ? reinterpret_cast<uint4_t *>(pool + target) : blocks + unit * W::ALL;
   for (unsigned word = tid; word < W::ALL; word += kMoveThreads) {
     unsigned c = word;
     uint4_t x = 0;
@@ -417,7 +440,7 @@ __global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
         x[e / 2] |= y << 16 * (e % 2);
       }
     }
-    to[word] = x;
+    to[word] = APART && keys != ~0u ? with_keys<D>(to[word], x, word, keys) : x;
   }
 }
 
@@ -454,12 +477,7 @@ __global__ __launch_bounds__(kMoveThreads) void paged_place_kernel(uint8_t *pool
       const unsigned c = tid + i * kMoveThreads;
       if (c >= W::ALL)
         continue;
-      const uint4_t old = to[c];
-#pragma unroll
-      for (unsigned j = 0; j < 4; ++j) {
-        const uint32_t bits = bits_of<D>(c, j, keys);
-        x[i][j] = (old[j] & ~bits) | (x[i][j] & bits);
-      }
+      x[i] = with_keys<D>(to[c], x[i], c, keys);
     }
   }
 #pragma unroll
@@ -534,17 +552,23 @@ hipError_t launch_paged_move(const int32_t *source, const int32_t *sourceTable,
   uint32_t *live = reinterpret_cast<uint32_t *>(blocks + move_units(p) * (40 * p.headDim / 16));
   const dim3 grid(paged_most_runs(p.tokens, p.sequences), p.kvHeads);
   uint8_t *pages = static_cast<uint8_t *>(pool);
-  auto run = [&](auto gather, auto place) {
-    hipLaunchKernelGGL(gather, grid, dim3(kMoveThreads), 0, stream, pages, g, source, sourceTable,
-                       live, blocks, invalid);
+  const bool apart = sourceTable != nullptr;
+  auto run = [&](auto move, auto gather, auto place) {
+    hipLaunchKernelGGL(apart ? move : gather, grid, dim3(kMoveThreads), 0, stream, pages, g, source,
+                       apart ? sourceTable : table, live, blocks, invalid);
     if (hipError_t e = hipGetLastError())
       return e;
+    if (apart)
+      return hipSuccess;
     hipLaunchKernelGGL(place, grid, dim3(kMoveThreads), 0, stream, pages, g, live, blocks, invalid);
     return hipGetLastError();
   };
-  return p.headDim == 256   ? run(paged_gather_kernel<256>, paged_place_kernel<256>)
-         : p.headDim == 128 ? run(paged_gather_kernel<128>, paged_place_kernel<128>)
-                            : run(paged_gather_kernel<64>, paged_place_kernel<64>);
+  return p.headDim == 256   ? run(paged_gather_kernel<256, true>, paged_gather_kernel<256, false>,
+                                  paged_place_kernel<256>)
+         : p.headDim == 128 ? run(paged_gather_kernel<128, true>, paged_gather_kernel<128, false>,
+                                  paged_place_kernel<128>)
+                            : run(paged_gather_kernel<64, true>, paged_gather_kernel<64, false>,
+                                  paged_place_kernel<64>);
 }
 
 } // namespace llmi

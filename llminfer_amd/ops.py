@@ -1355,28 +1355,30 @@ def bind_paged_move(pool: torch.Tensor, starts: torch.Tensor, past: torch.Tensor
                     source_table: torch.Tensor | None = None,
                     invalid: torch.Tensor | None = None) -> "Bound":
     """Keys and values moved as they are (llmi_hip_paged_move): those at
-    positions source [T] (int32, in any order) of their sequences' rows of
-    source_table (default: table) to positions past[s] + i of table, row i of
-    sequence s being source[starts[s] + i]. All are read before any is written,
-    so a sequence may be made shorter in its own pages. Keys stay rotated as
-    they were. A row whose source or target has no place is not moved and sets
-    bit 1 of invalid. The workspace is the bound call's own; keep a bound call
-    as long as a graph that it was captured into."""
+    positions source [T] (int32, in any order) of their sequences to positions
+    past[s] + i of row s of table, row i of sequence s being source[starts[s] +
+    i]. Without a source_table they are the table's own, all read before any is
+    written, so that a sequence may be made shorter in its pages; with one, of
+    the table's shape, they come from its pages, which must be none that rows go
+    to. Keys stay rotated as they were. A row whose source or target has no place
+    is not moved and sets bit 1 of invalid. The workspace is the bound call's
+    own; keep a bound call as long as a graph that it was captured into."""
     _require(source, torch.int32, "source")
     if source.dim() != 1:
         raise ValueError("source is [T]")
-    p = _paged(pool, starts, past, table, source.numel(), invalid)
-    if source_table is None:
-        source_table = table
-    _require(source_table, torch.int32, "source_table")
-    if source_table.shape != table.shape:
-        raise ValueError("source_table has the shape of table")
+    kv = _paged(pool, starts, past, table, source.numel(), invalid)
+    if source_table is not None:
+        _require(source_table, torch.int32, "source_table")
+        if source_table.shape != table.shape:
+            raise ValueError("source_table has the shape of table")
     _one_device(pool, starts, past, table, source, source_table, invalid)
     lib = _lib.load()
+    p = _lib.PagedMoveParams(kv, source_table is not None)
     ws = _private(lib.llmi_hip_paged_move_workspace_bytes(p), pool.device)
     b = Bound(lib.llmi_hip_paged_move,
               (_ptr(source), _ptr(source_table), _ptr(starts), _ptr(past), _ptr(table), _ptr(pool),
-               _ptr(invalid), p, _ptr(ws), _size(ws), _stream()), "pagedGather+pagedPlace")
+               _ptr(invalid), p, _ptr(ws), _size(ws), _stream()),
+              "+".join(kernel_names(_lib.OP_PAGED_MOVE, p)))
     b._keep = (pool, starts, past, table, source, source_table, invalid, ws)
     return b
 

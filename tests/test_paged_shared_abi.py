@@ -29,6 +29,7 @@ def free_params(**over):
 def test_param_structs():
     assert C.sizeof(_lib.PagedSharedParams) == 40
     assert C.sizeof(_lib.PagedForkParams) == 28
+    assert C.sizeof(_lib.PagedMoveParams) == 32
     assert C.sizeof(_lib.PagedFreeParams) == 16
 
 
@@ -37,7 +38,9 @@ def test_kv_refusals(over, status):
     lib = _lib.load()
     assert lib.llmi_hip_paged_gqa_shared(*[A16] * 7, FAR, A16, shared_params(**over), A16, MANY,
                                          None) == status
-    assert lib.llmi_hip_paged_move(*[A16] * 7, kv_params(**over), A16, MANY, None) == status
+    for apart in (0, 1):
+        assert lib.llmi_hip_paged_move(*[A16] * 7, _lib.PagedMoveParams(kv_params(**over), apart),
+                                       A16, MANY, None) == status
     if status != _lib.OK:
         fork = {k: v for k, v in over.items() if k != "tokens"}
         want = status if fork else _lib.INVALID_ARGUMENT
@@ -137,15 +140,19 @@ def test_free_refusals():
 
 def test_move_refusals():
     lib = _lib.load()
-    need = lib.llmi_hip_paged_move_workspace_bytes(kv_params())
-    assert need > 0
-    for k in range(6):  # invalid may be null, the rest not
-        bad = [A16] * 7
-        bad[k] = None
-        assert lib.llmi_hip_paged_move(*bad, kv_params(), A16, need, None) == _lib.INVALID_ARGUMENT
+    within, apart = (_lib.PagedMoveParams(kv_params(), x) for x in (0, 1))
+    need = lib.llmi_hip_paged_move_workspace_bytes(within)
+    assert need > 0 and lib.llmi_hip_paged_move_workspace_bytes(apart) == 0
+    for p in (within, apart):
+        for k in range(6):  # invalid may be null, the source's table within the pages
+            bad = [A16] * 7
+            bad[k] = None
+            if k != 1 or p is apart:
+                assert lib.llmi_hip_paged_move(*bad, p, A16, need, None) == _lib.INVALID_ARGUMENT
     for ws, size in ((None, need), (A16, need - 1), (A16 + 8, need)):
-        assert lib.llmi_hip_paged_move(*[A16] * 7, kv_params(), ws, size, None) == _lib.WORKSPACE
-    assert lib.llmi_hip_paged_move_workspace_bytes(kv_params(headDim=96)) == 0
+        assert lib.llmi_hip_paged_move(*[A16] * 7, within, ws, size, None) == _lib.WORKSPACE
+    wrong = _lib.PagedMoveParams(kv_params(headDim=96), 0)
+    assert lib.llmi_hip_paged_move_workspace_bytes(wrong) == 0
 
 
 def test_launches():
@@ -155,7 +162,9 @@ def test_launches():
     assert ops.kernel_names(_lib.OP_PAGED_FREE, free_params()) == ["pagedFree"]
     assert ops.kernel_names(_lib.OP_PAGED_FREE, free_params(pages=10**5)) == [
         "pagedFreeMark", "pagedFreeJoin", "pagedFreeList"]
-    assert ops.kernel_names(_lib.OP_PAGED_MOVE, kv_params()) == ["pagedGather", "pagedPlace"]
+    move = [_lib.PagedMoveParams(kv_params(), x) for x in (0, 1)]
+    assert ops.kernel_names(_lib.OP_PAGED_MOVE, move[0]) == ["pagedGather", "pagedPlace"]
+    assert ops.kernel_names(_lib.OP_PAGED_MOVE, move[1]) == ["pagedMove"]
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED, shared_params(heads=4))
     assert names[-1] == "pagedSharedMerge" and names[0] == "pagedGqaSplit"
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED,

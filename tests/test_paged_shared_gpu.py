@@ -185,20 +185,21 @@ def test_free_without_place(gpu, pages):
 
 # ---------------------------------------------------------------------- move
 
-MOVE = [  # (rows, past, span) of each sequence, hkv, dim, page, apart
-    ([(1, 0, 1)], 1, 64, 32, False),
-    ([(1, 40, 200)], 4, 256, 64, False),
-    ([(5, 100, 24)] * 6, 4, 256, 64, True),
-    ([(32, 32, 64)], 2, 128, 32, False),      # a whole block
-    ([(33, 31, 90), (0, 9, 9), (70, 1, 70)], 3, 128, 32, True),
-    ([(100, 0, 400)], 2, 256, 96, False),
-    ([(90, 5, 300), (64, 0, 64)], 2, 64, 32, False),
-    ([(3, i, 40) for i in range(70)], 1, 64, 32, False),
-    ([(300, 17, 1000)], 8, 128, 256, True),
+MOVE = [  # (rows, past, span) of each sequence, hkv, dim, page
+    ([(1, 0, 1)], 1, 64, 32),
+    ([(1, 40, 200)], 4, 256, 64),
+    ([(5, 100, 24)] * 6, 4, 256, 64),
+    ([(32, 32, 64)], 2, 128, 32),      # a whole block
+    ([(33, 31, 90), (0, 9, 9), (70, 1, 70)], 3, 128, 32),
+    ([(100, 0, 400)], 2, 256, 96),
+    ([(90, 5, 300), (64, 0, 64)], 2, 64, 32),
+    ([(3, i, 40) for i in range(70)], 1, 64, 32),
+    ([(300, 17, 1000)], 8, 128, 256),
 ]
 
 
-@pytest.mark.parametrize("seqs, hkv, dim, page, apart", MOVE)
+@pytest.mark.parametrize("seqs, hkv, dim, page", MOVE)
+@pytest.mark.parametrize("apart", [False, True])
 @pytest.mark.parametrize("order", ["ascending", "any", "repeated"])
 def test_move(gpu, seqs, hkv, dim, page, apart, order):
     """Bit for bit, everything else as it was; within a sequence's own pages and
@@ -331,6 +332,14 @@ class Group:
 
 
 SHARED = [  # groups, heads a KV head, hkv, dim, page
+    # 160 columns in 640, beside the sequences' own keys: tiles and runs of blocks
+    ([(256, [(1, 256 + 9 * i) for i in range(40)])], 4, 4, 256, 32),
+    ([(224, [(1, 230 + 31 * i % 97) for i in range(20)]), (96, [(1, 96 + i) for i in range(22)])],
+     8, 2, 128, 32),
+    ([(320, [(1, 320 + 7 * i) for i in range(50)]), (64, [(2, 70), (0, 80), (1, 64)] * 20)],
+     4, 2, 64, 64),
+    ([(64, [(1, 64 + i) for i in range(80)]), (0, [(1, 9)] * 9)], 8, 1, 64, 32),
+    ([(32, [(1, 3000)] + [(1, 40 + i) for i in range(47)])], 5, 4, 64, 32),
     ([(32, [(1, 32)])], 1, 1, 64, 32),
     ([(64, [(1, 64), (1, 100), (1, 65)])], 4, 2, 256, 64),
     ([(96, [(1, 100), (1, 97)]), (0, [(1, 10), (2, 0)]), (31, [(1, 40)])], 2, 2, 128, 32),

@@ -344,8 +344,10 @@ __device__ __forceinline__ uint4_t with_keys(uint4_t old, uint4_t x, unsigned c,
   return x;
 }
 
+// D threads: one has a word of key codes, one of value codes and perhaps one of
+// scales, whose loads are all in flight together.
 template <int D, bool APART>
-__global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
+__global__ __launch_bounds__(D) void paged_gather_kernel(
     uint8_t *pool, PagedView g, const int32_t *__restrict__ source,
     const int32_t *__restrict__ sourceTable, uint32_t *live, uint4_t *blocks, unsigned *invalid) {
   using W = Words<D>;
@@ -391,57 +393,61 @@ __global__ __launch_bounds__(kMoveThreads) void paged_gather_kernel(
   if (!keys)
     return;
   uint4_t *to = APART ? reinterpret_cast<uint4_t *>(pool + target) : blocks + unit * W::ALL;
-  for (unsigned word = tid; word < W::ALL; word += kMoveThreads) {
-    unsigned c = word;
-    uint4_t x = 0;
-    if (c < W::KEYS) {
-      const unsigned t = c / (D / 2), chunk = c % (D / 2) / (D >= 128 ? 16 : 8);
-      if constexpr (D >= 128) {
-        const unsigned key = key_of_row(t, c % 16), from = sKey[key];
-        x = *reinterpret_cast<const uint4_t *>(sBlock[key] + from / 8 % 2 * 8 * D +
-                                               (chunk * 16 + paged_row(from)) * 16);
-      } else {
-        for (unsigned n = 0; n < 2; ++n) {
-          const unsigned key = key_of_row(t, c % 8 * 2 + n), from = sKey[key];
-          const uint2 y = *reinterpret_cast<const uint2 *>(sBlock[key] + from / 8 % 2 * 8 * D +
-                                                           (chunk * 16 + paged_row(from)) * 8);
-          x[2 * n] = y.x;
-          x[2 * n + 1] = y.y;
-        }
-      }
-    } else if ((c -= W::KEYS) < W::SCALES) {
-      const unsigned t = c / (D / 8), group = c % (D / 8) / 4;
-      for (unsigned j = 0; j < 4; ++j) {
-        const unsigned key = key_of_row(t, c % 4 * 4 + j);
-        x[j] = *reinterpret_cast<const uint32_t *>(sBlock[key] + paged_key_scale(D, sKey[key], group));
-      }
-    } else if ((c -= W::SCALES) < W::KEYS) {
-      const unsigned st = c / 64, quad = c / 16 % 4, r = c % 16;
-      uint4_t y[8];
-      unsigned from[8];
-#pragma unroll
-      for (unsigned e = 0; e < 8; ++e) {
-        const unsigned key = key_of_slot(quad, e);
-        from[e] = sKey[key];
-        y[e] = *reinterpret_cast<const uint4_t *>(sBlock[key] +
-                                                  paged_value_word(D, quad_of(from[e]), 64 * st + r));
-      }
-#pragma unroll
-      for (unsigned e = 0; e < 8; ++e)
-        x |= (y[e] >> paged_nibble(slot_of(from[e])) & 15u) << paged_nibble(e);
+  uint4_t x[3] = {0, 0, 0}, y[8];
+  unsigned from[8];
+  { // key codes
+    const unsigned t = tid / (D / 2), chunk = tid % (D / 2) / (D >= 128 ? 16 : 8);
+    if constexpr (D >= 128) {
+      const unsigned key = key_of_row(t, tid % 16), of = sKey[key];
+      x[0] = *reinterpret_cast<const uint4_t *>(sBlock[key] + of / 8 % 2 * 8 * D +
+                                                (chunk * 16 + paged_row(of)) * 16);
     } else {
-      c -= W::KEYS;
-      const unsigned group = c / 8, bias = c / 4 % 2, quad = c % 4;
 #pragma unroll
-      for (unsigned e = 0; e < 8; ++e) {
-        const unsigned key = key_of_slot(quad, e), from = sKey[key];
-        const uint32_t y = *reinterpret_cast<const uint16_t *>(
-            sBlock[key] + paged_value_scale(D, quad_of(from), slot_of(from), group) + 64 * bias);
-        x[e / 2] |= y << 16 * (e % 2);
+      for (unsigned n = 0; n < 2; ++n) {
+        const unsigned key = key_of_row(t, tid % 8 * 2 + n), of = sKey[key];
+        const uint2 z = *reinterpret_cast<const uint2 *>(sBlock[key] + of / 8 % 2 * 8 * D +
+                                                         (chunk * 16 + paged_row(of)) * 8);
+        x[0][2 * n] = z.x;
+        x[0][2 * n + 1] = z.y;
       }
     }
-    to[word] = APART && keys != ~0u ? with_keys<D>(to[word], x, word, keys) : x;
   }
+  if (tid < W::SCALES) { // key scales
+    const unsigned t = tid / (D / 8), group = tid % (D / 8) / 4;
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const unsigned key = key_of_row(t, tid % 4 * 4 + j);
+      x[2][j] = *reinterpret_cast<const uint32_t *>(sBlock[key] + paged_key_scale(D, sKey[key], group));
+    }
+  }
+  // value codes: four channels of eight keys
+#pragma unroll
+  for (unsigned e = 0; e < 8; ++e) {
+    const unsigned key = key_of_slot(tid / 16 % 4, e);
+    from[e] = sKey[key];
+    y[e] = *reinterpret_cast<const uint4_t *>(
+        sBlock[key] + paged_value_word(D, quad_of(from[e]), 64 * (tid / 64) + tid % 16));
+  }
+  if (tid >= W::SCALES && tid < 2 * W::SCALES) { // value scales
+    const unsigned c = tid - W::SCALES, group = c / 8, bias = c / 4 % 2, quad = c % 4;
+#pragma unroll
+    for (unsigned e = 0; e < 8; ++e) {
+      const unsigned key = key_of_slot(quad, e), of = sKey[key];
+      const uint32_t z = *reinterpret_cast<const uint16_t *>(
+          sBlock[key] + paged_value_scale(D, quad_of(of), slot_of(of), group) + 64 * bias);
+      x[2][e / 2] |= z << 16 * (e % 2);
+    }
+  }
+#pragma unroll
+  for (unsigned e = 0; e < 8; ++e)
+    x[1] |= (y[e] >> paged_nibble(slot_of(from[e])) & 15u) << paged_nibble(e);
+  // (a block's words: key codes, key scales, value codes, value scales)
+  const unsigned at[3] = {tid, W::KEYS + W::SCALES + tid,
+                          tid < W::SCALES ? W::KEYS + tid : 2 * W::KEYS + tid};
+#pragma unroll
+  for (unsigned i = 0; i < 3; ++i)
+    if (i < 2 || tid < 2 * W::SCALES)
+      to[at[i]] = APART && keys != ~0u ? with_keys<D>(to[at[i]], x[i], at[i], keys) : x[i];
 }
 
 template <int D>
@@ -554,7 +560,7 @@ hipError_t launch_paged_move(const int32_t *source, const int32_t *sourceTable,
   uint8_t *pages = static_cast<uint8_t *>(pool);
   const bool apart = sourceTable != nullptr;
   auto run = [&](auto move, auto gather, auto place) {
-    hipLaunchKernelGGL(apart ? move : gather, grid, dim3(kMoveThreads), 0, stream, pages, g, source,
+    hipLaunchKernelGGL(apart ? move : gather, grid, dim3(p.headDim), 0, stream, pages, g, source,
                        apart ? sourceTable : table, live, blocks, invalid);
     if (hipError_t e = hipGetLastError())
       return e;

@@ -340,6 +340,10 @@ SHARED = [  # groups, heads a KV head, hkv, dim, page
      4, 2, 64, 64),
     ([(64, [(1, 64 + i) for i in range(80)]), (0, [(1, 9)] * 9)], 8, 1, 64, 32),
     ([(32, [(1, 3000)] + [(1, 40 + i) for i in range(47)])], 5, 4, 64, 32),
+    # more than 256 sequences, and than 64 groups, of each kind
+    ([(64, [(1, 64 + i % 40) for i in range(290)])], 4, 1, 64, 32),
+    ([(32, [(1, 32 + i)] * 25) for i in range(70)], 4, 1, 64, 32),
+    ([(64, [(1, 70), (1, 64)]) for _ in range(140)], 1, 1, 64, 32),
     ([(32, [(1, 32)])], 1, 1, 64, 32),
     ([(64, [(1, 64), (1, 100), (1, 65)])], 4, 2, 256, 64),
     ([(96, [(1, 100), (1, 97)]), (0, [(1, 10), (2, 0)]), (31, [(1, 40)])], 2, 2, 128, 32),
@@ -405,7 +409,7 @@ def test_shared_large_scores(gpu):
 
 
 
-@pytest.mark.parametrize("members", [3, 60])
+@pytest.mark.parametrize("members", [3, 60, 90])
 def test_shared_without_place(gpu, members):
     """A sequence shorter than its prefix or past its table is NaN as a whole, a
     missing shared page all of the group, a missing own page its rows; the
@@ -454,22 +458,37 @@ def test_shared_without_place(gpu, members):
     g.check(got, q, 1 / 16)
 
 
-def test_shared_odd_orders(gpu):
+@pytest.mark.parametrize("n", [20, 100])
+def test_shared_odd_orders(gpu, n):
     """Starts and groups out of order, overlapping or out of range: any values
     in the rows that are claimed twice, no fault, and the rows of no sequence
     as they were."""
     rng = np.random.default_rng(6)
-    g = Group(rng, [(64, [(2, 64 + i) for i in range(20)])], 1, 256, 32)
-    q = rows16(rng, 44, 4, 256)
-    for starts in (g.starts, ints([0, 40, 3, 20, 9] + [30] * 16), ints(range(100, 121)),
-                   ints(range(20, -1, -1)), ints([-5] * 10 + [50] * 11)):
-        for groups, prefix in (([0, 20], [64]), ([5, 2], [64]), ([0, 20, 0, 20, 0, 20], [64] * 5),
-                               ([-9, 100], [64]), ([30, 40], [64]), ([0] * 71, [32] * 70)):
+    g = Group(rng, [(64, [(2, 64 + i) for i in range(n)])], 1, 256, 32)
+    q = rows16(rng, 2 * n + 4, 4, 256)
+    for starts in (g.starts, ints([0, 40, 3, 20, 9] + [30] * (n - 4)), ints(range(5 * n, 6 * n + 1)),
+                   ints(range(n, -1, -1)), ints([-5] * 10 + [3 * n] * (n - 9))):
+        for groups, prefix in (([0, n], [64]), ([5, 2], [64]), ([0, n, 0, n, 0, n], [64] * 5),
+                               ([-9, 6 * n], [64]), ([n + 10, n + 20], [64]), ([0] * 71, [32] * 70)):
             out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
             g.call(q, starts=starts, groups=ints(groups), prefix=ints(prefix), out=out)
             torch.cuda.synchronize()
             if starts is g.starts:
-                assert (out[40:] == 7).all()
+                assert (out[2 * n:] == 7).all()
+
+
+@pytest.mark.parametrize("n", [6, 90])
+def test_shared_rows_are_apart(gpu, n):
+    """A query row of infinities or NaN changes no other row."""
+    rng = np.random.default_rng(13)
+    g = Group(rng, [(96, [(1, 100 + i) for i in range(n)])], 2, 128, 32)
+    q = rows16(rng, n, 8, 128)
+    bad = q.copy()
+    bad[1], bad[4, 3], bad[n - 1, :, 5] = np.nan, np.inf, -np.inf
+    got, want = (g.call(x).cpu().numpy() for x in (bad, q))
+    same = np.ones((n, 8), bool)
+    same[1] = same[4, 3] = same[n - 1] = False
+    assert np.array_equal(got[same], want[same]) and np.isnan(got[1]).all()
 
 
 def test_shared_is_plain_without_groups(gpu):
@@ -480,12 +499,13 @@ def test_shared_is_plain_without_groups(gpu):
     assert torch.equal(got, ops.paged_gqa(dev(q), g.pool, g.starts, g.past, g.table))
 
 
-def test_shared_replayed(gpu):
+@pytest.mark.parametrize("n", [9, 90])
+def test_shared_replayed(gpu, n):
     """A captured call is replayed on other lengths, groups and prefixes, with
     the eager result each time; two graphs bound on one stream run at once."""
     rng = np.random.default_rng(11)
-    g = Group(rng, [(512, [(1, 512 + 20 * i) for i in range(9)])], 2, 256, 64, extra=2)
-    q = [rows16(rng, 9, 8, 256) for _ in range(2)]
+    g = Group(rng, [(512, [(1, 512 + 20 * i) for i in range(n)])], 2, 256, 64, extra=2)
+    q = [rows16(rng, n, 8, 256) for _ in range(2)]
     dq = [dev(x) for x in q]
     outs = [torch.zeros_like(x) for x in dq]
     stream = torch.cuda.Stream()
@@ -505,6 +525,10 @@ def test_shared_replayed(gpu):
         g.past.copy_(dev((past - less).astype(np.int32)))
         g.prefix.fill_(prefix if less == 0 or prefix < 500 else 0)
         want = [g.call(x).cpu() for x in q]
+        for s in (0, 1, n // 2, n - 1):
+            p = int(past[s]) - less
+            exact, far = po.attention(q[0][s:s + 1], g.k[s][:p + 1], g.v[s][:p + 1], p, 1 / 16)
+            assert np.all(np.abs(want[0][s:s + 1].numpy().astype(np.float64) - exact) <= far)
         streams = [torch.cuda.Stream() for _ in graphs]
         torch.cuda.synchronize()
         for s, graph in zip(streams, graphs):

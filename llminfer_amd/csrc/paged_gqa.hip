@@ -669,15 +669,14 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
       return;
     float m = -INFINITY, l = 0.0f;
     vec y = 0.0f;
-    // column `column` of pieces [first, first + pieces); false where starts out of
+    // column `column` of a unit, its pieces [first, first + pieces); false where starts out of
     // order make more of them than the rows can have
     auto join = [&](const SharedPart &part, unsigned long long first, unsigned pieces,
                     unsigned column, unsigned turn) {
-      const unsigned unit = 1u << part.shift;
       if (first + pieces > part.most)
         return false;
-      const size_t place = ((size_t)first * g.kvHeads + kvh) * unit + column % unit;
-      const size_t step = (size_t)g.kvHeads * unit;
+      const size_t place = (((size_t)first * g.kvHeads + kvh) << part.shift) + column;
+      const size_t step = (size_t)g.kvHeads << part.shift;
       const float2 *ml = reinterpret_cast<const float2 *>(part.parts.ml) + place;
       const vec *po = reinterpret_cast<const vec *>(part.parts.o + place * D) + lane;
       for (unsigned i0 = (wave + turn) % W; i0 < pieces; i0 += 4 * W) {
@@ -715,7 +714,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
       const unsigned unit = column >> part.shift;
       return unit < note.units &&
              join(part, note.first + (unsigned long long)(note.units - 1 - unit) * note.pieces,
-                  note.pieces, column, turn);
+                  note.pieces, column - (unit << part.shift), turn);
     };
     const unsigned column = (row - lo) * G + h % G;
     bool whole;
@@ -728,11 +727,18 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
       if (turn == 1 && !both)
         whole = false; // its output is there
       else
-        whole = join(rest, from + mine.units + unit, turn, column, 0);
+        whole = join(rest, from + mine.units + unit, turn, column - (unit << rest.shift), 0);
     } else
       whole = join_units(rest, mine, column, 0);
-    if (both) // (`other` of a group: its first row)
-      whole = join_units(shared, of, (row - of.other) * G + h % G, turn) && whole;
+    if (both) { // (`other` of a group: its first row)
+      const unsigned at = (row - of.other) * G + h % G;
+      if (rest.runs) {
+        const unsigned width = min(max(of.units, 1u), 1u << shared.shift), unit = at / width;
+        whole = join(shared, of.first + (unsigned long long)unit * of.pieces, of.pieces,
+                     at - unit * width, turn) && whole;
+      } else
+        whole = join_units(shared, of, at, turn) && whole;
+    }
     if (W > 1) {
       sM[wave] = m;
       sL[wave] = l;

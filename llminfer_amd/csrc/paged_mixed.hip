@@ -374,11 +374,13 @@ void paged_mixed_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
       return;
     const SharedSeq s = paged_seq_of(g, lanes, seq);
     const unsigned pieces = x.shared.pieces(s), units = x.shared.units(s);
-    const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
+    // (units of as many columns each, in whole tiles)
+    const unsigned each = (s.rows * G + units - 1) / units, width = (each + 31) & ~31u;
+    const unsigned unit = local / pieces, piece = local % pieces;
     if (local == 0 && kvh == 0 && threadIdx.x == 0)
-      leave_note(g, s, seq, before, pieces, units);
+      g.notes[seq] = SharedNote{before, pieces, width, s.row0};
     tiles_piece<D, 1>(q, pool, g, out, invalid, queryHeads, x.shared, c, shared, s, seq, kvh, unit,
-                      piece, pieces, me);
+                      width, piece, pieces, me);
     return;
   }
   // this wave's run of own blocks

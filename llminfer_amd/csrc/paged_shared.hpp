@@ -28,7 +28,8 @@ struct SharedSeq {
 // many a unit has, its units, and the group whose partials are joined to them
 // (+ 1; 0: none), for a group its first row. Own keys in runs of blocks
 // (paged_mixed.hip): the first of its blocks among all, the blocks of a unit, its
-// first unit among all, and the group.
+// first unit among all, and the group; for a group beside them the columns of a
+// unit for the units, the first unit's pieces first.
 struct SharedNote {
   unsigned first, pieces, units, other;
 };

@@ -91,7 +91,7 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   if (local == 0 && kvh == 0 && threadIdx.x == 0)
     leave_note(g, s, seq, number, pieces, units);
   tiles_piece<D, 256 / D>(q, pool, g, out, invalid, queryHeads, split, c, parts, s, seq, kvh, unit,
-                          piece, pieces, number);
+                          Tiles<D, 256 / D>::UNIT, piece, pieces, number);
 }
 
 } // namespace

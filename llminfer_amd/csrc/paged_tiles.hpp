@@ -55,16 +55,16 @@ template <int N, int CT> __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(kMfma, CT * kAhead, 0);
 }
 
-// Unit `unit` of sequence s (number seq) over its piece `piece` of `pieces`; the
-// partial's number is `number`.
+// Unit `unit`, of `width` columns, of sequence s (number seq) over its piece `piece`
+// of `pieces`; the partial's number is `number`.
 template <int D, int CT, typename View>
 __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
                                             const uint8_t *__restrict__ pool, const View &g,
                                             half_t *out, unsigned *invalid, unsigned queryHeads,
                                             const Split &split, ScoreScale c, const Partials &parts,
                                             const typename View::Seq &s, unsigned seq, unsigned kvh,
-                                            unsigned unit, unsigned piece, unsigned pieces,
-                                            unsigned number) {
+                                            unsigned unit, unsigned width, unsigned piece,
+                                            unsigned pieces, unsigned number) {
   using T = Tiles<D, CT>;
   const unsigned G = queryHeads / g.kvHeads;
   const unsigned tid = threadIdx.x, lane = tid % 64, r = lane % 32, hi = lane / 32;
@@ -72,7 +72,10 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
   const unsigned half = wave / 4, tile0 = wave % 4 * CT;
 
   // this lane's columns (past the unit's last: some row's, not written)
-  const unsigned c0 = unit * T::UNIT, columns = min((unsigned)T::UNIT, s.rows * G - c0);
+  const unsigned c0 = unit * width, columns = min(width, s.rows * G - c0);
+  // A wave without a column only decodes: its products would take LDS and power
+  // from the others' (units of 88 of the 128 columns: 57 us, 59 with them).
+  const bool idle = !std::is_same<View, PagedView>::value && 32 * tile0 >= columns;
   unsigned visible[CT]; // a column's last key
   size_t row[CT];
 #pragma unroll
@@ -344,7 +347,7 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
 #pragma unroll
     for (int i = 0; i < T::EACH; ++i) {
       const unsigned at = half * T::EACH + i, b = b0 + T::BLOCKS * n + at;
-      if (b < b1)
+      if (b < b1 && !idle)
         consume(wide, b, keys + at * T::BLOCKB, values + at * T::BLOCKB);
     }
     if (half == 1)

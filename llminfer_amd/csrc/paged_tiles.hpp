@@ -72,10 +72,9 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
   const unsigned half = wave / 4, tile0 = wave % 4 * CT;
 
   // this lane's columns (past the unit's last: some row's, not written)
-  const unsigned c0 = unit * width, columns = min(width, s.rows * G - c0);
-  // A wave without a column only decodes: its products would take LDS and power
-  // from the others' (units of 88 of the 128 columns: 57 us, 59 with them).
-  const bool idle = !std::is_same<View, PagedView>::value && 32 * tile0 >= columns;
+  constexpr bool kShared = !std::is_same<View, PagedView>::value;
+  const unsigned most0 = kShared ? width : (unsigned)T::UNIT;
+  const unsigned c0 = unit * most0, columns = min(most0, s.rows * G - c0);
   unsigned visible[CT]; // a column's last key
   size_t row[CT];
 #pragma unroll
@@ -138,12 +137,12 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
   };
   const unsigned quad = unit16 / 16 % 4, rr = unit16 % 16;
   // (16 bytes of key codes: 32 channels of a key, at D 64 16 of two neighbours)
-  const unsigned keyRow = D >= 128 ? rr : 2 * (unit16 % 8);
-  const unsigned keyChunk = D >= 128 ? unit16 % (D / 2) / 16 * 2048 : unit16 % 32 / 8 * 1024;
-  const unsigned keyAt = slot * T::BLOCKB + keyChunk +
-                         (16 * (keyRow / 8) + 8 * (unit16 / (D / 2)) + keyRow % 8) * 16;
-  const unsigned keyScaleAt =
-      D >= 128 ? 4 * lane : 4 * (unit16 / 32 * 32 + unit16 % 32 / 16 * 16 + keyRow);
+  const unsigned two = 2 * (unit16 % 8);
+  const unsigned keyAt =
+      D >= 128 ? slot * T::BLOCKB + (unit16 % (D / 2) / 16) * 2048 +
+                     (16 * (rr / 8) + 8 * (unit16 / (D / 2)) + rr % 8) * 16
+               : slot * T::BLOCKB + (unit16 % 32 / 8) * 1024 +
+                     (16 * (two / 8) + 8 * (unit16 / 32) + two % 8) * 16;
   const unsigned valueAt = slot * T::BLOCKB + (unit16 / 64) * 4096 + quad * 512 + rr * 16;
   // The wave's part of step n has come. Behind the last key lies anything (what
   // is in page 0 from a missing page on), and 0 times that may be NaN: those
@@ -163,20 +162,21 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
   };
   auto decode_keys = [&](char *to) {
     const uint4_t keyCodes = *reinterpret_cast<const uint4_t *>(raw + 16 * lane);
-    const half2_t keyScale = *reinterpret_cast<const half2_t *>(raw + 2048 + keyScaleAt);
     if constexpr (D >= 128) {
+      const half2_t keyScale = *reinterpret_cast<const half2_t *>(raw + 2048 + 4 * lane);
 #pragma unroll
       for (int w = 0; w < 4; ++w)
         *reinterpret_cast<half8_t *>(to + keyAt + 512 * w) =
             paged_eight(keyCodes[w], keyScale, nibbles);
     } else {
-      const half2_t next = *reinterpret_cast<const half2_t *>(raw + 2052 + keyScaleAt);
+      const half2_t *scales = reinterpret_cast<const half2_t *>(raw + 2048) + unit16 / 32 * 32 +
+                              unit16 % 32 / 16 * 16 + two;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         *reinterpret_cast<half8_t *>(to + keyAt + 512 * w) =
-            paged_eight(keyCodes[w], keyScale, nibbles);
+            paged_eight(keyCodes[w], scales[0], nibbles);
         *reinterpret_cast<half8_t *>(to + keyAt + 512 * w + 16) =
-            paged_eight(keyCodes[2 + w], next, nibbles);
+            paged_eight(keyCodes[2 + w], scales[1], nibbles);
       }
     }
   };
@@ -347,7 +347,9 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
 #pragma unroll
     for (int i = 0; i < T::EACH; ++i) {
       const unsigned at = half * T::EACH + i, b = b0 + T::BLOCKS * n + at;
-      if (b < b1 && !idle)
+      // (a wave without a column only decodes: its products would take LDS from the
+      // others'; units of 88 of the 128 columns: 55 us, 59 with them)
+      if (b < b1 && (!kShared || 32 * tile0 < columns))
         consume(wide, b, keys + at * T::BLOCKB, values + at * T::BLOCKB);
     }
     if (half == 1)

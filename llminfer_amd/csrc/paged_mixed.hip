@@ -4,6 +4,24 @@
 // sequences' own keys, sixteen columns a unit (bound by memory and decoding), so
 // that both run at once. The partials of the two are joined by
 // paged_shared_merge_kernel.
+//
+// A workgroup of either kind takes a CU's LDS, so the plan gives each kind as many
+// CUs as make them end together, and own keys go by waves and not by workgroups:
+// a wave with a run of blocks waits for no other, and its runs are of equal
+// length whatever the sequences' are (pieces by workgroups, joined in LDS: 12 us
+// each, five of them waiting; 48 chats 57 us, 44 with runs).
+//
+// 48 sequences of 16 / 4 heads of 256, 16384 shared keys and up to 1024 of their
+// own, 13.3 GFLOP, take 39 us here and 44 with the join (paged_gqa: 137 to 142).
+// Tiles, 52 of a KV head's 64 workgroups, 20 blocks each: 6 us until the first
+// block is there (plan 1.5, table, block, one after the other), 1.15 us a block,
+// 4 to join the halves and write 24 MB of partials. Own keys, 10 blocks a wave:
+// 2.2 us a block of 10 KB and 9 us beside them, bound by decoding (550
+// instructions a block, two waves a SIMD). Matrix instructions take 15 % of the
+// time, vector instructions 31 %, waves wait for 52 %: barriers of a step, LDS and
+// the beginning. Six groups at head_dim 128: 48 us, own keys 1.2 us a block; two
+// of 187 rows in all at 64: 42 us, tiles 3.2 us a step of eight blocks, bound by
+// the softmax's vector instructions.
 #include "paged_tiles.hpp"
 
 namespace llmi {

@@ -2,6 +2,16 @@
 // children that share their parents' pages (fork), the pages that no sequence
 // holds (free), chosen keys and values put side by side (move). No arithmetic,
 // so bytes and latency are what there is to gain.
+//
+// In a loop: 64 children in pages of 256 keys of 4 heads of 256 (16 MB read, 20
+// written) 7.4 us, 5 TB/s, the rate of a copy; 16 children of one prompt 3.8 to 4
+// us, a launch with three dependent loads. The free ones of 400 thousand pages by
+// 500 rows of up to 1031 13.0 us (traced: marks 7.5, join 2.8, list 3.7; the bytes
+// would take 0.6), of 4096 by 16 rows 5.2 us. 8192 of 32749 keys of 4 heads of
+// 256 moved between pages 10.8 us: every line of the source is touched, 41 MB, and
+// 10 written, the rate of a copy; 6808 of 13 sequences' 8 heads of 128 9.2 us (23
+// MB and 9), 42 accepted drafts of 16 sequences 4.4 us. Within the same pages a
+// launch more and the rows once more through memory: 16.4, 14.1 and 7.6 us.
 #include "hip_common.hpp"
 #include "kernels.hpp"
 #include "paged_kv.hpp"
@@ -19,8 +29,10 @@ struct ForkView {
   unsigned pages, pageSize, kvHeads, sequences, tableStride;
 };
 
-// A workgroup copies one block of one head of a child's last page; the first
-// of a child writes its row of the table too.
+// A workgroup copies one block of one head of a child's last page (contiguous, all
+// of it in flight before it is stored); the first of a child writes its row of the
+// table too. The others, of blocks without keys, leave at once: how full the page
+// is only the device knows.
 template <int D>
 __global__ __launch_bounds__(kForkThreads) void paged_fork_kernel(ForkView g, uint4_t *pool,
                                                                   unsigned *invalid) {
@@ -195,6 +207,12 @@ __global__ __launch_bounds__(kFreeThreads) void paged_free_small_kernel(FreeView
   list_free<kSmall>(0, g.pages, 0, g.pages, free, count, [&](unsigned i) { return marks[i]; });
 }
 
+// Marks in up to 32 workgroups, each with bits of all pages in LDS, then joined, so
+// that no memory has to be cleared and nothing is atomic but bits in LDS; the join
+// and the list are launches of their own because a free page's rank needs all the
+// marks before it (marks of eight workgroups joined by those that list: 24 us).
+// One workgroup alone up to 8192 pages and 16384 slots: 5.2 us for 4096 pages,
+// against three launches.
 // What the launches leave each other: [part][words] marks, the words of a part
 // whole 16 bytes, [words] of all of them and how many pages of each kListed are
 // free.

@@ -656,11 +656,11 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
   const unsigned seq = n - 1;
   const int lo = max(g.starts[seq], 0), hi = g.starts[seq + 1];
   const SharedNote mine = g.notes[g.count + seq];
-  const unsigned run = rest.runs ? g.notes[g.count + g.all].first : 0u;
+  const SharedNote runs = rest.runs ? g.notes[g.count + g.all] : SharedNote{1, 1, 0, 0, 0};
   if ((int)row < lo || (int)row >= hi || mine.pieces == 0 || mine.other > g.count)
     return; // of no sequence, or its output is there
   const bool both = mine.other != 0;
-  SharedNote of{0, 0, 0, 0};
+  SharedNote of{0, 0, 0, 0, 0};
   if (both)
     of = shared.g.notes[mine.other - 1];
   for (unsigned h0 = blockIdx.y * kItems; h0 < queryHeads; h0 += gridDim.y * kItems) {
@@ -719,22 +719,28 @@ __global__ __launch_bounds__(kMergeThreads) void paged_shared_merge_kernel(
     const unsigned column = (row - lo) * G + h % G;
     bool whole;
     unsigned turn = mine.pieces;
-    if (rest.runs) { // (the note: first block, blocks of a unit, first unit)
-      const unsigned unit = column >> rest.shift;
-      const unsigned long long a = mine.first + (unsigned long long)unit * mine.pieces;
-      const unsigned long long from = a / run, to = (a + mine.pieces - 1) / run;
-      turn = (unsigned)(to - from + 1);
+    // the runs that have unit `unit` of a note: the first, and how many
+    auto runs_of = [](const SharedNote &note, unsigned unit, unsigned run, unsigned &count) {
+      const unsigned first = note.first + unit * note.pieces, from = first / run;
+      count = (first + note.pieces - 1) / run - from + 1;
+      return from;
+    };
+    if (rest.runs) {
+      const unsigned unit = column >> rest.shift, from = runs_of(mine, unit, runs.first, turn);
       if (turn == 1 && !both)
         whole = false; // its output is there
       else
-        whole = join(rest, from + mine.units + unit, turn, column - (unit << rest.shift), 0);
+        whole = join(rest, (unsigned long long)from + mine.units + unit, turn,
+                     column - (unit << rest.shift), 0);
     } else
       whole = join_units(rest, mine, column, 0);
     if (both) { // (`other` of a group: its first row)
       const unsigned at = (row - of.other) * G + h % G;
       if (rest.runs) {
-        const unsigned width = min(max(of.units, 1u), 1u << shared.shift), unit = at / width;
-        whole = join(shared, of.first + (unsigned long long)unit * of.pieces, of.pieces,
+        const unsigned width = min(max(of.width, 1u), 1u << shared.shift), unit = at / width;
+        unsigned count;
+        const unsigned from = runs_of(of, unit, runs.pieces, count);
+        whole = join(shared, (unsigned long long)from + (runs.units ? of.units + unit : 0u), count,
                      at - unit * width, turn) && whole;
       } else
         whole = join_units(shared, of, at, turn) && whole;
@@ -871,8 +877,8 @@ namespace {
 // Mixed from 96 columns a group and 640 in all KV heads on (128 columns of 8
 // heads of 128 on 8192 keys: 29 us, 35 Same; 768 of 4 heads of 256 on 16384: 44
 // and 61; below, its beginning and end cost more: 64 of 4 heads on 4096 keys 25
-// us, 18 Same; 128 of one head 18 and 12), as long as each unit has a workgroup.
-// Apart where it has not, or where the sequences have many rows themselves.
+// us, 18 Same; 128 of one head 18 and 12). Apart where the sequences have many rows
+// themselves, and where Mixed cannot count the blocks or divide the device.
 // Same has the pieces of its kernel's eight waves where the units are few (8
 // sequences on 4299 keys: 15.3 us, 17.2 with four), two rounds of four waves
 // otherwise (4 groups of 8 on 8192 keys: 25 us, 30 with six rounds or one).
@@ -892,21 +898,25 @@ SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) 
   s.rest = plan_for(p, group);
   s.sharedShift = s.shared.split.shift;
   s.restShift = s.rest.split.shift;
-  // (costs in us, of a workgroup: a block of 128 columns takes 1 at head_dim 256
-  // and 0.5 at 128 and 64, a wave's own block of 10 KB 2.2)
-  s.mixed = {7, 512 / p.headDim, kCus / p.kvHeads ? kCus / p.kvHeads : 1,
-             p.headDim == 256 ? 1.0f : 0.5f, 0.2f * p.headDim / 256, 0.5f};
+  // Costs in us of a workgroup, measured at each width: a block of 128 columns, an
+  // own block (eight waves have one each in 2.2, 1.2 or 0.8), an own unit; and the
+  // blocks of the 8 us that a second beginning takes.
+  const unsigned width = p.headDim == 256 ? 0 : p.headDim == 128 ? 1 : 2;
+  constexpr float kShared[] = {1.15f, 0.58f, 0.42f}, kOwn[] = {0.28f, 0.15f, 0.1f};
+  s.mixed = {512 / p.headDim, kCus / p.kvHeads, 7u << width, kShared[width], kOwn[width], 0.4f};
   const uint64_t units = most_units(of, group, 128), ownUnits = most_units(p, group, kColumns);
-  // own blocks of all units, which are counted in 32 bits
-  const uint64_t blocks = ownUnits * ((uint64_t)p.tableStride * p.pageSize / 32 + 1);
-  if (s.restShift != 4 || units >= s.mixed.cus || blocks >= 1u << 31) {
+  // the blocks of all units, which are counted in 32 bits
+  const uint64_t blocks = ((uint64_t)p.tableStride * p.pageSize / 32 + 1) *
+                          (units > ownUnits ? units : ownUnits);
+  const bool mixes = s.mixed.cus > 1 && blocks < 1u << 30;
+  if (s.restShift != 4 || (all / groups >= 96 && !mixes)) {
     s.how = SharedPlan::Apart;
     s.sharedPieces = most_pieces(of, group, s.shared.split);
     s.restPieces = most_pieces(p, group, s.rest.split);
   } else if (all / groups >= 96 && all * p.kvHeads >= 640) {
     s.how = SharedPlan::Mixed;
-    s.sharedShift = s.mixed.shift;
-    s.sharedPieces = s.mixed.cus;
+    s.sharedShift = 7;
+    s.sharedPieces = s.mixed.cus + units;
     s.restPieces = kMixedWaves * s.mixed.cus + ownUnits;
   } else {
     s.how = SharedPlan::Same;

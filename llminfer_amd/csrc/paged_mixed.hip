@@ -30,6 +30,7 @@ namespace {
 constexpr unsigned kColumns = 16; // of a unit of own keys
 constexpr unsigned kWaves = kMixedWaves;
 static_assert(kWaves == kThreads / 64, "the tiles' waves");
+constexpr unsigned kTileColumns = 128; // of a unit of shared keys, at most
 constexpr unsigned kLeastRun = 2; // blocks
 
 __device__ __forceinline__ float4_t mfma16x16x32(half8_t a, half8_t b, float4_t c) {
@@ -64,7 +65,10 @@ __device__ __forceinline__ void own_piece(const half_t *__restrict__ q,
   using Block = OwnBlock<D>;
   constexpr int TILES = D / 16;
   const unsigned G = queryHeads / g.kvHeads;
-  const unsigned tid = threadIdx.x, lane = tid % 64, quad = lane / 16, r = lane % 16;
+  unsigned tid = threadIdx.x;
+  asm volatile("" : "+v"(tid)); // (as in tiles_piece)
+  __builtin_assume(tid < kThreads);
+  const unsigned lane = tid % 64, quad = lane / 16, r = lane % 16;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const unsigned c0 = unit * kColumns, columns = min(kColumns, s.rows * G - c0);
   auto token_of = [&](unsigned col) { return min((c0 + col) / G, s.rows - 1); };
@@ -269,13 +273,14 @@ __device__ __forceinline__ void own_piece(const half_t *__restrict__ q,
     *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(lost ? 0.0f : m, sum);
 }
 
-// The two divisions. Groups' shared keys: pieces as Split has them, on `workers`
-// workgroups a KV head, one each. The sequences' own keys: the blocks of all
-// their units, one after the other, cut into runs of `run` blocks, one for each
-// wave of the other workgroups; a unit's pieces are where its blocks lie in them.
+// The two divisions. The blocks of all units of shared keys, one after the other,
+// are cut into runs, one for each of `workers` workgroups a KV head, those of all
+// units of own keys into runs, one for each wave of the other workgroups; a unit's
+// pieces are where its blocks lie in them. whole: units of shared keys begin with
+// a run, so that each workgroup has blocks of one unit and begins once.
 struct Mixed {
-  Split shared;
-  unsigned workers, run;
+  unsigned workers, sharedRun, ownRun;
+  bool whole;
 };
 __device__ __forceinline__ float wave_sum(float x) {
   x = group_sum<16>(x);
@@ -287,70 +292,76 @@ __device__ __forceinline__ float wave_sum(float x) {
 __device__ __forceinline__ unsigned own_units(const SharedSeq &q, unsigned group) {
   return q.step ? (q.rows * group + kColumns - 1) / kColumns : 0u;
 }
+__device__ __forceinline__ unsigned tile_units(const SharedSeq &q, unsigned group) {
+  return q.step ? 0u : (q.rows * group + kTileColumns - 1) / kTileColumns;
+}
+// Blocks of a unit of shared keys in the runs.
+__device__ __forceinline__ unsigned tile_blocks(const SharedSeq &q, const Mixed &x) {
+  const unsigned n = Split::blocks(q);
+  return x.whole ? (n + x.sharedRun - 1) / x.sharedRun * x.sharedRun : n;
+}
+// (the host sees to it that the blocks of all units of a kind are no more than 2^31)
 __device__ __forceinline__ Mixed mixed_split(const SharedView &g, const SharedLanes &lanes,
                                              unsigned group, const MixedPlan &plan) {
-  Mixed x{Split{group, plan.shift, plan.step, plan.step, 0.0f, true}, 0, 1};
-  float shared = 0.0f, units = 0.0f;
-  unsigned own = 0; // (the host sees to it that they are no more than 2^31)
+  unsigned shared = 0, own = 0, units = 0, tiles = 0;
   shared_chunks(g, lanes, [&](unsigned, const SharedSeq &q) {
-    shared += q.step == 0 ? lane_blocks(x.shared, q) : 0.0f;
-    const unsigned n = own_units(q, group);
-    own += n * Split::blocks(q);
-    units += (float)n;
+    const unsigned n = own_units(q, group), t = tile_units(q, group), blocks = Split::blocks(q);
+    shared += t * blocks;
+    own += n * blocks;
+    units += n;
+    tiles += t;
     return false;
   });
-  shared = wave_sum(shared);
-  units = wave_sum(units);
-  own = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(own), 63);
-  auto whole = [](float v) { // (below 2^30: no table has more blocks)
-    return uniform((unsigned)fminf(ceilf(v), 0x1p30f));
-  };
-  const float a = shared * plan.sharedCost, b = (float)own * plan.ownCost + units * plan.ownFixed;
-  const float cus = (float)plan.cus;
-  unsigned workers = shared == 0.0f ? 0u : max(1u, whole(cus * a / (a + b) - 0.5f));
-  workers = own == 0 ? plan.cus : min(workers, plan.cus - 1);
-  auto take = [](Split &s, unsigned chunk) {
-    const unsigned steps = (chunk + s.step - 1) & ~(s.step - 1);
-    s.chunk = uniform(steps ? steps : s.step);
-    s.inv = __builtin_amdgcn_rcpf((float)s.chunk);
-  };
-  take(x.shared, whole(shared * 1.0001f / (float)max(workers, 1u)));
-  // Every unit's last piece is rounded up: longer ones until each has a
-  // workgroup, undivided units at last (the host sees to it that they fit).
-  auto pieces = [&](bool undivided) { // (the groups come first)
-    unsigned n = 0;
-    shared_chunks(g, lanes, [&](unsigned c, const SharedSeq &q) {
-      if (q.step == 0)
-        n += x.shared.units(q) * (undivided ? 1u : x.shared.pieces(q));
-      return 64 * (c + 1) >= g.count;
-    });
-    return (unsigned)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
-  };
-  unsigned n = pieces(false);
-  for (int i = 0; i < 4 && n > workers; ++i) {
-    take(x.shared, max(x.shared.chunk + 1, (unsigned)fminf((float)x.shared.chunk * (float)n /
-                                                               (float)max(workers, 1u), 0x1p30f)));
-    n = pieces(false);
+  auto all = [](unsigned n) { return uniform((unsigned)__builtin_amdgcn_readlane((int)wave_scan(n), 63)); };
+  shared = all(shared);
+  own = all(own);
+  units = all(units);
+  tiles = all(tiles);
+  const float a = (float)(shared + tiles * plan.again) * plan.sharedCost;
+  const float b = (float)own * plan.ownCost + (float)units * plan.ownFixed;
+  unsigned workers = 0;
+  if (shared) {
+    workers = max(1u, uniform((unsigned)ceilf((float)plan.cus * a / (a + b) - 0.5f)));
+    workers = own ? min(workers, plan.cus - 1) : plan.cus;
   }
-  if (n > workers) {
-    take(x.shared, 1u << 30);
-    n = pieces(true);
+  Mixed x{workers, plan.step, 1, false};
+  if (workers) {
+    auto steps = [&](unsigned n) { return uniform((n + plan.step - 1) / plan.step * plan.step); };
+    const unsigned even = steps((shared + workers - 1) / workers);
+    // whole runs a unit: longer ones until there are no more than workgroups
+    unsigned n = 0, run = even;
+    for (int i = 0; i < 5; ++i) {
+      n = 0;
+      shared_chunks(g, lanes, [&](unsigned c, const SharedSeq &q) { // (the groups come first)
+        n += tile_units(q, group) * ((Split::blocks(q) + run - 1) / run);
+        return 64 * (c + 1) >= g.count;
+      });
+      n = all(n);
+      if (n <= workers)
+        break;
+      run = steps(max(run + 1, (unsigned)fminf((float)run * (float)n / (float)workers, 0x1p30f)));
+    }
+    x.whole = n <= workers && run <= even + plan.again;
+    x.sharedRun = x.whole ? run : even;
+    x.workers = x.whole ? n : (shared + even - 1) / even;
   }
-  x.workers = min(n, plan.cus);
   const unsigned waves = max(kWaves * (plan.cus - x.workers), 1u);
-  x.run = max(uniform((own + waves - 1) / waves), kLeastRun);
+  x.ownRun = max(uniform((own + waves - 1) / waves), kLeastRun);
   return x;
 }
 
-// The sequence that has block `at` of all own units: its first block and its
-// first unit among them; false behind the last.
-__device__ __forceinline__ bool find_own(const SharedView &g, const SharedLanes &lanes,
-                                         unsigned group, unsigned at, unsigned &seq,
-                                         unsigned &firstBlock, unsigned &firstUnit) {
+// The sequence whose units have block `at` of a kind, each units(q) units of
+// blocks(q) blocks: its first block and its first unit among all; false behind the
+// last.
+template <typename Units, typename Blocks>
+__device__ __forceinline__ bool find_block(const SharedView &g, const SharedLanes &lanes,
+                                           Units unitsOf, Blocks blocksOf, unsigned at,
+                                           unsigned &seq, unsigned &firstBlock,
+                                           unsigned &firstUnit) {
   bool found = false;
   firstBlock = firstUnit = 0;
   shared_chunks(g, lanes, [&](unsigned c, const SharedSeq &q) {
-    const unsigned units = own_units(q, group), n = units * Split::blocks(q);
+    const unsigned units = unitsOf(q), n = units * blocksOf(q);
     const unsigned blocks = wave_scan(n), sum = wave_scan(units);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(at - firstBlock < blocks);
     if (!past) {
@@ -368,65 +379,129 @@ __device__ __forceinline__ bool find_own(const SharedView &g, const SharedLanes 
   return found;
 }
 
+// A run of the blocks of a kind, taken unit by unit: each(s, seq, unit, first block
+// of the piece in its unit, blocks of the piece, of the unit, first block and unit
+// of the sequence), until it says false. s: the sequence, one of the first
+// `sequences` of the view (the groups come first).
+template <typename Units, typename Blocks, typename Count, typename Next,
+          typename Each>
+__device__ __forceinline__ void each_piece(const SharedView &g, const SharedLanes &lanes,
+                                           Units unitsOf, Blocks blocksOf, Count sequences,
+                                           unsigned at, unsigned run, Next next, Each each) {
+  unsigned seq, firstBlock, firstUnit;
+  const unsigned stop = at + run;
+  if (!find_block(g, lanes, unitsOf, blocksOf, at, seq, firstBlock, firstUnit))
+    return;
+  seq = uniform(seq);
+  firstBlock = uniform(firstBlock);
+  firstUnit = uniform(firstUnit);
+  SharedSeq s = paged_from_lane(paged_seq_of(g, lanes, seq), 0);
+  while (true) {
+    const unsigned units = uniform(unitsOf(s)), blocks = uniform(blocksOf(s));
+    while (at < stop && at - firstBlock < units * blocks) {
+      const unsigned unit = uniform((at - firstBlock) / blocks);
+      const unsigned b0 = uniform(at - firstBlock - unit * blocks);
+      const unsigned length = uniform(min(blocks - b0, stop - at));
+      if (!each(s, seq, unit, b0, length, blocks, firstBlock, firstUnit))
+        return;
+      at += length;
+    }
+    if (at >= stop || ++seq >= sequences())
+      return;
+    firstBlock += units * blocks;
+    firstUnit += units;
+    s = next(seq);
+  }
+}
+
+struct MixedArgs {
+  const half_t *q;
+  const uint8_t *pool;
+  SharedView g;
+  half_t *out;
+  unsigned *invalid;
+  unsigned queryHeads;
+  MixedPlan plan;
+  ScoreScale c;
+  Partials shared, rest;
+  unsigned mostShared, mostOwn;
+};
+// The arguments, read again: kept in registers over the pieces of a run they and
+// what comes of them fill the scalar ones, and with these full the tiles' products
+// wait for each operand (two groups at head_dim 64: 44 us, 42 so).
+__device__ __forceinline__ MixedArgs mixed_args() {
+  auto at = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const MixedArgs *)at;
+}
+
 template <int D>
 __global__ __attribute__((amdgpu_flat_work_group_size(kThreads, kThreads),
                           amdgpu_waves_per_eu(2, 2)))
-void paged_mixed_kernel(const half_t *__restrict__ q, const uint8_t *__restrict__ pool,
-                        SharedView g, half_t *out, unsigned *invalid, unsigned queryHeads,
-                        MixedPlan plan, ScoreScale c, Partials shared, Partials rest,
-                        unsigned mostShared, unsigned mostOwn) {
-  const unsigned G = queryHeads / g.kvHeads, kvh = blockIdx.x % g.kvHeads;
-  const unsigned me = blockIdx.x / g.kvHeads;
-  const SharedLanes lanes = paged_own(g);
-  const Mixed x = mixed_split(g, lanes, G, plan);
+void paged_mixed_kernel(MixedArgs args) {
+  const unsigned G = args.queryHeads / args.g.kvHeads, kvh = blockIdx.x % args.g.kvHeads;
+  const unsigned me = blockIdx.x / args.g.kvHeads;
+  const SharedLanes lanes = paged_own(args.g);
+  const Mixed x = mixed_split(args.g, lanes, G, args.plan);
   if (blockIdx.x == 0 && threadIdx.x == 0)
-    g.notes[g.count + g.all].first = x.run;
+    args.g.notes[args.g.count + args.g.all] =
+        SharedNote{x.ownRun, x.sharedRun, x.whole ? 0u : 1u, 0, 0};
   if (me < x.workers) {
-    unsigned seq, local, before;
-    if (me >= mostShared || // (starts out of order make more pieces than the rows can have)
-        !paged_find(g, lanes, me,
-                    [&](const SharedSeq &q) {
-                      return q.step == 0 ? x.shared.units(q) * x.shared.pieces(q) : 0u;
-                    },
-                    seq, local, before))
-      return;
-    const SharedSeq s = paged_seq_of(g, lanes, seq);
-    const unsigned pieces = x.shared.pieces(s), units = x.shared.units(s);
-    // (units of as many columns each, in whole tiles)
-    const unsigned each = (s.rows * G + units - 1) / units, width = (each + 31) & ~31u;
-    const unsigned unit = local / pieces, piece = local % pieces;
-    if (local == 0 && kvh == 0 && threadIdx.x == 0)
-      g.notes[seq] = SharedNote{before, pieces, width, s.row0};
-    tiles_piece<D, 1>(q, pool, g, out, invalid, queryHeads, x.shared, c, shared, s, seq, kvh, unit,
-                      width, piece, pieces, me);
+    bool again = false;
+    each_piece(
+        args.g, lanes, [&](const SharedSeq &q) {
+          const MixedArgs a = mixed_args();
+          return tile_units(q, a.queryHeads / a.g.kvHeads);
+        },
+        [&](const SharedSeq &q) { return tile_blocks(q, x); }, [&] { return mixed_args().g.count; }, me * x.sharedRun,
+        x.sharedRun,
+        [&](unsigned seq) {
+          const MixedArgs a = mixed_args();
+          return paged_from_lane(shared_seq(a.g, shared_groups(a.g), seq), 0);
+        },
+        [&](const SharedSeq &s, unsigned seq, unsigned unit, unsigned b0, unsigned length,
+            unsigned blocks, unsigned firstBlock, unsigned firstUnit) {
+          if (again)
+            __syncthreads(); // the piece before is done with its LDS
+          again = true;
+          const MixedArgs a = mixed_args();
+          const unsigned group = a.queryHeads / a.g.kvHeads, head = blockIdx.x % a.g.kvHeads;
+          const unsigned number = (x.whole ? 0u : firstUnit + unit) + blockIdx.x / a.g.kvHeads;
+          if (number >= a.mostShared) // (starts out of order: more than the rows can have)
+            return false;
+          // (units of as many columns each, in whole tiles)
+          const unsigned units = tile_units(s, group), each = (s.rows * group + units - 1) / units;
+          const unsigned width = uniform((each + 31) & ~31u);
+          if (unit == 0 && b0 == 0 && head == 0 && threadIdx.x == 0)
+            a.g.notes[seq] = SharedNote{firstBlock, blocks, firstUnit, s.row0, width};
+          tiles_piece<D, 1, false>(a.q, a.pool, a.g, a.out, a.invalid, a.queryHeads, a.c, a.shared,
+                                   s, seq, head, unit, width, b0,
+                                   uniform(min(length, Split::blocks(s) - b0)), false,
+                                   uniform(number));
+          return !x.whole;
+        });
     return;
   }
   // this wave's run of own blocks
   const unsigned worker = uniform((me - x.workers) * kWaves + threadIdx.x / 64);
-  unsigned at = worker * x.run, seq, firstBlock, firstUnit;
-  const unsigned stop = at + x.run;
-  if (!find_own(g, lanes, G, at, seq, firstBlock, firstUnit))
-    return;
-  SharedSeq s = paged_from_lane(paged_seq_of(g, lanes, seq), 0);
-  while (true) {
-    const unsigned units = uniform(own_units(s, G)), blocks = uniform(Split::blocks(s));
-    for (; at < stop && at - firstBlock < units * blocks;) {
-      const unsigned unit = (at - firstBlock) / blocks, b0 = (at - firstBlock) % blocks;
-      const unsigned length = min(blocks - b0, stop - at), number = worker + firstUnit + unit;
-      if (at == firstBlock && kvh == 0 && threadIdx.x % 64 == 0)
-        g.notes[seq] = SharedNote{firstBlock, s.ok ? blocks : 0u, firstUnit, s.begin ? s.group + 1 : 0u};
-      if (number >= mostOwn)
-        return;
-      own_piece<D>(q, pool, g, out, invalid, queryHeads, c, rest, s, kvh, unit, s.begin + b0,
-                   s.begin + b0 + length, length == blocks && !s.joined(), number);
-      at += length;
-    }
-    if (at >= stop || ++seq >= g.sequences)
-      return;
-    firstBlock += units * blocks;
-    firstUnit += units;
-    s = paged_from_lane(shared_seq(g, lanes.groups, seq), 0);
-  }
+  each_piece(
+      args.g, lanes, [&](const SharedSeq &q) { return own_units(q, G); },
+      [&](const SharedSeq &q) { return Split::blocks(q); }, [&] { return args.g.sequences; }, worker * x.ownRun,
+      x.ownRun,
+      [&](unsigned seq) { return paged_from_lane(shared_seq(args.g, lanes.groups, seq), 0); },
+      [&](const SharedSeq &s, unsigned seq, unsigned unit, unsigned b0, unsigned length,
+          unsigned blocks, unsigned firstBlock, unsigned firstUnit) {
+        const unsigned number = worker + firstUnit + unit;
+        if (number >= args.mostOwn)
+          return false;
+        if (unit == 0 && b0 == 0 && kvh == 0 && threadIdx.x % 64 == 0)
+          args.g.notes[seq] = SharedNote{firstBlock, s.ok ? blocks : 0u, firstUnit,
+                                         s.begin ? s.group + 1 : 0u, 0};
+        own_piece<D>(args.q, args.pool, args.g, args.out, args.invalid, args.queryHeads, args.c,
+                     args.rest, s, kvh, unit, s.begin + b0, s.begin + b0 + length,
+                     length == blocks && !s.joined(), number);
+        return true;
+      });
 }
 
 } // namespace
@@ -435,9 +510,10 @@ hipError_t launch_paged_mixed(const half_t *q, const uint8_t *pool, const Shared
                               unsigned *invalid, unsigned queryHeads, const MixedPlan &plan,
                               ScoreScale c, Partials shared, Partials rest, unsigned mostShared,
                               unsigned mostOwn, hipStream_t stream) {
+  const MixedArgs args{q, pool, g, out, invalid, queryHeads, plan, c, shared, rest, mostShared,
+                       mostOwn};
   auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(plan.cus * g.kvHeads), dim3(kThreads), 0, stream, q, pool, g,
-                       out, invalid, queryHeads, plan, c, shared, rest, mostShared, mostOwn);
+    hipLaunchKernelGGL(kernel, dim3(plan.cus * g.kvHeads), dim3(kThreads), 0, stream, args);
     return hipGetLastError();
   };
   return g.dim == 256   ? run(paged_mixed_kernel<256>)

@@ -156,12 +156,13 @@ hipError_t launch_paged_tiles(const half_t *q, const uint8_t *pool, const View &
                               Partials parts, unsigned pieces, hipStream_t stream);
 
 // The kernel for groups with many rows in all and sequences with few
-// (paged_mixed.hip): units of 2^shift columns of the shared keys, whole steps of
-// blocks, on `cus` workgroups a KV head, and the time that a block of a unit of
-// shared keys, a block of a unit of own keys and a unit of own keys take of one.
+// (paged_mixed.hip): whole steps of blocks, `cus` workgroups a KV head, the blocks
+// of shared keys whose time a workgroup loses by beginning a second time, and the
+// time that a block of a unit of shared keys, a block of a unit of own keys and a
+// unit of own keys take of a workgroup.
 constexpr unsigned kMixedWaves = 8; // of a workgroup
 struct MixedPlan {
-  unsigned shift, step, cus;
+  unsigned step, cus, again;
   float sharedCost, ownCost, ownFixed;
 };
 hipError_t launch_paged_mixed(const half_t *q, const uint8_t *pool, const SharedView &g, half_t *out,

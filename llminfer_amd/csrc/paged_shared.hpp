@@ -25,13 +25,14 @@ struct SharedSeq {
 };
 
 // What the workgroups of a sequence leave for the join: its first piece, how
-// many a unit has, its units, and the group whose partials are joined to them
-// (+ 1; 0: none), for a group its first row. Own keys in runs of blocks
-// (paged_mixed.hip): the first of its blocks among all, the blocks of a unit, its
-// first unit among all, and the group; for a group beside them the columns of a
-// unit for the units, the first unit's pieces first.
+// many a unit has, its units (the last unit's pieces first), and the group whose
+// partials are joined to them (+ 1; 0: none), for a group its first row. Of runs of
+// blocks (paged_mixed.hip): the first of its blocks among all, the blocks of a unit,
+// its first unit among all, the same, and for a group the columns of a unit; and in
+// a note behind all others the blocks of a run of own keys, of one of shared keys,
+// and whether units of these are parted anywhere (1) or at whole runs (0).
 struct SharedNote {
-  unsigned first, pieces, units, other;
+  unsigned first, pieces, units, other, width, unused[3]; // (32 bytes)
 };
 
 // Sequences base .. base + sequences - 1 of `count` groups and then `all`
@@ -40,7 +41,7 @@ struct SharedNote {
 struct SharedView : PagedView {
   typedef SharedSeq Seq;
   const int32_t *groups, *prefix;
-  SharedNote *notes; // [count + all], and one with the blocks of a run
+  SharedNote *notes; // [count + all], and one of the runs
   unsigned count, all, base;
 };
 
@@ -211,7 +212,8 @@ __device__ __forceinline__ void leave_note(const SharedView &g, const SharedSeq 
                                            unsigned first, unsigned pieces, unsigned units) {
   const bool join = s.ok && (s.joined() || pieces > 1);
   g.notes[g.base + seq] =
-      SharedNote{first, join ? pieces : 0u, units, s.step == 0 ? s.row0 : s.begin ? s.group + 1 : 0u};
+      SharedNote{first, join ? pieces : 0u, units,
+                 s.step == 0 ? s.row0 : s.begin ? s.group + 1 : 0u, 0};
 }
 
 } // namespace llmi

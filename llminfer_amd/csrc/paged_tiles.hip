@@ -90,8 +90,10 @@ void paged_tiles_kernel(const half_t *__restrict__ q, const uint8_t *__restrict_
   const unsigned unit = units - 1 - local / pieces, piece = local % pieces;
   if (local == 0 && kvh == 0 && threadIdx.x == 0)
     leave_note(g, s, seq, number, pieces, units);
-  tiles_piece<D, 256 / D>(q, pool, g, out, invalid, queryHeads, split, c, parts, s, seq, kvh, unit,
-                          Tiles<D, 256 / D>::UNIT, piece, pieces, number);
+  const unsigned length = split.length(s, pieces);
+  tiles_piece<D, 256 / D, true>(q, pool, g, out, invalid, queryHeads, c, parts, s, seq, kvh,
+                                unit, Tiles<D, 256 / D>::UNIT, s.first() + piece * length, length,
+                                pieces == 1, number);
 }
 
 } // namespace

@@ -44,30 +44,36 @@ constexpr int kBufferWord3 = 0x00020000; // gfx9 raw buffer descriptor, dword 3
 // The order that the scheduler gives a run of products, N operands read from
 // LDS and CT products for each: some reads ahead of the first, then one after
 // each operand's products.
-template <int N, int CT> __device__ __forceinline__ void reads_ahead() {
-  constexpr int kMfma = 0x008, kRead = 0x100, kAhead = CT == 1 ? 4 : 3;
-  __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+template <int N, int CT, int AHEAD> __device__ __forceinline__ void reads_ahead() {
+  constexpr int kMfma = 0x008, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kRead, AHEAD, 0);
 #pragma unroll
-  for (int i = 0; i < N - kAhead; ++i) {
+  for (int i = 0; i < N - AHEAD; ++i) {
     __builtin_amdgcn_sched_group_barrier(kMfma, CT, 0);
     __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
   }
-  __builtin_amdgcn_sched_group_barrier(kMfma, CT * kAhead, 0);
+  __builtin_amdgcn_sched_group_barrier(kMfma, CT * AHEAD, 0);
 }
 
-// Unit `unit`, of `width` columns, of sequence s (number seq) over its piece `piece`
-// of `pieces`; the partial's number is `number`.
-template <int D, int CT, typename View>
+// Unit `unit`, of `width` columns, of sequence s (number seq) over `length` blocks
+// of its keys from block `begin` on, all that it has if it is `undivided`; the
+// partial's number is `number`. MASKED: some columns do not see the last keys.
+template <int D, int CT, bool MASKED, typename View>
 __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
                                             const uint8_t *__restrict__ pool, const View &g,
                                             half_t *out, unsigned *invalid, unsigned queryHeads,
-                                            const Split &split, ScoreScale c, const Partials &parts,
+                                            ScoreScale c, const Partials &parts,
                                             const typename View::Seq &s, unsigned seq, unsigned kvh,
-                                            unsigned unit, unsigned width, unsigned piece,
-                                            unsigned pieces, unsigned number) {
+                                            unsigned unit, unsigned width, unsigned begin,
+                                            unsigned length, bool undivided, unsigned number) {
   using T = Tiles<D, CT>;
   const unsigned G = queryHeads / g.kvHeads;
-  const unsigned tid = threadIdx.x, lane = tid % 64, r = lane % 32, hi = lane / 32;
+  unsigned tid = threadIdx.x;
+  if constexpr (!std::is_same<View, PagedView>::value) {
+    asm volatile("" : "+v"(tid)); // (what comes of it is not kept from piece to piece: spilled)
+    __builtin_assume(tid < kThreads);
+  }
+  const unsigned lane = tid % 64, r = lane % 32, hi = lane / 32;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const unsigned half = wave / 4, tile0 = wave % 4 * CT;
 
@@ -99,8 +105,7 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
   // not in the pool, whose columns' outputs are NaN
   const unsigned whole = s.keys();
   unsigned end = whole;
-  const unsigned length = split.length(s, pieces);
-  const unsigned b0 = min(s.first() + piece * length, most / 32 + 1);
+  const unsigned b0 = min(begin, most / 32 + 1);
   const unsigned b1 = min(b0 + length, most / 32 + 1);
   const unsigned steps = (b1 - b0 + T::BLOCKS - 1) / T::BLOCKS;
 
@@ -195,6 +200,9 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
   };
 
   // ---- the products: Q^T operands, outputs
+  // (with a fourth at head_dim 256 a run's state makes it too many registers, and
+  // the scheduler takes none of them ahead)
+  constexpr int kAhead = CT == 1 && (D < 256 || MASKED) ? 4 : 3;
   half8_t qv[CT][T::STEPS];
 #pragma unroll
   for (int j = 0; j < CT; ++j)
@@ -229,14 +237,14 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
       for (int j = 0; j < CT; ++j)
         x[j] = mfma32x32x16(key, qv[j][n], x[j]);
     }
-    reads_ahead<T::STEPS, CT>();
+    reads_ahead<T::STEPS, CT, kAhead>();
     if constexpr (kWide)
 #pragma unroll
       for (int j = 0; j < CT; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
           x[j][v] = scaled_score(x[j][v], c.c);
-    if (base + 31 > least) {
+    if (MASKED && base + 31 > least) {
 #pragma unroll
       for (int j = 0; j < CT; ++j)
 #pragma unroll
@@ -290,7 +298,7 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
         for (int j = 0; j < CT; ++j)
           o[j][i] = mfma32x32x16(value, w[j][n], o[j][i]);
       }
-    reads_ahead<2 * T::OUT, CT>();
+    reads_ahead<2 * T::OUT, CT, kAhead>();
     __builtin_amdgcn_s_setprio(0);
   };
 
@@ -425,14 +433,14 @@ __device__ __forceinline__ void tiles_piece(const half_t *__restrict__ q,
         for (int e = 0; e < 4; ++e)
           y[e] = o[j][i][4 * v + e] * a + z[e] * b;
         const unsigned at = 32 * i + 8 * v + 4 * hi;
-        if (pieces == 1 && !s.joined())
+        if (undivided && !s.joined())
           *reinterpret_cast<half4_t *>(out + row[j] + at) =
               half4_t{(half_t)(y[0] * inv), (half_t)(y[1] * inv), (half_t)(y[2] * inv),
                       (half_t)(y[3] * inv)};
         else
           *reinterpret_cast<float4_t *>(parts.o + part * D + at) = y;
       }
-    if ((pieces > 1 || s.joined()) && hi == 0)
+    if ((!undivided || s.joined()) && hi == 0)
       *reinterpret_cast<float2 *>(parts.ml + 2 * part) = make_float2(top, sum);
   }
 }

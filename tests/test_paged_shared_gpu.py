@@ -290,7 +290,7 @@ class Group:
         prefix are shared, its last keys are each sequence's own copy."""
         self.seqs = [s for _, members in groups for s in members]
         width = max([-(-(r + p) // page) for r, p in self.seqs] + [1]) + extra
-        need = sum(-(-k // page) + len(m) * width for k, m in groups)
+        need = sum(k // page + len(m) * (width - k // page) for k, m in groups)
         numbers = iter(rng.permutation(need + 2).tolist())
         self.pool = random_pool(rng, need + 2, page, hkv, dim)
         self.table, self.k, self.v = [], [], []
@@ -298,16 +298,18 @@ class Group:
             whole = keys // page
             common = [next(numbers) for _ in range(whole)]
             shared = [rows16(rng, keys, hkv, dim, size=size) for _ in range(2)]
-            for r, p in members:
+            kept = [po.kept(x) for x in shared]
+            for i, (r, p) in enumerate(members):
                 n = r + p - keys
                 own = [rows16(rng, n, hkv, dim, size=size) for _ in range(2)]
                 self.table.append(common + [next(numbers) for _ in range(width - whole)])
-                self.k.append(po.kept(np.concatenate((shared[0], own[0]))))
-                self.v.append(po.kept(np.concatenate((shared[1], own[1]))))
+                self.k.append((kept[0], po.kept(own[0])))
+                self.v.append((kept[1], po.kept(own[1])))
                 row = dev(np.array(self.table[-1:], np.int32))
-                k, v = (np.concatenate((a, b)) for a, b in zip(shared, own))
+                first = whole * page if i else 0  # the shared pages are filled once
+                k, v = (np.concatenate((a[first:], b)) for a, b in zip(shared, own))
                 if len(k):
-                    ops.paged_append(dev(k), dev(v), self.pool, ints([0, len(k)]), ints([0]), row)
+                    ops.paged_append(dev(k), dev(v), self.pool, ints([0, len(k)]), ints([first]), row)
         self.table = dev(np.array(self.table, np.int32))
         self.rows = [r for r, _ in self.seqs]
         self.starts = ints(np.cumsum([0] + self.rows))
@@ -321,11 +323,14 @@ class Group:
         return ops.paged_gqa_shared(dev(q), self.pool, args.pop("starts"), args.pop("past"),
                                     args.pop("table"), args.pop("groups"), args.pop("prefix"), **args)
 
+    def cached(self, s, n):
+        return (np.concatenate(x)[:n] for x in (self.k[s], self.v[s]))
+
     def check(self, got, q, scale, skip=()):
         at = 0
         for s, (r, p) in enumerate(self.seqs):
             if r and s not in skip:
-                want, far = po.attention(q[at:at + r], self.k[s][:r + p], self.v[s][:r + p], p, scale)
+                want, far = po.attention(q[at:at + r], *self.cached(s, r + p), p, scale)
                 err = np.abs(got[at:at + r].astype(np.float64) - want)
                 assert np.all(err <= far), (s, (err - far).max(), np.isnan(got[at:at + r]).any())
             at += r
@@ -371,6 +376,24 @@ def test_shared(gpu, groups, per, hkv, dim, page, scale):
     got = g.call(q, scale=scale, invalid=word).cpu().numpy()
     assert word.item() == 0
     g.check(got, q, 1 / np.sqrt(np.float32(dim)) if scale is None else scale)
+
+
+@pytest.mark.parametrize("groups, per, hkv, dim, page, some", [
+    ([(1280, [(1, 1280 + i % 8) for i in range(288)])], 4, 16, 256, 64, range(0, 288, 31)),
+    ([(2048, [(1, 2050)] * 130), (1800, [(1, 1800 + i) for i in range(70)])], 8, 8, 128, 128,
+     [0, 1, 99, 129, 130, 160, 199]),
+    ([(3968, [(1, 3970 + i % 3) for i in range(300)])], 4, 16, 64, 128, range(0, 300, 43)),
+    ([(96, [(1, 96 + i % 60) for i in range(700)])], 4, 32, 64, 32, range(0, 700, 77)),
+])
+def test_shared_parted_units(gpu, groups, per, hkv, dim, page, some):
+    """So many units of shared keys that the workgroups' runs of blocks part them
+    anywhere, or that there are more of them than workgroups."""
+    rng = np.random.default_rng(hkv + dim)
+    g = Group(rng, groups, hkv, dim, page)
+    q = rows16(rng, sum(g.rows), per * hkv, dim)
+    got = g.call(q)
+    g.check(got.cpu().numpy(), q, 1 / np.sqrt(np.float32(dim)), set(range(len(g.rows))) - set(some))
+    assert torch.equal(got, g.call(q)) and not got.isnan().any()
 
 
 def test_shared_reads_the_first_table(gpu):
@@ -527,7 +550,7 @@ def test_shared_replayed(gpu, n):
         want = [g.call(x).cpu() for x in q]
         for s in (0, 1, n // 2, n - 1):
             p = int(past[s]) - less
-            exact, far = po.attention(q[0][s:s + 1], g.k[s][:p + 1], g.v[s][:p + 1], p, 1 / 16)
+            exact, far = po.attention(q[0][s:s + 1], *g.cached(s, p + 1), p, 1 / 16)
             assert np.all(np.abs(want[0][s:s + 1].numpy().astype(np.float64) - exact) <= far)
         streams = [torch.cuda.Stream() for _ in graphs]
         torch.cuda.synchronize()

@@ -587,7 +587,9 @@ LLMI_HIP_API size_t llmi_hip_paged_gqa_shared_workspace_bytes(PagedSharedParams 
  * children may have one parent), of length L = past[parent[i]]: its row of
  * tableOut has the parent's first L / pageSize pages, then spare[i], a page of
  * its own, into which the blocks of the parent's next page that hold its last L
- * % pageSize keys are copied, then -1 to the row's end; pastOut[i] = L. With
+ * % pageSize keys are copied, then -1 to the row's end; pastOut[i] = L. (Where
+ * that is none, the page is held, as llmi_hip_paged_free counts, from the child's
+ * first key of its own on.) With
  * spare[i] negative it takes over the parent's row as it is, which at most one
  * child of a parent can do. (A full row has no place for a spare page, which
  * stays unused.)

@@ -902,7 +902,7 @@ SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) 
   // own block (eight waves have one each in 2.2, 1.2 or 0.8), an own unit; and the
   // blocks of the 8 us that a second beginning takes.
   const unsigned width = p.headDim == 256 ? 0 : p.headDim == 128 ? 1 : 2;
-  constexpr float kShared[] = {1.15f, 0.58f, 0.42f}, kOwn[] = {0.28f, 0.15f, 0.1f};
+  constexpr float kShared[] = {1.04f, 0.52f, 0.38f}, kOwn[] = {0.28f, 0.15f, 0.1f};
   s.mixed = {512 / p.headDim, kCus / p.kvHeads, 7u << width, kShared[width], kOwn[width], 0.4f};
   const uint64_t units = most_units(of, group, 128), ownUnits = most_units(p, group, kColumns);
   // the blocks of all units, which are counted in 32 bits

@@ -282,13 +282,6 @@ struct Mixed {
   unsigned workers, sharedRun, ownRun;
   bool whole;
 };
-__device__ __forceinline__ float wave_sum(float x) {
-  x = group_sum<16>(x);
-  LanePair p = pair16(x);
-  x = p.a + p.b;
-  p = pair32(x);
-  return p.a + p.b;
-}
 __device__ __forceinline__ unsigned own_units(const SharedSeq &q, unsigned group) {
   return q.step ? (q.rows * group + kColumns - 1) / kColumns : 0u;
 }

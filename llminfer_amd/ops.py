@@ -1278,8 +1278,9 @@ def bind_paged_fork(pool: torch.Tensor, table: torch.Tensor, past: torch.Tensor,
     parent[i] of table [S, n] and past [S] as row i of table_out [N, n] and
     past_out [N] (all int32). It shares the parent's whole pages and gets a copy
     of the page that is not full in page spare[i], or with spare[i] negative
-    takes over the parent's row as it is. Spare pages are apart and none of a
-    sequence's (paged_free has them). A parent that is not one of the
+    takes over the parent's row as it is. Where that page has no key yet, the
+    spare one is the child's next (paged_free counts it from its first key on).
+    Spare pages are apart and none of a sequence's (paged_free has them). A parent that is not one of the
     sequences, or does not fit its row: a row of -1 of length -1; a page that is
     not in the pool: -1 in its place; both set bit 1 of invalid."""
     _require_pool(pool)

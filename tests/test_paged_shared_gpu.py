@@ -693,6 +693,44 @@ def test_other_stream_and_order(gpu):
     assert torch.equal(free, ops.paged_free(g.table, g.past, 32, g.pool.shape[0])[0])
 
 
+@pytest.mark.parametrize("n", [6, 50])
+def test_a_pool_past_4_gib(gpu, n):
+    """Pages at the end of 6.5 GB hold what those of a small pool do after the same
+    calls: offsets in bytes need more than 32 bits."""
+    rng = np.random.default_rng(n)
+    page, hkv, dim, pages = 32, 4, 256, 160_000
+    g = Group(rng, [(256, [(1, 290 + 5 * i) for i in range(n)])], hkv, dim, page, extra=2)
+    small = g.pool.shape[0]
+    spare = ints(range(small, small + n))
+    pool = torch.cat((g.pool, torch.zeros_like(g.pool[:n])))
+    far = torch.empty((pages, *pool.shape[1:]), dtype=torch.uint8, device="cuda")
+    assert far.nbytes > 1 << 32
+    far[-small - n:] = pool
+    to = pages - small - n
+    q = rows16(rng, n, 4 * hkv, dim)
+    want = g.call(q)
+    assert not want.isnan().any()
+    g.pool, table = far, g.table
+    assert torch.equal(g.call(q, table=table + to), want)
+    seen = []
+    rows = [20 + i % 14 for i in range(n)]
+    source = [int(x) for r in rows for x in np.sort(rng.permutation(280)[:r])]
+    for where, add in ((pool, 0), (far, to)):
+        mine = table + add
+        ops.paged_move(where, ints(np.cumsum([0] + rows)), ints([256] * n), mine, ints(source))
+        ops.paged_move(where, ints([0, 20]), ints([260]), mine[n - 1:], ints(range(256, 276)),
+                       mine[1:2])
+        t, past = ops.paged_fork(where, mine, g.past, ints(range(n - 1, -1, -1)), spare + add)
+        # (with the pages of their next rows)
+        free, count = ops.paged_free(t, past + 1, page, where.shape[0])
+        k, v = ops.paged_read(where, ints(range(0, 290 * n + 1, 290)), ints([0] * n), t, 290 * n)
+        held = t[t >= 0].unique() - add
+        seen.append((t - add * (t >= 0), past, k, v, held, count - where.shape[0]))
+        assert not torch.isin(held + add, free).any()
+    for a, b in zip(*seen):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------- refusals
 
 def test_refuses(gpu):

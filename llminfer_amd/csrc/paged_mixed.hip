@@ -9,19 +9,26 @@
 // CUs as make them end together, and own keys go by waves and not by workgroups:
 // a wave with a run of blocks waits for no other, and its runs are of equal
 // length whatever the sequences' are (pieces by workgroups, joined in LDS: 12 us
-// each, five of them waiting; 48 chats 57 us, 44 with runs).
+// each, five of them waiting; 48 chats 57 us, 44 with runs). Shared keys go by
+// workgroups, which begin a unit in 8 us: a run of blocks each, of one unit where
+// there are fewer units than workgroups, else wherever the runs part them (900
+// sequences of 8 heads of 128, 29 units for 32 workgroups a KV head, behind 4096
+// keys: 156 us, 411 with whole units of as many blocks each).
 //
 // 48 sequences of 16 / 4 heads of 256, 16384 shared keys and up to 1024 of their
-// own, 13.3 GFLOP, take 39 us here and 44 with the join (paged_gqa: 137 to 142).
-// Tiles, 52 of a KV head's 64 workgroups, 20 blocks each: 6 us until the first
-// block is there (plan 1.5, table, block, one after the other), 1.15 us a block,
-// 4 to join the halves and write 24 MB of partials. Own keys, 10 blocks a wave:
-// 2.2 us a block of 10 KB and 9 us beside them, bound by decoding (550
-// instructions a block, two waves a SIMD). Matrix instructions take 15 % of the
-// time, vector instructions 31 %, waves wait for 52 %: barriers of a step, LDS and
-// the beginning. Six groups at head_dim 128: 48 us, own keys 1.2 us a block; two
-// of 187 rows in all at 64: 42 us, tiles 3.2 us a step of eight blocks, bound by
-// the softmax's vector instructions.
+// own, 13.3 GFLOP, take 38 us here and 41.5 with the join (paged_gqa: 137 to 142).
+// Tiles, 48 of a KV head's 64 workgroups, 22 blocks each: 6 us until the first
+// block is there (plan 1.5, table, block, one after the other), 1 us a block, 4 to
+// join the halves and write 22 MB of partials. A step of two blocks is 3800 cycles
+// of a SIMD with two waves, whose own take 1200 of decoding each, 1030 and 1050 of
+// products (512 and 512 of them the matrix cores'; LDS gives 192 KB a step and
+// takes 64, 2000 cycles of its own) and 660 of softmax; no wave waits for loads.
+// Own keys, 8 blocks a wave: 2.2 us a block of 10 KB, two waves a SIMD, bound by
+// decoding (550 instructions a block). Matrix instructions take 16 % of the
+// time, vector instructions 32 %, waves wait for 43 %. Six groups at head_dim 128:
+// 45 us with the join, own keys 1.2 us a block; two of 187 rows in all at 64:
+// 42 us, tiles 3.2 us a step of eight blocks, bound by the softmax's vector
+// instructions.
 #include "paged_tiles.hpp"
 
 namespace llmi {
@@ -420,8 +427,9 @@ struct MixedArgs {
   unsigned mostShared, mostOwn;
 };
 // The arguments, read again: kept in registers over the pieces of a run they and
-// what comes of them fill the scalar ones, and with these full the tiles' products
-// wait for each operand (two groups at head_dim 64: 44 us, 42 so).
+// what comes of them fill the scalar ones, and with these full the compiler takes
+// no operand of the tiles' products ahead (16 drafts: 56 us, 52.6 so; six groups
+// 48 and 44).
 __device__ __forceinline__ MixedArgs mixed_args() {
   auto at = __builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(at));

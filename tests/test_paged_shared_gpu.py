@@ -693,6 +693,33 @@ def test_other_stream_and_order(gpu):
     assert torch.equal(free, ops.paged_free(g.table, g.past, 32, g.pool.shape[0])[0])
 
 
+def test_two_at_once(gpu):
+    """Bound calls in flight on two streams, each with its own workspace."""
+    rng = np.random.default_rng(2)
+    calls = []
+    for groups, per, hkv, dim, page in (SHARED[0], SHARED[1], SHARED[9], SHARED[14]):
+        g = Group(rng, groups, hkv, dim, page)
+        q = dev(rows16(rng, sum(g.rows), per * hkv, dim))
+        out = torch.empty_like(q)
+        free, count = ints(range(g.pool.shape[0])), ints([0])
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            bound = [ops.bind_paged_gqa_shared(q, g.pool, g.starts, g.past, g.table, g.groups,
+                                               g.prefix, out),
+                     ops.bind_paged_free(g.table, g.past, page, free, count)]
+        want = g.call(q.cpu().numpy()), ops.paged_free(g.table, g.past, page, free.numel())[0]
+        calls.append((bound, out, free, want))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for bound, *_ in calls:
+            for b in bound:
+                b()
+    torch.cuda.synchronize()
+    for _, out, free, want in calls:
+        assert torch.equal(out, want[0]) and torch.equal(free, want[1])
+
+
 @pytest.mark.parametrize("n", [6, 50])
 def test_a_pool_past_4_gib(gpu, n):
     """Pages at the end of 6.5 GB hold what those of a small pool do after the same

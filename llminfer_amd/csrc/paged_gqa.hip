@@ -874,11 +874,18 @@ namespace {
 //  Mixed  shared keys in tiles of 128 columns, beside them own keys in units of
 //         16, by one launch (paged_mixed.hip);
 //  Apart  each by a launch of its own, as its columns ask for.
-// Mixed from 96 columns a group and 640 in all KV heads on (128 columns of 8
-// heads of 128 on 8192 keys: 29 us, 35 Same; 768 of 4 heads of 256 on 16384: 44
-// and 61; below, its beginning and end cost more: 64 of 4 heads on 4096 keys 25
-// us, 18 Same; 128 of one head 18 and 12). Apart where the sequences have many rows
-// themselves, and where Mixed cannot count the blocks or divide the device.
+// Mixed where it saves more than its beginning and end cost: the time of the shared
+// keys goes by units, about 1.1 of 16 columns and 2.6 of 128, times KV heads and keys,
+// of which the host knows how many a table has place for, and takes 16384 where that
+// is more. On 8192 keys, in us, Same and Mixed: 4 heads of 256, a group of 64 columns
+// 22.3 and 27.4, of 96 29.4 and 29.9, 4 of 49 42.5 and 35.6, 16 of 18 51 and 67, 16 of
+// 38 80 and 66; 8 heads of 128, a group of 64 22.3 and 23.0, of 96 30.2 and 24.9, 4 of
+// 24 29.3 and 29.1, of 49 40 and 38; 8 heads of 64, a group of 128 21.8 and 23.4, 4
+// of 60 27 and 33, 16 of 38 59 and 55. On 2048 keys Same is up to 6 us faster at
+// these, on 32768 Mixed up to 35 (a group of 96 of 4 heads of 256 62 and 40, of 128 of
+// 8 heads of 64 52 and 32).
+// Apart where the sequences have many rows themselves, and for tiles where Mixed
+// cannot count the blocks or divide the device.
 // Same has the pieces of its kernel's eight waves where the units are few (8
 // sequences on 4299 keys: 15.3 us, 17.2 with four), two rounds of four waves
 // otherwise (4 groups of 8 on 8192 keys: 25 us, 30 with six rounds or one).
@@ -909,11 +916,15 @@ SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) 
   const uint64_t blocks = ((uint64_t)p.tableStride * p.pageSize / 32 + 1) *
                           (units > ownUnits ? units : ownUnits);
   const bool mixes = s.mixed.cus > 1 && blocks < 1u << 30;
-  if (s.restShift != 4 || (all / groups >= 96 && !mixes)) {
+  const uint64_t columns = (all + groups - 1) / groups, most = (uint64_t)p.tableStride * p.pageSize;
+  const float saved = (float)p.kvHeads * groups *
+                      (1.1f * ((columns + 15) / 16) - 2.6f * ((columns + 127) / 128)) *
+                      ((most < 16384 ? most : 16384) / 8192.0f);
+  if (s.restShift != 4 || (columns >= 96 && !mixes)) {
     s.how = SharedPlan::Apart;
     s.sharedPieces = most_pieces(of, group, s.shared.split);
     s.restPieces = most_pieces(p, group, s.rest.split);
-  } else if (all / groups >= 96 && all * p.kvHeads >= 640) {
+  } else if (mixes && saved > (p.headDim == 64 ? 60.0f : 18.0f)) {
     s.how = SharedPlan::Mixed;
     s.sharedShift = 7;
     s.sharedPieces = s.mixed.cus + units;

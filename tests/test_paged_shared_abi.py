@@ -168,8 +168,13 @@ def test_launches():
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED, shared_params(heads=4))
     assert names[-1] == "pagedSharedMerge" and names[0] == "pagedGqaSplit"
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED,
-                             shared_params(heads=16, kvHeads=4, headDim=256, tokens=48, sequences=48))
+                             shared_params(heads=16, kvHeads=4, headDim=256, tokens=48, sequences=48,
+                                           pages=2000, tableStride=256))
     assert names == ["pagedGqaMixed", "pagedSharedMerge"]
+    names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED,
+                             shared_params(heads=16, kvHeads=4, headDim=256, tokens=48, sequences=48,
+                                           tableStride=9))
+    assert names == ["pagedGqaSplit", "pagedSharedMerge"]
     names = ops.kernel_names(_lib.OP_PAGED_GQA_SHARED,
                              shared_params(heads=16, kvHeads=4, headDim=256, tokens=400, sequences=4))
     assert names == ["pagedGqaTiles", "pagedGqaTiles", "pagedSharedMerge"]

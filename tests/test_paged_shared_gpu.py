@@ -283,7 +283,9 @@ def test_move_without_place(gpu):
 # -------------------------------------------------------------------- shared
 
 class Group:
-    """Sequences behind one prefix: a pool and its table, as forks leave them."""
+    """Sequences behind one prefix: a pool and its table, as forks leave them, whose
+    rows have place for `places` keys at least."""
+    places = 0
 
     def __init__(self, rng, groups, hkv, dim, page, size=1.0, extra=0):
         """groups: (prefix, [(rows, past) of each sequence]). Whole pages of a
@@ -310,7 +312,9 @@ class Group:
                 k, v = (np.concatenate((a[first:], b)) for a, b in zip(shared, own))
                 if len(k):
                     ops.paged_append(dev(k), dev(v), self.pool, ints([0, len(k)]), ints([first]), row)
-        self.table = dev(np.array(self.table, np.int32))
+        self.table = np.array(self.table, np.int32)
+        unused = max(self.places // page - width, 0)
+        self.table = dev(np.pad(self.table, ((0, 0), (0, unused)), constant_values=-1))
         self.rows = [r for r, _ in self.seqs]
         self.starts = ints(np.cumsum([0] + self.rows))
         self.past = ints(p for _, p in self.seqs)
@@ -334,6 +338,13 @@ class Group:
                 err = np.abs(got[at:at + r].astype(np.float64) - want)
                 assert np.all(err <= far), (s, (err - far).max(), np.isnan(got[at:at + r]).any())
             at += r
+
+
+@pytest.fixture(params=[0, 16384], ids=["short", "long"])
+def room(request, monkeypatch):
+    """Tables that are as long as their sequences, and longer: the host divides the
+    work by what a table has place for."""
+    monkeypatch.setattr(Group, "places", request.param)
 
 
 SHARED = [  # groups, heads a KV head, hkv, dim, page
@@ -366,6 +377,7 @@ SHARED = [  # groups, heads a KV head, hkv, dim, page
 ]
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("groups, per, hkv, dim, page", SHARED)
 @pytest.mark.parametrize("scale", [None, -0.3, 0.0])
 def test_shared(gpu, groups, per, hkv, dim, page, scale):
@@ -378,6 +390,7 @@ def test_shared(gpu, groups, per, hkv, dim, page, scale):
     g.check(got, q, 1 / np.sqrt(np.float32(dim)) if scale is None else scale)
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("groups, per, hkv, dim, page, some", [
     ([(1280, [(1, 1280 + i % 8) for i in range(288)])], 4, 16, 256, 64, range(0, 288, 31)),
     ([(2048, [(1, 2050)] * 130), (1800, [(1, 1800 + i) for i in range(70)])], 8, 8, 128, 128,
@@ -409,6 +422,7 @@ def test_shared_reads_the_first_table(gpu):
     g.check(got, q, 1 / 16)
 
 
+@pytest.mark.usefixtures("room")
 def test_shared_outside_groups(gpu):
     """Sequences before, between and behind the groups share nothing; rows of no
     sequence stay."""
@@ -422,6 +436,7 @@ def test_shared_outside_groups(gpu):
     assert (got[-3:] == 7).all()
 
 
+@pytest.mark.usefixtures("room")
 def test_shared_large_scores(gpu):
     """Scores far past the weights' range, in both parts."""
     rng = np.random.default_rng(4)
@@ -430,6 +445,7 @@ def test_shared_large_scores(gpu):
     g.check(g.call(q).cpu().numpy(), q, 1 / np.sqrt(128))
 
 
+@pytest.mark.usefixtures("room")
 
 
 @pytest.mark.parametrize("members", [3, 60, 90])
@@ -481,6 +497,7 @@ def test_shared_without_place(gpu, members):
     g.check(got, q, 1 / 16)
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("n", [20, 100])
 def test_shared_odd_orders(gpu, n):
     """Starts and groups out of order, overlapping or out of range: any values
@@ -500,6 +517,7 @@ def test_shared_odd_orders(gpu, n):
                 assert (out[2 * n:] == 7).all()
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("n", [6, 90])
 def test_shared_rows_are_apart(gpu, n):
     """A query row of infinities or NaN changes no other row."""
@@ -522,6 +540,7 @@ def test_shared_is_plain_without_groups(gpu):
     assert torch.equal(got, ops.paged_gqa(dev(q), g.pool, g.starts, g.past, g.table))
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("n", [9, 90])
 def test_shared_replayed(gpu, n):
     """A captured call is replayed on other lengths, groups and prefixes, with
@@ -693,6 +712,7 @@ def test_other_stream_and_order(gpu):
     assert torch.equal(free, ops.paged_free(g.table, g.past, 32, g.pool.shape[0])[0])
 
 
+@pytest.mark.usefixtures("room")
 def test_two_at_once(gpu):
     """Bound calls in flight on two streams, each with its own workspace."""
     rng = np.random.default_rng(2)
@@ -720,6 +740,7 @@ def test_two_at_once(gpu):
         assert torch.equal(out, want[0]) and torch.equal(free, want[1])
 
 
+@pytest.mark.usefixtures("room")
 @pytest.mark.parametrize("n", [6, 50])
 def test_a_pool_past_4_gib(gpu, n):
     """Pages at the end of 6.5 GB hold what those of a small pool do after the same
@@ -738,12 +759,12 @@ def test_a_pool_past_4_gib(gpu, n):
     want = g.call(q)
     assert not want.isnan().any()
     g.pool, table = far, g.table
-    assert torch.equal(g.call(q, table=table + to), want)
+    there = torch.where(table >= 0, table + to, table)
+    assert torch.equal(g.call(q, table=there), want)
     seen = []
     rows = [20 + i % 14 for i in range(n)]
     source = [int(x) for r in rows for x in np.sort(rng.permutation(280)[:r])]
-    for where, add in ((pool, 0), (far, to)):
-        mine = table + add
+    for where, add, mine in ((pool, 0, table), (far, to, there)):
         ops.paged_move(where, ints(np.cumsum([0] + rows)), ints([256] * n), mine, ints(source))
         ops.paged_move(where, ints([0, 20]), ints([260]), mine[n - 1:], ints(range(256, 276)),
                        mine[1:2])

@@ -115,3 +115,91 @@ def test_own_tiles_without_place(gpu, members, per, dim, rows):
     g = fresh()
     g.past[2], g.past[members - 1] = prefix - 1, g.table.shape[1] * page
     expect(g, {2: 0, members - 1: 0})
+
+
+# ----------------------------- pieces that take their blocks' places by turns
+
+class Pages:
+    """Sequences behind one prefix in a pool of any bytes with finite scales: what
+    it holds is what ops.paged_read says."""
+
+    def __init__(self, seed, prefix, seqs, hkv, dim, page, places=0):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        common = prefix // page
+        owned = [-(-(r + p) // page) - common for r, p in seqs]
+        width = max(common + max(owned), places // page)
+        order = 1 + torch.randperm(common + sum(owned), generator=g, device="cuda").int()
+        pages = order.numel() + 1  # (page 0 is none of the sequences')
+        self.pool = torch.randint(0, 256, (pages, hkv, page // 32, 40 * dim), generator=g,
+                                  dtype=torch.uint8, device="cuda")
+        for at in (16 * dim, 36 * dim):
+            scale = 0.05 * torch.randn(pages, hkv, page // 32, 2 * dim, generator=g, device="cuda")
+            self.pool[..., at:at + 4 * dim] = scale.half().view(torch.uint8)
+        self.table = torch.full((len(seqs), width), -1, dtype=torch.int32, device="cuda")
+        self.table[:, :common] = order[:common]
+        at = common
+        for s, n in enumerate(owned):
+            self.table[s, common:common + n] = order[at:at + n]
+            at += n
+        self.seqs, self.rows = seqs, [r for r, _ in seqs]
+        self.starts, self.past = ints(np.cumsum([0] + self.rows)), ints(p for _, p in seqs)
+        self.groups, self.prefix = ints([0, len(seqs)]), ints([prefix])
+
+    def check(self, got, q, s, heads):
+        """Rows of sequence s, some query heads."""
+        at, (r, p) = sum(self.rows[:s]), self.seqs[s]
+        k, v = ops.paged_read(self.pool, ints([0, r + p]), ints([0]), self.table[s:s + 1].contiguous(),
+                              r + p)
+        per = q.shape[1] // k.shape[1]
+        for h in heads:
+            kv = (x[:, h // per:h // per + 1].cpu().numpy() for x in (k, v))
+            want, far = po.attention(q[at:at + r, h:h + 1], *kv, p, 1 / np.sqrt(np.float32(q.shape[2])))
+            assert np.all(np.abs(got[at:at + r, h:h + 1].astype(np.float64) - want) <= far), (s, h)
+
+
+# With 128 KV heads two workgroups have one: the first all shared keys, a unit of 48
+# columns, the second's eight waves the own keys, equal runs of them. Places are
+# looked up for 64 steps of 512 / dim shared blocks, and for 64 own blocks, at once.
+LONG = [  # dim, page, prefix, own keys of the long sequences, how many of 48 they are
+    (64, 128, 17408, 3000, 6),   # 544 shared blocks, 68 steps; 594 own, runs of 75
+    (128, 64, 9216, 40, 1),      # 288 shared blocks, 72 steps
+    (128, 32, 4096, 3001, 6),
+    (256, 128, 5120, 2990, 6),   # 160 shared blocks, 80 steps
+]
+
+
+@pytest.mark.parametrize("dim, page, prefix, rest, many", LONG)
+def test_long_runs(gpu, dim, page, prefix, rest, many):
+    """Runs that look their blocks' places up more than once, and a page that is
+    missing behind the first time."""
+    hkv, S = 128, 48
+    # (the others' columns make one unit; the long ones lie first, so that runs part them)
+    seqs = [(1, prefix + rest - 3 * i) for i in range(many)]
+    seqs += [(1, prefix + i % 20) for i in range(S - many)]
+
+    def fresh():
+        return Pages(dim, prefix, seqs, hkv, dim, page, 16384)
+
+    q = rows16(np.random.default_rng(dim), S, hkv, dim)
+    g = fresh()
+    word = ints([0])
+    what, got = called(g, q, invalid=word)
+    assert what == "pagedGqaMixed+pagedSharedMerge" and word.item() == 0 and not np.isnan(got).any()
+    for s in (0, many - 1, many, S - 1):
+        g.check(got, q, s, (0, 77, 127))
+    assert np.array_equal(called(g, q)[1], got)
+    # own block 70, of a run from block 0 on, and the last page of another sequence
+    for s, key in ((0, min(70 * 32, rest)), (many - 1, rest - 3 * (many - 1))):
+        g = fresh()
+        g.pool[0] = 0xFF
+        g.table[s, (prefix + key) // page] = -1
+        word.zero_()
+        lost = called(g, q, invalid=word)[1]
+        assert word.item() == 2 and np.isnan(lost[s]).all()
+        others = np.arange(S) != s
+        assert np.array_equal(lost[others], got[others])
+    g = fresh()
+    g.pool[0] = 0xFF
+    g.table[0, (prefix - 32) // page] = g.pool.shape[0]  # the last shared one
+    word.zero_()
+    assert np.isnan(called(g, q, invalid=word)[1]).all() and word.item() == 2

@@ -203,3 +203,75 @@ def test_long_runs(gpu, dim, page, prefix, rest, many):
     g.table[0, (prefix - 32) // page] = g.pool.shape[0]  # the last shared one
     word.zero_()
     assert np.isnan(called(g, q, invalid=word)[1]).all() and word.item() == 2
+
+
+# -------------------------------------------------- starts and groups in disorder
+
+def claimed(starts, tokens):
+    """Rows that a sequence has, of starts in any order."""
+    rows = np.zeros(tokens, bool)
+    for a, b in zip(starts, starts[1:]):
+        lo = min(max(a, 0), tokens)
+        rows[lo:min(max(b, lo), tokens)] = True
+    return rows
+
+
+@pytest.mark.parametrize("n, rows, dim, places, what", [
+    (20, 2, 256, 0, "pagedGqaSplit+pagedSharedMerge"),
+    (100, 2, 256, 0, "pagedGqaSplit+pagedSharedMerge"),
+    (30, 2, 256, 16384, "pagedGqaMixed+pagedSharedMerge"),
+    (100, 2, 256, 16384, "pagedGqaMixed+pagedSharedMerge"),
+    (100, 2, 64, 16384, "pagedGqaMixed+pagedSharedMerge"),
+    (9, 48, 256, 0, TILES),
+    (70, 48, 256, 0, TILES),
+])
+def test_disorder_stays_in_its_rows(gpu, n, rows, dim, places, what):
+    """Starts and groups out of order, overlapping or out of range change no row
+    that no sequence has, and nothing behind the output or a workspace of exactly
+    the size that is asked for, whatever it held. In order again, the result is what
+    it was."""
+    rng = np.random.default_rng(n)
+    g = Group(rng, [(64, [(rows, 64 + i) for i in range(n)])], 1, dim, 32)
+    g.table = torch.nn.functional.pad(g.table, (0, max(places // 32 - g.table.shape[1], 0)), value=-1)
+    T = rows * n + 4
+    q = dev(rows16(rng, T, 4, dim))
+    lib, guard = _lib.load(), 4096
+    around = torch.empty(q.numel() + 2 * guard, dtype=torch.float16, device="cuda")
+    out = around[guard:-guard].view(q.shape)
+    assert out.data_ptr() % 16 == 0
+    kv = _lib.PagedKvParams(g.pool.shape[0], 32, 1, dim, n, g.table.shape[1], T)
+    stream = torch.cuda.current_stream().cuda_stream
+    ordered = [rows * i for i in range(n + 1)]
+
+    def call(starts, groups, prefix, fill):
+        p = _lib.PagedSharedParams(_lib.PagedGqaParams(kv, 4, 0.1), len(prefix))
+        need = lib.llmi_hip_paged_gqa_shared_workspace_bytes(p)
+        ws = torch.full((need + 2 * guard,), fill, dtype=torch.uint8, device="cuda")
+        ws[:guard] = ws[-guard:] = 99
+        around.fill_(7)
+        arrays = [ints(x) for x in (starts, groups, prefix)]
+        _lib.check(lib.llmi_hip_paged_gqa_shared(
+            q.data_ptr(), arrays[0].data_ptr(), g.past.data_ptr(), g.table.data_ptr(),
+            arrays[1].data_ptr(), arrays[2].data_ptr(), g.pool.data_ptr(), out.data_ptr(), None, p,
+            ws.data_ptr() + guard, need, stream))
+        torch.cuda.synchronize()
+        assert (ws[:guard] == 99).all() and (ws[-guard:] == 99).all()
+        assert (around[:guard] == 7).all() and (around[-guard:] == 7).all()
+        left = dev(~claimed(starts, T))
+        assert (out[left] == 7).all(), (starts[:9], groups, prefix)
+        return p, out.clone()
+
+    p, want = call(ordered, [0, n], [64], 0)
+    assert "+".join(ops.kernel_names(_lib.OP_PAGED_GQA_SHARED, p)) == what
+    assert not (want[:rows * n] == 7).all(-1).any()
+    disorders = [ordered, [0, 20 * rows, 3, 10 * rows, 9] + [15 * rows] * (n - 4),
+                 list(range(T, T + n + 1)), list(range(n, -1, -1)),
+                 [-5] * (n // 2) + [rows * n + 2] * (n + 1 - n // 2),
+                 [2**31 - 1] * 2 + [-2**31] * (n - 2) + [T + 9]]
+    for starts in disorders:
+        for groups, prefix in (([0, n], [64]), ([5, 2], [64]), ([0, n, 0, n, 0, n], [64] * 5),
+                               ([-9, 6 * n], [64]), ([n + 10, n + 20], [64]), ([0] * 71, [32] * 70),
+                               ([2**31 - 1, -2**31], [2**31 - 1])):
+            for fill in (0xFF, 0x01):
+                call(starts, groups, prefix, fill)
+    assert torch.equal(call(ordered, [0, n], [64], 0xFF)[1], want)

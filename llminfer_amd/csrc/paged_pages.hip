@@ -88,6 +88,8 @@ constexpr unsigned kWindow = 1u << 19; // pages whose marks one workgroup has in
 constexpr unsigned kListed = 4096;     // pages whose entries one workgroup writes
 constexpr unsigned kSmall = 8192;      // pages of a pool that one workgroup has alone
 constexpr unsigned kMarkers = 32;      // workgroups that mark, at most
+constexpr unsigned kSlots = 8;         // of a row that a lane has: 512 slots are a piece of it
+constexpr unsigned kRows = 4;          // pieces that a wave has in flight
 
 struct FreeView {
   const int32_t *table, *lengths;
@@ -99,7 +101,6 @@ struct FreeView {
 // pieces of rows in flight.
 __device__ __forceinline__ void mark_held(const FreeView &g, unsigned part, unsigned parts,
                                           unsigned window, uint32_t *marks, unsigned *invalid) {
-  constexpr unsigned kRows = 4, kSlots = 8;
   const unsigned tid = threadIdx.x, lane = tid % 64, first = window * kWindow;
   const unsigned wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const unsigned mine = min(kWindow, g.pages - first);
@@ -211,8 +212,12 @@ __global__ __launch_bounds__(kFreeThreads) void paged_free_small_kernel(FreeView
 // that no memory has to be cleared and nothing is atomic but bits in LDS; the join
 // and the list are launches of their own because a free page's rank needs all the
 // marks before it (marks of eight workgroups joined by those that list: 24 us).
-// One workgroup alone up to 8192 pages and 16384 slots: 5.2 us for 4096 pages,
-// against three launches.
+// The time goes by pieces of rows, not by slots: short rows are a piece each. One
+// workgroup alone up to 8192 pages and 96 pieces, a round and a half of its waves
+// (at 8192 pages, one workgroup and three launches: 65 rows of 256 7.4 and 10.1 us,
+// 96 10.2 and 10.7, 127 11.3 and 11.0, 500 of 65 29 and 10.2); 32 pieces a marking
+// workgroup, up to the most (1000 rows of 32 in 400 thousand pages: 12.2 us, 58 in
+// one; 4000 of 16 15.3 and, in three, 74).
 // What the launches leave each other: [part][words] marks, the words of a part
 // whole 16 bytes, [words] of all of them and how many pages of each kListed are
 // free.
@@ -292,11 +297,16 @@ __global__ __launch_bounds__(kFreeThreads) void paged_free_list_kernel(FreeMarks
                      [&](unsigned i) { return sWord[i - first / 32]; });
 }
 
+uint64_t free_pieces(const PagedFreeParams &p) {
+  return (uint64_t)p.sequences * ((p.tableStride + 64 * kSlots - 1) / (64 * kSlots));
+}
 unsigned free_markers(const PagedFreeParams &p) {
-  const uint64_t slots = (uint64_t)p.sequences * p.tableStride, parts = slots / 16384;
+  const uint64_t parts = free_pieces(p) / 32;
   return parts < 1 ? 1u : parts < kMarkers ? (unsigned)parts : kMarkers;
 }
-bool free_small(const PagedFreeParams &p) { return p.pages <= kSmall && free_markers(p) == 1; }
+bool free_small(const PagedFreeParams &p) {
+  return p.pages <= kSmall && free_pieces(p) <= 96;
+}
 
 // -------------------------------------------------------------------- move
 //

@@ -7,7 +7,7 @@ import torch
 
 from llminfer_amd import _lib, ops
 from tests import paged_oracle as po
-from tests.test_paged_shared_gpu import Group, dev, ints, rows16
+from tests.test_paged_shared_gpu import Group, dev, free_oracle, ints, rows16
 
 pytestmark = pytest.mark.gpu
 
@@ -275,3 +275,27 @@ def test_disorder_stays_in_its_rows(gpu, n, rows, dim, places, what):
             for fill in (0xFF, 0x01):
                 call(starts, groups, prefix, fill)
     assert torch.equal(call(ordered, [0, n], [64], 0xFF)[1], want)
+
+
+# ------------------------------------------------------------------ free pages
+
+@pytest.mark.parametrize("sequences, width, launches", [
+    (96, 256, 1), (97, 256, 3), (48, 513, 1), (49, 513, 3), (96, 1, 1), (97, 1, 3),
+    (12, 4096, 1), (12, 4097, 3), (1000, 32, 3), (2100, 7, 3), (2, 20_000, 1),
+])
+@pytest.mark.parametrize("pages", [33, 8192])
+def test_free_by_pieces(gpu, sequences, width, launches, pages):
+    """One workgroup for up to 96 pieces of 512 slots of rows, short rows a piece
+    each; up to 32 workgroups that mark."""
+    rng = np.random.default_rng(width + sequences)
+    p = _lib.PagedFreeParams(pages, 32, sequences, width)
+    assert len(ops.kernel_names(_lib.OP_PAGED_FREE, p)) == launches
+    for most in (width, 3):
+        table = rng.integers(0, pages, (sequences, width), dtype=np.int32)
+        lengths = rng.integers(0, min(width, most) * 32 + 1, sequences)
+        lengths[rng.random(sequences) < 0.6] = 0
+        want, count, bad = free_oracle(table, lengths, 32, pages)
+        word = ints([0])
+        free, n = ops.paged_free(dev(table), ints(lengths), 32, pages, word)
+        assert not bad and word.item() == 0 and n.item() == count
+        assert np.array_equal(free.cpu().numpy(), want)

@@ -17,8 +17,8 @@
 //
 // 48 sequences of 16 / 4 heads of 256, 16384 shared keys and up to 1024 of their
 // own, 13.3 GFLOP, take 38 us here and 41.5 with the join (paged_gqa: 137 to 142).
-// Tiles, 48 of a KV head's 64 workgroups, 22 blocks each: 6 us until the first
-// block is there (plan 1.5, table, block, one after the other), 1 us a block, 4 to
+// Tiles, 48 of a KV head's 64 workgroups, 22 blocks each: 7 us until the first
+// block is there (plan 2, table, block, one after the other), 1 us a block, 4 to
 // join the halves and write 22 MB of partials. A step of two blocks is 3800 cycles
 // of a SIMD with two waves, whose own take 1200 of decoding each, 1030 and 1050 of
 // products (512 and 512 of them the matrix cores'; LDS gives 192 KB a step and
@@ -27,8 +27,11 @@
 // decoding (550 instructions a block). Matrix instructions take 16 % of the
 // time, vector instructions 32 %, waves wait for 43 %. Six groups at head_dim 128:
 // 45 us with the join, own keys 1.2 us a block; two of 187 rows in all at 64:
-// 42 us, tiles 3.2 us a step of eight blocks, bound by the softmax's vector
-// instructions.
+// 42 us, tiles 2.9 us a step of eight blocks, of which a wave's softmax is 2300 to
+// 3000 of 6600 cycles. At 256 a lane has all of its 256 registers; at 128 and 64 it
+// has 166 and 129: there the tiles' 128 KB of LDS, the same at every width, leave
+// room for two waves a SIMD only, which keep the vector units active for 48 % of
+// their cycles and the matrix cores for 14 to 17 %.
 #include "paged_tiles.hpp"
 
 namespace llmi {

@@ -883,7 +883,12 @@ namespace {
 // 24 29.3 and 29.1, of 49 40 and 38; 8 heads of 64, a group of 128 21.8 and 23.4, 4
 // of 60 27 and 33, 16 of 38 59 and 55. On 2048 keys Same is up to 6 us faster at
 // these, on 32768 Mixed up to 35 (a group of 96 of 4 heads of 256 62 and 40, of 128 of
-// 8 heads of 64 52 and 32).
+// 8 heads of 64 52 and 32). And what the plan costs Same, whose workgroups, two a CU at
+// a time, each look at all groups and sequences, about 1.3 us for 64 of them, 2.6 where
+// the groups are more than a wave's lanes; those of Mixed are all there at once. Behind
+// 512 keys: 257 sequences in 6 groups, 4 heads of 256, 45 and 29; 500 in 125 153 and
+// 101; 1000 in 250 563 and 209, 8 heads of 128 1005 and 288, 4000 in 1000 17950 and
+// 1384; 256 in 128, 4 heads of 256, 71 and 74, and behind 2048 120 and 283.
 // Apart where the sequences have many rows themselves, and for tiles where Mixed
 // cannot count the blocks or divide the device.
 // Same has the pieces of its kernel's eight waves where the units are few (8
@@ -920,11 +925,13 @@ SharedPlan shared_plan(const PagedKvParams &p, unsigned group, unsigned groups) 
   const float saved = (float)p.kvHeads * groups *
                       (1.1f * ((columns + 15) / 16) - 2.6f * ((columns + 127) / 128)) *
                       ((most < 16384 ? most : 16384) / 8192.0f);
+  const float rounds = (float)p.kvHeads * (ownUnits + groups * ((columns + 15) / 16)) / (2 * kCus);
+  const float plans = rounds * ((p.sequences + groups) / 64.0f) * (groups > 64 ? 2.6f : 1.3f);
   if (s.restShift != 4 || (columns >= 96 && !mixes)) {
     s.how = SharedPlan::Apart;
     s.sharedPieces = most_pieces(of, group, s.shared.split);
     s.restPieces = most_pieces(p, group, s.rest.split);
-  } else if (mixes && saved > (p.headDim == 64 ? 60.0f : 18.0f)) {
+  } else if (mixes && saved + plans > (p.headDim == 64 ? 60.0f : 18.0f)) {
     s.how = SharedPlan::Mixed;
     s.sharedShift = 7;
     s.sharedPieces = s.mixed.cus + units;

@@ -170,14 +170,15 @@ __device__ __forceinline__ SharedSeq paged_from_lane(const SharedSeq &own, unsig
 }
 __device__ __forceinline__ SharedSeq paged_seq_of(const SharedView &g, const SharedLanes &own,
                                                   unsigned seq) {
-  SharedSeq q;
-  shared_chunks(g, own, [&](unsigned c, const SharedSeq &s) {
-    if (c != seq / 64)
-      return false;
-    q = paged_from_lane(s, seq % 64);
-    return true;
-  });
-  return q;
+  if (seq < 64)
+    return paged_from_lane(own.a, seq);
+  if (seq < 128)
+    return paged_from_lane(own.b, seq - 64);
+  if (seq < 192)
+    return paged_from_lane(own.c, seq - 128);
+  if (seq < 256)
+    return paged_from_lane(own.d, seq - 192);
+  return paged_from_lane(shared_seq(g, own.groups, seq / 64 * 64 + threadIdx.x % 64), seq % 64);
 }
 
 template <typename Count>

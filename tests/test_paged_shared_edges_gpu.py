@@ -299,3 +299,42 @@ def test_free_by_pieces(gpu, sequences, width, launches, pages):
         free, n = ops.paged_free(dev(table), ints(lengths), 32, pages, word)
         assert not bad and word.item() == 0 and n.item() == count
         assert np.array_equal(free.cpu().numpy(), want)
+
+
+# ------------------------------------------- groups and sequences by the hundred
+
+MANY = [  # groups, sequences of each, heads a KV head, hkv, dim, page, launches of how
+    (250, 4, 4, 4, 64, 32, "pagedGqaMixed"),
+    (130, 5, 4, 8, 128, 32, "pagedGqaMixed"),
+    (66, 9, 2, 4, 256, 64, "pagedGqaMixed"),
+    (6, 60, 4, 4, 256, 32, "pagedGqaMixed"),
+    (130, 2, 4, 2, 64, 32, "pagedGqaSplit"),
+    (40, 3, 4, 4, 128, 32, "pagedGqaSplit"),
+]
+
+
+@pytest.mark.parametrize("groups, members, per, hkv, dim, page, how", MANY)
+def test_many_groups(gpu, groups, members, per, hkv, dim, page, how):
+    """Where the plan of every workgroup, which looks at all groups and sequences,
+    is most of the work, the launch with few workgroups is taken."""
+    rng = np.random.default_rng(groups + dim)
+    each = [(64 + 32 * (i % 3), [(1, 130 + (7 * i + j) % 60) for j in range(members)])
+            for i in range(groups)]
+    each[groups // 2] = (96, [(0, 99), (2, 96)])
+    g = Group(rng, each, hkv, dim, page)
+    q = rows16(rng, sum(g.rows), per * hkv, dim)
+    word = ints([0])
+    what, got = called(g, q, invalid=word)
+    assert what == how + "+pagedSharedMerge" and word.item() == 0 and not np.isnan(got).any()
+    last = len(g.rows) - 1
+    some = {0, 1, members, 63, 64, 127, 128, 191, 192, 255, 256, 257, last - 1, last,
+            members * (groups // 2) + 1}
+    scale, others = 1 / np.sqrt(np.float32(dim)), set(range(last + 1)) - some
+    g.check(got, q, scale, others)
+    g.past[last // 2] = -1
+    lost = called(g, q, invalid=word)[1]
+    at = np.cumsum([0] + g.rows)
+    here = np.zeros(len(q), bool)
+    here[at[last // 2]:at[last // 2 + 1]] = True
+    assert word.item() == 2 and np.isnan(lost[here]).all() and not np.isnan(lost[~here]).any()
+    g.check(lost, q, scale, others | {last // 2})

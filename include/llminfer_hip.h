@@ -575,7 +575,8 @@ LLMI_HIP_API size_t llmi_hip_paged_gqa_workspace_bytes(PagedGqaParams p);
  * paged_gqa. Sizes, limits, errors and the workspace
  * (llmi_hip_paged_gqa_shared_workspace_bytes) are as there; groups at most
  * 2^22 - 1. The workspace is the larger one where many rows share keys (16 / 4
- * heads of 256: 72 MB for 48 rows, 151 for 1000; paged_gqa 29 and 92). */
+ * heads of 256: 72 MB for 48 rows, 151 for 1000, 282 for 1000 in 250 groups;
+ * paged_gqa 29 and 92). */
 LLMI_HIP_API int llmi_hip_paged_gqa_shared(const uint16_t *q, const int32_t *starts,
                                            const int32_t *past, const int32_t *table,
                                            const int32_t *groups, const int32_t *prefix,

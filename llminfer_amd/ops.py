@@ -1231,9 +1231,9 @@ def bind_paged_gqa_shared(q: torch.Tensor, pool: torch.Tensor, starts: torch.Ten
     table of its first sequence. A sequence whose past is shorter than its
     group's prefix has no place: NaN, and bit 1 of invalid. Pays with many rows
     behind a long prefix, not below some thousand keys, and paged_gqa is faster with
-    tens of rows a sequence or two sequences a group. The workspace is the bound call's own (16 / 4 heads of 256: 72 MB for
-    48 rows, 151 for 1000, 282 for 1000 in 250 groups); keep a bound call as long as a graph that it was
-    captured into."""
+    tens of rows a sequence or two sequences a group. The workspace is the bound
+    call's own (16 / 4 heads of 256: 72 MB for 48 rows, 151 for 1000, 282 for 1000 in
+    250 groups); keep a bound call as long as a graph that it was captured into."""
     for t, n in ((q, "q"), (out, "out")):
         _require(t, torch.float16, n)
     if q.dim() != 3 or out.shape != q.shape:
